@@ -145,6 +145,21 @@ unsafe extern "C" {
         scales: *const QwArray, biases: *const QwArray, global_scale: *const QwArray,
         linear_bias: *const QwArray, group_size: c_int, bits: c_int, mode: *const c_char,
         y: *mut QwArray, stream: *mut c_void) -> c_int;
+    pub fn qw_quantized_linear_lora(x: *const QwArray, w: *const QwArray, scales: *const QwArray,
+        biases: *const QwArray, linear_bias: *const QwArray, lora_a: *const QwArray,
+        lora_b: *const QwArray, lora_scales: *const QwArray, adapter_idx: *const QwArray,
+        group_size: c_int, bits: c_int, mode: *const c_char, y: *mut QwArray,
+        workspace: *mut c_void, workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn qw_quantized_linear_lora_workspace(m: i64, n: i64, rank: i64, bytes: *mut i64) -> c_int;
+    pub fn qw_lora_backward(x: *const QwArray, dy: *const QwArray, lora_a: *const QwArray,
+        lora_b: *const QwArray, lora_scales: *const QwArray, adapter_idx: *const QwArray,
+        accumulate_dx: c_int, dx: *mut QwArray, da: *mut QwArray, db: *mut QwArray,
+        workspace: *mut c_void, workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn qw_lora_backward_workspace(m: i64, n: i64, k: i64, rank: i64, adapters: i64,
+        bytes: *mut i64) -> c_int;
+    pub fn qw_topk_distill(logits: *const QwArray, teacher_idx: *const QwArray,
+        teacher_values: *const QwArray, temperature: *const QwArray, row_weights: *const QwArray,
+        loss: *mut QwArray, dlogits: *mut QwArray, stream: *mut c_void) -> c_int;
     pub fn qw_dequantize(w: *const QwArray, scales: *const QwArray, biases: *const QwArray,
         group_size: c_int, bits: c_int, mode: *const c_char, out: *mut QwArray,
         stream: *mut c_void) -> c_int;

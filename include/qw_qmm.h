@@ -272,6 +272,84 @@ int qw_quantized_linear_forward_global_scale(const qw_array* x, const qw_array* 
                                              const qw_array* linear_bias, int group_size, int bits,
                                              const char* mode, qw_array* y, void* stream);
 
+/* ---------------------------------------------------------------- adapters
+ * Low-rank adapters of many requests beside one quantized projection.  A
+ * stack of L adapters of rank R (a lower rank is padded with zeros) is
+ *   lora_a f16 [L, R, K], lora_b f16 [L, N, R], lora_scales f32 [L] (nullable:
+ *   all 1; the usual alpha / rank), R 1..128, L up to 4096,
+ * and row m of x (leading dimensions flattened) takes adapter adapter_idx[m]
+ * (u32 [M], in any order; nullable: adapter 0 for every row).  An id of L or
+ * more, such as 0xFFFFFFFF, means no adapter; what x holds in such a row never
+ * reaches an adapter's result.
+ *
+ * Workspaces: these calls allocate no scratch.  The caller passes at least the
+ * bytes that the matching _workspace query reports (for the current device),
+ * 256-byte aligned, contents unspecified before and after; it must not be used
+ * by another call until this one has ended on the GPU (two captured graphs
+ * that may run at the same time need one each).  The first matmul call on a
+ * device creates its status word, so make one before a stream capture.
+ *
+ * y = x @ dequantize(w).T + linear_bias + scale * (x @ A.T) @ B.T with the A, B
+ * and scale of each row's adapter: y f16 [..., N], the sum of the three terms
+ * in fp32 rounded once.  x, w, scales, biases, linear_bias (nullable) as in
+ * qw_quantized_linear_forward; y must not overlap x.  With more than 16 rows
+ * the rank-space product scale * x A^T feeds the tensor cores as fp16 (so it
+ * must stay below 65504); with up to 16 it stays fp32.
+ * No counterpart in the reference, whose linears carry no adapters. */
+int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_array* scales, const qw_array* biases,
+                             const qw_array* linear_bias, const qw_array* lora_a, const qw_array* lora_b,
+                             const qw_array* lora_scales, const qw_array* adapter_idx, int group_size, int bits,
+                             const char* mode, qw_array* y, void* workspace, int64_t workspace_bytes, void* stream);
+/* Workspace bytes of qw_quantized_linear_lora for m rows of x against n output
+ * columns with adapters of this rank. */
+int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64_t* bytes);
+
+/* Gradient of the adapters' term: with h = scale * x A^T and g = scale * dy B
+ * of each row's adapter,
+ *   da[l] = sum over the rows m of adapter l of g[m]^T x[m]    f32 [L, R, K]
+ *   db[l] = sum over the rows m of adapter l of dy[m]^T h[m]   f32 [L, N, R]
+ *   dx[m] = g[m] A                                             f16 [..., K]
+ * da, db and dx are nullable (not all three) and are written whole: adapters
+ * without rows get zeros, rows without an adapter a zero dx.  With
+ * accumulate_dx != 0, dx += g A instead, rounded once per element (the caller
+ * put the frozen projection's dy @ dequantize(w) there), and rows without an
+ * adapter are left as they are.  x f16 [..., K] (rows may be strided as in
+ * qw_quantized_matmul), K a multiple of 64; dy f16 [..., N] row-contiguous; dx
+ * must not overlap x or dy.  Products are accumulated in fp32; h and g enter
+ * the sums over rows with 22 significant bits relative to their largest
+ * magnitude in the adapter.  Results do not depend on scheduling: the same
+ * inputs give the same bits.  Non-finite values in dy or x of an adapter's
+ * rows make that adapter's gradients non-finite. */
+int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora_a, const qw_array* lora_b,
+                     const qw_array* lora_scales, const qw_array* adapter_idx, int accumulate_dx, qw_array* dx,
+                     qw_array* da, qw_array* db, void* workspace, int64_t workspace_bytes, void* stream);
+/* Workspace bytes of qw_lora_backward for m rows, k inputs, n outputs and this
+ * many adapters of this rank. */
+int qw_lora_backward_workspace(int64_t m, int64_t n, int64_t k, int64_t rank, int64_t adapters, int64_t* bytes);
+
+/* ---------------------------------------------------------------- distillation
+ * Loss of a student's logits against a teacher's stored top logits (what
+ * qw_topk or qw_quantized_matmul_topk returned), and its gradient, in one
+ * pass over the logits.  For row m with p = softmax(teacher_values[m] / T) over
+ * its valid entries and q = softmax(logits[m] / T) over all V columns:
+ *   loss[m]    = w T^2 sum_j p_j (log p_j - log q_{i_j})
+ *   dlogits[m] = w T (q - sum_j p_j e_{i_j})        (the gradient of loss[m])
+ * logits f16, bf16 or f32 [..., V]; teacher_idx u32 [..., k] and teacher_values
+ * f16, bf16 or f32 [..., k], 1 <= k <= 1024, in any order; an id of V or more
+ * (0xFFFFFFFF) is no entry, and ids given twice count twice.  temperature T
+ * (f32 scalar in device memory, positive; nullable: 1), row_weights w (f32 [M];
+ * nullable: all 1).  loss f32 [M]; dlogits (nullable) has the logits' type and
+ * shape and may be the logits' own buffer.  A small type needs weights that
+ * carry a loss scale: values below its range round to zero.
+ * Rows with w = 0 get a zero loss and gradient whatever their logits hold, as
+ * do rows without a valid entry (or whose valid entries are all -inf).  Logits
+ * of -inf have q = 0; where the teacher gives such a column weight the loss is
+ * +inf, and the gradient follows the formula.
+ * No counterpart in the reference, which does not train. */
+int qw_topk_distill(const qw_array* logits, const qw_array* teacher_idx, const qw_array* teacher_values,
+                    const qw_array* temperature, const qw_array* row_weights, qw_array* loss, qw_array* dlogits,
+                    void* stream);
+
 /* out f16 [N, K] = scales * q + biases, each product and sum rounded to fp16
  * (the fp16 op-by-op evaluation of MLX's CPU backend).
  * Replaces: dequantize, lib.rs:1152-1159, mlx_cxx_bridge.cpp:3019-3069. */

@@ -7,13 +7,15 @@ its NVLink peer allreduce.
 The compute lives in libqwqmm.so (C ABI in include/qw_qmm.h); this package is
 the Python mirror of the reference's operator surface on torch tensors.
 """
-from .ops import (QuantizedFusedLinear, QuantizedLinear, QuantizedMlp, compiled_moe_expert_forward,
-                  compiled_swiglu_activation, decode_schedule, dequantize, device_status, quantize_weights,
+from .ops import (LoraAdapters, QuantizedFusedLinear, QuantizedLinear, QuantizedMlp, compiled_moe_expert_forward,
+                  compiled_swiglu_activation, decode_schedule, dequantize, device_status, lora_backward, quantize_weights,
                   quantized_linear_forward,
-                  quantized_linear_forward_global_scale, quantized_matmul, quantized_matmul_argmax,
-                  quantized_matmul_chain, quantized_matmul_swiglu, quantized_matmul_topk, swiglu_mlp, topk)
+                  quantized_linear_forward_global_scale, quantized_linear_lora, quantized_matmul, quantized_matmul_argmax,
+                  quantized_matmul_chain, quantized_matmul_swiglu, quantized_matmul_topk, swiglu_mlp, topk,
+                  topk_distillation)
 
 __all__ = [
+    "LoraAdapters",
     "QuantizedFusedLinear",
     "QuantizedLinear",
     "QuantizedMlp",
@@ -22,9 +24,11 @@ __all__ = [
     "decode_schedule",
     "dequantize",
     "device_status",
+    "lora_backward",
     "quantize_weights",
     "quantized_linear_forward",
     "quantized_linear_forward_global_scale",
+    "quantized_linear_lora",
     "quantized_matmul",
     "quantized_matmul_argmax",
     "quantized_matmul_chain",
@@ -32,4 +36,5 @@ __all__ = [
     "quantized_matmul_topk",
     "swiglu_mlp",
     "topk",
+    "topk_distillation",
 ]

@@ -1129,6 +1129,292 @@ int qw_quantize(const qw_array* w, int group_size, int bits, const char* mode, q
   return QW_OK;
 }
 
+// ------------------------------------------------- low-rank adapters
+namespace {
+
+// Whether the byte ranges of two contiguous arrays share memory.
+size_t dtype_bytes(int dtype) { return dtype == QW_F16 || dtype == QW_BF16 ? 2 : 4; }
+bool overlap(const qw_array* a, const qw_array* b, int64_t a_ld = 0, int64_t b_ld = 0) {
+  auto span = [](const qw_array* t, int64_t ld) -> size_t {
+    const int64_t n = numel(t);
+    if (n == 0) return 0;
+    const int64_t last = t->shape[t->ndim - 1];
+    return (size_t)(ld ? (n / last - 1) * ld + last : n) * dtype_bytes(t->dtype);
+  };
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a->data), pb = reinterpret_cast<uintptr_t>(b->data);
+  return pa < pb + span(b, b_ld) && pb < pa + span(a, a_ld);
+}
+
+// The adapters of a call over M rows of x: A f16 [L, R, K], B f16 [L, N, R],
+// scales f32 [L] (nullable), idx u32 [M] (nullable).  Fills p.a .. p.R.
+int check_adapters(const qw_array* lora_a, const qw_array* lora_b, const qw_array* lora_scales,
+                   const qw_array* adapter_idx, int64_t M, int64_t N, int64_t K, LoraArgs* p) {
+  int rc;
+  if ((rc = check_array(lora_a, "lora_a")) || (rc = check_array(lora_b, "lora_b")) ||
+      (lora_scales && (rc = check_array(lora_scales, "lora_scales"))) ||
+      (adapter_idx && (rc = check_array(adapter_idx, "adapter_idx"))))
+    return rc;
+  if (lora_a->dtype != QW_F16 || lora_b->dtype != QW_F16)
+    return fail(QW_EUNSUPPORTED, std::string("lora_a and lora_b must be float16, got ") + dtype_name(lora_a->dtype) +
+                                     " and " + dtype_name(lora_b->dtype));
+  if (lora_a->ndim != 3 || lora_b->ndim != 3)
+    return fail(QW_EINVAL, "lora_a must be 3-D [L, R, K] and lora_b 3-D [L, N, R]");
+  const int64_t L = lora_a->shape[0], R = lora_a->shape[1];
+  if (lora_a->shape[2] != K)
+    return fail(QW_EINVAL, "lora_a's width " + std::to_string(lora_a->shape[2]) + " does not match the input width " +
+                               std::to_string(K));
+  if (lora_b->shape[0] != L || lora_b->shape[1] != N || lora_b->shape[2] != R)
+    return fail(QW_EINVAL, "lora_b must be [" + std::to_string(L) + ", " + std::to_string(N) + ", " +
+                               std::to_string(R) + "] to match lora_a and the output width");
+  if (R < 1) return fail(QW_EINVAL, "the adapters' rank must be at least 1");
+  if (R > kLoraMaxRank)
+    return fail(QW_EUNSUPPORTED, "rank " + std::to_string(R) + " is above the supported " +
+                                     std::to_string(kLoraMaxRank));
+  if (L > kLoraMaxAdapters)
+    return fail(QW_EUNSUPPORTED, std::to_string(L) + " adapters are above the supported " +
+                                     std::to_string(kLoraMaxAdapters));
+  if (lora_scales && (lora_scales->dtype != QW_F32 || numel(lora_scales) != L))
+    return fail(QW_EINVAL, "lora_scales must be float32 with one element per adapter");
+  if (adapter_idx && (adapter_idx->dtype != QW_U32 || numel(adapter_idx) != M))
+    return fail(QW_EINVAL, "adapter_idx must be uint32 with one element per row of x");
+  if (!aligned(lora_a->data, 16) || !aligned(lora_b->data, 16) || (lora_scales && !aligned(lora_scales->data, 4)) ||
+      (adapter_idx && !aligned(adapter_idx->data, 4)))
+    return fail(QW_EINVAL, "lora_a and lora_b must be 16-byte aligned, lora_scales and adapter_idx 4-byte aligned");
+  p->a = lora_a->data;
+  p->b = lora_b->data;
+  p->scales = lora_scales ? static_cast<const float*>(lora_scales->data) : nullptr;
+  p->idx = adapter_idx ? static_cast<const uint32_t*>(adapter_idx->data) : nullptr;
+  p->M = M;
+  p->N = N;
+  p->K = K;
+  p->L = L;
+  p->R = (int)R;
+  return QW_OK;
+}
+
+constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Bytes of the decode kernel's scratch at the start of a forward workspace.
+size_t lora_skinny_bytes(int64_t M, int64_t N, int64_t K, int dev) {
+  if (M > 16) return 0;
+  SkinnyArgs sa{};
+  sa.M = M;
+  sa.N = N;
+  sa.K = K;
+  return align256(skinny_scratch_bytes(sa, dev));
+}
+
+int check_workspace(const void* workspace, int64_t have, size_t need) {
+  if (have < 0 || (size_t)have < need)
+    return fail(QW_EINVAL, "the workspace has " + std::to_string(have) + " bytes, the call needs " +
+                               std::to_string(need));
+  if (need && !workspace) return fail(QW_EINVAL, "workspace is null");
+  if (!aligned(workspace, 256)) return fail(QW_EINVAL, "the workspace must be 256-byte aligned");
+  return QW_OK;
+}
+
+}  // namespace
+
+int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64_t* bytes) {
+  set_error("");
+  if (!bytes) return fail(QW_EINVAL, "bytes is null");
+  if (m < 0 || n < 0 || rank < 1 || rank > kLoraMaxRank || m > ((int64_t)1 << 30) || n > ((int64_t)1 << 30))
+    return fail(QW_EINVAL, "m, n or rank out of range");
+  int dev = 0;
+  const cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  *bytes = (int64_t)(lora_skinny_bytes(m, n, 0, dev) + lora_forward_bytes(m, n, rank));
+  return QW_OK;
+}
+
+int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_array* scales, const qw_array* biases,
+                             const qw_array* linear_bias, const qw_array* lora_a, const qw_array* lora_b,
+                             const qw_array* lora_scales, const qw_array* adapter_idx, int group_size, int bits,
+                             const char* mode, qw_array* y, void* workspace, int64_t workspace_bytes, void* stream_v) {
+  set_error("");
+  int rc;
+  SkinnyArgs sa;
+  if ((rc = check_qmm_call(x, w, scales, biases, 1, group_size, bits, mode, y, &sa))) return rc;
+  if (y->dtype != QW_F16) return fail(QW_EINVAL, "linear forward output must be float16");
+  if (linear_bias) {
+    if ((rc = check_array(linear_bias, "linear_bias"))) return rc;
+    if (linear_bias->dtype != QW_F16 || numel(linear_bias) != sa.N)
+      return fail(QW_EINVAL, "linear_bias must be float16 with N elements");
+  }
+  LoraArgs la{};
+  if ((rc = check_adapters(lora_a, lora_b, lora_scales, adapter_idx, sa.M, sa.N, sa.K, &la))) return rc;
+  if (sa.M == 0 || sa.N == 0) return QW_OK;
+  if (sa.M > ((int64_t)1 << 30)) return fail(QW_EUNSUPPORTED, "x has more rows than supported");
+  if (overlap(x, y, sa.x_ld)) return fail(QW_EINVAL, "y must not overlap x");
+  la.x = sa.x;
+  la.x_ld = sa.x_ld;
+  int dev = 0;
+  cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  const size_t skinny = lora_skinny_bytes(sa.M, sa.N, sa.K, dev);
+  if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, sa.N, la.R)))) return rc;
+  DeviceRes* res = nullptr;
+  std::string err;
+  if (!device_res(dev, &res, &err)) return fail(QW_ENOMEM, err);
+  cudaStream_t stream = as_stream(stream_v);
+  void* lws = static_cast<uint8_t*>(workspace) + skinny;
+  if (skinny) {
+    ce = cudaMemsetAsync(workspace, 0, skinny_zeroed_bytes(sa), stream);
+    if (ce != cudaSuccess) return cuda_fail(ce, "cudaMemsetAsync");
+  }
+  if ((ce = launch_lora_shrink(la, lws, stream)) != cudaSuccess) return cuda_fail(ce, "adapter launch");
+  if (sa.M <= 16) {
+    sa.y = lora_forward_product(la, lws);
+    sa.y_f32 = true;
+    sa.status = res->status;
+    Scratch sc{workspace, skinny};
+    ce = launch_skinny(sa, sc, stream, pdl_enabled(), &err);
+    if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "skinny launch") : fail(QW_ECUDA, err);
+  } else {
+    PrefillArgs pa{sa.x, sa.w, sa.scales, sa.biases, lora_forward_product(la, lws), true, sa.M, sa.N, sa.K,
+                   res->status};
+    pa.x_ld = sa.x_ld;
+    pa.bits = bits;
+    pa.group_size = group_size;
+    ce = launch_prefill(pa, stream, pdl_enabled(), &err);
+    if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "prefill launch") : fail(QW_ECUDA, err);
+  }
+  ce = launch_lora_expand(la, lws, linear_bias ? linear_bias->data : nullptr, y->data, stream);
+  return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter launch");
+}
+
+int qw_lora_backward_workspace(int64_t m, int64_t n, int64_t k, int64_t rank, int64_t adapters, int64_t* bytes) {
+  set_error("");
+  if (!bytes) return fail(QW_EINVAL, "bytes is null");
+  if (m < 0 || n < 0 || k < 0 || rank < 1 || rank > kLoraMaxRank || adapters < 0 || adapters > kLoraMaxAdapters ||
+      m > ((int64_t)1 << 30) || n > ((int64_t)1 << 30) || k > ((int64_t)1 << 28))
+    return fail(QW_EINVAL, "m, n, k, rank or adapters out of range");
+  int dev = 0;
+  const cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  *bytes = (int64_t)lora_backward_bytes(m, n, k, rank, adapters, device_info(dev).sm_count);
+  return QW_OK;
+}
+
+int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora_a, const qw_array* lora_b,
+                     const qw_array* lora_scales, const qw_array* adapter_idx, int accumulate_dx, qw_array* dx,
+                     qw_array* da, qw_array* db, void* workspace, int64_t workspace_bytes, void* stream_v) {
+  set_error("");
+  int rc;
+  if (!x) return fail(QW_EINVAL, "x is null");
+  if (x->ndim < 1 || x->ndim > 4) return fail(QW_EINVAL, "x must have 1 to 4 dimensions");
+  const int64_t K = x->shape[x->ndim - 1];
+  LoraArgs la{};
+  if ((rc = check_x_rows(x, K, &la.x_ld)) || (rc = check_array(dy, "dy"))) return rc;
+  if (x->dtype != QW_F16 || dy->dtype != QW_F16)
+    return fail(QW_EUNSUPPORTED, std::string("x and dy must be float16, got ") + dtype_name(x->dtype) + " and " +
+                                     dtype_name(dy->dtype));
+  if (K < 1 || K % 64 != 0) return fail(QW_EINVAL, "x's last dimension must be a multiple of 64");
+  const int64_t N = dy->shape[dy->ndim - 1];
+  const int64_t M = numel(x) / K;
+  if (N < 1 || numel(dy) / N != M)
+    return fail(QW_EINVAL, "dy must have shape [..., N] with the leading dimensions of x");
+  if (M > ((int64_t)1 << 24) || N > ((int64_t)1 << 30) || K > ((int64_t)1 << 28))
+    return fail(QW_EUNSUPPORTED, "x or dy beyond the supported range");
+  if ((rc = check_adapters(lora_a, lora_b, lora_scales, adapter_idx, M, N, K, &la))) return rc;
+  if ((dx && (rc = check_array(dx, "dx"))) || (da && (rc = check_array(da, "da"))) ||
+      (db && (rc = check_array(db, "db"))))
+    return rc;
+  if (!dx && !da && !db) return fail(QW_EINVAL, "dx, da and db are all null");
+  if (dx && (dx->dtype != QW_F16 || dx->shape[dx->ndim - 1] != K || numel(dx) != M * K))
+    return fail(QW_EINVAL, "dx must be float16 [..., K] with the leading dimensions of x");
+  auto same_shape = [](const qw_array* a, const qw_array* b) {
+    return a->ndim == 3 && a->shape[0] == b->shape[0] && a->shape[1] == b->shape[1] && a->shape[2] == b->shape[2];
+  };
+  if (da && (da->dtype != QW_F32 || !same_shape(da, lora_a)))
+    return fail(QW_EINVAL, "da must be float32 with lora_a's shape");
+  if (db && (db->dtype != QW_F32 || !same_shape(db, lora_b)))
+    return fail(QW_EINVAL, "db must be float32 with lora_b's shape");
+  if ((M && !aligned(x->data, 16)) || (dx && !aligned(dx->data, 16)) || (da && !aligned(da->data, 16)) ||
+      (db && !aligned(db->data, 16)))
+    return fail(QW_EINVAL, "x, dx, da and db must be 16-byte aligned");
+  if (M && !aligned(dy->data, 2)) return fail(QW_EINVAL, "dy is misaligned");
+  if (dx && (overlap(dx, x, 0, la.x_ld) || overlap(dx, dy)))
+    return fail(QW_EINVAL, "dx must not overlap x or dy");
+  int dev = 0;
+  const cudaError_t cd = cudaGetDevice(&dev);
+  if (cd != cudaSuccess) return cuda_fail(cd, "cudaGetDevice");
+  const int sms = device_info(dev).sm_count;
+  if ((rc = check_workspace(workspace, workspace_bytes, lora_backward_bytes(M, N, K, la.R, la.L, sms)))) return rc;
+  la.x = x->data;
+  LoraGrads g{};
+  g.dy = dy->data;
+  g.dy_ld = N;
+  g.dx = dx ? dx->data : nullptr;
+  g.add_dx = accumulate_dx != 0;
+  g.da = da ? static_cast<float*>(da->data) : nullptr;
+  g.db = db ? static_cast<float*>(db->data) : nullptr;
+  const cudaError_t ce = launch_lora_backward(la, g, workspace, sms, as_stream(stream_v));
+  return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter gradient launch");
+}
+
+// ------------------------------------------------------ distillation
+int qw_topk_distill(const qw_array* logits, const qw_array* teacher_idx, const qw_array* teacher_values,
+                    const qw_array* temperature, const qw_array* row_weights, qw_array* loss, qw_array* dlogits,
+                    void* stream) {
+  set_error("");
+  int rc;
+  if ((rc = check_array(logits, "logits")) || (rc = check_array(teacher_idx, "teacher_idx")) ||
+      (rc = check_array(teacher_values, "teacher_values")) ||
+      (temperature && (rc = check_array(temperature, "temperature"))) ||
+      (row_weights && (rc = check_array(row_weights, "row_weights"))) || (rc = check_array(loss, "loss")) ||
+      (dlogits && (rc = check_array(dlogits, "dlogits"))))
+    return rc;
+  auto real = [](const qw_array* a) { return a->dtype == QW_F16 || a->dtype == QW_BF16 || a->dtype == QW_F32; };
+  if (!real(logits) || !real(teacher_values))
+    return fail(QW_EUNSUPPORTED, "logits and teacher_values must be float16, bfloat16 or float32");
+  const int64_t V = logits->shape[logits->ndim - 1];
+  const int64_t k = teacher_idx->shape[teacher_idx->ndim - 1];
+  if (V < 1) return fail(QW_EINVAL, "rows of logits are empty");
+  const int64_t M = numel(logits) / V;
+  if (k < 1) return fail(QW_EINVAL, "teacher_idx must hold at least one entry per row");
+  if (k > distill_max_top())
+    return fail(QW_EUNSUPPORTED, std::to_string(k) + " teacher entries per row are above the supported " +
+                                     std::to_string(distill_max_top()));
+  if (V > ((int64_t)1 << 30) || M > ((int64_t)1 << 28))
+    return fail(QW_EUNSUPPORTED, "logits beyond the supported range");
+  if (teacher_idx->dtype != QW_U32 || numel(teacher_idx) != M * k)
+    return fail(QW_EINVAL, "teacher_idx must be uint32 [..., k] with the leading dimensions of the logits");
+  if (teacher_values->shape[teacher_values->ndim - 1] != k || numel(teacher_values) != M * k)
+    return fail(QW_EINVAL, "teacher_values must have teacher_idx's shape");
+  if (temperature && (temperature->dtype != QW_F32 || numel(temperature) != 1))
+    return fail(QW_EINVAL, "temperature must be a float32 scalar");
+  if (row_weights && (row_weights->dtype != QW_F32 || numel(row_weights) != M))
+    return fail(QW_EINVAL, "row_weights must be float32 with one element per row of logits");
+  if (loss->dtype != QW_F32 || numel(loss) != M)
+    return fail(QW_EINVAL, "loss must be float32 with one element per row of logits");
+  if (dlogits && (dlogits->dtype != logits->dtype || dlogits->shape[dlogits->ndim - 1] != V ||
+                  numel(dlogits) != M * V))
+    return fail(QW_EINVAL, "dlogits must have the logits' type and shape");
+  if (!aligned(logits->data, dtype_bytes(logits->dtype)) ||
+      (dlogits && !aligned(dlogits->data, dtype_bytes(logits->dtype))) || !aligned(teacher_idx->data, 4) ||
+      !aligned(teacher_values->data, dtype_bytes(teacher_values->dtype)) || !aligned(loss->data, 4) ||
+      (temperature && !aligned(temperature->data, 4)) || (row_weights && !aligned(row_weights->data, 4)))
+    return fail(QW_EINVAL, "an array is misaligned");
+  if (dlogits && dlogits->data != logits->data && overlap(dlogits, logits))
+    return fail(QW_EINVAL, "dlogits must be the logits' own buffer or not overlap it");
+  DistillArgs a{};
+  a.logits = logits->data;
+  a.idx = static_cast<const uint32_t*>(teacher_idx->data);
+  a.values = teacher_values->data;
+  a.temperature = temperature ? static_cast<const float*>(temperature->data) : nullptr;
+  a.weights = row_weights ? static_cast<const float*>(row_weights->data) : nullptr;
+  a.loss = static_cast<float*>(loss->data);
+  a.dlogits = dlogits ? dlogits->data : nullptr;
+  a.M = M;
+  a.V = V;
+  a.k = (int)k;
+  a.dtype = logits->dtype;
+  a.values_dtype = teacher_values->dtype;
+  const cudaError_t ce = launch_distill(a, as_stream(stream));
+  return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "distillation launch");
+}
+
 const char* qw_last_error(void) { return qw::last_error(); }
 
 int qw_device_status(int device, unsigned int* status, int clear) {

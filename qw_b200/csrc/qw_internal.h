@@ -167,6 +167,54 @@ cudaError_t launch_allreduce(const ArComm& c, const float* partial, void* out, b
 // and synchronized), cleared when `clear`; 0 when no such call ran there.
 cudaError_t static_scratch_status(int device, unsigned int* v, bool clear);
 
+// Low-rank adapters beside a projection (qw_lora.cu): row m of x takes
+// adapter idx[m] (idx null: adapter 0; idx[m] >= L: none).
+struct LoraArgs {
+  const void* x;          // fp16 [M][K], rows x_ld apart
+  const void* a;          // fp16 [L][R][K]
+  const void* b;          // fp16 [L][N][R]
+  const float* scales;    // [L] (null: all 1)
+  const uint32_t* idx;    // [M]
+  int64_t M, N, K, L;
+  int64_t x_ld;
+  int R;
+};
+struct LoraGrads {
+  const void* dy;  // fp16 [M][N], rows dy_ld apart
+  int64_t dy_ld;
+  void* dx;        // fp16 [M][K] or null
+  bool add_dx;     // dx += instead of dx =
+  float* da;       // [L][R][K] or null
+  float* db;       // [L][N][R] or null
+};
+constexpr int kLoraMaxRank = 128;
+constexpr int64_t kLoraMaxAdapters = 4096;
+// Forward workspace after the decode kernel's scratch.
+size_t lora_forward_bytes(int64_t M, int64_t N, int64_t R);
+cudaError_t launch_lora_shrink(const LoraArgs& p, void* ws, cudaStream_t stream);
+// fp32 [M][N] within the workspace: where the projection's product goes.
+float* lora_forward_product(const LoraArgs& p, void* ws);
+cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, cudaStream_t stream);
+size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);
+cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, cudaStream_t stream);
+
+// Distillation from a teacher's top logits (qw_distill.cu).
+struct DistillArgs {
+  const void* logits;        // [M][V]
+  const uint32_t* idx;       // [M][k], ids >= V: no entry
+  const void* values;        // [M][k], of type values_dtype
+  const float* temperature;  // scalar or null (1)
+  const float* weights;      // [M] or null (all 1)
+  float* loss;               // [M]
+  void* dlogits;             // [M][V] or null
+  int64_t M, V;
+  int k;
+  int dtype;                 // qw_dtype of logits and dlogits
+  int values_dtype;          // qw_dtype of values
+};
+int distill_max_top();
+cudaError_t launch_distill(const DistillArgs& p, cudaStream_t stream);
+
 // Quantize / dequantize kernels (affine, 4-bit, group 64 for now).
 cudaError_t launch_dequantize(const uint32_t* w, const void* scales, const void* biases, void* out, int64_t N,
                               int64_t K, int group_size, int bits, int rounding, cudaStream_t stream);

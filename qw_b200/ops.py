@@ -212,6 +212,87 @@ def quantized_linear_forward_global_scale(x, w, scales, biases, global_scale=Non
     return out
 
 
+def _one_device(x: torch.Tensor, *tensors):
+    """Every operand on x's device (the library is given bare addresses)."""
+    for t in tensors:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"operands on {x.device} and {t.device}")
+    return torch.cuda.device(x.device)
+
+
+def _workspace(query, x: torch.Tensor, *sizes) -> torch.Tensor:
+    """Scratch of one call, of the current stream (inside a capture: of the graph's own pool)."""
+    n = ctypes.c_int64(0)
+    _lib.check(query(*[int(s) for s in sizes], ctypes.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=x.device)
+
+
+def quantized_linear_lora(x: torch.Tensor, w, scales, biases, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                          lora_scales: Optional[torch.Tensor] = None, adapter_idx: Optional[torch.Tensor] = None,
+                          linear_bias: Optional[torch.Tensor] = None, group_size: int = 64, bits: int = 4,
+                          mode: str = "affine", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ dequantize(w).T + linear_bias + s (x @ A.T) @ B.T with the adapter
+    (A, B, s) of each row, many adapters in one call: ``lora_a`` fp16
+    [L, R, K], ``lora_b`` fp16 [L, N, R], ``lora_scales`` fp32 [L] (None: 1),
+    ``adapter_idx`` int32, one per row in any order, -1 for none (None: adapter
+    0 for every row)."""
+    if out is None:
+        out = torch.empty(*x.shape[:-1], w.shape[0], dtype=torch.float16, device=x.device)
+    L = _lib.load()
+    with _one_device(x, w, scales, biases, lora_a, lora_b, lora_scales, adapter_idx, linear_bias, out):
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        ws = _workspace(L.qw_quantized_linear_lora_workspace, x, rows, w.shape[0], lora_a.shape[1])
+        _lib.check(L.qw_quantized_linear_lora(
+            _arr(x), _arr(w), _arr(scales), _arr(biases), _arr(linear_bias), _arr(lora_a), _arr(lora_b),
+            _arr(lora_scales), _arr(adapter_idx), group_size, bits, _mode(mode), _arr(out), ws.data_ptr(),
+            ws.numel(), _stream(x)))
+    return out
+
+
+def lora_backward(x: torch.Tensor, dy: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                  lora_scales: Optional[torch.Tensor] = None, adapter_idx: Optional[torch.Tensor] = None,
+                  dx: Optional[torch.Tensor] = None):
+    """Gradient of quantized_linear_lora's adapters: (dx fp16 like x, da fp32
+    [L, R, K], db fp32 [L, N, R]).  Given ``dx`` (the frozen projection's
+    dy @ dequantize(w)), the adapters' part is added to it in place; otherwise
+    a new tensor holds that part alone."""
+    accumulate = dx is not None
+    if dx is None:
+        dx = torch.empty(x.shape, dtype=torch.float16, device=x.device)
+    da = torch.empty(lora_a.shape, dtype=torch.float32, device=x.device)
+    db = torch.empty(lora_b.shape, dtype=torch.float32, device=x.device)
+    L = _lib.load()
+    with _one_device(x, dy, lora_a, lora_b, lora_scales, adapter_idx, dx):
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        ws = _workspace(L.qw_lora_backward_workspace, x, rows, dy.shape[-1], x.shape[-1], lora_a.shape[1],
+                        lora_a.shape[0])
+        _lib.check(L.qw_lora_backward(_arr(x), _arr(dy), _arr(lora_a), _arr(lora_b), _arr(lora_scales),
+                                      _arr(adapter_idx), int(accumulate), _arr(dx), _arr(da), _arr(db),
+                                      ws.data_ptr(), ws.numel(), _stream(x)))
+    return dx, da, db
+
+
+def topk_distillation(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_values: torch.Tensor,
+                      temperature: Optional[torch.Tensor] = None, row_weights: Optional[torch.Tensor] = None,
+                      grad: bool = True, dlogits: Optional[torch.Tensor] = None):
+    """(loss fp32 [...], dlogits like logits or None): T^2 KL(teacher || student)
+    of each row, the teacher a softmax over its stored top logits (``topk``,
+    ``quantized_matmul_topk``), times ``row_weights``, with its gradient.
+    ``teacher_idx`` int32 or int64 (int64 costs a cast), -1 for no entry;
+    ``temperature`` an fp32 tensor of one element on the device (None: 1).
+    ``dlogits`` (optional) receives the gradient and may be ``logits``."""
+    if teacher_idx.dtype == torch.int64:
+        teacher_idx = teacher_idx.to(torch.int32)
+    if dlogits is None and grad:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    loss = torch.empty(logits.shape[:-1] or (1,), dtype=torch.float32, device=logits.device)
+    with _one_device(logits, teacher_idx, teacher_values, temperature, row_weights, dlogits):
+        _lib.check(_lib.load().qw_topk_distill(_arr(logits), _arr(teacher_idx), _arr(teacher_values),
+                                               _arr(temperature), _arr(row_weights), _arr(loss), _arr(dlogits),
+                                               _stream(logits)))
+    return loss, dlogits
+
+
 def dequantize(w, scales, biases, group_size: int = 64, bits: int = 4, mode: str = "affine",
                rounding: int = 0, out=None) -> torch.Tensor:
     """Full-precision weights from the quantized triple (lib.rs:1152-1159).
@@ -257,17 +338,38 @@ def device_status(device: int = 0, clear: bool = True) -> int:
     return int(v.value)
 
 
+class LoraAdapters:
+    """A stack of low-rank adapters of one projection: ``a`` fp16 [L, R, K],
+    ``b`` fp16 [L, N, R], ``scales`` fp32 [L] (None: 1).  Attached to a
+    QuantizedLinear (its ``lora``), whose forward then takes the adapter of each
+    row."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: Optional[torch.Tensor] = None):
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"adapters must be [L, R, K] and [L, N, R], got {list(a.shape)} and {list(b.shape)}")
+        self.a, self.b, self.scales = a, b, scales
+
+    def backward(self, x: torch.Tensor, dy: torch.Tensor, adapter_idx: Optional[torch.Tensor] = None, dx=None):
+        """(dx, da, db) of the adapters' term (lora_backward)."""
+        return lora_backward(x, dy, self.a, self.b, self.scales, adapter_idx, dx=dx)
+
+
 class QuantizedLinear:
     """A quantized weight triple and its forward, after mlxcel-core's
     ``QuantizedWeight`` (layers.rs:35-174) and the quantized arm of
-    ``UnifiedLinear::forward`` (layers.rs:2023-2093)."""
+    ``UnifiedLinear::forward`` (layers.rs:2023-2093).  With ``lora`` (adapters
+    of many requests, LoraAdapters) forward adds each row's adapter."""
 
     def __init__(self, w, scales, biases, group_size: int = 64, bits: int = 4, mode: str = "affine",
-                 bias: Optional[torch.Tensor] = None, global_scale: Optional[torch.Tensor] = None):
+                 bias: Optional[torch.Tensor] = None, global_scale: Optional[torch.Tensor] = None,
+                 lora: Optional[LoraAdapters] = None):
+        if lora is not None and global_scale is not None:
+            raise ValueError("a projection with a global scale takes no adapters")
         self.weight, self.scales, self.biases = w, scales, biases
         self.group_size, self.bits, self.mode = group_size, bits, mode
         self.bias = bias
         self.global_scale = global_scale
+        self.lora = lora
 
     @property
     def out_features(self) -> int:
@@ -277,7 +379,11 @@ class QuantizedLinear:
     def in_features(self) -> int:
         return self.weight.shape[1] * 32 // self.bits
 
-    def forward(self, x: torch.Tensor, out=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.lora is not None:
+            return quantized_linear_lora(x, self.weight, self.scales, self.biases, self.lora.a, self.lora.b,
+                                         self.lora.scales, adapter_idx, self.bias, self.group_size, self.bits,
+                                         self.mode, out=out)
         if self.global_scale is not None:
             return quantized_linear_forward_global_scale(x, self.weight, self.scales, self.biases,
                                                          self.global_scale, self.bias, self.group_size,
@@ -314,14 +420,16 @@ class QuantizedFusedLinear:
                 raise ValueError("fused planes must share input width and quantization")
             if l.bias is not None or l.global_scale is not None:
                 raise ValueError("fused planes take no linear bias or global scale")
+            if l.lora is not None:
+                raise ValueError("attach adapters to the fused projection, not to its planes")
         cat = lambda ts: torch.cat(ts, 0).contiguous()  # noqa: E731
         fused = QuantizedLinear(cat([l.weight for l in linears]), cat([l.scales for l in linears]),
                                 cat([l.biases for l in linears]) if first.biases is not None else None,
                                 first.group_size, first.bits, first.mode)
         return cls(fused, [l.out_features for l in linears])
 
-    def forward(self, x: torch.Tensor, out=None):
-        y = self.linear(x, out=out)
+    def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None):
+        y = self.linear(x, out=out, adapter_idx=adapter_idx)
         views, c = [], 0
         for n in self.sizes:
             views.append(y[..., c:c + n])
@@ -336,8 +444,8 @@ class QuantizedMlp:
     reference's ``Mlp`` (qwen3_next.rs:449-487).  The gate and up projections
     run as one fused kernel when ``fuse_mlp_input_projections``
     (qwen3_next.rs:406-447) would fuse them: same group size, bits and mode,
-    no linear biases and no global scales; otherwise as two matmuls followed
-    by the activation (the reference's Separate arm).  A checkpoint that
+    no linear biases, no global scales and no adapters; otherwise as two matmuls
+    followed by the activation (the reference's Separate arm).  A checkpoint that
     stores them concatenated is split into two row views by ``from_fused``."""
 
     def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear):
@@ -345,6 +453,7 @@ class QuantizedMlp:
         self.fused = (gate.group_size == up.group_size and gate.bits == up.bits and gate.mode == up.mode
                       and gate.bias is None and up.bias is None
                       and gate.global_scale is None and up.global_scale is None
+                      and gate.lora is None and up.lora is None
                       and gate.out_features == up.out_features)
 
     @classmethod
@@ -358,14 +467,14 @@ class QuantizedMlp:
                             gate_up.group_size, gate_up.bits, gate_up.mode)
         return cls(g, u, down)
 
-    def forward_hidden(self, x: torch.Tensor, out=None) -> torch.Tensor:
+    def forward_hidden(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
         g, u = self.gate, self.up
         if self.fused:
             return quantized_matmul_swiglu(x, g.weight, g.scales, g.biases, u.weight, u.scales, u.biases,
                                            g.group_size, g.bits, g.mode, out=out)
-        return compiled_swiglu_activation(g(x), u(x), out=out)
+        return compiled_swiglu_activation(g(x, adapter_idx=adapter_idx), u(x, adapter_idx=adapter_idx), out=out)
 
-    def forward(self, x: torch.Tensor, out=None) -> torch.Tensor:
-        return self.down(self.forward_hidden(x), out=out)
+    def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return self.down(self.forward_hidden(x, adapter_idx=adapter_idx), out=out, adapter_idx=adapter_idx)
 
     __call__ = forward
