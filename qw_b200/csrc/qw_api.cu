@@ -1411,7 +1411,11 @@ int qw_topk_distill(const qw_array* logits, const qw_array* teacher_idx, const q
   a.k = (int)k;
   a.dtype = logits->dtype;
   a.values_dtype = teacher_values->dtype;
-  const cudaError_t ce = launch_distill(a, as_stream(stream));
+  if (M == 0) return QW_OK;
+  int dev = 0;
+  cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  ce = launch_distill(a, device_info(dev).sm_count, as_stream(stream));
   return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "distillation launch");
 }
 

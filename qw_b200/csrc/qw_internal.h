@@ -213,7 +213,7 @@ struct DistillArgs {
   int values_dtype;          // qw_dtype of values
 };
 int distill_max_top();
-cudaError_t launch_distill(const DistillArgs& p, cudaStream_t stream);
+cudaError_t launch_distill(const DistillArgs& p, int sm_count, cudaStream_t stream);
 
 // Quantize / dequantize kernels (affine, 4-bit, group 64 for now).
 cudaError_t launch_dequantize(const uint32_t* w, const void* scales, const void* biases, void* out, int64_t N,
