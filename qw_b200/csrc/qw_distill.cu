@@ -6,18 +6,20 @@
 // HBM-bound: z has to be read once and dz written once.  q needs the whole
 // row's maximum and sum before the first dz can leave, so a row is held on chip
 // in between: a thread-block cluster of up to 8 CTAs per row, each CTA a
-// contiguous share of it in registers (kVec 16-byte vectors a thread, 64 KB a
-// CTA of 512 threads, two CTAs an SM, so that one row's loads run under
-// another's stores).  What a share has beyond that (rows of more than 512 KB)
-// is read a second time, from L2.
-//   1. every thread issues its loads of z; while they fly, the teacher's k
-//      entries are read, their softmax taken by each warp alone, and the z they
-//      point at gathered;
-//   2. maximum and sum of exponentials by thread, warp and CTA; each CTA then
-//      stores (maximum, sum, its part of sum_j p_j (t_j - z_j)) into every CTA
-//      of the cluster, and one cluster barrier later every thread has the row's;
-//   3. dz = w T q from the registers, then the columns the teacher names are
-//      written again by the CTA that owns them, behind a barrier.
+// contiguous share of it in shared memory (up to 72 KB, three CTAs of 256
+// threads an SM; longer rows up to 200 KB a CTA).  What a share has beyond that
+// (rows of more than 1.6 MB) is read a second time, from L2.  Clusters are
+// persistent: behind each vector of dz that a thread writes, it starts the
+// asynchronous copy of the next row's vector into the same place, which only
+// this thread reads, so loads run under the stores and the reductions and need
+// no barrier of their own.
+//   1. the teacher's k entries go to shared memory, every warp takes their
+//      softmax's normaliser alone, and the z they point at are fetched;
+//   2. maximum and sum of exponentials by thread and warp; each warp stores
+//      (maximum, sum, its part of sum_j p_j (t_j - z_j)) into every CTA of the
+//      cluster, and one cluster barrier later every warp joins them;
+//   3. dz = w T q, then the columns the teacher names are written again by the
+//      CTA that owns them, behind a barrier.
 // Sums and exponentials are fp32 (ex2.approx, relative error 2^-22); the loss,
 // a difference of two log-normalisers, is put together in fp64 from them.
 // Rows start at any element: up to 15 bytes before the first 16-byte boundary
@@ -25,6 +27,8 @@
 // threads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "../../include/qw_qmm.h"
 #include "qw_internal.h"
@@ -35,8 +39,8 @@ namespace qw {
 namespace {
 
 constexpr int kTopMax = 1024;    // teacher entries per row
-constexpr int kVec = 8;          // 16-byte vectors a thread holds
 constexpr int kClusterMax = 8;   // CTAs per row
+constexpr int kWarpsMax = 8;     // warps per CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -60,7 +64,41 @@ struct Vec {
   static constexpr int N = 16 / (int)sizeof(T);
   static __device__ __forceinline__ void load(const uint4& v, float (&f)[N]);
   static __device__ __forceinline__ uint4 pack(const float (&f)[N]);
+  static __device__ __forceinline__ uint4 max(const uint4& a, const uint4& b);  // elementwise, numbers over NaN
+  static __device__ __forceinline__ uint4 fill(float v) {
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = v;
+    return pack(f);
+  }
 };
+template <typename H2>
+__device__ __forceinline__ uint4 max_pairs(const uint4& a, const uint4& b) {
+  uint4 r;
+  const uint32_t *pa = &a.x, *pb = &b.x;
+  uint32_t* pr = &r.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const H2 h = __hmax2(*reinterpret_cast<const H2*>(pa + i), *reinterpret_cast<const H2*>(pb + i));
+    pr[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return r;
+}
+template <>
+__device__ __forceinline__ uint4 Vec<__half>::max(const uint4& a, const uint4& b) {
+  return max_pairs<__half2>(a, b);
+}
+template <>
+__device__ __forceinline__ uint4 Vec<__nv_bfloat16>::max(const uint4& a, const uint4& b) {
+  return max_pairs<__nv_bfloat162>(a, b);
+}
+template <>
+__device__ __forceinline__ uint4 Vec<float>::max(const uint4& a, const uint4& b) {
+  auto mx = [](uint32_t x, uint32_t y) {
+    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+  };
+  return make_uint4(mx(a.x, b.x), mx(a.y, b.y), mx(a.z, b.z), mx(a.w, b.w));
+}
 template <>
 __device__ __forceinline__ void Vec<__half>::load(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -126,211 +164,336 @@ __device__ __forceinline__ F warp_sum(F v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// A maximum to subtract: that of values which are all -inf counts as 0.
-__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+// Exponentials of a share are taken relative to a reference: the largest
+// exponent z c (c = log2(e) / T) rounded up to a whole number, so that one fused
+// multiply-add makes an argument, z c - ref, and every term is at most 1.  Where
+// the largest exponent is beyond +-kFar the product's own rounding (and that of
+// c) would show, so z - max is taken first, the reference being max c; that
+// costs an addition an element.  References follow from the maximum, and shares
+// are joined by 2^(their difference), taken in fp64.
+constexpr float kFar = 64.f;
+struct Ref {
+  float sub, off;  // argument of z: (z - sub) c - off
+  bool far;
+  double ref;
+};
+__device__ __forceinline__ Ref make_ref(float zmax, float c) {
+  Ref r{0.f, 0.f, false, -INFINITY};
+  if (zmax == -INFINITY) return r;  // nothing here: every exponential is 0
+  const float top = zmax * c;
+  r.far = !(fabsf(top) <= kFar);
+  if (r.far) {
+    r.sub = zmax;
+    r.ref = (double)zmax * (double)c;
+  } else {
+    r.off = ceilf(top);
+    r.ref = r.off;
+  }
+  return r;
+}
 
-// What a CTA tells its cluster of its share: largest logit, sum of
-// exponentials relative to it, and sum_j p_j (t_j - z_j) / T of its columns.
-struct Share {
+// What a warp tells its cluster: the largest of its logits, the sum of their
+// exponentials relative to that maximum's reference, and sum_j p_j (t_j - z_j)
+// over its teacher entries.
+struct __align__(16) Share {
   double gap;
   float max, sum;
 };
 
-template <typename T, int TH>
-__global__ void __launch_bounds__(TH, 1024 / TH) distill_rows_kernel(const DistillArgs p) {
+// One row's layout: `head` single elements up to the first 16-byte boundary,
+// then vectors, of which this thread has those at `first` + e TH N for e TH <
+// `count`, then `tail` single elements.
+struct RowLayout {
+  int first;   // element index of this thread's first vector
+  int count;   // vectors from it to the end of the CTA's share
+  int edge;    // the single element of this thread, -1: none
+  int lo, hi;  // the CTA's columns
+};
+template <typename T>
+__device__ __forceinline__ RowLayout row_layout(const T* z, int V, uint32_t rank, uint32_t C) {
+  constexpr int N = Vec<T>::N;
+  const int off = (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T);
+  const int head = off < V ? off : V;
+  const uint32_t nv = (uint32_t)(V - head) / N;
+  const int tail = V - head - (int)nv * N;
+  const int v0 = (int)(nv * rank / C), v1 = (int)(nv * (rank + 1) / C);
+  const int tid = threadIdx.x;
+  RowLayout r;
+  r.first = head + (v0 + tid) * N;
+  r.count = v1 - v0 - tid;
+  r.edge = -1;
+  if (rank == 0 && tid < head) r.edge = tid;
+  if (rank == C - 1 && tid >= 32 && tid < 32 + tail) r.edge = V - tail + (tid - 32);
+  r.lo = rank == 0 ? 0 : head + v0 * N;
+  r.hi = rank == C - 1 ? V : head + v1 * N;
+  return r;
+}
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Shared memory: `held` vectors per thread, then ids [2][k], tval [2][k], zval [k].
+template <typename T, int TH, int PER_SM>
+__global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillArgs p, const int held) {
   using VT = Vec<T>;
-  __shared__ uint32_t ids[kTopMax];
-  __shared__ float tval[kTopMax];
-  __shared__ float zval[kTopMax];  // the logit each entry of this CTA's columns points at
-  __shared__ Share warp_share[TH / 32];
-  __shared__ Share shares[kClusterMax];
+  constexpr int kWarps = TH / 32;
+  static_assert(kWarps <= kWarpsMax && kWarps * kClusterMax <= 64, "two shares a lane");
+  extern __shared__ uint4 smem[];
+  __shared__ Share shares_buf[2][kClusterMax * kWarps];
   uint32_t rank, C;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
-  const int tid = threadIdx.x, lane = tid % 32;
-  const int64_t m = blockIdx.x / C;
-  const int64_t V = p.V;
-  const T* z = reinterpret_cast<const T*>(p.logits) + m * V;
-  T* dz = p.dlogits ? reinterpret_cast<T*>(p.dlogits) + m * V : nullptr;
-  const int off = (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T);
-  const int head = off < V ? off : (int)V;
-  const int nv = (int)((V - head) / VT::N);
-  const int tail = (int)(V - head - (int64_t)nv * VT::N);
-  const int v0 = (int)((int64_t)nv * rank / C), v1 = (int)((int64_t)nv * (rank + 1) / C);
-  const uint32_t e0 = rank == 0 ? 0u : (uint32_t)(head + v0 * VT::N);
-  const uint32_t e1 = rank == C - 1 ? (uint32_t)V : (uint32_t)(head + v1 * VT::N);
-  const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-  // the single element of this thread, if it has one
-  int64_t edge = -1;
-  if (rank == 0 && tid < head) edge = tid;
-  if (rank == C - 1 && tid >= 32 && tid < 32 + tail) edge = V - tail + (tid - 32);
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int V = (int)p.V, M = (int)p.M;
+  const T* const z0 = reinterpret_cast<const T*>(p.logits);
+  uint32_t* const teacher = reinterpret_cast<uint32_t*>(smem + (size_t)held * TH);
+  float* const zval = reinterpret_cast<float*>(teacher) + 4 * p.k;
+  const uint32_t mine = smem_u32(smem + tid);  // this thread's vectors, TH apart
+  const int inside = held * TH;                // e below it is held
+  const int stride = (int)(gridDim.x / C);
+  int m = (int)(blockIdx.x / C);
 
-  uint4 d[kVec];
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    const int i = v0 + tid + e * TH;
-    if (i < v1) d[e] = __ldcg(zv + i);
+  // What of a row is loaded while the row before it is written: this thread's
+  // teacher entry, the weight, the vectors and the single element.
+  uint32_t id_next = 0xFFFFFFFFu;
+  float val_next = 0.f, w_next = 1.f, ze = -INFINITY;
+  auto fetch_teacher = [&](int row) {
+    if (tid < p.k) {
+      id_next = p.idx[(int64_t)row * p.k + tid];
+      val_next = load_value(p, (int64_t)row * p.k + tid);
+    }
+    if (p.weights) w_next = p.weights[row];
+  };
+  fetch_teacher(m);
+  {
+    const T* z = z0 + (int64_t)m * V;
+    const RowLayout lay = row_layout(z, V, rank, C);
+    const int n = lay.count < inside ? lay.count : inside;
+#pragma unroll 4
+    for (int e = 0; e < n; e += TH) copy_async16(mine + e * 16, z + lay.first + e * VT::N);
+    if (lay.edge >= 0) ze = to_f32(z[lay.edge]);
   }
-  const float ze = edge >= 0 ? to_f32(z[edge]) : -INFINITY;
-
-  const float w = p.weights ? p.weights[m] : 1.f;
   const float temp = p.temperature ? *p.temperature : 1.f;
   const float inv = 1.f / temp;
   const float c = inv * kLog2e;
-  for (int j = tid; j < p.k; j += TH) {
-    const uint32_t id = p.idx[m * p.k + j];
-    const bool ok = (int64_t)id < V;
-    ids[j] = ok ? id : 0xFFFFFFFFu;
-    tval[j] = ok ? load_value(p, m * p.k + j) : -INFINITY;
-  }
-  __syncthreads();
-  float tmax = -INFINITY, tsum = 0.f;
-  for (int j = lane; j < p.k; j += 32) tmax = fmaxf(tmax, tval[j]);
-  tmax = warp_max(tmax);
-  const bool svec = dz && (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0);
-  auto store = [&](int i, const float (&f)[VT::N]) {
-    if (svec) {
-      reinterpret_cast<uint4*>(dz + head)[i] = VT::pack(f);
-    } else {
-#pragma unroll
-      for (int q = 0; q < VT::N; ++q) dz[head + (int64_t)i * VT::N + q] = from_f32<T>(f[q]);
-    }
-  };
-  if (w == 0.f || tmax == -INFINITY) {  // no weight, or nothing to learn from (the whole cluster takes this branch)
-    if (rank == 0 && tid == 0) p.loss[m] = 0.f;
-    if (dz) {
-      const float zero[VT::N] = {};
-      for (int i = v0 + tid; i < v1; i += TH) store(i, zero);
-      if (edge >= 0) dz[edge] = from_f32<T>(0.f);
-    }
-    return;
-  }
-  for (int j = lane; j < p.k; j += 32) tsum += ex2((tval[j] - tmax) * c);
-  tsum = warp_sum(tsum);
-  double gap = 0.0;
-  for (int j = tid; j < p.k; j += TH) {
-    if (ids[j] >= e0 && ids[j] < e1) {
-      const float zj = to_f32(z[ids[j]]);
-      const float pj = ex2((tval[j] - tmax) * c) / tsum;
-      zval[j] = zj;
-      if (pj > 0.f) gap += zj == -INFINITY ? (double)INFINITY : (double)pj * ((double)tval[j] - (double)zj);
-    }
-  }
 
-  // maximum and sum of this thread's, warp's, CTA's and cluster's logits
-  float mx = ze;
+  // Buffers alternate so that a barrier of their own guards none of them: the
+  // teacher's by row, the shares by row that reached the cluster barrier (a CTA
+  // may be ahead of its cluster by rows that skip it, but by one barrier only).
+  int met = 0;
+  for (int parity = 0; m < M; parity ^= 1) {
+    uint32_t* const ids = teacher + parity * p.k;
+    float* const tval = reinterpret_cast<float*>(teacher) + (2 + parity) * p.k;
+    Share* const shares = shares_buf[met];
+    const T* const z = z0 + (int64_t)m * V;
+    T* const dz = p.dlogits ? reinterpret_cast<T*>(p.dlogits) + (int64_t)m * V : nullptr;
+    const float w = w_next;
+    const RowLayout cur = row_layout(z, V, rank, C);
+    const int n = cur.count < inside ? cur.count : inside;
+    const int next = m + stride;
+
+    // the teacher's entries of the row
+    const uint32_t my_id = id_next < (uint32_t)V && tid < p.k ? id_next : 0xFFFFFFFFu;
+    const float my_val = my_id != 0xFFFFFFFFu ? val_next : -INFINITY;
+    if (tid < p.k) {
+      ids[tid] = my_id;
+      tval[tid] = my_val;
+    }
+    for (int j = tid + TH; j < p.k; j += TH) {
+      const uint32_t id = p.idx[(int64_t)m * p.k + j];
+      const float v = load_value(p, (int64_t)m * p.k + j);
+      ids[j] = id < (uint32_t)V ? id : 0xFFFFFFFFu;
+      tval[j] = id < (uint32_t)V ? v : -INFINITY;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float tmax = -INFINITY, tsum = 0.f;
+    for (int j = lane; j < p.k; j += 32) tmax = fmaxf(tmax, tval[j]);
+    tmax = warp_max(tmax);
+    // Writes the row from `value` of each element and, behind each vector's
+    // store, starts the next row's copy into its place.
+    auto write_row = [&](auto&& value) {
+      const bool aligned = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
+      auto store = [&](int at, const uint4& v) {
+        float f[VT::N];
+        VT::load(v, f);
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    if (v0 + tid + e * TH < v1) {
+        for (int q = 0; q < VT::N; ++q) f[q] = value(f[q]);
+        if (aligned) {
+          *reinterpret_cast<uint4*>(dz + at) = VT::pack(f);
+        } else {  // dlogits start at another offset from a 16-byte boundary than logits
+#pragma unroll
+          for (int q = 0; q < VT::N; ++q) dz[at + q] = from_f32<T>(f[q]);
+        }
+      };
+      RowLayout lay{};
+      int nn = 0;
+      const T* const zn = z0 + (int64_t)next * V;
+      if (next < M) {
+        fetch_teacher(next);
+        lay = row_layout(zn, V, rank, C);
+        nn = lay.count < inside ? lay.count : inside;
+      }
+      if (dz) {
+#pragma unroll 2
+        for (int e = 0; e < n; e += TH) {
+          store(cur.first + e * VT::N, lds16(mine + e * 16));
+          if (e < nn) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+        }
+        for (int e = inside; e < cur.count; e += TH) {
+          const int at = cur.first + e * VT::N;
+          store(at, __ldcg(reinterpret_cast<const uint4*>(z + at)));
+        }
+        if (cur.edge >= 0) dz[cur.edge] = from_f32<T>(value(ze));
+        // a row of another alignment may have one vector more
+        for (int e = (n + TH - 1) / TH * TH; e < nn; e += TH)
+          if (e >= 0) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+      } else {
+        for (int e = 0; e < nn; e += TH) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+      }
+      ze = next < M && lay.edge >= 0 ? to_f32(zn[lay.edge]) : -INFINITY;
+    };
+    if (w == 0.f || tmax == -INFINITY) {  // no weight, or nothing to learn from: the whole cluster takes this branch
+      if (rank == 0 && tid == 0) p.loss[m] = 0.f;
+      write_row([](float) { return 0.f; });
+      m = next;
+      continue;
+    }
+    const bool mine_in = my_id >= (uint32_t)cur.lo && my_id < (uint32_t)cur.hi;
+    float my_z = 0.f;
+    if (mine_in) my_z = to_f32(z[my_id]);
+    for (int j = lane; j < p.k; j += 32) tsum += ex2((tval[j] - tmax) * c);
+    tsum = warp_sum(tsum);
+
+    // maximum and sum of this thread's, warp's and cluster's logits
+    uint4 mv = VT::fill(-INFINITY);
+    auto over_rest = [&](auto&& f) {  // what is not held
+      for (int e = inside; e < cur.count; e += TH)
+        f(__ldcg(reinterpret_cast<const uint4*>(z + cur.first + e * VT::N)));
+    };
+#pragma unroll 4
+    for (int e = 0; e < n; e += TH) mv = VT::max(mv, lds16(mine + e * 16));
+    over_rest([&](const uint4& v) { mv = VT::max(mv, v); });
+    float mx = ze;
+    {
       float f[VT::N];
-      VT::load(d[e], f);
+      VT::load(mv, f);
 #pragma unroll
       for (int q = 0; q < VT::N; ++q) mx = fmaxf(mx, f[q]);
     }
-  }
-  for (int i = v0 + tid + kVec * TH; i < v1; i += TH) {
-    float f[VT::N];
-    VT::load(__ldcg(zv + i), f);
+    mx = warp_max(mx);
+    const Ref wr = make_ref(mx, c);
+    float sum = cur.edge >= 0 ? ex2((ze - wr.sub) * c - wr.off) : 0.f;
+    auto add_all = [&](auto far) {
+      auto add = [&](const uint4& v) {
+        float f[VT::N];
+        VT::load(v, f);
+        float part[2] = {0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < VT::N; ++q) mx = fmaxf(mx, f[q]);
-  }
-  mx = warp_max(mx);
-  float sub = finite_max(mx);
-  float sum = edge >= 0 ? ex2((ze - sub) * c) : 0.f;
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    if (v0 + tid + e * TH < v1) {
-      float f[VT::N];
-      VT::load(d[e], f);
-      float part = 0.f;
-#pragma unroll
-      for (int q = 0; q < VT::N; ++q) part += ex2((f[q] - sub) * c);
-      sum += part;
-    }
-  }
-  for (int i = v0 + tid + kVec * TH; i < v1; i += TH) {
-    float f[VT::N];
-    VT::load(__ldcg(zv + i), f);
-    float part = 0.f;
-#pragma unroll
-    for (int q = 0; q < VT::N; ++q) part += ex2((f[q] - sub) * c);
-    sum += part;
-  }
-  sum = warp_sum(sum);
-  gap = warp_sum(gap);
-  if (lane == 0) warp_share[tid / 32] = Share{gap, mx, sum};
-  __syncthreads();
-  if (tid < 32) {
-    const Share s = lane < TH / 32 ? warp_share[lane] : Share{0.0, -INFINITY, 0.f};
-    const float cm = warp_max(s.max);
-    const float cs = warp_sum(s.sum * ex2((finite_max(s.max) - finite_max(cm)) * c));
-    const double cg = warp_sum(s.gap);
-    if (lane < C) {  // into CTA `lane` of the cluster
+        for (int q = 0; q < VT::N; ++q)
+          part[q & 1] += ex2(decltype(far)::value ? (f[q] - wr.sub) * c : fmaf(f[q], c, -wr.off));
+        sum += part[0] + part[1];
+      };
+#pragma unroll 4
+      for (int e = 0; e < n; e += TH) add(lds16(mine + e * 16));
+      over_rest(add);
+    };
+    if (wr.far) add_all(std::true_type{});
+    else add_all(std::false_type{});
+    sum = warp_sum(sum);
+    double gap = 0.0;
+    auto entry = [&](int j, float t, float zj) {
+      zval[j] = zj;
+      const float pj = ex2((t - tmax) * c) / tsum;
+      if (pj > 0.f) gap += zj == -INFINITY ? (double)INFINITY : (double)pj * ((double)t - (double)zj);
+    };
+    if (mine_in) entry(tid, my_val, my_z);
+    for (int j = tid + TH; j < p.k; j += TH)
+      if (ids[j] >= (uint32_t)cur.lo && ids[j] < (uint32_t)cur.hi) entry(j, tval[j], to_f32(z[ids[j]]));
+    if (__any_sync(0xffffffffu, gap != 0.0)) gap = warp_sum(gap);
+    if (lane < C) {  // this warp's share into CTA `lane` of the cluster
       uint32_t to;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&shares[rank])), "r"((uint32_t)lane));
-      asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to + (uint32_t)offsetof(Share, max)), "f"(cm),
-                   "f"(cs)
+      asm("mapa.shared::cluster.u32 %0, %1, %2;"
+          : "=r"(to)
+          : "r"(smem_u32(&shares[rank * kWarps + warp])), "r"((uint32_t)lane));
+      asm volatile("st.shared::cluster.f64 [%0], %1;\nst.shared::cluster.v2.f32 [%0+8], {%2, %3};" ::"r"(to), "d"(gap),
+                   "f"(mx), "f"(sum)
                    : "memory");
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(cg) : "memory");
     }
-  }
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  float zmax = -INFINITY, zsum = 0.f;
-  for (uint32_t r = 0; r < C; ++r) zmax = fmaxf(zmax, shares[r].max);
-  sub = finite_max(zmax);
-  for (uint32_t r = 0; r < C; ++r) zsum += shares[r].sum * ex2((finite_max(shares[r].max) - sub) * c);
-  if (rank == 0 && tid == 0) {
-    double g = 0.0;
-    for (uint32_t r = 0; r < C; ++r) g += shares[r].gap;
-    // log of p's normaliser over q's; an empty student row (zsum 0) makes it -inf and the loss +inf
-    const double norm = ((double)tmax - (double)sub) * inv + log((double)tsum) - log((double)zsum);
-    const double kl = isinf(g) ? g : g * inv - norm;
-    p.loss[m] = (float)((double)w * temp * temp * kl);
-  }
-  if (!dz) return;
-
-  const float scale = zsum > 0.f ? w * temp / zsum : (zsum == 0.f ? 0.f : zsum);
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    const int i = v0 + tid + e * TH;
-    if (i < v1) {
-      float f[VT::N];
-      VT::load(d[e], f);
-#pragma unroll
-      for (int q = 0; q < VT::N; ++q) f[q] = ex2((f[q] - sub) * c) * scale;
-      store(i, f);
-    }
-  }
-  for (int i = v0 + tid + kVec * TH; i < v1; i += TH) {
-    float f[VT::N];
-    VT::load(__ldcg(zv + i), f);
-#pragma unroll
-    for (int q = 0; q < VT::N; ++q) f[q] = ex2((f[q] - sub) * c) * scale;
-    store(i, f);
-  }
-  if (edge >= 0) dz[edge] = from_f32<T>(ex2((ze - sub) * c) * scale);
-  __syncthreads();
-  // the teacher's columns of this CTA: the first entry of an id writes it, with the mass of all its entries
-  for (int j = tid; j < p.k; j += TH) {
-    const uint32_t id = ids[j];
-    if (id < e0 || id >= e1) continue;
-    float mass = 0.f;
-    bool first = true;
-    for (int i = 0; i < p.k; ++i) {
-      if (ids[i] == id) {
-        first = first && i >= j;
-        mass += ex2((tval[i] - tmax) * c);
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    met ^= 1;
+    // two shares a lane, joined by every warp
+    const int n_shares = (int)C * kWarps;
+    Share sa{0.0, -INFINITY, 0.f}, sb = sa;
+    if (lane < n_shares) sa = shares[lane];
+    if (lane + 32 < n_shares) sb = shares[lane + 32];
+    const float zmax = warp_max(fmaxf(sa.max, sb.max));
+    const Ref row = make_ref(zmax, c);
+    auto joined = [&](const Share& s) {
+      return s.max == -INFINITY ? s.sum : s.sum * ex2((float)(make_ref(s.max, c).ref - row.ref));
+    };
+    const float zsum = warp_sum(joined(sa) + joined(sb));
+    const float scale = zsum == 0.f ? 0.f : w * temp / zsum;
+    if (row.far) write_row([&](float x) { return ex2((x - row.sub) * c) * scale; });
+    else write_row([&](float x) { return ex2(fmaf(x, c, -row.off)) * scale; });
+    if (rank == 0 && warp == kWarps - 1) {
+      const double g = warp_sum(sa.gap + sb.gap);
+      if (lane == 0) {
+        // log of p's normaliser over q's; a student row of -inf alone has an infinite gap
+        const double norm = (double)tmax * inv + log((double)tsum) -
+                            (row.ref * 0.69314718055994531 + log((double)zsum));
+        p.loss[m] = (float)((double)w * temp * temp * (isinf(g) ? g : g * inv - norm));
       }
     }
-    if (first) dz[id] = from_f32<T>(ex2((zval[j] - sub) * c) * scale - w * temp * (mass / tsum));
+    if (dz) {
+      __syncthreads();
+      // the teacher's columns of this CTA, a warp an entry: the first entry of
+      // an id writes it, with the mass of all its entries
+      for (int j = warp; j < p.k; j += kWarps) {
+        const uint32_t id = ids[j];
+        if (id < (uint32_t)cur.lo || id >= (uint32_t)cur.hi) continue;
+        float mass = 0.f;
+        bool first = true;
+        for (int i = lane; i < p.k; i += 32) {
+          if (ids[i] == id) {
+            first = first && i >= j;
+            mass += ex2((tval[i] - tmax) * c);
+          }
+        }
+        first = __all_sync(0xffffffffu, first);
+        mass = warp_sum(mass);
+        if (first && lane == 0)
+          dz[id] = from_f32<T>(ex2((zval[j] - row.sub) * c - row.off) * scale - w * temp * (mass / tsum));
+      }
+    }
+    m = next;
   }
 }
 
-template <typename T, int TH>
+constexpr int64_t kMaxSmem = 227 * 1024 - 2048;  // dynamic shared memory a CTA may take
+
+template <typename T, int TH, int PER_SM>
 cudaError_t launch_rows(const DistillArgs& p, int cluster, cudaStream_t stream) {
+  auto* kernel = distill_rows_kernel<T, TH, PER_SM>;
+  // vectors per thread that cover a CTA's share of any row, as far as shared memory goes
+  const int64_t nv = (p.V * (int64_t)sizeof(T) / 16 + cluster - 1) / cluster + 1;
+  int64_t held = (nv + TH - 1) / TH;
+  const int64_t top_bytes = (int64_t)p.k * 20;
+  if (held * TH * 16 + top_bytes > kMaxSmem) held = (kMaxSmem - top_bytes) / (TH * 16);
+  const size_t smem = (size_t)(held * TH * 16 + top_bytes);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.M * cluster));
+  cfg.gridDim = dim3((unsigned)cluster);
   cfg.blockDim = dim3(TH);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -339,18 +502,43 @@ cudaError_t launch_rows(const DistillArgs& p, int cluster, cudaStream_t stream) 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, distill_rows_kernel<T, TH>, p);
+  // as many clusters as the GPU holds at once (asked once per size), each walking rows a grid apart
+  static thread_local int configured_dev = -1, asked_cluster = 0, resident = 0;
+  static thread_local size_t asked_smem = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e;
+  if (configured_dev != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+    if (e != cudaSuccess) return e;
+    configured_dev = dev;
+    asked_cluster = 0;
+  }
+  if (asked_cluster != cluster || asked_smem != smem) {
+    if ((e = cudaOccupancyMaxActiveClusters(&resident, kernel, &cfg)) != cudaSuccess) return e;
+    if (resident < 1) return cudaErrorInvalidConfiguration;
+    asked_cluster = cluster;
+    asked_smem = smem;
+  }
+  const int64_t clusters = p.M < resident ? p.M : resident;
+  cfg.gridDim = dim3((unsigned)(clusters * cluster));
+  return cudaLaunchKernelEx(&cfg, kernel, p, (int)held);
 }
 
 template <typename T>
 cudaError_t launch_type(const DistillArgs& p, int sm_count, cudaStream_t stream) {
   const int64_t bytes = p.V * (int64_t)sizeof(T);
-  if (bytes <= 128 * kVec * 16) return launch_rows<T, 128>(p, 1, stream);
-  // as many CTAs as hold the row in registers; with few rows, more, down to 8 KB a CTA, while they fit the SMs
-  int64_t cluster = (bytes + 512 * kVec * 16 - 1) / (512 * kVec * 16);
+  if (bytes <= 16384) return launch_rows<T, 128, 8>(p, 1, stream);
+#ifndef DS
+#define DS 72
+#define DP 3
+#define DT 256
+#endif
+  // shares of at most 72 KB; with few rows more CTAs, down to 8 KB a CTA, while they fit the SMs
+  int64_t cluster = (bytes + DS * 1024 - 1) / (DS * 1024);
   while (cluster < kClusterMax && p.M * (cluster + 1) <= sm_count && bytes / (cluster + 1) >= 8192) ++cluster;
   if (cluster > kClusterMax) cluster = kClusterMax;
-  return launch_rows<T, 512>(p, (int)cluster, stream);
+  return launch_rows<T, DT, DP>(p, (int)cluster, stream);
 }
 
 }  // namespace
