@@ -241,8 +241,10 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
+// EVEN: every row of logits and of dlogits starts on a 16-byte boundary and has
+// whole vectors, so that one layout serves all.
 // Shared memory: `held` vectors per thread, then ids [2][k], tval [2][k], zval [k].
-template <typename T, int TH, int PER_SM>
+template <typename T, int TH, int PER_SM, bool EVEN>
 __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillArgs p, const int held) {
   using VT = Vec<T>;
   constexpr int kWarps = TH / 32;
@@ -274,9 +276,9 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     if (p.weights) w_next = p.weights[row];
   };
   fetch_teacher(m);
+  RowLayout lay = row_layout(z0 + (int64_t)m * V, V, rank, C);
   {
     const T* z = z0 + (int64_t)m * V;
-    const RowLayout lay = row_layout(z, V, rank, C);
     const int n = lay.count < inside ? lay.count : inside;
 #pragma unroll 4
     for (int e = 0; e < n; e += TH) copy_async16(mine + e * 16, z + lay.first + e * VT::N);
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     const T* const z = z0 + (int64_t)m * V;
     T* const dz = p.dlogits ? reinterpret_cast<T*>(p.dlogits) + (int64_t)m * V : nullptr;
     const float w = w_next;
-    const RowLayout cur = row_layout(z, V, rank, C);
+    const RowLayout cur = lay;
     const int n = cur.count < inside ? cur.count : inside;
     const int next = m + stride;
 
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     // Writes the row from `value` of each element and, behind each vector's
     // store, starts the next row's copy into its place.
     auto write_row = [&](auto&& value) {
-      const bool aligned = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
+      const bool aligned = EVEN || ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
       auto store = [&](int at, const uint4& v) {
         float f[VT::N];
         VT::load(v, f);
@@ -335,32 +337,38 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
           for (int q = 0; q < VT::N; ++q) dz[at + q] = from_f32<T>(f[q]);
         }
       };
-      RowLayout lay{};
-      int nn = 0;
       const T* const zn = z0 + (int64_t)next * V;
+      int nn = -1;
       if (next < M) {
         fetch_teacher(next);
-        lay = row_layout(zn, V, rank, C);
+        if (!EVEN) lay = row_layout(zn, V, rank, C);
         nn = lay.count < inside ? lay.count : inside;
       }
       if (dz) {
+        if (EVEN && next < M) {
 #pragma unroll 2
-        for (int e = 0; e < n; e += TH) {
-          store(cur.first + e * VT::N, lds16(mine + e * 16));
-          if (e < nn) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+          for (int e = 0; e < n; e += TH) {
+            store(cur.first + e * VT::N, lds16(mine + e * 16));
+            copy_async16(mine + e * 16, zn + cur.first + e * VT::N);
+          }
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < n || e < nn; e += TH) {
+            if (e < n) store(cur.first + e * VT::N, lds16(mine + e * 16));
+            if (e < nn) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+          }
         }
+#pragma unroll 1
         for (int e = inside; e < cur.count; e += TH) {
           const int at = cur.first + e * VT::N;
           store(at, __ldcg(reinterpret_cast<const uint4*>(z + at)));
         }
-        if (cur.edge >= 0) dz[cur.edge] = from_f32<T>(value(ze));
-        // a row of another alignment may have one vector more
-        for (int e = (n + TH - 1) / TH * TH; e < nn; e += TH)
-          if (e >= 0) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
+        if (!EVEN && cur.edge >= 0) dz[cur.edge] = from_f32<T>(value(ze));
       } else {
+#pragma unroll 1
         for (int e = 0; e < nn; e += TH) copy_async16(mine + e * 16, zn + lay.first + e * VT::N);
       }
-      ze = next < M && lay.edge >= 0 ? to_f32(zn[lay.edge]) : -INFINITY;
+      if (!EVEN) ze = next < M && lay.edge >= 0 ? to_f32(zn[lay.edge]) : -INFINITY;
     };
     if (w == 0.f || tmax == -INFINITY) {  // no weight, or nothing to learn from: the whole cluster takes this branch
       if (rank == 0 && tid == 0) p.loss[m] = 0.f;
@@ -377,6 +385,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     // maximum and sum of this thread's, warp's and cluster's logits
     uint4 mv = VT::fill(-INFINITY);
     auto over_rest = [&](auto&& f) {  // what is not held
+#pragma unroll 1
       for (int e = inside; e < cur.count; e += TH)
         f(__ldcg(reinterpret_cast<const uint4*>(z + cur.first + e * VT::N)));
     };
@@ -458,21 +467,26 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
       __syncthreads();
       // the teacher's columns of this CTA, a warp an entry: the first entry of
       // an id writes it, with the mass of all its entries
-      for (int j = warp; j < p.k; j += kWarps) {
-        const uint32_t id = ids[j];
-        if (id < (uint32_t)cur.lo || id >= (uint32_t)cur.hi) continue;
-        float mass = 0.f;
-        bool first = true;
-        for (int i = lane; i < p.k; i += 32) {
-          if (ids[i] == id) {
-            first = first && i >= j;
-            mass += ex2((tval[i] - tmax) * c);
+      for (int j0 = warp; j0 < p.k; j0 += 32 * kWarps) {
+        const int jl = j0 + lane * kWarps;
+        const uint32_t idl = jl < p.k ? ids[jl] : 0xFFFFFFFFu;
+        for (uint32_t in = __ballot_sync(0xffffffffu, idl >= (uint32_t)cur.lo && idl < (uint32_t)cur.hi); in;
+             in &= in - 1) {
+          const int j = j0 + (__ffs(in) - 1) * kWarps;
+          const uint32_t id = __shfl_sync(0xffffffffu, idl, __ffs(in) - 1);
+          float mass = 0.f;
+          bool first = true;
+          for (int i = lane; i < p.k; i += 32) {
+            if (ids[i] == id) {
+              first = first && i >= j;
+              mass += ex2((tval[i] - tmax) * c);
+            }
           }
+          if (!__all_sync(0xffffffffu, first)) continue;
+          mass = warp_sum(mass);
+          if (lane == 0)
+            dz[id] = from_f32<T>(ex2((zval[j] - row.sub) * c - row.off) * scale - w * temp * (mass / tsum));
         }
-        first = __all_sync(0xffffffffu, first);
-        mass = warp_sum(mass);
-        if (first && lane == 0)
-          dz[id] = from_f32<T>(ex2((zval[j] - row.sub) * c - row.off) * scale - w * temp * (mass / tsum));
       }
     }
     m = next;
@@ -480,10 +494,11 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
 }
 
 constexpr int64_t kMaxSmem = 227 * 1024 - 2048;  // dynamic shared memory a CTA may take
+constexpr int64_t kShareBytes = 72 * 1024;       // share of a row that lets three CTAs sit on an SM
 
-template <typename T, int TH, int PER_SM>
-cudaError_t launch_rows(const DistillArgs& p, int cluster, cudaStream_t stream) {
-  auto* kernel = distill_rows_kernel<T, TH, PER_SM>;
+template <typename T, int TH, int PER_SM, bool EVEN>
+cudaError_t launch_even(const DistillArgs& p, int cluster, cudaStream_t stream) {
+  auto* kernel = distill_rows_kernel<T, TH, PER_SM, EVEN>;
   // vectors per thread that cover a CTA's share of any row, as far as shared memory goes
   const int64_t nv = (p.V * (int64_t)sizeof(T) / 16 + cluster - 1) / cluster + 1;
   int64_t held = (nv + TH - 1) / TH;
@@ -525,20 +540,23 @@ cudaError_t launch_rows(const DistillArgs& p, int cluster, cudaStream_t stream) 
   return cudaLaunchKernelEx(&cfg, kernel, p, (int)held);
 }
 
+template <typename T, int TH, int PER_SM>
+cudaError_t launch_rows(const DistillArgs& p, int cluster, cudaStream_t stream) {
+  const bool even = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.dlogits) |
+                      (uintptr_t)(p.V * (int64_t)sizeof(T))) & 15) == 0;
+  return even ? launch_even<T, TH, PER_SM, true>(p, cluster, stream)
+              : launch_even<T, TH, PER_SM, false>(p, cluster, stream);
+}
+
 template <typename T>
 cudaError_t launch_type(const DistillArgs& p, int sm_count, cudaStream_t stream) {
   const int64_t bytes = p.V * (int64_t)sizeof(T);
   if (bytes <= 16384) return launch_rows<T, 128, 8>(p, 1, stream);
-#ifndef DS
-#define DS 72
-#define DP 3
-#define DT 256
-#endif
   // shares of at most 72 KB; with few rows more CTAs, down to 8 KB a CTA, while they fit the SMs
-  int64_t cluster = (bytes + DS * 1024 - 1) / (DS * 1024);
+  int64_t cluster = (bytes + kShareBytes - 1) / kShareBytes;
   while (cluster < kClusterMax && p.M * (cluster + 1) <= sm_count && bytes / (cluster + 1) >= 8192) ++cluster;
   if (cluster > kClusterMax) cluster = kClusterMax;
-  return launch_rows<T, DT, DP>(p, (int)cluster, stream);
+  return launch_rows<T, 256, 3>(p, (int)cluster, stream);
 }
 
 }  // namespace
