@@ -1223,7 +1223,8 @@ int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64
   int dev = 0;
   const cudaError_t ce = cudaGetDevice(&dev);
   if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
-  *bytes = (int64_t)(lora_skinny_bytes(m, n, 0, dev) + lora_forward_bytes(m, n, rank));
+  *bytes = (int64_t)(lora_skinny_bytes(m, n, 0, dev) +
+                     lora_forward_bytes(m, n, (int)rank, m > 16 ? prefill_token_tile(m) : 0));
   return QW_OK;
 }
 
@@ -1252,35 +1253,39 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
   cudaError_t ce = cudaGetDevice(&dev);
   if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
   const size_t skinny = lora_skinny_bytes(sa.M, sa.N, sa.K, dev);
-  if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, sa.N, la.R)))) return rc;
+  const int token_tile = sa.M > 16 ? prefill_token_tile(sa.M) : 0;
+  if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, sa.N, la.R, token_tile))))
+    return rc;
   DeviceRes* res = nullptr;
   std::string err;
   if (!device_res(dev, &res, &err)) return fail(QW_ENOMEM, err);
   cudaStream_t stream = as_stream(stream_v);
   void* lws = static_cast<uint8_t*>(workspace) + skinny;
-  if (skinny) {
-    ce = cudaMemsetAsync(workspace, 0, skinny_zeroed_bytes(sa), stream);
-    if (ce != cudaSuccess) return cuda_fail(ce, "cudaMemsetAsync");
-  }
-  if ((ce = launch_lora_shrink(la, lws, stream)) != cudaSuccess) return cuda_fail(ce, "adapter launch");
+  const void* bias = linear_bias ? linear_bias->data : nullptr;
+  const bool pdl = pdl_enabled();
+  sa.status = res->status;
+  // The decode kernel's counters are cleared by the first launch.
+  ce = launch_lora_rank(la, token_tile, lws, workspace, skinny ? skinny_zeroed_bytes(sa) : 0,
+                        device_info(dev).sm_count, pdl, stream);
+  if (ce != cudaSuccess) return cuda_fail(ce, "adapter launch");
   if (sa.M <= 16) {
     sa.y = lora_forward_product(la, lws);
     sa.y_f32 = true;
-    sa.status = res->status;
     Scratch sc{workspace, skinny};
-    ce = launch_skinny(sa, sc, stream, pdl_enabled(), &err);
+    ce = launch_skinny(sa, sc, stream, pdl, &err);
     if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "skinny launch") : fail(QW_ECUDA, err);
-  } else {
-    PrefillArgs pa{sa.x, sa.w, sa.scales, sa.biases, lora_forward_product(la, lws), true, sa.M, sa.N, sa.K,
-                   res->status};
-    pa.x_ld = sa.x_ld;
-    pa.bits = bits;
-    pa.group_size = group_size;
-    ce = launch_prefill(pa, stream, pdl_enabled(), &err);
-    if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "prefill launch") : fail(QW_ECUDA, err);
+    ce = launch_lora_expand(la, lws, bias, y->data, pdl, stream);
+    return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter launch");
   }
-  ce = launch_lora_expand(la, lws, linear_bias ? linear_bias->data : nullptr, y->data, stream);
-  return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter launch");
+  const PrefillLora lora = lora_prefill_operands(la, token_tile, lws, bias);
+  PrefillArgs pa{sa.x, sa.w, sa.scales, sa.biases, y->data, false, sa.M, sa.N, sa.K, res->status};
+  pa.x_ld = sa.x_ld;
+  pa.bits = bits;
+  pa.group_size = group_size;
+  pa.lora = &lora;
+  ce = launch_prefill(pa, stream, pdl, &err);
+  if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "prefill launch") : fail(QW_ECUDA, err);
+  return QW_OK;
 }
 
 int qw_lora_backward_workspace(int64_t m, int64_t n, int64_t k, int64_t rank, int64_t adapters, int64_t* bytes) {

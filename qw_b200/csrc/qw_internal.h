@@ -104,6 +104,18 @@ size_t skinny_zeroed_bytes(const SkinnyArgs& a);
 int check_qmm_call(const qw_array* x, const qw_array* w, const qw_array* scales, const qw_array* biases,
                    int transpose, int group_size, int bits, const char* mode, qw_array* y, SkinnyArgs* sa);
 
+// Adapters of a prefill call, as further columns of its reduction: for every
+// token tile, the adapters its tokens name.
+struct PrefillLora {
+  const void* h;             // fp16 [M][R8], R8 the rank rounded up to 8, zero-padded
+  const void* b;             // fp16 [L][N][R]
+  const uint32_t* idx;       // [M] or null (adapter 0)
+  const uint32_t* tile_n;    // [token tiles]
+  const uint32_t* tile_ids;  // [token tiles][tokens per tile]
+  const void* bias;          // fp16 [N] or null
+  int R, L;
+};
+
 // Prefill path (tcgen05, M >= 17).
 struct PrefillArgs {
   const void* x;
@@ -122,7 +134,10 @@ struct PrefillArgs {
   const uint32_t* w2 = nullptr;
   const void* scales2 = nullptr;
   const void* biases2 = nullptr;
+  const PrefillLora* lora = nullptr;  // adapters and bias added to the products (not SwiGLU; y fp16)
 };
+// Tokens per tile of a prefill call over M rows.
+int prefill_token_tile(int64_t M);
 cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream, bool pdl, std::string* err);
 bool prefill_available();
 
@@ -189,12 +204,18 @@ struct LoraGrads {
 };
 constexpr int kLoraMaxRank = 128;
 constexpr int64_t kLoraMaxAdapters = 4096;
-// Forward workspace after the decode kernel's scratch.
-size_t lora_forward_bytes(int64_t M, int64_t N, int64_t R);
-cudaError_t launch_lora_shrink(const LoraArgs& p, void* ws, cudaStream_t stream);
-// fp32 [M][N] within the workspace: where the projection's product goes.
+// Forward workspace (after the decode kernel's scratch): token_tile 0 for at
+// most 16 rows, else prefill_token_tile(M).
+size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile);
+// h = s x A^T into the workspace, with the token tiles' adapter lists where
+// token_tile != 0, and `zero_bytes` (rounded up to 16) at `zero` cleared.
+cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes, int sm_count,
+                             bool pdl, cudaStream_t stream);
+// fp32 [M][N] within the workspace of at most 16 rows: the projection's product.
 float* lora_forward_product(const LoraArgs& p, void* ws);
-cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, cudaStream_t stream);
+cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, bool pdl, cudaStream_t stream);
+// What the tcgen05 kernel adds to its products, from the workspace.
+PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias);
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);
 cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, cudaStream_t stream);
 

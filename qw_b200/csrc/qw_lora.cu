@@ -4,6 +4,13 @@
 // and the gradient of that term:
 //   h = s x A^T, g = s dy B, dA = g^T x, dB = dy^T h, dx = g A
 // with the sums over the rows of each adapter.
+//
+// Forward, three launches chained by programmatic dependent launch:
+//   rank_rows     h = s x A^T (below);
+//   the projection's own kernel: the decode kernel (at most 16 rows) into an
+//                 fp32 product, or the tcgen05 kernel, which takes h and B as
+//                 further columns of its reduction and writes y itself;
+//   expand_rows   (at most 16 rows) y = fp16(product + h B^T + bias).
 #include <cuda_fp16.h>
 
 #include "qw_internal.h"
@@ -42,20 +49,246 @@ __global__ void __launch_bounds__(kThreads) shrink_rows_kernel(LoraArgs p, const
   }
 }
 
-__global__ void __launch_bounds__(kThreads) expand_rows_kernel(LoraArgs p, const float* y32, const float* h,
-                                                               const __half* bias, __half* y) {
-  const int64_t nb = (p.N + kThreads - 1) / kThreads;
-  const int64_t m = blockIdx.x / nb;
-  const int64_t n = (blockIdx.x % nb) * kThreads + threadIdx.x;
-  if (n >= p.N) return;
-  const int64_t a = adapter_of(p, m);
-  float acc = y32[m * p.N + n];
-  if (a >= 0) {
-    const __half* b = reinterpret_cast<const __half*>(p.b) + (a * p.N + n) * p.R;
-    for (int r = 0; r < p.R; ++r) acc += h[m * p.R + r] * __half2float(b[r]);
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// h = s x A^T for the forward.  Memory- and latency-bound: x is read once and
+// the A of every adapter present once per 16 rows; the products are few.
+//
+// A cluster takes a tile of 16 rows and every G-th of the adapters its rows
+// name (a row belongs to one of them, so groups write disjoint rows); its CTAs
+// and their warps split K.  A warp's operands come straight from memory in
+// mma.sync m16n8k16 fragment order: one 16-byte load a lane brings a row's 8
+// consecutive k for two products' slots, the order of k within a sum being
+// free as long as x and A agree, so no shared memory, no barrier and no copy
+// stands between the loads and the products, and a warp keeps U steps of 32 k
+// in flight.  Each adapter has its own accumulators: what a row that is not its
+// own, or A of another, holds never meets it.  Sums over warps and CTAs go
+// through (distributed) shared memory in a fixed order.
+//
+// Blocks behind the tiles' list, for the tcgen05 kernel, the adapters of every
+// token tile in ascending order, and zero the decode kernel's counters.
+struct RankRows {
+  LoraArgs p;
+  float* h32;         // [M][R] fp32 (at most 16 rows), or
+  __half* h16;        // [M][R8] fp16, zero-padded rank
+  int R8;
+  int tiles, groups;  // row tiles, adapter groups per tile
+  int token_tile;     // rows of a token tile (0: no lists)
+  int token_tiles;
+  uint32_t* tile_n;   // [token_tiles] adapters of the tile
+  uint32_t* tile_ids; // [token_tiles][token_tile]
+  uint4* zero;        // cleared by the blocks behind the lists
+  int zero_vecs;
+};
+
+template <int RT, int WARPS, int U>
+__global__ void __launch_bounds__(WARPS * 32) rank_rows_kernel(const RankRows q) {
+  constexpr int RP = 8 * RT;
+  extern __shared__ float red[];  // [WARPS][16][RP], then the CTA's sum [16][RP]
+  __shared__ uint32_t row_id[16];
+  __shared__ uint32_t list[16];
+  __shared__ int list_n;
+  __shared__ uint32_t bits[kLoraMaxAdapters / 32];
+  const LoraArgs& p = q.p;
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t rank = cluster_rank(), C = cluster_size();
+  const int unit = (int)(blockIdx.x / C);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  if (unit >= q.tiles * q.groups) {
+    if (rank != 0) return;
+    const int t = unit - q.tiles * q.groups;
+    if (t >= q.token_tiles) {
+      for (int i = tid; i < q.zero_vecs; i += WARPS * 32) q.zero[i] = make_uint4(0u, 0u, 0u, 0u);
+      return;
+    }
+    for (int i = tid; i < (int)kLoraMaxAdapters / 32; i += WARPS * 32) bits[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < q.token_tile; i += WARPS * 32) {
+      const int64_t m = (int64_t)t * q.token_tile + i;
+      if (m < p.M) {
+        const int64_t a = adapter_of(p, m);
+        if (a >= 0) atomicOr(&bits[a / 32], 1u << (a % 32));
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {  // a lane the bits of 4 words
+      uint32_t w[kLoraMaxAdapters / 1024], n = 0;
+#pragma unroll
+      for (int i = 0; i < (int)kLoraMaxAdapters / 1024; ++i) {
+        w[i] = bits[lane * (kLoraMaxAdapters / 1024) + i];
+        n += __popc(w[i]);
+      }
+      uint32_t before = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+      }
+      if (lane == 31) q.tile_n[t] = before;
+      before -= n;
+#pragma unroll
+      for (int i = 0; i < (int)kLoraMaxAdapters / 1024; ++i)
+        for (uint32_t b = w[i]; b; b &= b - 1)
+          q.tile_ids[(size_t)t * q.token_tile + before++] =
+              (uint32_t)((lane * (kLoraMaxAdapters / 1024) + i) * 32 + __ffs(b) - 1);
+    }
+    return;
   }
-  if (bias) acc += __half2float(bias[n]);
-  y[m * p.N + n] = __float2half_rn(acc);
+
+  const int64_t m0 = (int64_t)(unit / q.groups) * 16;
+  const int group = unit % q.groups;
+  if (warp == 0) {
+    const int64_t a = lane < 16 && m0 + lane < p.M ? adapter_of(p, m0 + lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, (int)a);
+    const bool first = a >= 0 && __ffs(same) - 1 == lane;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, first);
+    if (lane < 16) row_id[lane] = (uint32_t)a;
+    if (first) list[__popc(leaders & ((1u << lane) - 1u))] = (uint32_t)a;
+    if (lane == 0) list_n = __popc(leaders);
+  }
+  __syncthreads();
+  const int n = list_n;
+  const int steps = (int)(p.K / 32);
+  const int s0 = (int)((int64_t)steps * rank / C), s1 = (int)((int64_t)steps * (rank + 1) / C);
+  const int r = lane / 4, kq = (lane % 4) * 8;
+  float* const mine = red + warp * 16 * RP;
+  float* const cta = red + WARPS * 16 * RP;
+  for (int j = group; j < n; j += q.groups) {
+    const uint32_t a = list[j];
+    const bool own0 = row_id[r] == a, own1 = row_id[r + 8] == a;
+    const __half* x0 = reinterpret_cast<const __half*>(p.x) + (m0 + r) * p.x_ld + kq;
+    const __half* x1 = x0 + 8 * p.x_ld;
+    const __half* w0 = reinterpret_cast<const __half*>(p.a) + ((int64_t)a * p.R + r) * p.K + kq;
+    float acc[RT][4];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (int s = s0 + warp; s < s1; s += WARPS * U) {
+      uint4 xa[U], xb[U], w[U][RT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t k = (int64_t)(s + u * WARPS) * 32;
+        const bool in = s + u * WARPS < s1;
+        xa[u] = in && own0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
+        xb[u] = in && own1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          w[u][t] = in && r + 8 * t < p.R ? __ldg(reinterpret_cast<const uint4*>(w0 + (int64_t)t * 8 * p.K + k)) : zero;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          mma_16816(acc[t], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][t].x, w[u][t].y);
+          mma_16816(acc[t], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][t].z, w[u][t].w);
+        }
+    }
+    __syncthreads();  // the sums of the adapter before are read
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float2* d0 = reinterpret_cast<float2*>(mine + r * RP + t * 8 + (lane % 4) * 2);
+      float2* d1 = reinterpret_cast<float2*>(mine + (r + 8) * RP + t * 8 + (lane % 4) * 2);
+      *d0 = make_float2(acc[t][0], acc[t][1]);
+      *d1 = make_float2(acc[t][2], acc[t][3]);
+    }
+    __syncthreads();
+    const float scale = p.scales ? p.scales[a] : 1.f;
+    for (int i = tid; i < 16 * RP; i += WARPS * 32) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) v += red[w * 16 * RP + i];
+      cta[i] = v;
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    for (int i = (int)rank * WARPS * 32 + tid; i < 16 * RP; i += (int)C * WARPS * 32) {
+      const int row = i / RP, c = i % RP;
+      if (row_id[row] != a) continue;
+      float v = 0.f;
+      for (uint32_t k = 0; k < C; ++k) v += C > 1 ? ld_cluster_f32(&cta[i], k) : cta[i];
+      v *= scale;
+      if (q.h32) {
+        if (c < p.R) q.h32[(m0 + row) * p.R + c] = v;
+      } else if (c < q.R8) {
+        // one rounding to fp16: the tensor cores take y's second product in fp16
+        q.h16[(m0 + row) * q.R8 + c] = __float2half_rn(v);
+      }
+    }
+    if (C > 1) cluster_sync();  // the peers' sums are read before they change or go
+  }
+}
+
+// y = fp16(product + h B^T + bias) for at most 16 rows.  Bound by the launch and
+// one trip to memory: a thread has a column and every fourth row; B's lines are
+// asked for before the wait for the projection.
+template <int RV>  // R = 8 RV (0: any rank)
+__global__ void __launch_bounds__(256) expand_rows_kernel(const LoraArgs p, const float* y32, const float* h,
+                                                          const __half* bias, __half* y, int row_groups) {
+  extern __shared__ float hs[];  // [M][R]
+  const int cols = 256 / row_groups;
+  const int64_t n = (int64_t)blockIdx.x * cols + threadIdx.x % cols;
+  const int rg = threadIdx.x / cols;
+  const __half* b0 = reinterpret_cast<const __half*>(p.b);
+  if (n < p.N) {
+    for (int m = rg; m < p.M; m += row_groups) {
+      const int64_t a = adapter_of(p, m);
+      if (a < 0) continue;
+      const char* line = reinterpret_cast<const char*>(b0 + (a * p.N + n) * p.R);
+      for (int i = 0; i < p.R * 2; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + i));
+    }
+  }
+  pdl_wait();
+  for (int i = threadIdx.x; i < (int)p.M * p.R; i += 256) hs[i] = __ldcg(h + i);
+  __syncthreads();
+  if (n >= p.N) return;
+  const float bn = bias ? __half2float(bias[n]) : 0.f;
+#pragma unroll 4
+  for (int m = rg; m < p.M; m += row_groups) {
+    const int64_t a = adapter_of(p, m);
+    float acc = __ldcg(y32 + m * p.N + n) + bn;
+    if (a >= 0) {
+      const __half* b = b0 + (a * p.N + n) * p.R;
+      float part = 0.f;
+      if constexpr (RV > 0) {
+#pragma unroll
+        for (int v = 0; v < RV; ++v) {
+          const uint4 w = __ldg(reinterpret_cast<const uint4*>(b) + v);
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ws[i]));
+            part = fmaf(hs[m * 8 * RV + 8 * v + 2 * i], f.x, part);
+            part = fmaf(hs[m * 8 * RV + 8 * v + 2 * i + 1], f.y, part);
+          }
+        }
+      } else {
+        for (int i = 0; i < p.R; ++i) part = fmaf(hs[m * p.R + i], __half2float(b[i]), part);
+      }
+      acc += part;
+    }
+    y[m * p.N + n] = __float2half_rn(acc);
+  }
 }
 
 __global__ void __launch_bounds__(kThreads) dx_rows_kernel(LoraArgs p, const float* g, __half* dx, bool add) {
@@ -89,23 +322,144 @@ __global__ void __launch_bounds__(kThreads) outer_rows_kernel(LoraArgs p, const 
 
 }  // namespace
 
-size_t lora_forward_bytes(int64_t M, int64_t N, int64_t R) {
-  return (size_t)M * R * sizeof(float) + (size_t)M * N * sizeof(float);
+namespace {
+
+constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+int round8(int r) { return (r + 7) / 8 * 8; }
+
+// Forward workspace: at most 16 rows, h fp32 then the projection's fp32
+// product; above, h fp16 (zero-padded rank) and the token tiles' lists.
+struct ForwardSpace {
+  size_t second, third, end;
+};
+ForwardSpace forward_space(int64_t M, int64_t N, int R, int token_tile) {
+  ForwardSpace f;
+  if (token_tile == 0) {
+    f.second = align256((size_t)M * R * sizeof(float));
+    f.third = f.end = f.second + align256((size_t)M * N * sizeof(float));
+  } else {
+    const size_t tiles = (size_t)((M + token_tile - 1) / token_tile);
+    f.second = align256((size_t)M * round8(R) * sizeof(__half));
+    f.third = f.second + align256(tiles * sizeof(uint32_t));
+    f.end = f.third + align256(tiles * token_tile * sizeof(uint32_t));
+  }
+  return f;
 }
 
-cudaError_t launch_lora_shrink(const LoraArgs& p, void* ws, cudaStream_t stream) {
-  shrink_rows_kernel<false><<<(unsigned)p.M, kThreads, 0, stream>>>(p, (const __half*)p.x, p.x_ld, p.K,
-                                                                    (const __half*)p.a, (float*)ws);
-  return cudaGetLastError();
+template <int RT, int WARPS, int U>
+cudaError_t launch_rank_rows(RankRows& q, int sm_count, bool pdl, cudaStream_t stream) {
+  // K over the warps, then over up to 8 CTAs while a warp has more than U
+  // steps; the tile's adapters over groups while SMs are free.
+  const int steps = (int)(q.p.K / 32);
+  int C = (steps + WARPS * U - 1) / (WARPS * U);
+  C = C > 8 ? 8 : C;
+  while (C > 1 && (int64_t)q.tiles * C > 2 * sm_count) --C;
+  int64_t groups = 2 * sm_count / ((int64_t)q.tiles * C);
+  const int64_t most = q.p.L < 16 ? q.p.L : 16;
+  groups = groups > most ? most : groups;
+  groups = groups < 1 ? 1 : groups;
+  q.groups = (int)groups;
+  constexpr int smem = (WARPS + 1) * 16 * 8 * RT * (int)sizeof(float);
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(rank_rows_kernel<RT, WARPS, U>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured_dev = dev;
+  }
+  const int64_t units = (int64_t)q.tiles * q.groups + q.token_tiles + (q.zero_vecs ? 1 : 0);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * C));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, rank_rows_kernel<RT, WARPS, U>, q);
 }
 
-float* lora_forward_product(const LoraArgs& p, void* ws) { return (float*)ws + p.M * p.R; }
+}  // namespace
 
-cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.N + kThreads - 1) / kThreads * p.M));
-  expand_rows_kernel<<<grid, kThreads, 0, stream>>>(p, lora_forward_product(p, ws), (const float*)ws,
-                                                    (const __half*)bias, (__half*)y);
-  return cudaGetLastError();
+size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile) { return forward_space(M, N, R, token_tile).end; }
+
+cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes, int sm_count,
+                             bool pdl, cudaStream_t stream) {
+  const ForwardSpace f = forward_space(p.M, p.N, p.R, token_tile);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  RankRows q{};
+  q.p = p;
+  q.R8 = round8(p.R);
+  if (token_tile == 0) {
+    q.h32 = reinterpret_cast<float*>(base);
+  } else {
+    q.h16 = reinterpret_cast<__half*>(base);
+    q.token_tile = token_tile;
+    q.token_tiles = (int)((p.M + token_tile - 1) / token_tile);
+    q.tile_n = reinterpret_cast<uint32_t*>(base + f.second);
+    q.tile_ids = reinterpret_cast<uint32_t*>(base + f.third);
+  }
+  q.tiles = (int)((p.M + 15) / 16);
+  q.zero = static_cast<uint4*>(zero);
+  q.zero_vecs = (int)((zero_bytes + 15) / 16);
+  if (p.R <= 8) return launch_rank_rows<1, 16, 6>(q, sm_count, pdl, stream);
+  if (p.R <= 16) return launch_rank_rows<2, 16, 4>(q, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_rank_rows<4, 16, 3>(q, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_rank_rows<8, 8, 3>(q, sm_count, pdl, stream);
+  return launch_rank_rows<16, 8, 1>(q, sm_count, pdl, stream);
+}
+
+float* lora_forward_product(const LoraArgs& p, void* ws) {
+  return reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + forward_space(p.M, p.N, p.R, 0).second);
+}
+
+PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias) {
+  const ForwardSpace f = forward_space(p.M, p.N, p.R, token_tile);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  PrefillLora l{};
+  l.h = base;
+  l.b = p.b;
+  l.idx = p.idx;
+  l.tile_n = reinterpret_cast<uint32_t*>(base + f.second);
+  l.tile_ids = reinterpret_cast<uint32_t*>(base + f.third);
+  l.bias = bias;
+  l.R = p.R;
+  l.L = (int)p.L;
+  return l;
+}
+
+cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, bool pdl, cudaStream_t stream) {
+  const int row_groups = p.M >= 4 ? 4 : 1;
+  const int cols = 256 / row_groups;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.N + cols - 1) / cols));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = (size_t)p.M * p.R * sizeof(float);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const float* y32 = lora_forward_product(p, ws);
+  const float* h = static_cast<const float*>(ws);
+  const __half* bi = static_cast<const __half*>(bias);
+  __half* yo = static_cast<__half*>(y);
+  switch (p.R) {
+    case 8: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<1>, p, y32, h, bi, yo, row_groups);
+    case 16: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<2>, p, y32, h, bi, yo, row_groups);
+    case 32: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<4>, p, y32, h, bi, yo, row_groups);
+    case 64: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<8>, p, y32, h, bi, yo, row_groups);
+    default: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<0>, p, y32, h, bi, yo, row_groups);
+  }
 }
 
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count) {

@@ -22,6 +22,17 @@
 // them with one shuffle per token and writes silu(gate) * up (64 outputs per
 // tile, each op rounded to fp16).
 //
+// LORA (a separate instantiation): adapters beside the projection, as further
+// columns of the reduction.  A token tile that names n adapters of rank R gets
+// ceil(n R8 / 64) more k blocks (R8 the rank rounded up to 8): block columns
+// (adapter, r) hold lora_b of the tile's weight rows as A and h = s x A^T, fp16,
+// of the tokens that take that adapter as B, zero for the others.  The dequant
+// warps write both (TMEM and the swizzled x slot), the producer only passes
+// the stage on.  2048 x 17408 x 5120 with 8 adapters of rank 32: the product
+// alone 291 us, a separate pass over y would read and write 214 MB more (33 us).
+// A zero times another adapter's infinity would be NaN: non-finite lora_b values
+// enter as zero and are added, for the tokens that own them, in the epilogue.
+//
 // The weights the MMA consumes are exactly qw_dequantize's (fp16(fp16(s*q)
 // + b)): pairs (1024 + q_even, 1024 + 16 q_odd) come from one prmt and one
 // and, fma.rn.f16x2 with (s, s/16) and (-1024 s, -64 s) gives fp16(s*q)
@@ -57,13 +68,16 @@ struct PfCfg {
   // barriers: xfull, wpfull, wpempty, afull, aempty (per stage), dfull, dempty
   static constexpr int NBAR = 5 * STAGES + 2;
   static constexpr int OFF_BAR = OFF_WP + STAGES * WP_STAGE;
-  static constexpr int SMEM = OFF_BAR + NBAR * 8 + 64 + 1024;
+  // LORA: per tile parity and half of the blocks, whether a weight row has non-finite lora_b values
+  static constexpr int OFF_BAD = OFF_BAR + NBAR * 8 + 64;
+  static constexpr int SMEM = OFF_BAD + 1024;
+  static constexpr int SMEM_LORA = SMEM + 4 * BM;
   // TMEM: D (BT fp32 columns) at 0, then the A stages (32 columns each)
   static constexpr uint32_t D_COL = 0;
   static constexpr uint32_t A_COL = BT >= 128 ? BT : 128;
   static constexpr uint32_t TMEM_COLS = A_COL + 32 * STAGES <= 256 ? 256 : 512;
   static_assert(A_COL + 32 * STAGES <= 512, "TMEM columns");
-  static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert(SMEM_LORA <= 232448, "shared memory budget");
 };
 constexpr int DQW = 8;             // dequant / epilogue warps: 2 per TMEM lane quarter
 constexpr int THREADS = (2 + DQW) * 32;
@@ -82,7 +96,32 @@ struct PrefillParams {
   const __half* scales2;
   const __half* biases2;
   unsigned int* status;
+  PrefillLora lora;  // LORA
+  int lora_r8;       // rank rounded up to 8, in 8-wide chunks
 };
+
+// 8 consecutive ranks of one lora_b row from rank r0 on, zero past the rank.
+__device__ __forceinline__ uint4 lora_chunk(const __half* row, int r0, int R) {
+  if (R % 8 == 0) return __ldg(reinterpret_cast<const uint4*>(row + r0));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = r0 + 2 * i < R ? __half_as_ushort(row[r0 + 2 * i]) : 0;
+    const uint32_t hi = r0 + 2 * i + 1 < R ? __half_as_ushort(row[r0 + 2 * i + 1]) : 0;
+    w[i] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Two fp16 values with non-finite ones (exponent all ones) replaced by zero.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool* bad) {
+  const bool lo = (w & 0x7C00u) == 0x7C00u, hi = (w & 0x7C000000u) == 0x7C000000u;
+  *bad = *bad || lo || hi;
+  return (lo ? 0u : w & 0xFFFFu) | (hi ? 0u : w & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t lora_adapter_of(const PrefillLora& l, int tok, int M) {
+  if (tok >= M) return 0xFFFFFFFFu;
+  return l.idx ? l.idx[tok] : 0u;
+}
 
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
   // K-major, 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
@@ -121,7 +160,7 @@ __device__ __forceinline__ void dequant_group_slow(const uint32_t (&wd)[4], __ha
   }
 }
 
-template <int BITS, int BT_>
+template <int BITS, int BT_, bool LORA>
 __global__ void __launch_bounds__(THREADS, 1)
     qmm_prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                        const __grid_constant__ CUtensorMap tm_w2, const PrefillParams p) {
@@ -147,6 +186,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   const int total_tiles = p.n_tiles * p.m_tiles;
+  uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [parity][half][BM]
+  // k blocks of a token tile: the weights' groups, then its adapters'
+  auto blocks_of = [&](int mt) {
+    if constexpr (LORA) return p.groups + ((int)__ldcg(p.lora.tile_n + mt) * p.lora_r8 + 7) / 8;
+    else return p.groups;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -182,7 +227,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t it = 0;
       for (int tile = blockIdx.x; tile < total_tiles && !*abort_flag; tile += gridDim.x) {
         const int nt = tile / p.m_tiles, mt = tile % p.m_tiles;
-        for (int g = 0; g < p.groups; ++g, ++it) {
+        const int blocks = blocks_of(mt);
+        for (int g = 0; g < blocks; ++g, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (it >= STAGES) {
@@ -193,6 +239,11 @@ __global__ void __launch_bounds__(THREADS, 1)
               *abort_flag = 1;
               break;
             }
+          }
+          if (LORA && g >= p.groups) {  // the dequant warps fill the stage
+            mbar_arrive(&xfull[s]);
+            mbar_arrive(&wpfull[s]);
+            continue;
           }
           mbar_arrive_expect_tx(&xfull[s], X_STAGE);
           tma_load_2d(smem + OFF_X + s * X_STAGE, &tm_x, &xfull[s], g * kGroup, mt * BT);
@@ -211,13 +262,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------------------------------------------------- MMA issuer
     constexpr uint32_t idesc = idesc_f16(BM, BT);
     uint32_t it = 0, tile_count = 0;
+    if (LORA) pdl_wait();  // the lists are the previous kernel's
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++tile_count) {
       // the epilogue has drained D from the previous tile
       if (tile_count > 0 && !*abort_flag &&
           !mbar_wait(dempty, (tile_count - 1) & 1, p.status, kDevTimeoutAccum))
         *abort_flag = 1;
       tc_fence_after();
-      for (int g = 0; g < p.groups; ++g, ++it) {
+      const int blocks = blocks_of(tile % p.m_tiles);
+      for (int g = 0; g < blocks; ++g, ++it) {
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
         if (!*abort_flag) {
@@ -258,9 +311,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const __half* biases = up_lane ? p.biases2 : p.biases;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     pdl_wait();
-    uint32_t tile_count = 0;
+    uint32_t tile_count = 0, it0 = 0;  // it0: k blocks of the tiles before
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++tile_count) {
       const int nt = tile / p.m_tiles, mt = tile % p.m_tiles;
+      const int blocks = blocks_of(mt);
+      bool bad = false;  // this row has non-finite lora_b values in the blocks of this warp
       const int row = nt * p.tile_rows + row_in_tile;
       const bool row_ok = row < p.N;
       const __half* srow = scales + (size_t)(row_ok ? row : 0) * p.sb_groups;
@@ -270,10 +325,65 @@ __global__ void __launch_bounds__(THREADS, 1)
       // MMA block-times per block of its own.
       __half s_next = (row_ok && khalf < p.groups) ? srow[khalf / p.gsh] : __float2half(0.f);
       __half b_next = (row_ok && khalf < p.groups) ? brow[khalf / p.gsh] : __float2half(0.f);
-      for (int g = khalf; g < p.groups; g += 2) {
-        const uint32_t it = tile_count * (uint32_t)p.groups + (uint32_t)g;
+      for (int g = khalf; g < blocks; g += 2) {
+        const uint32_t it = it0 + (uint32_t)g;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
+        if (LORA && g >= p.groups) {
+          // columns (adapter, r) of this block: chunk c (8 wide) of the tile's list
+          const int n = (int)__ldcg(p.lora.tile_n + mt);
+          const uint32_t* list = p.lora.tile_ids + (size_t)mt * BT;
+          const __half* lb = reinterpret_cast<const __half*>(p.lora.b);
+          const int c0 = (g - p.groups) * 8;
+          uint32_t out[2][16];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const int j = (c0 + c) / p.lora_r8, r0 = (c0 + c) % p.lora_r8 * 8;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (j < n && row_ok) {
+              v = lora_chunk(lb + ((size_t)__ldcg(list + j) * p.N + row) * p.lora.R, r0, p.lora.R);
+              v.x = finite_pair(v.x, &bad);
+              v.y = finite_pair(v.y, &bad);
+              v.z = finite_pair(v.z, &bad);
+              v.w = finite_pair(v.w, &bad);
+            }
+            out[c / 4][4 * (c % 4)] = v.x;
+            out[c / 4][4 * (c % 4) + 1] = v.y;
+            out[c / 4][4 * (c % 4) + 2] = v.z;
+            out[c / 4][4 * (c % 4) + 3] = v.w;
+          }
+          if (!*abort_flag && !mbar_wait(&wpfull[s], ph, p.status, kDevTimeoutFull)) *abort_flag = 1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&wpempty[s]);
+          if (it >= STAGES && !*abort_flag && !mbar_wait(&aempty[s], ph ^ 1, p.status, kDevTimeoutEmpty))
+            *abort_flag = 1;
+          // h of the tokens that take each column's adapter, at the places TMA's 128-byte swizzle gives them
+          for (int t = quarter * 32 + lane; t < BT; t += BM) {
+            const int tok = mt * BT + t;
+            const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
+            const uint4* h = reinterpret_cast<const uint4*>(p.lora.h) + (size_t)(tok < p.M ? tok : 0) * p.lora_r8;
+            uint8_t* dst = smem + OFF_X + s * X_STAGE + t * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const int j = (c0 + c) / p.lora_r8, rc = (c0 + c) % p.lora_r8;
+              const bool own = j < n && a == __ldcg(list + j);
+              *reinterpret_cast<uint4*>(dst + ((c ^ (t & 7)) << 4)) = own ? __ldcg(h + rc) : make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+          if (g + 2 >= blocks) bad_rows[((tile_count & 1) * 2 + khalf) * BM + quarter * 32 + lane] = bad;
+          tc_fence_after();
+          tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
+          tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&afull[s]);
+          continue;
+        }
+        // a half of the blocks may hold none of the adapters'
+        if (LORA && g + 2 >= blocks)
+          bad_rows[((tile_count & 1) * 2 + khalf) * BM + quarter * 32 + lane] = 0;
         const __half sc = s_next, bi = b_next;
         if (g + 2 < p.groups && row_ok) {  // prefetch this warp's next block's scale/bias
           s_next = srow[(g + 2) / p.gsh];
@@ -358,8 +468,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&afull[s]);
       }
       // ---------------------------------------------------------- epilogue
+      it0 += (uint32_t)blocks;
       if (!*abort_flag && !mbar_wait(dfull, tile_count & 1, p.status, kDevTimeoutAccum)) *abort_flag = 1;
       tc_fence_after();
+      float bias = 0.f;
+      if (LORA) {
+        if (p.lora.bias && row_ok) bias = __half2float(reinterpret_cast<const __half*>(p.lora.bias)[row]);
+        bad = bad_rows[(tile_count & 1) * 2 * BM + quarter * 32 + lane];
+        if (blocks > 1) bad = bad || bad_rows[((tile_count & 1) * 2 + 1) * BM + quarter * 32 + lane];
+      }
 #pragma unroll 1
       for (int cb = khalf * (BT / 32); cb < (khalf + 1) * (BT / 32); ++cb) {
         uint32_t v[16];
@@ -395,7 +512,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int tok = mt * BT + cb * 16 + q;
           if (tok < p.M) {
             const size_t idx = (size_t)tok * p.N + row;
-            const float f = __uint_as_float(v[q]);
+            float f = __uint_as_float(v[q]);
+            if constexpr (LORA) {
+              f += bias;
+              if (bad) {  // the non-finite terms of this token's own adapter
+                const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
+                const __half* h = reinterpret_cast<const __half*>(p.lora.h) + (size_t)tok * 8 * p.lora_r8;
+                const __half* b = reinterpret_cast<const __half*>(p.lora.b) + ((size_t)a * p.N + row) * p.lora.R;
+                for (int r = 0; a < (uint32_t)p.lora.L && r < p.lora.R; ++r) {
+                  const float bv = __half2float(b[r]);
+                  if (!isfinite(bv)) f += __half2float(h[r]) * bv;
+                }
+              }
+              reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
+              continue;
+            }
             if (p.y_f32) reinterpret_cast<float*>(p.y)[idx] = f;
             else reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
           }
@@ -421,8 +552,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 bool prefill_available() { return true; }
 
 namespace {
-template <int BITS, int BT>
+template <int BITS, int BT, bool LORA>
 cudaError_t launch_cfg(const PrefillArgs& a, cudaStream_t stream, bool pdl, std::string* err) {
+  constexpr int smem = LORA ? PfCfg<BITS, BT>::SMEM_LORA : PfCfg<BITS, BT>::SMEM;
   using Cfg = PfCfg<BITS, BT>;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -430,7 +562,7 @@ cudaError_t launch_cfg(const PrefillArgs& a, cudaStream_t stream, bool pdl, std:
   static thread_local int configured_dev = -1;
   if (configured_dev != dev) {
     cudaError_t e =
-        cudaFuncSetAttribute(qmm_prefill_kernel<BITS, BT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+        cudaFuncSetAttribute(qmm_prefill_kernel<BITS, BT, LORA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     configured_dev = dev;
   }
@@ -452,6 +584,10 @@ cudaError_t launch_cfg(const PrefillArgs& a, cudaStream_t stream, bool pdl, std:
   p.scales2 = reinterpret_cast<const __half*>(a.swiglu ? a.scales2 : a.scales);
   p.biases2 = reinterpret_cast<const __half*>(a.swiglu ? a.biases2 : a.biases);
   p.status = a.status;
+  if (LORA) {
+    p.lora = *a.lora;
+    p.lora_r8 = (a.lora->R + 7) / 8;
+  }
   CUtensorMap tx, tw, tw2;
   if (!encode_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.x, (uint64_t)a.K, (uint64_t)a.M,
                       (uint64_t)(a.x_ld ? a.x_ld : a.K) * 2, kGroup, BT, CU_TENSOR_MAP_SWIZZLE_128B, err))
@@ -469,14 +605,14 @@ cudaError_t launch_cfg(const PrefillArgs& a, cudaStream_t stream, bool pdl, std:
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, qmm_prefill_kernel<BITS, BT>, tx, tw, tw2, p);
+  return cudaLaunchKernelEx(&cfg, qmm_prefill_kernel<BITS, BT, LORA>, tx, tw, tw2, p);
 }
 }  // namespace
 
@@ -486,8 +622,16 @@ cudaError_t launch_prefill(const PrefillArgs& a, cudaStream_t stream, bool pdl, 
     return cudaErrorInvalidValue;
   }
   // narrow token tiles for at most 32 rows of x
-  if (a.M <= 32) return a.bits == 4 ? launch_cfg<4, 32>(a, stream, pdl, err) : launch_cfg<8, 32>(a, stream, pdl, err);
-  return a.bits == 4 ? launch_cfg<4, 256>(a, stream, pdl, err) : launch_cfg<8, 256>(a, stream, pdl, err);
+  if (a.lora) {
+    if (a.M <= 32)
+      return a.bits == 4 ? launch_cfg<4, 32, true>(a, stream, pdl, err) : launch_cfg<8, 32, true>(a, stream, pdl, err);
+    return a.bits == 4 ? launch_cfg<4, 256, true>(a, stream, pdl, err) : launch_cfg<8, 256, true>(a, stream, pdl, err);
+  }
+  if (a.M <= 32)
+    return a.bits == 4 ? launch_cfg<4, 32, false>(a, stream, pdl, err) : launch_cfg<8, 32, false>(a, stream, pdl, err);
+  return a.bits == 4 ? launch_cfg<4, 256, false>(a, stream, pdl, err) : launch_cfg<8, 256, false>(a, stream, pdl, err);
 }
+
+int prefill_token_tile(int64_t M) { return M <= 32 ? 32 : 256; }
 
 }  // namespace qw
