@@ -112,6 +112,7 @@ struct PrefillLora {
   const uint32_t* idx;       // [M] or null (adapter 0)
   const uint32_t* tile_n;    // [token tiles]
   const uint32_t* tile_ids;  // [token tiles][tokens per tile]
+  const uint32_t* slots;     // [M] place of the token's adapter in its tile's list (none: 0xFFFFFFFF)
   const void* bias;          // fp16 [N] or null
   int R, L;
 };

@@ -96,6 +96,7 @@ struct RankRows {
   int token_tiles;
   uint32_t* tile_n;   // [token_tiles] adapters of the tile
   uint32_t* tile_ids; // [token_tiles][token_tile]
+  uint32_t* slots;    // [M] place of the row's adapter in its tile's list
   uint4* zero;        // cleared by the blocks behind the lists
   int zero_vecs;
 };
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(WARPS * 32) rank_rows_kernel(const RankRows q)
   __shared__ uint32_t row_id[16];
   __shared__ uint32_t list[16];
   __shared__ int list_n;
-  __shared__ uint32_t bits[kLoraMaxAdapters / 32];
+  __shared__ uint32_t bits[kLoraMaxAdapters / 32], before[kLoraMaxAdapters / 32];
   const LoraArgs& p = q.p;
   pdl_wait();
   pdl_launch_dependents();
@@ -132,26 +133,35 @@ __global__ void __launch_bounds__(WARPS * 32) rank_rows_kernel(const RankRows q)
       }
     }
     __syncthreads();
+    constexpr int kWords = (int)kLoraMaxAdapters / 32;
     if (warp == 0) {  // a lane the bits of 4 words
-      uint32_t w[kLoraMaxAdapters / 1024], n = 0;
+      uint32_t w[kWords / 32], n = 0;
 #pragma unroll
-      for (int i = 0; i < (int)kLoraMaxAdapters / 1024; ++i) {
-        w[i] = bits[lane * (kLoraMaxAdapters / 1024) + i];
+      for (int i = 0; i < kWords / 32; ++i) {
+        w[i] = bits[lane * (kWords / 32) + i];
         n += __popc(w[i]);
       }
-      uint32_t before = n;
+      uint32_t at = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
+        const uint32_t v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
       }
-      if (lane == 31) q.tile_n[t] = before;
-      before -= n;
+      if (lane == 31) q.tile_n[t] = at;
+      at -= n;
 #pragma unroll
-      for (int i = 0; i < (int)kLoraMaxAdapters / 1024; ++i)
+      for (int i = 0; i < kWords / 32; ++i) {
+        before[lane * (kWords / 32) + i] = at;
         for (uint32_t b = w[i]; b; b &= b - 1)
-          q.tile_ids[(size_t)t * q.token_tile + before++] =
-              (uint32_t)((lane * (kLoraMaxAdapters / 1024) + i) * 32 + __ffs(b) - 1);
+          q.tile_ids[(size_t)t * q.token_tile + at++] = (uint32_t)((lane * (kWords / 32) + i) * 32 + __ffs(b) - 1);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < q.token_tile; i += WARPS * 32) {
+      const int64_t m = (int64_t)t * q.token_tile + i;
+      if (m >= p.M) break;
+      const int64_t a = adapter_of(p, m);
+      q.slots[m] = a < 0 ? 0xFFFFFFFFu : before[a / 32] + __popc(bits[a / 32] & ((1u << (a % 32)) - 1u));
     }
     return;
   }
@@ -330,18 +340,19 @@ int round8(int r) { return (r + 7) / 8 * 8; }
 // Forward workspace: at most 16 rows, h fp32 then the projection's fp32
 // product; above, h fp16 (zero-padded rank) and the token tiles' lists.
 struct ForwardSpace {
-  size_t second, third, end;
+  size_t second, third, fourth, end;
 };
 ForwardSpace forward_space(int64_t M, int64_t N, int R, int token_tile) {
   ForwardSpace f;
   if (token_tile == 0) {
     f.second = align256((size_t)M * R * sizeof(float));
-    f.third = f.end = f.second + align256((size_t)M * N * sizeof(float));
+    f.third = f.fourth = f.end = f.second + align256((size_t)M * N * sizeof(float));
   } else {
     const size_t tiles = (size_t)((M + token_tile - 1) / token_tile);
     f.second = align256((size_t)M * round8(R) * sizeof(__half));
     f.third = f.second + align256(tiles * sizeof(uint32_t));
-    f.end = f.third + align256(tiles * token_tile * sizeof(uint32_t));
+    f.fourth = f.third + align256(tiles * token_tile * sizeof(uint32_t));
+    f.end = f.fourth + align256((size_t)M * sizeof(uint32_t));
   }
   return f;
 }
@@ -406,6 +417,7 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     q.token_tiles = (int)((p.M + token_tile - 1) / token_tile);
     q.tile_n = reinterpret_cast<uint32_t*>(base + f.second);
     q.tile_ids = reinterpret_cast<uint32_t*>(base + f.third);
+    q.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);
@@ -430,6 +442,7 @@ PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, c
   l.idx = p.idx;
   l.tile_n = reinterpret_cast<uint32_t*>(base + f.second);
   l.tile_ids = reinterpret_cast<uint32_t*>(base + f.third);
+  l.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
   l.bias = bias;
   l.R = p.R;
   l.L = (int)p.L;

@@ -26,9 +26,9 @@
 // columns of the reduction.  A token tile that names n adapters of rank R gets
 // ceil(n R8 / 64) more k blocks (R8 the rank rounded up to 8): block columns
 // (adapter, r) hold lora_b of the tile's weight rows as A and h = s x A^T, fp16,
-// of the tokens that take that adapter as B, zero for the others.  The dequant
-// warps write both (TMEM and the swizzled x slot), the producer only passes
-// the stage on.  2048 x 17408 x 5120 with 8 adapters of rank 32: the product
+// of the tokens that take that adapter as B, zero for the others.  Four more
+// warps write both (TMEM and the swizzled x slot) while the dequant warps are at
+// the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8 adapters of rank 32: the product
 // alone 291 us, a separate pass over y would read and write 214 MB more (33 us).
 // A zero times another adapter's infinity would be NaN: non-finite lora_b values
 // enter as zero and are added, for the tokens that own them, in the epilogue.
@@ -68,10 +68,11 @@ struct PfCfg {
   // barriers: xfull, wpfull, wpempty, afull, aempty (per stage), dfull, dempty
   static constexpr int NBAR = 5 * STAGES + 2;
   static constexpr int OFF_BAR = OFF_WP + STAGES * WP_STAGE;
-  // LORA: per tile parity and half of the blocks, whether a weight row has non-finite lora_b values
+  // LORA: per tile parity, whether a weight row has non-finite lora_b values
   static constexpr int OFF_BAD = OFF_BAR + NBAR * 8 + 64;
+  static constexpr int OFF_XGO = OFF_BAD + 2 * BM;  // LORA: barriers, the producer has freed the stage for an adapters' block
   static constexpr int SMEM = OFF_BAD + 1024;
-  static constexpr int SMEM_LORA = SMEM + 4 * BM;
+  static constexpr int SMEM_LORA = SMEM + 2 * BM + 8 * STAGES;
   // TMEM: D (BT fp32 columns) at 0, then the A stages (32 columns each)
   static constexpr uint32_t D_COL = 0;
   static constexpr uint32_t A_COL = BT >= 128 ? BT : 128;
@@ -81,6 +82,7 @@ struct PfCfg {
 };
 constexpr int DQW = 8;             // dequant / epilogue warps: 2 per TMEM lane quarter
 constexpr int THREADS = (2 + DQW) * 32;
+constexpr int THREADS_LORA = THREADS + 128;  // and four warps that stage the adapters' blocks
 
 struct PrefillParams {
   int M, N, K;
@@ -161,7 +163,7 @@ __device__ __forceinline__ void dequant_group_slow(const uint32_t (&wd)[4], __ha
 }
 
 template <int BITS, int BT_, bool LORA>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
     qmm_prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                        const __grid_constant__ CUtensorMap tm_w2, const PrefillParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -186,7 +188,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   const int total_tiles = p.n_tiles * p.m_tiles;
-  uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [parity][half][BM]
+  uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [parity][BM]
+  uint64_t* const xgo = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_XGO);  // LORA
   // k blocks of a token tile: the weights' groups, then its adapters'
   auto blocks_of = [&](int mt) {
     if constexpr (LORA) return p.groups + ((int)__ldcg(p.lora.tile_n + mt) * p.lora_r8 + 7) / 8;
@@ -200,6 +203,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&wpempty[s], DQW / 2);  // the four warps (lane quarters) that own the group
       mbar_init(&afull[s], DQW / 2);
       mbar_init(&aempty[s], 1);
+      if (LORA) mbar_init(&xgo[s], 1);
     }
     mbar_init(dfull, 1);
     mbar_init(dempty, DQW);
@@ -240,9 +244,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               break;
             }
           }
-          if (LORA && g >= p.groups) {  // the dequant warps fill the stage
+          if (LORA && g >= p.groups) {  // the stage is free: the adapters' warps fill it
             mbar_arrive(&xfull[s]);
             mbar_arrive(&wpfull[s]);
+            mbar_arrive(&xgo[s]);
             continue;
           }
           mbar_arrive_expect_tx(&xfull[s], X_STAGE);
@@ -294,6 +299,90 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) tc_commit(dfull);
       __syncwarp();
     }
+  } else if (LORA && warp >= 2 + DQW) {
+    // ------------------------------- the adapters' k blocks (A in TMEM, x slot)
+    const int quarter = warp & 3;
+    const int lane_row = quarter * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const __half* lb = reinterpret_cast<const __half*>(p.lora.b);
+    const uint4* hb = reinterpret_cast<const uint4*>(p.lora.h);
+    const int r8 = p.lora_r8;
+    pdl_wait();
+    // xgo[s] completes a phase per adapters' block in stage s, and its next one only after these warps have
+    // passed the stage on (wpempty), so its parity is that of the blocks counted here
+    uint32_t it0 = 0, tile_count = 0, parities = 0;
+    for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++tile_count) {
+      const int nt = tile / p.m_tiles, mt = tile % p.m_tiles;
+      const int blocks = blocks_of(mt);
+      const int n = (int)__ldcg(p.lora.tile_n + mt);
+      const uint32_t* list = p.lora.tile_ids + (size_t)mt * BT;
+      const int row = nt * BM + lane_row;
+      const bool row_ok = row < p.N;
+      bool bad = false;
+      for (int g = p.groups; g < blocks; ++g) {
+        const int s = (int)((it0 + (uint32_t)g) % STAGES);
+        // chunk c (8 wide) of the block is ranks 8 rc .. of entry j of the tile's list
+        const int j0 = (g - p.groups) * 8 / r8, rc0 = (g - p.groups) * 8 % r8;
+        uint4 v[8];
+        {
+          int j = j0, rc = rc0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            v[c] = make_uint4(0u, 0u, 0u, 0u);
+            if (j < n && row_ok)
+              v[c] = lora_chunk(lb + ((size_t)__ldcg(list + j) * p.N + row) * p.lora.R, rc * 8, p.lora.R);
+            if (++rc == r8) rc = 0, ++j;
+          }
+        }
+        uint32_t slot[BT > BM ? BT / BM : 1];
+#pragma unroll
+        for (int i = 0; i < (BT > BM ? BT / BM : 1); ++i) {
+          const int tok = mt * BT + lane_row + i * BM;
+          slot[i] = lane_row + i * BM < BT && tok < p.M ? __ldcg(p.lora.slots + tok) : 0xFFFFFFFFu;
+        }
+        if (!*abort_flag && !mbar_wait(&xgo[s], (parities >> s) & 1u, p.status, kDevTimeoutFull)) *abort_flag = 1;
+        parities ^= 1u << s;
+        // h of the tokens that take each column's adapter, at the places TMA's 128-byte swizzle gives them
+#pragma unroll
+        for (int i = 0; i < (BT > BM ? BT / BM : 1); ++i) {
+          const int t = lane_row + i * BM;
+          if (t >= BT) continue;
+          const uint4* h = hb + (size_t)(mt * BT + t) * r8;
+          uint4 hv[8];
+          int j = j0, rc = rc0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            hv[c] = make_uint4(0u, 0u, 0u, 0u);
+            if ((uint32_t)j == slot[i]) hv[c] = __ldcg(h + rc);
+            if (++rc == r8) rc = 0, ++j;
+          }
+          uint8_t* dst = smem + OFF_X + s * X_STAGE + t * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(dst + ((c ^ (t & 7)) << 4)) = hv[c];
+        }
+        fence_proxy_async_smem();
+        uint32_t out[2][16];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          out[c / 4][4 * (c % 4)] = finite_pair(v[c].x, &bad);
+          out[c / 4][4 * (c % 4) + 1] = finite_pair(v[c].y, &bad);
+          out[c / 4][4 * (c % 4) + 2] = finite_pair(v[c].z, &bad);
+          out[c / 4][4 * (c % 4) + 3] = finite_pair(v[c].w, &bad);
+        }
+        if (g + 1 == blocks) bad_rows[(tile_count & 1) * BM + lane_row] = bad;
+        tc_fence_after();
+        tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
+        tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&wpempty[s]);
+          mbar_arrive(&afull[s]);
+        }
+      }
+      it0 += (uint32_t)blocks;
+    }
   } else {
     // ---------------------------------------------- dequant + epilogue
     const int dw = warp - 2;                 // 0..7
@@ -315,7 +404,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++tile_count) {
       const int nt = tile / p.m_tiles, mt = tile % p.m_tiles;
       const int blocks = blocks_of(mt);
-      bool bad = false;  // this row has non-finite lora_b values in the blocks of this warp
       const int row = nt * p.tile_rows + row_in_tile;
       const bool row_ok = row < p.N;
       const __half* srow = scales + (size_t)(row_ok ? row : 0) * p.sb_groups;
@@ -325,65 +413,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       // MMA block-times per block of its own.
       __half s_next = (row_ok && khalf < p.groups) ? srow[khalf / p.gsh] : __float2half(0.f);
       __half b_next = (row_ok && khalf < p.groups) ? brow[khalf / p.gsh] : __float2half(0.f);
-      for (int g = khalf; g < blocks; g += 2) {
+      for (int g = khalf; g < p.groups; g += 2) {
         const uint32_t it = it0 + (uint32_t)g;
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
-        if (LORA && g >= p.groups) {
-          // columns (adapter, r) of this block: chunk c (8 wide) of the tile's list
-          const int n = (int)__ldcg(p.lora.tile_n + mt);
-          const uint32_t* list = p.lora.tile_ids + (size_t)mt * BT;
-          const __half* lb = reinterpret_cast<const __half*>(p.lora.b);
-          const int c0 = (g - p.groups) * 8;
-          uint32_t out[2][16];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const int j = (c0 + c) / p.lora_r8, r0 = (c0 + c) % p.lora_r8 * 8;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (j < n && row_ok) {
-              v = lora_chunk(lb + ((size_t)__ldcg(list + j) * p.N + row) * p.lora.R, r0, p.lora.R);
-              v.x = finite_pair(v.x, &bad);
-              v.y = finite_pair(v.y, &bad);
-              v.z = finite_pair(v.z, &bad);
-              v.w = finite_pair(v.w, &bad);
-            }
-            out[c / 4][4 * (c % 4)] = v.x;
-            out[c / 4][4 * (c % 4) + 1] = v.y;
-            out[c / 4][4 * (c % 4) + 2] = v.z;
-            out[c / 4][4 * (c % 4) + 3] = v.w;
-          }
-          if (!*abort_flag && !mbar_wait(&wpfull[s], ph, p.status, kDevTimeoutFull)) *abort_flag = 1;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&wpempty[s]);
-          if (it >= STAGES && !*abort_flag && !mbar_wait(&aempty[s], ph ^ 1, p.status, kDevTimeoutEmpty))
-            *abort_flag = 1;
-          // h of the tokens that take each column's adapter, at the places TMA's 128-byte swizzle gives them
-          for (int t = quarter * 32 + lane; t < BT; t += BM) {
-            const int tok = mt * BT + t;
-            const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
-            const uint4* h = reinterpret_cast<const uint4*>(p.lora.h) + (size_t)(tok < p.M ? tok : 0) * p.lora_r8;
-            uint8_t* dst = smem + OFF_X + s * X_STAGE + t * 128;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const int j = (c0 + c) / p.lora_r8, rc = (c0 + c) % p.lora_r8;
-              const bool own = j < n && a == __ldcg(list + j);
-              *reinterpret_cast<uint4*>(dst + ((c ^ (t & 7)) << 4)) = own ? __ldcg(h + rc) : make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-          fence_proxy_async_smem();
-          if (g + 2 >= blocks) bad_rows[((tile_count & 1) * 2 + khalf) * BM + quarter * 32 + lane] = bad;
-          tc_fence_after();
-          tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
-          tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&afull[s]);
-          continue;
-        }
-        // a half of the blocks may hold none of the adapters'
-        if (LORA && g + 2 >= blocks)
-          bad_rows[((tile_count & 1) * 2 + khalf) * BM + quarter * 32 + lane] = 0;
         const __half sc = s_next, bi = b_next;
         if (g + 2 < p.groups && row_ok) {  // prefetch this warp's next block's scale/bias
           s_next = srow[(g + 2) / p.gsh];
@@ -472,10 +505,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!*abort_flag && !mbar_wait(dfull, tile_count & 1, p.status, kDevTimeoutAccum)) *abort_flag = 1;
       tc_fence_after();
       float bias = 0.f;
+      bool bad = false;  // non-finite lora_b values in this row
       if (LORA) {
         if (p.lora.bias && row_ok) bias = __half2float(reinterpret_cast<const __half*>(p.lora.bias)[row]);
-        bad = bad_rows[(tile_count & 1) * 2 * BM + quarter * 32 + lane];
-        if (blocks > 1) bad = bad || bad_rows[((tile_count & 1) * 2 + 1) * BM + quarter * 32 + lane];
+        bad = blocks > p.groups && bad_rows[(tile_count & 1) * BM + quarter * 32 + lane];
       }
 #pragma unroll 1
       for (int cb = khalf * (BT / 32); cb < (khalf + 1) * (BT / 32); ++cb) {
@@ -604,7 +637,7 @@ cudaError_t launch_cfg(const PrefillArgs& a, cudaStream_t stream, bool pdl, std:
   int grid = di.sm_count < tiles ? di.sm_count : tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(LORA ? THREADS_LORA : THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
