@@ -1354,7 +1354,7 @@ int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora
   g.add_dx = accumulate_dx != 0;
   g.da = da ? static_cast<float*>(da->data) : nullptr;
   g.db = db ? static_cast<float*>(db->data) : nullptr;
-  const cudaError_t ce = launch_lora_backward(la, g, workspace, sms, as_stream(stream_v));
+  const cudaError_t ce = launch_lora_backward(la, g, workspace, sms, pdl_enabled(), as_stream(stream_v));
   return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter gradient launch");
 }
 

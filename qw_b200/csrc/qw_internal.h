@@ -195,6 +195,13 @@ struct LoraArgs {
   int64_t x_ld;
   int R;
 };
+// Adapter lists of a forward's token tiles (tile 0: none).
+struct TokenLists {
+  int tile, tiles;   // tokens per tile, tiles
+  uint32_t* n;       // [tiles] adapters of the tile
+  uint32_t* ids;     // [tiles][tile]
+  uint32_t* slots;   // [M] place of the row's adapter in its tile's list (none: 0xFFFFFFFF)
+};
 struct LoraGrads {
   const void* dy;  // fp16 [M][N], rows dy_ld apart
   int64_t dy_ld;
@@ -218,7 +225,11 @@ cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, vo
 // What the tcgen05 kernel adds to its products, from the workspace.
 PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias);
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);
-cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, cudaStream_t stream);
+cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
+                                 cudaStream_t stream);
+// h = s x A^T in fp16 [M][R8] and the token tiles' lists, for a long forward.
+cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, int sm_count, bool pdl,
+                                 cudaStream_t stream);
 
 // Distillation from a teacher's top logits (qw_distill.cu).
 struct DistillArgs {

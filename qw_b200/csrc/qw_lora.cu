@@ -14,61 +14,12 @@
 #include <cuda_fp16.h>
 
 #include "qw_internal.h"
+#include "qw_lora.cuh"
 #include "qw_ptx.cuh"
 
 namespace qw {
 
 namespace {
-
-constexpr int kThreads = 256;
-
-__device__ __forceinline__ int64_t adapter_of(const LoraArgs& p, int64_t m) {
-  const uint32_t a = p.idx ? p.idx[m] : 0u;
-  return (int64_t)a < p.L ? (int64_t)a : -1;
-}
-
-// out[m][r] = s sum_i v[m][i] W[r][i] (TRANS: W[i][r]) in fp32, zero without an adapter.
-template <bool TRANS>
-__global__ void __launch_bounds__(kThreads) shrink_rows_kernel(LoraArgs p, const __half* v, int64_t ld, int64_t len,
-                                                               const __half* w, float* out) {
-  const int64_t m = blockIdx.x;
-  const int64_t a = adapter_of(p, m);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const __half* row = v + m * ld;
-  for (int r = warp; r < p.R; r += kThreads / 32) {
-    float acc = 0.f;
-    if (a >= 0) {
-      const __half* wa = w + a * len * p.R;
-      for (int64_t i = lane; i < len; i += 32)
-        acc += __half2float(row[i]) * __half2float(TRANS ? wa[i * p.R + r] : wa[r * len + i]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      acc *= p.scales ? p.scales[a] : 1.f;
-    }
-    if (lane == 0) out[m * p.R + r] = acc;
-  }
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
 
 // h = s x A^T for the forward.  Memory- and latency-bound: x is read once and
 // the A of every adapter present once per 16 rows; the products are few.
@@ -85,30 +36,25 @@ __device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
 // through (distributed) shared memory in a fixed order.
 //
 // Blocks behind the tiles' list, for the tcgen05 kernel, the adapters of every
-// token tile in ascending order, and zero the decode kernel's counters.
+// token tile, and zero the decode kernel's counters.
 struct RankRows {
   LoraArgs p;
   float* h32;         // [M][R] fp32 (at most 16 rows), or
   __half* h16;        // [M][R8] fp16, zero-padded rank
   int R8;
   int tiles, groups;  // row tiles, adapter groups per tile
-  int token_tile;     // rows of a token tile (0: no lists)
-  int token_tiles;
-  uint32_t* tile_n;   // [token_tiles] adapters of the tile
-  uint32_t* tile_ids; // [token_tiles][token_tile]
-  uint32_t* slots;    // [M] place of the row's adapter in its tile's list
+  TokenLists lists;
   uint4* zero;        // cleared by the blocks behind the lists
   int zero_vecs;
 };
 
 template <int RT, int WARPS, int U>
-__global__ void __launch_bounds__(WARPS * 32) rank_rows_kernel(const RankRows q) {
+__global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows q) {
   constexpr int RP = 8 * RT;
   extern __shared__ float red[];  // [WARPS][16][RP], then the CTA's sum [16][RP]
   __shared__ uint32_t row_id[16];
   __shared__ uint32_t list[16];
   __shared__ int list_n;
-  __shared__ uint32_t bits[kLoraMaxAdapters / 32], before[kLoraMaxAdapters / 32];
   const LoraArgs& p = q.p;
   pdl_wait();
   pdl_launch_dependents();
@@ -119,49 +65,10 @@ __global__ void __launch_bounds__(WARPS * 32) rank_rows_kernel(const RankRows q)
   if (unit >= q.tiles * q.groups) {
     if (rank != 0) return;
     const int t = unit - q.tiles * q.groups;
-    if (t >= q.token_tiles) {
+    if (t < q.lists.tiles) {
+      token_list(p, q.lists, t);
+    } else {
       for (int i = tid; i < q.zero_vecs; i += WARPS * 32) q.zero[i] = make_uint4(0u, 0u, 0u, 0u);
-      return;
-    }
-    for (int i = tid; i < (int)kLoraMaxAdapters / 32; i += WARPS * 32) bits[i] = 0u;
-    __syncthreads();
-    for (int i = tid; i < q.token_tile; i += WARPS * 32) {
-      const int64_t m = (int64_t)t * q.token_tile + i;
-      if (m < p.M) {
-        const int64_t a = adapter_of(p, m);
-        if (a >= 0) atomicOr(&bits[a / 32], 1u << (a % 32));
-      }
-    }
-    __syncthreads();
-    constexpr int kWords = (int)kLoraMaxAdapters / 32;
-    if (warp == 0) {  // a lane the bits of 4 words
-      uint32_t w[kWords / 32], n = 0;
-#pragma unroll
-      for (int i = 0; i < kWords / 32; ++i) {
-        w[i] = bits[lane * (kWords / 32) + i];
-        n += __popc(w[i]);
-      }
-      uint32_t at = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += v;
-      }
-      if (lane == 31) q.tile_n[t] = at;
-      at -= n;
-#pragma unroll
-      for (int i = 0; i < kWords / 32; ++i) {
-        before[lane * (kWords / 32) + i] = at;
-        for (uint32_t b = w[i]; b; b &= b - 1)
-          q.tile_ids[(size_t)t * q.token_tile + at++] = (uint32_t)((lane * (kWords / 32) + i) * 32 + __ffs(b) - 1);
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < q.token_tile; i += WARPS * 32) {
-      const int64_t m = (int64_t)t * q.token_tile + i;
-      if (m >= p.M) break;
-      const int64_t a = adapter_of(p, m);
-      q.slots[m] = a < 0 ? 0xFFFFFFFFu : before[a / 32] + __popc(bits[a / 32] & ((1u << (a % 32)) - 1u));
     }
     return;
   }
@@ -301,35 +208,6 @@ __global__ void __launch_bounds__(256) expand_rows_kernel(const LoraArgs p, cons
   }
 }
 
-__global__ void __launch_bounds__(kThreads) dx_rows_kernel(LoraArgs p, const float* g, __half* dx, bool add) {
-  const int64_t nb = (p.K + kThreads - 1) / kThreads;
-  const int64_t m = blockIdx.x / nb;
-  const int64_t k = (blockIdx.x % nb) * kThreads + threadIdx.x;
-  if (k >= p.K) return;
-  const int64_t a = adapter_of(p, m);
-  if (a < 0 && add) return;
-  float acc = add ? __half2float(dx[m * p.K + k]) : 0.f;
-  if (a >= 0) {
-    const __half* w = reinterpret_cast<const __half*>(p.a) + a * p.R * p.K + k;
-    for (int r = 0; r < p.R; ++r) acc += g[m * p.R + r] * __half2float(w[r * p.K]);
-  }
-  dx[m * p.K + k] = __float2half_rn(acc);
-}
-
-// out[a][r][i] (TRANS: out[a][i][r]) = sum over the adapter's rows of t[m][r] v[m][i].
-template <bool TRANS>
-__global__ void __launch_bounds__(kThreads) outer_rows_kernel(LoraArgs p, const __half* v, int64_t ld, int64_t len,
-                                                              const float* t, float* out) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int r = blockIdx.y;
-  const int64_t a = blockIdx.z;
-  if (i >= len) return;
-  float acc = 0.f;
-  for (int64_t m = 0; m < p.M; ++m)
-    if (adapter_of(p, m) == a) acc += t[m * p.R + r] * __half2float(v[m * ld + i]);
-  out[TRANS ? (a * len + i) * p.R + r : (a * p.R + r) * len + i] = acc;
-}
-
 }  // namespace
 
 namespace {
@@ -380,7 +258,7 @@ cudaError_t launch_rank_rows(RankRows& q, int sm_count, bool pdl, cudaStream_t s
     if (e != cudaSuccess) return e;
     configured_dev = dev;
   }
-  const int64_t units = (int64_t)q.tiles * q.groups + q.token_tiles + (q.zero_vecs ? 1 : 0);
+  const int64_t units = (int64_t)q.tiles * q.groups + q.lists.tiles + (q.zero_vecs ? 1 : 0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * C));
   cfg.blockDim = dim3(WARPS * 32);
@@ -413,11 +291,15 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     q.h32 = reinterpret_cast<float*>(base);
   } else {
     q.h16 = reinterpret_cast<__half*>(base);
-    q.token_tile = token_tile;
-    q.token_tiles = (int)((p.M + token_tile - 1) / token_tile);
-    q.tile_n = reinterpret_cast<uint32_t*>(base + f.second);
-    q.tile_ids = reinterpret_cast<uint32_t*>(base + f.third);
-    q.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
+    q.lists.tile = token_tile;
+    q.lists.tiles = (int)((p.M + token_tile - 1) / token_tile);
+    q.lists.n = reinterpret_cast<uint32_t*>(base + f.second);
+    q.lists.ids = reinterpret_cast<uint32_t*>(base + f.third);
+    q.lists.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
+#ifndef TILE_M
+#define TILE_M 512
+#endif
+    if (p.M >= TILE_M) return launch_lora_products(p, q.lists, q.h16, sm_count, pdl, stream);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);
@@ -473,28 +355,6 @@ cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, vo
     case 64: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<8>, p, y32, h, bi, yo, row_groups);
     default: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<0>, p, y32, h, bi, yo, row_groups);
   }
-}
-
-size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count) {
-  return (size_t)M * R * 2 * sizeof(float);
-}
-
-cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, cudaStream_t stream) {
-  float* h = (float*)ws;
-  float* gg = h + p.M * p.R;
-  const __half* x = (const __half*)p.x;
-  const __half* dy = (const __half*)g.dy;
-  if (p.M) {
-    shrink_rows_kernel<false><<<(unsigned)p.M, kThreads, 0, stream>>>(p, x, p.x_ld, p.K, (const __half*)p.a, h);
-    shrink_rows_kernel<true><<<(unsigned)p.M, kThreads, 0, stream>>>(p, dy, g.dy_ld, p.N, (const __half*)p.b, gg);
-  }
-  const unsigned kb = (unsigned)((p.K + kThreads - 1) / kThreads), nb = (unsigned)((p.N + kThreads - 1) / kThreads);
-  if (g.dx && p.M) dx_rows_kernel<<<(unsigned)(kb * p.M), kThreads, 0, stream>>>(p, gg, (__half*)g.dx, g.add_dx);
-  if (g.da && kb)
-    outer_rows_kernel<false><<<dim3(kb, p.R, (unsigned)p.L), kThreads, 0, stream>>>(p, x, p.x_ld, p.K, gg, g.da);
-  if (g.db && nb)
-    outer_rows_kernel<true><<<dim3(nb, p.R, (unsigned)p.L), kThreads, 0, stream>>>(p, dy, g.dy_ld, p.N, h, g.db);
-  return cudaGetLastError();
 }
 
 }  // namespace qw

@@ -1,0 +1,963 @@
+// qw_lora_grad.cu -- gradient of the adapters beside a projection (and the
+// rank-space product of a long forward):
+//   h = s x A^T, g = s dy B                    per row, its adapter's A, B, s
+//   dA = g^T x, dB = dy^T h                    sums over the adapter's rows
+//   dx = g A (+ dx)
+// Three launches, chained by programmatic dependent launch:
+//   plan     sorts the rows by adapter and cuts each adapter's rows into chunks;
+//   products h and g, fp32, and the largest magnitude of each per adapter
+//            (runs beside the plan until its results);
+//   sums     dA, dB and dx, a chunk of rows and 256 columns at a time.
+// x and dy are read twice, once across their width and once along their rows;
+// everything else is rank-sized.
+#include <cuda_fp16.h>
+
+#include "qw_internal.h"
+#include "qw_lora.cuh"
+#include "qw_ptx.cuh"
+
+namespace qw {
+
+namespace {
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // 0 bytes read: 16 zeros written
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
+                                                  uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+// Eight halves from any address, those at or past `n` zero.
+__device__ __forceinline__ uint4 load_halves(const __half* p, int64_t n) {
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = i < n ? __half_as_ushort(p[i]) : 0u;
+  return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+}
+
+// ---------------------------------------------------------------- products
+// v W of each row's adapter, a tile of rows at a time: out[m][r] = s sum_i
+// v[m][i] W[i][r].  HBM-bound by v (read once); mma.sync keeps up (2 R products a
+// value read, R at most 128).
+//
+// A cluster takes a tile of 64 MT rows and its CTAs split the reduction; a CTA
+// walks 64 values of it at a time, four copies deep (cp.async), and within those
+// the adapters that the tile's rows name, so v is staged once however mixed the
+// rows are.  A warp has 16 MT rows.  One whose rows all share an adapter adds
+// straight into its accumulators; another sums each adapter's 64 values apart and
+// keeps them for the rows that own it, so no row's sum ever meets another
+// adapter's values (a zero weight would not stop their infinities).  Sums over
+// the cluster go through distributed shared memory in rank order.
+constexpr int kStages = 4;
+constexpr int kProdThreads = 128;
+constexpr int kChunk = 64;  // reduction values per step
+
+struct Product {
+  const __half* v;  // [M][len], rows ld apart
+  int64_t ld, len;
+  const __half* w;  // [L][R][len], or with `trans` [L][len][R]
+  float* out32;     // [M][RP] fp32, RP the kernel's padded rank (null: out16)
+  __half* out16;    // [M][R8] fp16
+  uint32_t* amax;   // [L] largest magnitude of out32, as fp32 bits
+};
+struct Products {
+  LoraArgs p;
+  Product a, b;      // b.v null: one product
+  __half* dx_zero;   // [M][K]: rows without an adapter are cleared (nullable)
+  int R8;
+  int tiles;         // row tiles
+  TokenLists lists;  // forward
+};
+
+// Row pitch in bytes of a [64][RP] tile whose rows are the reduction (an odd number of 16-byte pieces).
+constexpr int trans_pitch(int rp) { return rp * 2 + 16; }
+template <int RT, int MT>
+struct ProdCfg {
+  static constexpr int RP = 8 * RT;
+  static constexpr int BR = 64 * MT;
+  static constexpr int V_STAGE = BR * 128;
+  static constexpr int W_STAGE = 64 * trans_pitch(RP) > RP * 128 ? 64 * trans_pitch(RP) : RP * 128;
+  static constexpr int STAGE = V_STAGE + W_STAGE;
+  static constexpr int SUMS = BR * RP * 4;
+  static constexpr int SMEM = kStages * STAGE > SUMS ? kStages * STAGE : SUMS;
+};
+
+template <int RT, int MT, bool TRANS>
+__device__ void product_tile(const Products& q, const Product& f, int tile, uint32_t rank, uint32_t C, uint8_t* smem,
+                             uint32_t* row_id, uint32_t* row_slot, uint32_t* list, uint32_t* slot_max, int* list_n) {
+  using Cfg = ProdCfg<RT, MT>;
+  constexpr int RP = Cfg::RP, BR = Cfg::BR;
+  const LoraArgs& p = q.p;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int64_t m0 = (int64_t)tile * BR;
+
+  // the tile's adapters in order of first appearance
+  for (int i = tid; i < BR; i += kProdThreads) {
+    row_id[i] = m0 + i < p.M ? (uint32_t)adapter_of(p, m0 + i) : 0xFFFFFFFFu;
+    slot_max[i] = 0u;
+  }
+  if (tid == 0) *list_n = 0;
+  __syncthreads();
+  for (int i = tid; i < BR; i += kProdThreads) {
+    const uint32_t a = row_id[i];
+    int first = i;
+    if (a != 0xFFFFFFFFu)
+      for (int k = i - 1; k >= 0; --k) first = row_id[k] == a ? k : first;
+    row_slot[i] = a == 0xFFFFFFFFu ? a : (uint32_t)first;
+  }
+  __syncthreads();
+  if (warp == 0) {  // the leaders' places, in row order
+    int n = 0;
+    for (int b = 0; b < BR; b += 32) {
+      const bool lead = row_slot[b + lane] == (uint32_t)(b + lane);
+      const uint32_t m = __ballot_sync(0xffffffffu, lead);
+      const int at = n + __popc(m & ((1u << lane) - 1u));
+      if (lead) {
+        list[at] = row_id[b + lane];
+        list[BR + b + lane] = (uint32_t)at;
+      }
+      n += __popc(m);
+    }
+    if (lane == 0) *list_n = n;
+  }
+  __syncthreads();
+  for (int i = tid; i < BR; i += kProdThreads)
+    if (row_slot[i] != 0xFFFFFFFFu) row_slot[i] = list[BR + row_slot[i]];
+  const int n = *list_n;
+  if (!TRANS && q.dx_zero) {  // rows without an adapter
+    for (int row = warp; row < BR && m0 + row < p.M; row += kProdThreads / 32) {
+      if (row_id[row] != 0xFFFFFFFFu) continue;
+      uint4* dst = reinterpret_cast<uint4*>(q.dx_zero + (m0 + row) * p.K);
+      for (int64_t c = rank * 32 + lane; c < p.K / 8; c += C * 32) dst[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  if (n == 0) {  // the whole cluster: nobody's rows
+    pdl_wait();  // a kernel behind this one counts on the plan, too
+    return;
+  }
+
+  // this warp's rows: lane / 4 and + 8 of each m tile
+  uint32_t rid[MT][2];
+  uint32_t any = 0xFFFFFFFFu;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      rid[t][h] = row_id[warp * 16 * MT + t * 16 + lane / 4 + 8 * h];
+      any = rid[t][h] < any ? rid[t][h] : any;
+    }
+  const uint32_t low = __reduce_min_sync(0xffffffffu, any);
+  bool mine = true;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) mine = mine && (rid[t][h] == low || rid[t][h] == 0xFFFFFFFFu);
+  const bool single = __all_sync(0xffffffffu, mine);
+
+  const int chunks = (int)((f.len + kChunk - 1) / kChunk);
+  const int c0 = (int)((int64_t)chunks * rank / C), c1 = (int)((int64_t)chunks * (rank + 1) / C);
+  const int steps = (c1 - c0) * n;
+  const uint32_t base = smem_u32(smem);
+  const bool v16 = f.ld % 8 == 0 && f.len % 8 == 0 && (reinterpret_cast<uintptr_t>(f.v) & 15) == 0;
+  const bool w16 = !TRANS || p.R % 8 == 0;
+  auto load = [&](int step) {
+    const int64_t i0 = (int64_t)(c0 + step / n) * kChunk;
+    const int j = step % n;
+    if (j == 0) {
+      const uint32_t dst = base + (uint32_t)((step / n) % kStages) * Cfg::STAGE;
+#pragma unroll
+      for (int k = 0; k < BR * 8 / kProdThreads; ++k) {
+        const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
+        const int64_t i = i0 + piece * 8;
+        const bool in = m0 + row < p.M && i < f.len;
+        const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
+        const uint32_t at = dst + row * 128 + ((piece ^ (row & 7)) << 4);
+        if (v16) cp_async16(at, src, in);
+        else sts16(at, load_halves(src, in ? f.len - i : 0));
+      }
+    }
+    const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
+    const __half* w = f.w + (int64_t)list[j] * p.R * f.len;
+    constexpr int kPieces = TRANS ? 64 * RT : RP * 8;
+#pragma unroll
+    for (int k = 0; k < (kPieces + kProdThreads - 1) / kProdThreads; ++k) {
+      const int e = k * kProdThreads + tid;
+      if (TRANS) {
+        const int row = e / RT, r = e % RT * 8;
+        const bool in = i0 + row < f.len && r < p.R;
+        const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
+        const uint32_t at = dst + row * trans_pitch(RP) + r * 2;
+        if (w16) cp_async16(at, src, in);
+        else sts16(at, load_halves(src, in ? p.R - r : 0));
+      } else {
+        const int r = e / 8, piece = e % 8;
+        const bool in = r < p.R && i0 + piece * 8 < f.len;
+        cp_async16(dst + r * 128 + ((piece ^ (r & 7)) << 4), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
+      }
+    }
+  };
+
+  float acc[MT][RT][4];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[t][r][0] = acc[t][r][1] = acc[t][r][2] = acc[t][r][3] = 0.f;
+  auto multiply = [&](int step, float (&d)[MT][RT][4]) {
+    const uint32_t vs = base + (uint32_t)((step / n) % kStages) * Cfg::STAGE;
+    const uint32_t ws = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t a[MT][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int row = warp * 16 * MT + t * 16 + (lane & 15), piece = kk * 2 + (lane >> 4);
+        ldmatrix_x4(vs + row * 128 + ((piece ^ (row & 7)) << 4), a[t][0], a[t][1], a[t][2], a[t][3]);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r += 2) {
+        uint32_t b[4];
+        if (TRANS) {
+          const int row = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+          ldmatrix_x4_trans(ws + row * trans_pitch(RP) + (r + (lane >> 4)) * 16, b[0], b[1], b[2], b[3]);
+        } else {
+          const int row = (r + (lane >> 4)) * 8 + (lane & 7), piece = kk * 2 + ((lane >> 3) & 1);
+          ldmatrix_x4(ws + row * 128 + ((piece ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          mma_16816(d[t][r], a[t][0], a[t][1], a[t][2], a[t][3], b[0], b[1]);
+          mma_16816(d[t][r + 1], a[t][0], a[t][1], a[t][2], a[t][3], b[2], b[3]);
+        }
+      }
+    }
+  };
+
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (s < steps) load(s);
+    cp_async_commit();
+  }
+  for (int step = 0; step < steps; ++step) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();
+    if (step + kStages - 1 < steps) load(step + kStages - 1);
+    cp_async_commit();
+    const uint32_t a = list[step % n];
+    bool own = false;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) own = own || rid[t][0] == a || rid[t][1] == a;
+    if (!__any_sync(0xffffffffu, own)) continue;
+    if (single) {
+      multiply(step, acc);
+    } else {
+      float part[MT][RT][4];
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) part[t][r][0] = part[t][r][1] = part[t][r][2] = part[t][r][3] = 0.f;
+      multiply(step, part);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][r][i] = rid[t][i / 2] == a ? acc[t][r][i] + part[t][r][i] : acc[t][r][i];
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(smem);  // [BR][RP]
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(sums + (warp * 16 * MT + t * 16 + lane / 4 + 8 * h) * RP + r * 8 + (lane % 4) * 2) =
+            make_float2(acc[t][r][2 * h], acc[t][r][2 * h + 1]);
+  if (C > 1) cluster_sync();
+  else __syncthreads();
+  pdl_wait();  // the maxima's start values are the plan's (at the forward: nothing to wait for any more)
+  for (int i = (int)rank * kProdThreads + tid; i < BR * RP / 4; i += (int)C * kProdThreads) {
+    const int row = i * 4 / RP, c = i * 4 % RP;
+    const uint32_t a = row_id[row];
+    if (a == 0xFFFFFFFFu) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t k = 0; k < C; ++k) {
+      const float4 t = ld_cluster_f32x4(sums + i * 4, k);
+      v.x += t.x;
+      v.y += t.y;
+      v.z += t.z;
+      v.w += t.w;
+    }
+    const float s = p.scales ? p.scales[a] : 1.f;
+    v.x *= s;
+    v.y *= s;
+    v.z *= s;
+    v.w *= s;
+    if (f.out32) {
+      *reinterpret_cast<float4*>(f.out32 + (m0 + row) * RP + c) = v;
+      const uint32_t b0 = __float_as_uint(fabsf(v.x)), b1 = __float_as_uint(fabsf(v.y));
+      const uint32_t b2 = __float_as_uint(fabsf(v.z)), b3 = __float_as_uint(fabsf(v.w));
+      const uint32_t lo = b0 > b1 ? b0 : b1, hi = b2 > b3 ? b2 : b3;
+      atomicMax(&slot_max[row_slot[row]], lo > hi ? lo : hi);  // a NaN is above every number
+    } else if (c < q.R8) {
+      // one rounding to fp16: the tensor cores take y's second product in fp16
+      const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(f.out16 + (m0 + row) * q.R8 + c) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+  }
+  if (f.out32) {
+    __syncthreads();
+    for (int i = tid; i < n; i += kProdThreads)
+      if (slot_max[i]) atomicMax(f.amax + list[i], slot_max[i]);
+  }
+  if (C > 1) cluster_sync();  // the peers' sums are read before they go
+}
+
+template <int RT, int MT>
+__global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Products q) {
+  constexpr int BR = ProdCfg<RT, MT>::BR;
+  extern __shared__ __align__(128) uint8_t prod_smem[];
+  __shared__ uint32_t row_id[BR], row_slot[BR], list[2 * BR], slot_max[BR];
+  __shared__ int list_n;
+  const uint32_t rank = cluster_rank(), C = cluster_size();
+  const int unit = (int)(blockIdx.x / C);
+  // The operands were there before the kernel that this launch may overlap (the
+  // plan started its dependents only once they were); a forward waits.
+  if (q.lists.tile) pdl_wait();
+  pdl_launch_dependents();
+  if (unit < q.tiles) {
+    product_tile<RT, MT, false>(q, q.a, unit, rank, C, prod_smem, row_id, row_slot, list, slot_max, &list_n);
+  } else if (q.b.v && unit < 2 * q.tiles) {
+    product_tile<RT, MT, true>(q, q.b, unit - q.tiles, rank, C, prod_smem, row_id, row_slot, list, slot_max, &list_n);
+  } else if (rank == 0) {
+    token_list(q.p, q.lists, unit - q.tiles);
+  }
+}
+
+template <int RT, int MT>
+cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
+  using Cfg = ProdCfg<RT, MT>;
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(lora_products_kernel<RT, MT>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e != cudaSuccess) return e;
+    configured_dev = dev;
+  }
+  q.tiles = (int)((q.p.M + Cfg::BR - 1) / Cfg::BR);
+  const int products = q.b.v ? 2 : 1;
+  int64_t most = (q.a.len + kChunk - 1) / kChunk;
+  if (q.b.v && (q.b.len + kChunk - 1) / kChunk > most) most = (q.b.len + kChunk - 1) / kChunk;
+  // two CTAs an SM from the clusters' splits
+  int C = most < 8 ? (int)most : 8;
+  while (C > 1 && (int64_t)products * q.tiles * C > 2 * sm_count) --C;
+  const int64_t units = (int64_t)products * q.tiles + q.lists.tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * C));
+  cfg.blockDim = dim3(kProdThreads);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, lora_products_kernel<RT, MT>, q);
+}
+
+// 128-row tiles (a W fragment serves two m tiles) once they fill the GPU; ranks
+// above 64 keep 64 rows, whose accumulators fit the registers.
+cudaError_t dispatch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
+  const bool wide = q.p.M >= 1024;
+  if (q.p.R <= 16) return wide ? launch_products<2, 2>(q, sm_count, pdl, stream) : launch_products<2, 1>(q, sm_count, pdl, stream);
+  if (q.p.R <= 32) return wide ? launch_products<4, 2>(q, sm_count, pdl, stream) : launch_products<4, 1>(q, sm_count, pdl, stream);
+  if (q.p.R <= 64) return wide ? launch_products<8, 2>(q, sm_count, pdl, stream) : launch_products<8, 1>(q, sm_count, pdl, stream);
+  return launch_products<16, 1>(q, sm_count, pdl, stream);
+}
+int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+
+// -------------------------------------------------------------------- plan
+// Rows sorted by adapter (stable) and cut into chunks.  One CTA: each warp
+// counts the adapters of its share of the rows, the counts become positions, and
+// each warp places its rows; a warp owns its counters, so nothing is atomic.
+struct Chunk {
+  int adapter, start, count;  // rows order[start .. start + count)
+  int index, of;              // which of the adapter's chunks
+  int joint, slot0;           // of an adapter of several chunks: its place among those, and its first partial sum's
+};
+struct Plan {
+  int* total;       // chunks
+  Chunk* chunks;
+  int* order;       // [M] rows by adapter
+  uint32_t* amax;   // [2][L] largest magnitude of h and g, as fp32 bits
+  uint32_t* count;  // [joint][tiles] chunks of a sum that are done
+};
+
+constexpr int kPlanThreads = 1024;
+
+__device__ int block_scan(int v, int* warp_tot) {  // exclusive prefix over the CTA
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_tot[warp] = incl;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; ++w) before += warp_tot[w];
+  return before + incl - v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs p, const Plan plan, int warps,
+                                                                 int chunk_rows, int64_t counters) {
+  extern __shared__ int hist[];  // [warps][L]
+  __shared__ int warp_tot[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int L = (int)p.L;
+  for (int i = tid; i < 2 * L; i += kPlanThreads) plan.amax[i] = 0u;
+  for (int64_t i = tid; i < counters; i += kPlanThreads) plan.count[i] = 0u;
+  for (int i = tid; i < warps * L; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  const int64_t per = ((p.M + warps - 1) / warps + 31) / 32 * 32;
+  const int64_t r0 = per * warp, r1 = r0 + per < p.M ? r0 + per : p.M;
+  int* const mine = hist + warp * L;
+  auto walk = [&](auto&& place) {
+    if (warp >= warps) return;
+    for (int64_t b = r0; b < r1; b += 32) {
+      const int64_t m = b + lane;
+      const int a = m < r1 ? (int)adapter_of(p, m) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int at = a >= 0 ? mine[a] : 0;
+      __syncwarp();
+      if (a >= 0 && rank == 0) mine[a] = at + __popc(same);
+      __syncwarp();
+      if (a >= 0) place(m, at + rank);
+    }
+  };
+  walk([](int64_t, int) {});
+  __syncthreads();
+  constexpr int kPer = (int)kLoraMaxAdapters / kPlanThreads;
+  int rows[kPer], sum = 0;
+  for (int i = 0; i < kPer; ++i) {
+    const int a = tid * kPer + i;
+    rows[i] = 0;
+    for (int w = 0; w < warps && a < L; ++w) rows[i] += hist[w * L + a];
+    sum += rows[i];
+  }
+  int start = block_scan(sum, warp_tot);
+  int cuts[kPer], n_cuts = 0, joints = 0, parts = 0;
+  for (int i = 0; i < kPer; ++i) {
+    cuts[i] = tid * kPer + i < L ? (rows[i] + chunk_rows - 1) / chunk_rows : 0;
+    if (cuts[i] == 0 && tid * kPer + i < L) cuts[i] = 1;  // an adapter without rows has zeros to write
+    n_cuts += cuts[i];
+    joints += cuts[i] > 1;
+    parts += cuts[i] > 1 ? cuts[i] : 0;
+  }
+  int chunk = block_scan(n_cuts, warp_tot);
+  int joint = block_scan(joints, warp_tot);
+  int slot = block_scan(parts, warp_tot);
+  if (tid == kPlanThreads - 1) *plan.total = chunk + n_cuts;
+  for (int i = 0; i < kPer; ++i) {
+    const int a = tid * kPer + i;
+    if (a >= L) break;
+    for (int k = 0; k < cuts[i]; ++k) {
+      const int left = rows[i] - k * chunk_rows;
+      plan.chunks[chunk++] =
+          Chunk{a, start + k * chunk_rows, left < chunk_rows ? left : chunk_rows, k, cuts[i], joint, slot};
+    }
+    joint += cuts[i] > 1;
+    slot += cuts[i] > 1 ? cuts[i] : 0;
+    for (int w = 0; w < warps; ++w) {  // counts to positions
+      const int c = hist[w * L + a];
+      hist[w * L + a] = start;
+      start += c;
+    }
+  }
+  __syncthreads();
+  walk([&](int64_t m, int at) { plan.order[at] = (int)m; });
+}
+
+// -------------------------------------------------------------------- sums
+// A chunk of an adapter's rows and 256 columns of x (dA, and dx of those rows)
+// or of dy (dB) at a time, by a persistent grid.  Rows come 64 a step by
+// cp.async, three steps deep, their h or g beside them.  Products run over rows,
+// so both operands are read through transposing ldmatrix; D is [columns][ranks].
+//
+// The tensor cores take fp16, h and g are fp32: scaled by a power of two that
+// puts the adapter's largest magnitude below 2^15, each is split into the nearest
+// fp16 and the nearest fp16 of the rest (22 bits together) and both halves are
+// multiplied, so dA and dB keep what an fp32 product would.
+//
+// A sum of several chunks is joined by the last CTA to finish one of them, from
+// fp32 partial sums in chunk order, so that results do not depend on timing.
+constexpr int kCols(int rp) { return rp > 64 ? 128 : 256; }  // columns of an item, 32 a warp
+constexpr int kRows = 64;  // rows per step
+
+struct Sums {
+  LoraArgs p;
+  const __half* dy;
+  int64_t dy_ld;
+  const float *h, *g;  // [M][RP]
+  Plan plan;
+  __half* dx;
+  float *da, *db;
+  float* part;         // [chunk of a joint sum][tiles][columns][RP]
+  bool add_dx;
+  int x_tiles, tiles;  // column tiles of x, and of x and dy together
+};
+
+template <int RT>
+struct SumCfg {
+  static constexpr int RP = 8 * RT;
+  static constexpr int COLS = kCols(RP);
+  static constexpr int THREADS = COLS;
+  static constexpr int STAGES = 3;
+  static constexpr int ROW = COLS * 2;              // bytes of a V or lora_a row, 16-byte pieces swizzled by row
+  static constexpr int V_STAGE = kRows * ROW;
+  static constexpr int G_STAGE = kRows * RP * 4;
+  static constexpr int PITCH = RP * 2 + 16;          // of the split h or g, [64][RP] fp16
+  static constexpr int OFF_G = STAGES * V_STAGE;
+  static constexpr int OFF_HI = OFF_G + 2 * G_STAGE;  // a step's is free once it is split
+  static constexpr int OFF_LO = OFF_HI + kRows * PITCH;
+  static constexpr int OFF_A = OFF_LO + kRows * PITCH;  // lora_a [RP][columns]
+  static constexpr int OFF_DX = OFF_A + RP * ROW;      // dx, [16 rows][32 columns] fp32 a warp
+  static constexpr int SMEM = OFF_DX + THREADS / 32 * 16 * 32 * 4;
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+};
+
+template <int RT>
+__global__ void __launch_bounds__(SumCfg<RT>::THREADS) lora_sums_kernel(const Sums q) {
+  using Cfg = SumCfg<RT>;
+  constexpr int RP = Cfg::RP, STAGES = Cfg::STAGES, COLS = Cfg::COLS, THREADS = Cfg::THREADS, PIECES = COLS / 8;
+  extern __shared__ __align__(128) uint8_t sum_smem[];
+  __shared__ int last;
+  const LoraArgs& p = q.p;
+  const uint32_t base = smem_u32(sum_smem);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  pdl_wait();
+  const int total = *q.plan.total;
+  const int64_t items = (int64_t)total * q.tiles;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const Chunk ck = q.plan.chunks[item / q.tiles];
+    const int tile = (int)(item % q.tiles);
+    const bool is_x = tile < q.x_tiles;
+    const int64_t col0 = (int64_t)(is_x ? tile : tile - q.x_tiles) * COLS;
+    const int64_t width = is_x ? p.K : p.N;
+    const __half* v = is_x ? reinterpret_cast<const __half*>(p.x) : q.dy;
+    const int64_t ld = is_x ? p.x_ld : q.dy_ld;
+    const float* t = is_x ? q.g : q.h;
+    float* out = is_x ? q.da : q.db;
+    const bool want_dx = is_x && q.dx;
+    if (!out && !want_dx) continue;
+    const bool v16 = ld % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(v) & 15) == 0;
+    // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
+    const uint32_t top = q.plan.amax[(is_x ? p.L : 0) + ck.adapter];
+    int e = top == 0u || top >= 0x7F800000u ? 0 : 14 - ((int)(top >> 23) - 127);
+    e = e > 126 ? 126 : (e < -126 ? -126 : e);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+
+    auto load = [&](int step) {
+      const int s = step % STAGES;
+#pragma unroll
+      for (int k = 0; k < kRows * PIECES / THREADS; ++k) {
+        const int row = (k * THREADS + tid) / PIECES, piece = tid % PIECES;
+        const int64_t c = col0 + piece * 8;
+        const bool in = step * kRows + row < ck.count && c < width;
+        const __half* src = v + (in ? q.plan.order[ck.start + step * kRows + row] * ld + c : 0);
+        const uint32_t at = base + s * Cfg::V_STAGE + row * Cfg::ROW + ((piece ^ (row & 7)) << 4);
+        if (v16) cp_async16(at, src, in);
+        else sts16(at, load_halves(src, in ? width - c : 0));
+      }
+#pragma unroll
+      for (int k = 0; k < kRows * RP / 4 / THREADS; ++k) {
+        const int i = k * THREADS + tid, row = i / (RP / 4), piece = i % (RP / 4);
+        const bool in = step * kRows + row < ck.count;
+        const float* src = t + (in ? (int64_t)q.plan.order[ck.start + step * kRows + row] * RP + piece * 4 : 0);
+        cp_async16(base + Cfg::OFF_G + (step % 2) * Cfg::G_STAGE + i * 16, src, in);
+      }
+    };
+    const int steps = (ck.count + kRows - 1) / kRows;
+    __syncthreads();  // the item before has left shared memory
+    if (want_dx) {    // with the first step's group
+#pragma unroll
+      for (int k = 0; k < RP * PIECES / THREADS; ++k) {
+        const int i = k * THREADS + tid, r = i / PIECES, piece = i % PIECES;
+        const bool in = r < p.R && col0 + piece * 8 < width;
+        const __half* src = reinterpret_cast<const __half*>(p.a) +
+                            (in ? ((int64_t)ck.adapter * p.R + r) * p.K + col0 + piece * 8 : 0);
+        cp_async16(base + Cfg::OFF_A + r * Cfg::ROW + ((piece ^ (r & 7)) << 4), src, in);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (s < steps) load(s);
+      cp_async_commit();
+    }
+    float acc[2][RT][4];  // columns 32 warp + 16 i + .., ranks
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.f;
+    for (int step = 0; step < steps; ++step) {
+      cp_async_wait<STAGES - 2>();
+      __syncthreads();
+      // split h or g
+      const uint32_t gs = base + Cfg::OFF_G + (step % 2) * Cfg::G_STAGE;
+#pragma unroll
+      for (int k = 0; k < kRows * RP / 4 / THREADS; ++k) {
+        const int i = k * THREADS + tid, row = i / (RP / 4), c = i % (RP / 4) * 4;
+        float f[4];
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                     : "r"(gs + i * 16)
+                     : "memory");
+        __half hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          f[x] *= up;
+          hi[x] = __float2half_rn(f[x]);
+          lo[x] = __float2half_rn(f[x] - __half2float(hi[x]));
+        }
+        auto pack = [](const __half (&h)[4]) {
+          return make_uint2((uint32_t)__half_as_ushort(h[0]) | ((uint32_t)__half_as_ushort(h[1]) << 16),
+                            (uint32_t)__half_as_ushort(h[2]) | ((uint32_t)__half_as_ushort(h[3]) << 16));
+        };
+        const uint2 a = pack(hi), b = pack(lo);
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + Cfg::OFF_HI + row * Cfg::PITCH + c * 2), "r"(a.x),
+                     "r"(a.y)
+                     : "memory");
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + Cfg::OFF_LO + row * Cfg::PITCH + c * 2), "r"(b.x),
+                     "r"(b.y)
+                     : "memory");
+      }
+      __syncthreads();
+      if (step + STAGES - 1 < steps) load(step + STAGES - 1);
+      cp_async_commit();
+      const uint32_t vs = base + (step % STAGES) * Cfg::V_STAGE;
+      if (out) {
+#pragma unroll
+        for (int kk = 0; kk < kRows / 16; ++kk) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // V^T: [16 columns][16 rows]
+            const int row = kk * 16 + (lane >> 4) * 8 + (lane & 7);
+            const int piece = warp * 4 + i * 2 + ((lane >> 3) & 1);
+            ldmatrix_x4_trans(vs + row * Cfg::ROW + ((piece ^ (row & 7)) << 4), a[i][0], a[i][1], a[i][2], a[i][3]);
+          }
+          const int row = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t ts = base + (half ? Cfg::OFF_LO : Cfg::OFF_HI) + row * Cfg::PITCH + (lane >> 4) * 16;
+#pragma unroll
+            for (int r = 0; r < RT; r += 2) {
+              uint32_t b[4];
+              ldmatrix_x4_trans(ts + r * 16, b[0], b[1], b[2], b[3]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                mma_16816(acc[i][r], a[i][0], a[i][1], a[i][2], a[i][3], b[0], b[1]);
+                mma_16816(acc[i][r + 1], a[i][0], a[i][1], a[i][2], a[i][3], b[2], b[3]);
+              }
+            }
+          }
+        }
+      }
+      if (want_dx) {
+        // dx of the step's rows: [64 rows][32 columns] a warp, ranks the reduction
+#pragma unroll 1
+        for (int mt = 0; mt < kRows / 16; ++mt) {
+          if (step * kRows + mt * 16 >= ck.count) break;
+          float d[4][4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) d[c][0] = d[c][1] = d[c][2] = d[c][3] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < RP / 16; ++kk) {
+            uint32_t hi[4], lo[4];
+            const uint32_t at = (uint32_t)((mt * 16 + (lane & 15)) * Cfg::PITCH + kk * 32 + (lane >> 4) * 16);
+            ldmatrix_x4(base + Cfg::OFF_HI + at, hi[0], hi[1], hi[2], hi[3]);
+            ldmatrix_x4(base + Cfg::OFF_LO + at, lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              uint32_t b[4];
+              const int r = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), piece = warp * 4 + c + (lane >> 4);
+              ldmatrix_x4_trans(base + Cfg::OFF_A + r * Cfg::ROW + ((piece ^ (r & 7)) << 4), b[0], b[1], b[2], b[3]);
+              mma_16816(d[c], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
+              mma_16816(d[c + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
+              mma_16816(d[c], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
+              mma_16816(d[c + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+            }
+          }
+          // through shared memory (this warp's 64 bytes of each row) into rows of 16-byte stores
+          float* stage = reinterpret_cast<float*>(sum_smem + Cfg::OFF_DX) + warp * 16 * 32;  // [16][32] fp32
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int row = lane / 4 + 8 * h, col = c * 8 + (lane % 4) * 2;
+              *reinterpret_cast<float2*>(stage + row * 32 + (col ^ ((row & 7) << 2))) =
+                  make_float2(d[c][2 * h] * down, d[c][2 * h + 1] * down);
+            }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int i = k * 32 + lane, row = i / 4, col = i % 4 * 8;  // 8 columns a lane
+            const int at = step * kRows + mt * 16 + row;
+            const int64_t cg = col0 + warp * 32 + col;
+            if (at < ck.count && cg < width) {
+              uint4* dst = reinterpret_cast<uint4*>(q.dx + q.plan.order[ck.start + at] * p.K + cg);
+              uint4 old = make_uint4(0u, 0u, 0u, 0u);
+              if (q.add_dx) old = *dst;
+              uint32_t* o = &old.x;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 f = *reinterpret_cast<const float2*>(stage + row * 32 + ((col + 2 * x) ^ ((row & 7) << 2)));
+                float2 s = __half22float2(*reinterpret_cast<const __half2*>(&o[x]));
+                s.x += f.x;
+                s.y += f.y;
+                const __half2 r = __floats2half2_rn(s.x, s.y);
+                o[x] = *reinterpret_cast<const uint32_t*>(&r);
+              }
+              *dst = old;
+            }
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    if (!out) continue;
+    // D[column][rank] of this chunk, then the sum's
+    auto put = [&](auto&& f) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) f(warp * 32 + i * 16 + lane / 4 + 8 * h, r * 8 + (lane % 4) * 2, acc[i][r] + 2 * h);
+    };
+    if (ck.of > 1) {
+      const int64_t sum = (int64_t)ck.joint * q.tiles + tile;
+      // slot of the adapter's first chunk; its next ones follow, q.tiles apart
+      float* slots = q.part + ((int64_t)ck.slot0 * q.tiles + tile) * COLS * RP;
+      const int64_t apart = (int64_t)q.tiles * COLS * RP;
+      put([&](int c, int r, float* a) {
+        __stcg(reinterpret_cast<float2*>(slots + ck.index * apart + c * RP + r), make_float2(a[0], a[1]));
+      });
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) last = atomicAdd(q.plan.count + sum, 1u) == (uint32_t)ck.of - 1;
+      __syncthreads();
+      if (!last) continue;
+      __threadfence();
+      put([&](int c, int r, float* a) {
+        float2 s = make_float2(0.f, 0.f);
+        for (int k = 0; k < ck.of; ++k) {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(slots + k * apart + c * RP + r));
+          s.x += x.x;
+          s.y += x.y;
+        }
+        a[0] = s.x;
+        a[1] = s.y;
+      });
+    }
+    const int64_t a0 = (int64_t)ck.adapter * p.R * width;
+    put([&](int c, int r, float* a) {
+      if (col0 + c >= width) return;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (r + x < p.R)
+          out[is_x ? a0 + (int64_t)(r + x) * width + col0 + c : a0 + (col0 + c) * p.R + r + x] = a[x] * down;
+    });
+  }
+}
+
+constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// How a gradient call is cut: chunks long enough that the column tiles alone
+// fill the GPU, shorter ones only where they would not.
+struct GradSpace {
+  int RP, x_tiles, tiles, chunk_rows;
+  int64_t max_chunks, joints;
+  size_t h, g, chunks, order, amax, count, part, end;
+};
+GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_count) {
+  GradSpace s;
+  s.RP = padded_rank(R);
+  const int cols = kCols(s.RP);
+  s.x_tiles = (int)((K + cols - 1) / cols);
+  s.tiles = s.x_tiles + (int)((N + cols - 1) / cols);
+  // about two items an SM
+  int64_t cuts = (2 * (int64_t)sm_count + s.tiles - 1) / s.tiles;
+  const int64_t most = (M + kRows - 1) / kRows;
+  cuts = cuts > most ? most : cuts;
+  cuts = cuts < 1 ? 1 : cuts;
+  s.chunk_rows = (int)(((M + cuts - 1) / cuts + kRows - 1) / kRows * kRows);
+  if (s.chunk_rows < kRows) s.chunk_rows = kRows;
+  s.max_chunks = M / s.chunk_rows + L;
+  s.joints = M / (s.chunk_rows + 1);  // adapters of more than chunk_rows rows
+  if (s.joints > L) s.joints = L;
+  const int64_t parts = s.joints ? M / s.chunk_rows + s.joints : 0;  // their chunks
+  size_t at = 256;  // the chunks' total
+  auto take = [&](size_t bytes) {
+    const size_t was = at;
+    at += align256(bytes);
+    return was;
+  };
+  s.h = take((size_t)M * s.RP * sizeof(float));
+  s.g = take((size_t)M * s.RP * sizeof(float));
+  s.chunks = take((size_t)s.max_chunks * sizeof(Chunk));
+  s.order = take((size_t)M * sizeof(int));
+  s.amax = take((size_t)2 * L * sizeof(uint32_t));
+  s.count = take((size_t)s.joints * s.tiles * sizeof(uint32_t));
+  s.part = take((size_t)parts * s.tiles * cols * s.RP * sizeof(float));
+  s.end = at;
+  return s;
+}
+
+template <int RT>
+cudaError_t launch_sums(const Sums& q, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
+  using Cfg = SumCfg<RT>;
+  static thread_local int configured_dev = -1, per_sm = 1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    cudaError_t e = cudaFuncSetAttribute(lora_sums_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e == cudaSuccess)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, lora_sums_kernel<RT>, Cfg::THREADS, Cfg::SMEM);
+    if (e != cudaSuccess) return e;
+    if (per_sm < 1) return cudaErrorInvalidConfiguration;
+    configured_dev = dev;
+  }
+  const int64_t grid = items < (int64_t)sm_count * per_sm ? items : (int64_t)sm_count * per_sm;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RT>, q);
+}
+
+}  // namespace
+
+cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, int sm_count, bool pdl,
+                                 cudaStream_t stream) {
+  Products q{};
+  q.p = p;
+  q.R8 = (p.R + 7) / 8 * 8;
+  q.a.v = static_cast<const __half*>(p.x);
+  q.a.ld = p.x_ld;
+  q.a.len = p.K;
+  q.a.w = static_cast<const __half*>(p.a);
+  q.a.out16 = static_cast<__half*>(h16);
+  q.lists = lists;
+  return dispatch_products(q, sm_count, pdl, stream);
+}
+
+size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count) {
+  return grad_space(M, N, K, (int)R, L, sm_count).end;
+}
+
+cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
+                                 cudaStream_t stream) {
+  cudaError_t e;
+  const GradSpace s = grad_space(p.M, p.N, p.K, p.R, p.L, sm_count);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  if (p.L == 0) {  // nobody has an adapter
+    return g.dx && !g.add_dx && p.M ? cudaMemsetAsync(g.dx, 0, (size_t)p.M * p.K * sizeof(__half), stream)
+                                    : cudaSuccess;
+  }
+  Plan plan;
+  plan.total = reinterpret_cast<int*>(base);
+  plan.chunks = reinterpret_cast<Chunk*>(base + s.chunks);
+  plan.order = reinterpret_cast<int*>(base + s.order);
+  plan.amax = reinterpret_cast<uint32_t*>(base + s.amax);
+  plan.count = reinterpret_cast<uint32_t*>(base + s.count);
+  {
+    // a warp's counters for every adapter; as many warps as fit 192 KB
+    int warps = (int)(192 * 1024 / (p.L * 4));
+    warps = warps > 32 ? 32 : warps;
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+      e = cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024);
+      if (e != cudaSuccess) return e;
+      configured_dev = dev;
+    }
+    lora_plan_kernel<<<1, kPlanThreads, (size_t)warps * p.L * 4, stream>>>(p, plan, warps, s.chunk_rows,
+                                                                          s.joints * s.tiles);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  if (p.M) {
+    Products q{};
+    q.p = p;
+    q.R8 = (p.R + 7) / 8 * 8;
+    q.a.v = static_cast<const __half*>(p.x);
+    q.a.ld = p.x_ld;
+    q.a.len = p.K;
+    q.a.w = static_cast<const __half*>(p.a);
+    q.a.out32 = reinterpret_cast<float*>(base + s.h);
+    q.a.amax = plan.amax;
+    q.b.v = static_cast<const __half*>(g.dy);
+    q.b.ld = g.dy_ld;
+    q.b.len = p.N;
+    q.b.w = static_cast<const __half*>(p.b);
+    q.b.out32 = reinterpret_cast<float*>(base + s.g);
+    q.b.amax = plan.amax + p.L;
+    q.dx_zero = g.add_dx ? nullptr : static_cast<__half*>(g.dx);
+    if ((e = dispatch_products(q, sm_count, pdl, stream)) != cudaSuccess) return e;
+  }
+  Sums q{};
+  q.p = p;
+  q.dy = static_cast<const __half*>(g.dy);
+  q.dy_ld = g.dy_ld;
+  q.h = reinterpret_cast<const float*>(base + s.h);
+  q.g = reinterpret_cast<const float*>(base + s.g);
+  q.plan = plan;
+  q.dx = static_cast<__half*>(g.dx);
+  q.da = g.da;
+  q.db = g.db;
+  q.part = reinterpret_cast<float*>(base + s.part);
+  q.add_dx = g.add_dx;
+  q.x_tiles = s.x_tiles;
+  q.tiles = s.tiles;
+  const int64_t items = s.max_chunks * s.tiles;
+  if (p.R <= 16) return launch_sums<2>(q, items, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_sums<4>(q, items, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_sums<8>(q, items, sm_count, pdl, stream);
+  return launch_sums<16>(q, items, sm_count, pdl, stream);
+}
+
+}  // namespace qw

@@ -41,6 +41,8 @@
 // per-element path.  Accumulation is fp32 in the tensor cores.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "qw_internal.h"
 #include "qw_ptx.cuh"
 
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
         if (!*abort_flag && !mbar_wait(&xgo[s], (parities >> s) & 1u, p.status, kDevTimeoutFull)) *abort_flag = 1;
         parities ^= 1u << s;
         // h of the tokens that take each column's adapter, at the places TMA's 128-byte swizzle gives them
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < (BT > BM ? BT / BM : 1); ++i) {
           const int t = lane_row + i * BM;
           if (t >= BT) continue;
@@ -510,61 +512,66 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
         if (p.lora.bias && row_ok) bias = __half2float(reinterpret_cast<const __half*>(p.lora.bias)[row]);
         bad = blocks > p.groups && bad_rows[(tile_count & 1) * BM + quarter * 32 + lane];
       }
+      auto store_tile = [&](auto with_bad) {
 #pragma unroll 1
-      for (int cb = khalf * (BT / 32); cb < (khalf + 1) * (BT / 32); ++cb) {
-        uint32_t v[16];
-        tmem_ld_32x32b_x16(tmem + lane_base + D_COL + cb * 16, v);
-        tmem_wait_ld();
-        if (p.swiglu) {
-          // lane l < 16 finishes tokens 0-7 of the block and lane l + 16
-          // tokens 8-15: each sends its partner the half the partner needs
-          float g[8], u[8];
+        for (int cb = khalf * (BT / 32); cb < (khalf + 1) * (BT / 32); ++cb) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(tmem + lane_base + D_COL + cb * 16, v);
+          tmem_wait_ld();
+          if (p.swiglu) {
+            // lane l < 16 finishes tokens 0-7 of the block and lane l + 16
+            // tokens 8-15: each sends its partner the half the partner needs
+            float g[8], u[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float mine_lo = __uint_as_float(v[q]), mine_hi = __uint_as_float(v[q + 8]);
-            const float other = __shfl_xor_sync(0xffffffffu, up_lane ? mine_lo : mine_hi, 16);
-            g[q] = up_lane ? other : mine_lo;
-            u[q] = up_lane ? mine_hi : other;
+            for (int q = 0; q < 8; ++q) {
+              const float mine_lo = __uint_as_float(v[q]), mine_hi = __uint_as_float(v[q + 8]);
+              const float other = __shfl_xor_sync(0xffffffffu, up_lane ? mine_lo : mine_hi, 16);
+              g[q] = up_lane ? other : mine_lo;
+              u[q] = up_lane ? mine_hi : other;
+            }
+            if (!row_ok || *abort_flag) continue;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int tok = mt * BT + cb * 16 + (up_lane ? 8 : 0) + q;
+              if (tok < p.M) {
+                const size_t idx = (size_t)tok * p.N + row;
+                const float h = swiglu_f16(g[q], u[q]);
+                if (p.y_f32) reinterpret_cast<float*>(p.y)[idx] = h;
+                else reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(h);
+              }
+            }
+            continue;
           }
           if (!row_ok || *abort_flag) continue;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int tok = mt * BT + cb * 16 + (up_lane ? 8 : 0) + q;
+          for (int q = 0; q < 16; ++q) {
+            const int tok = mt * BT + cb * 16 + q;
             if (tok < p.M) {
               const size_t idx = (size_t)tok * p.N + row;
-              const float h = swiglu_f16(g[q], u[q]);
-              if (p.y_f32) reinterpret_cast<float*>(p.y)[idx] = h;
-              else reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(h);
-            }
-          }
-          continue;
-        }
-        if (!row_ok || *abort_flag) continue;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int tok = mt * BT + cb * 16 + q;
-          if (tok < p.M) {
-            const size_t idx = (size_t)tok * p.N + row;
-            float f = __uint_as_float(v[q]);
-            if constexpr (LORA) {
-              f += bias;
-              if (bad) {  // the non-finite terms of this token's own adapter
-                const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
-                const __half* h = reinterpret_cast<const __half*>(p.lora.h) + (size_t)tok * 8 * p.lora_r8;
-                const __half* b = reinterpret_cast<const __half*>(p.lora.b) + ((size_t)a * p.N + row) * p.lora.R;
-                for (int r = 0; a < (uint32_t)p.lora.L && r < p.lora.R; ++r) {
-                  const float bv = __half2float(b[r]);
-                  if (!isfinite(bv)) f += __half2float(h[r]) * bv;
+              float f = __uint_as_float(v[q]);
+              if constexpr (LORA) {
+                f += bias;
+                if (decltype(with_bad)::value && bad) {  // the non-finite terms of this token's own adapter
+                  const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
+                  const __half* h = reinterpret_cast<const __half*>(p.lora.h) + (size_t)tok * 8 * p.lora_r8;
+                  const __half* b = reinterpret_cast<const __half*>(p.lora.b) + ((size_t)a * p.N + row) * p.lora.R;
+                  for (int r = 0; a < (uint32_t)p.lora.L && r < p.lora.R; ++r) {
+                    const float bv = __half2float(b[r]);
+                    if (!isfinite(bv)) f += __half2float(h[r]) * bv;
+                  }
                 }
+                reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
+                continue;
               }
-              reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
-              continue;
+              if (p.y_f32) reinterpret_cast<float*>(p.y)[idx] = f;
+              else reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
             }
-            if (p.y_f32) reinterpret_cast<float*>(p.y)[idx] = f;
-            else reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
           }
         }
-      }
+      };
+      // a branch an element for the rare case would cost the whole epilogue (2048 x 17408 x 5120: 45 us of 499)
+      if (LORA && __any_sync(0xffffffffu, bad)) store_tile(std::true_type{});
+      else store_tile(std::false_type{});
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dempty);
