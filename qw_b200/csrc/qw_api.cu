@@ -1265,7 +1265,7 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
   const bool pdl = pdl_enabled();
   sa.status = res->status;
   // The decode kernel's counters are cleared by the first launch.
-  ce = launch_lora_rank(la, token_tile, lws, workspace, skinny ? skinny_zeroed_bytes(sa) : 0,
+  ce = launch_lora_rank(la, token_tile, lws, workspace, skinny ? skinny_zeroed_bytes(sa) : 0, res->status,
                         device_info(dev).sm_count, pdl, stream);
   if (ce != cudaSuccess) return cuda_fail(ce, "adapter launch");
   if (sa.M <= 16) {
@@ -1347,7 +1347,11 @@ int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora
   const int sms = device_info(dev).sm_count;
   if ((rc = check_workspace(workspace, workspace_bytes, lora_backward_bytes(M, N, K, la.R, la.L, sms)))) return rc;
   la.x = x->data;
+  DeviceRes* res = nullptr;
+  std::string err;
+  if (!device_res(dev, &res, &err)) return fail(QW_ENOMEM, err);
   LoraGrads g{};
+  g.status = res->status;
   g.dy = dy->data;
   g.dy_ld = N;
   g.dx = dx ? dx->data : nullptr;

@@ -48,27 +48,49 @@ __device__ __forceinline__ uint4 load_halves(const __half* p, int64_t n) {
   return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
+// ------------------------------------------------------- tensor-core operands
+// Shared-memory operands of tcgen05.mma, all with the 128-byte swizzle: rows of
+// 128 bytes (64 halves), 16-byte piece q of row i at place q ^ (i & 7), eight rows
+// to an atom of 1024 bytes.
+//   along K: the rows are the operand's M or N and hold 64 k; a step of 16 k is 32
+//            bytes further on.
+//   along MN: the rows are k and hold 64 of M or N, the next 64 are `next` bytes
+//            away; a step of 16 k is 16 rows further on.
+__device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint64_t operand_k(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t operand_mn(uint32_t addr, uint32_t next) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16, D fp32, A and B fp16 (each along K, or along MN), M x N.
+constexpr uint32_t mma_desc(int m, int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
 // ---------------------------------------------------------------- products
-// v W of each row's adapter, a tile of rows at a time: out[m][r] = s sum_i
-// v[m][i] W[i][r].  HBM-bound by v (read once); mma.sync keeps up (2 R products a
-// value read, R at most 128).
+// v W of each row's adapter, a tile of 128 rows at a time: out[m][r] = s sum_i
+// v[m][i] W[i][r].  HBM-bound by v, which is read once.
 //
-// A cluster takes a tile of 64 MT rows and its CTAs split the reduction; a CTA
-// walks 64 values of it at a time, four copies deep (cp.async), and within those
-// the adapters that the tile's rows name, so v is staged once however mixed the
-// rows are.  A warp has 16 MT rows.  One whose rows all share an adapter adds
-// straight into its accumulators; another sums each adapter's 64 values apart and
-// keeps them for the rows that own it, so no row's sum ever meets another
-// adapter's values (a zero weight would not stop their infinities).  Sums over
-// the cluster go through distributed shared memory in rank order.
+// A cluster takes a tile and its CTAs split the reduction; a CTA walks 64 values
+// of it at a time, four copies deep (cp.async), and within those the adapters
+// that the tile's rows name, so v is staged once however mixed the rows are.
+// Every adapter has columns of its own in TMEM (four adapters at a time, two
+// above rank 64) and a row reads those of its own adapter: no row's sum ever
+// meets another adapter's values.  Sums over the cluster go through distributed
+// shared memory in rank order.
 constexpr int kStages = 4;
 constexpr int kProdThreads = 128;
 constexpr int kChunk = 64;  // reduction values per step
+constexpr int kTileRows = 128;
 
 struct Product {
   const __half* v;  // [M][len], rows ld apart
   int64_t ld, len;
-  const __half* w;  // [L][R][len], or with `trans` [L][len][R]
+  const __half* w;  // [L][R][len], or for the second product [L][len][R]
   float* out32;     // [M][RP] fp32, RP the kernel's padded rank (null: out16)
   __half* out16;    // [M][R8] fp16
   uint32_t* amax;   // [L] largest magnitude of out32, as fp32 bits
@@ -80,66 +102,72 @@ struct Products {
   int R8;
   int tiles;         // row tiles
   TokenLists lists;  // forward
+  unsigned int* status;
 };
 
-// Row pitch in bytes of a [64][RP] tile whose rows are the reduction (an odd number of 16-byte pieces).
-constexpr int trans_pitch(int rp) { return rp * 2 + 16; }
-template <int RT, int MT>
+template <int RP>
 struct ProdCfg {
-  static constexpr int RP = 8 * RT;
-  static constexpr int BR = 64 * MT;
-  static constexpr int V_STAGE = BR * 128;
-  static constexpr int W_STAGE = 64 * trans_pitch(RP) > RP * 128 ? 64 * trans_pitch(RP) : RP * 128;
+  static constexpr int BLOCK = RP > 64 ? 128 : 64;    // TMEM columns of an adapter
+  static constexpr int COLUMNS = 256;                 // two CTAs an SM
+  static constexpr int GROUP = COLUMNS / BLOCK;       // adapters at a time
+  static constexpr int V_STAGE = kTileRows * 128;
+  static constexpr int W_STAGE = 64 * BLOCK * 2;
   static constexpr int STAGE = V_STAGE + W_STAGE;
-  static constexpr int SUMS = BR * RP * 4;
-  static constexpr int SMEM = kStages * STAGE > SUMS ? kStages * STAGE : SUMS;
+  static constexpr int PITCH = RP + 4;                // floats of a row of sums
+  static constexpr int SUMS = kTileRows * PITCH * 4;
+  static constexpr int SMEM = (kStages * STAGE > SUMS ? kStages * STAGE : SUMS) + 1024;
+  static_assert(SMEM <= (RP > 64 ? 224 : 112) * 1024, "two CTAs an SM up to rank 64");
 };
 
-template <int RT, int MT, bool TRANS>
+struct ProdShared {
+  uint32_t row_id[kTileRows], row_slot[kTileRows], list[2 * kTileRows], slot_max[kTileRows];
+  uint64_t done[kStages];
+  int list_n;
+  uint32_t tmem;
+};
+
+template <int RP, bool TRANS>
 __device__ void product_tile(const Products& q, const Product& f, int tile, uint32_t rank, uint32_t C, uint8_t* smem,
-                             uint32_t* row_id, uint32_t* row_slot, uint32_t* list, uint32_t* slot_max, int* list_n) {
-  using Cfg = ProdCfg<RT, MT>;
-  constexpr int RP = Cfg::RP, BR = Cfg::BR;
+                             ProdShared& sh) {
+  using Cfg = ProdCfg<RP>;
   const LoraArgs& p = q.p;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int64_t m0 = (int64_t)tile * BR;
+  const int64_t m0 = (int64_t)tile * kTileRows;
 
-  // the tile's adapters in order of first appearance
-  for (int i = tid; i < BR; i += kProdThreads) {
-    row_id[i] = m0 + i < p.M ? (uint32_t)adapter_of(p, m0 + i) : 0xFFFFFFFFu;
-    slot_max[i] = 0u;
-  }
-  if (tid == 0) *list_n = 0;
+  // the tile's adapters in order of first appearance, and each row's place among them
+  sh.row_id[tid] = m0 + tid < p.M ? (uint32_t)adapter_of(p, m0 + tid) : 0xFFFFFFFFu;
+  sh.slot_max[tid] = 0u;
   __syncthreads();
-  for (int i = tid; i < BR; i += kProdThreads) {
-    const uint32_t a = row_id[i];
-    int first = i;
-    if (a != 0xFFFFFFFFu)
-      for (int k = i - 1; k >= 0; --k) first = row_id[k] == a ? k : first;
-    row_slot[i] = a == 0xFFFFFFFFu ? a : (uint32_t)first;
-  }
-  __syncthreads();
-  if (warp == 0) {  // the leaders' places, in row order
-    int n = 0;
-    for (int b = 0; b < BR; b += 32) {
-      const bool lead = row_slot[b + lane] == (uint32_t)(b + lane);
-      const uint32_t m = __ballot_sync(0xffffffffu, lead);
-      const int at = n + __popc(m & ((1u << lane) - 1u));
-      if (lead) {
-        list[at] = row_id[b + lane];
-        list[BR + b + lane] = (uint32_t)at;
-      }
-      n += __popc(m);
+  const uint32_t my_id = sh.row_id[tid];
+  {
+    const uint4* ids = reinterpret_cast<const uint4*>(sh.row_id);
+    int first = tid;
+    for (int k = tid / 4; k >= 0; --k) {  // four rows at a time, downwards
+      const uint4 w = ids[k];
+      first = w.w == my_id && 4 * k + 3 < first ? 4 * k + 3 : first;
+      first = w.z == my_id && 4 * k + 2 < first ? 4 * k + 2 : first;
+      first = w.y == my_id && 4 * k + 1 < first ? 4 * k + 1 : first;
+      first = w.x == my_id && 4 * k < first ? 4 * k : first;
     }
-    if (lane == 0) *list_n = n;
+    const bool lead = my_id != 0xFFFFFFFFu && first == tid;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, lead);
+    if (lane == 0) sh.row_slot[warp] = __popc(leaders);
+    __syncthreads();
+    int at = __popc(leaders & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) at += (int)sh.row_slot[w];
+    if (tid == kProdThreads - 1) sh.list_n = at + lead;
+    if (lead) {
+      sh.list[at] = my_id;
+      sh.list[kTileRows + tid] = (uint32_t)at;
+    }
+    __syncthreads();
+    sh.row_slot[tid] = my_id == 0xFFFFFFFFu ? my_id : sh.list[kTileRows + first];
   }
-  __syncthreads();
-  for (int i = tid; i < BR; i += kProdThreads)
-    if (row_slot[i] != 0xFFFFFFFFu) row_slot[i] = list[BR + row_slot[i]];
-  const int n = *list_n;
+  const int n = sh.list_n;
+  const int my_slot = (int)sh.row_slot[tid];  // -1: none
   if (!TRANS && q.dx_zero) {  // rows without an adapter
-    for (int row = warp; row < BR && m0 + row < p.M; row += kProdThreads / 32) {
-      if (row_id[row] != 0xFFFFFFFFu) continue;
+    for (int row = warp; row < kTileRows && m0 + row < p.M; row += kProdThreads / 32) {
+      if (sh.row_id[row] != 0xFFFFFFFFu) continue;
       uint4* dst = reinterpret_cast<uint4*>(q.dx_zero + (m0 + row) * p.K);
       for (int64_t c = rank * 32 + lane; c < p.K / 8; c += C * 32) dst[c] = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -149,220 +177,205 @@ __device__ void product_tile(const Products& q, const Product& f, int tile, uint
     return;
   }
 
-  // this warp's rows: lane / 4 and + 8 of each m tile
-  uint32_t rid[MT][2];
-  uint32_t any = 0xFFFFFFFFu;
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      rid[t][h] = row_id[warp * 16 * MT + t * 16 + lane / 4 + 8 * h];
-      any = rid[t][h] < any ? rid[t][h] : any;
-    }
-  const uint32_t low = __reduce_min_sync(0xffffffffu, any);
-  bool mine = true;
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) mine = mine && (rid[t][h] == low || rid[t][h] == 0xFFFFFFFFu);
-  const bool single = __all_sync(0xffffffffu, mine);
-
   const int chunks = (int)((f.len + kChunk - 1) / kChunk);
   const int c0 = (int)((int64_t)chunks * rank / C), c1 = (int)((int64_t)chunks * (rank + 1) / C);
-  const int steps = (c1 - c0) * n;
   const uint32_t base = smem_u32(smem);
   const bool v16 = f.ld % 8 == 0 && f.len % 8 == 0 && (reinterpret_cast<uintptr_t>(f.v) & 15) == 0;
   const bool w16 = !TRANS || p.R % 8 == 0;
-  auto load = [&](int step) {
-    const int64_t i0 = (int64_t)(c0 + step / n) * kChunk;
-    const int j = step % n;
-    if (j == 0) {
-      const uint32_t dst = base + (uint32_t)((step / n) % kStages) * Cfg::STAGE;
-#pragma unroll
-      for (int k = 0; k < BR * 8 / kProdThreads; ++k) {
-        const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
-        const int64_t i = i0 + piece * 8;
-        const bool in = m0 + row < p.M && i < f.len;
-        const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
-        const uint32_t at = dst + row * 128 + ((piece ^ (row & 7)) << 4);
-        if (v16) cp_async16(at, src, in);
-        else sts16(at, load_halves(src, in ? f.len - i : 0));
-      }
-    }
-    const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
-    const __half* w = f.w + (int64_t)list[j] * p.R * f.len;
-    constexpr int kPieces = TRANS ? 64 * RT : RP * 8;
-#pragma unroll
-    for (int k = 0; k < (kPieces + kProdThreads - 1) / kProdThreads; ++k) {
-      const int e = k * kProdThreads + tid;
-      if (TRANS) {
-        const int row = e / RT, r = e % RT * 8;
-        const bool in = i0 + row < f.len && r < p.R;
-        const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
-        const uint32_t at = dst + row * trans_pitch(RP) + r * 2;
-        if (w16) cp_async16(at, src, in);
-        else sts16(at, load_halves(src, in ? p.R - r : 0));
-      } else {
-        const int r = e / 8, piece = e % 8;
-        const bool in = r < p.R && i0 + piece * 8 < f.len;
-        cp_async16(dst + r * 128 + ((piece ^ (r & 7)) << 4), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
-      }
-    }
+  bool ok = true;        // a bounded wait that ran out: go on without waiting
+  uint32_t parities = 0; // of done[i], a bit each: flips with every use waited for
+  auto wait_step = [&](int step) {
+    const int i = step % kStages;
+    ok = ok && mbar_wait(&sh.done[i], (parities >> i) & 1u, q.status, kDevTimeoutAccum);
+    parities ^= 1u << i;
   };
 
-  float acc[MT][RT][4];
+  for (int j0 = 0; j0 < n; j0 += Cfg::GROUP) {
+    const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
+    const int steps = (c1 - c0) * nj;
+    auto load = [&](int step) {
+      const int64_t i0 = (int64_t)(c0 + step / nj) * kChunk;
+      const int j = step % nj;
+      if (j == 0) {
+        const uint32_t dst = base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE;
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < RT; ++r) acc[t][r][0] = acc[t][r][1] = acc[t][r][2] = acc[t][r][3] = 0.f;
-  auto multiply = [&](int step, float (&d)[MT][RT][4]) {
-    const uint32_t vs = base + (uint32_t)((step / n) % kStages) * Cfg::STAGE;
-    const uint32_t ws = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t a[MT][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row = warp * 16 * MT + t * 16 + (lane & 15), piece = kk * 2 + (lane >> 4);
-        ldmatrix_x4(vs + row * 128 + ((piece ^ (row & 7)) << 4), a[t][0], a[t][1], a[t][2], a[t][3]);
+        for (int k = 0; k < kTileRows * 8 / kProdThreads; ++k) {
+          const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
+          const int64_t i = i0 + piece * 8;
+          const bool in = m0 + row < p.M && i < f.len;
+          const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
+          const uint32_t at = dst + swizzled(row, piece);
+          if (v16) cp_async16(at, src, in);
+          else sts16(at, load_halves(src, in ? f.len - i : 0));
+        }
       }
+      const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
+      const __half* w = f.w + (int64_t)sh.list[j0 + j] * p.R * f.len;
+      constexpr int kPieces = 8 * RP;
 #pragma unroll
-      for (int r = 0; r < RT; r += 2) {
-        uint32_t b[4];
+      for (int k = 0; k < kPieces / kProdThreads; ++k) {
+        const int e = k * kProdThreads + tid;
         if (TRANS) {
-          const int row = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-          ldmatrix_x4_trans(ws + row * trans_pitch(RP) + (r + (lane >> 4)) * 16, b[0], b[1], b[2], b[3]);
+          const int row = e / (RP / 8), r = e % (RP / 8) * 8;
+          const bool in = i0 + row < f.len && r < p.R;
+          const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
+          const uint32_t at = dst + (r / 64) * 8192 + swizzled(row, r % 64 / 8);
+          if (w16) cp_async16(at, src, in);
+          else sts16(at, load_halves(src, in ? p.R - r : 0));
         } else {
-          const int row = (r + (lane >> 4)) * 8 + (lane & 7), piece = kk * 2 + ((lane >> 3) & 1);
-          ldmatrix_x4(ws + row * 128 + ((piece ^ (row & 7)) << 4), b[0], b[1], b[2], b[3]);
+          const int r = e / 8, piece = e % 8;
+          const bool in = r < p.R && i0 + piece * 8 < f.len;
+          cp_async16(dst + swizzled(r, piece), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
         }
+      }
+    };
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          mma_16816(d[t][r], a[t][0], a[t][1], a[t][2], a[t][3], b[0], b[1]);
-          mma_16816(d[t][r + 1], a[t][0], a[t][1], a[t][2], a[t][3], b[2], b[3]);
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (s < steps) load(s);
+      cp_async_commit();
+    }
+    for (int step = 0; step < steps; ++step) {
+      cp_async_wait<kStages - 2>();
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (tid == 0) {
+        tc_fence_after();
+        const int chunk = step / nj, j = step % nj;
+        const uint64_t a = operand_k(base + (uint32_t)(chunk % kStages) * Cfg::STAGE);
+        const uint32_t ws = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
+        const uint64_t b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
+        constexpr uint32_t kDesc = mma_desc(kTileRows, TRANS ? Cfg::BLOCK : RP, false, TRANS);
+#pragma unroll
+        for (int kk = 0; kk < kChunk / 16; ++kk)
+          tc_mma_ss(sh.tmem + j * Cfg::BLOCK, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
+                    chunk > 0 || kk > 0);
+        tc_commit(&sh.done[step % kStages]);
+      }
+      // the products that read the stage loaded next are the previous step's
+      if (step > 0) wait_step(step - 1);
+      if (step + kStages - 1 < steps) load(step + kStages - 1);
+      cp_async_commit();
+    }
+    if (steps > 0) wait_step(steps - 1);
+    tc_fence_after();
+    cp_async_wait<0>();
+    __syncthreads();
+
+    // each row's own columns, to shared memory
+    float* const sums = reinterpret_cast<float*>(smem);
+    for (int b = 0; b < nj; ++b) {
+      const bool own = my_slot == j0 + b;
+      if (!__any_sync(0xffffffffu, own)) continue;
+#pragma unroll
+      for (int c = 0; c < RP; c += 16) {
+        uint32_t v[16];
+        if (steps > 0) {
+          tmem_ld_32x32b_x16(sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::BLOCK + c, v);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0u;  // this CTA has no part of the reduction
+        }
+        if (own) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(sums + tid * Cfg::PITCH + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
     }
-  };
-
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (s < steps) load(s);
-    cp_async_commit();
-  }
-  for (int step = 0; step < steps; ++step) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    if (step + kStages - 1 < steps) load(step + kStages - 1);
-    cp_async_commit();
-    const uint32_t a = list[step % n];
-    bool own = false;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) own = own || rid[t][0] == a || rid[t][1] == a;
-    if (!__any_sync(0xffffffffu, own)) continue;
-    if (single) {
-      multiply(step, acc);
-    } else {
-      float part[MT][RT][4];
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) part[t][r][0] = part[t][r][1] = part[t][r][2] = part[t][r][3] = 0.f;
-      multiply(step, part);
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][r][i] = rid[t][i / 2] == a ? acc[t][r][i] + part[t][r][i] : acc[t][r][i];
+    tc_fence_before();
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    pdl_wait();  // the maxima's start values are the plan's (a forward has waited)
+    for (int i = (int)rank * kProdThreads + tid; i < kTileRows * RP / 4; i += (int)C * kProdThreads) {
+      const int row = i / (RP / 4), c = i % (RP / 4) * 4;
+      const int slot = (int)sh.row_slot[row];
+      if (slot < j0 || slot >= j0 + nj) continue;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t k = 0; k < C; ++k) {
+        const float4 t = ld_cluster_f32x4(sums + row * Cfg::PITCH + c, k);
+        v.x += t.x;
+        v.y += t.y;
+        v.z += t.z;
+        v.w += t.w;
+      }
+      const float s = p.scales ? p.scales[sh.row_id[row]] : 1.f;
+      v.x *= s;
+      v.y *= s;
+      v.z *= s;
+      v.w *= s;
+      if (f.out32) {
+        *reinterpret_cast<float4*>(f.out32 + (m0 + row) * RP + c) = v;
+        const uint32_t b0 = __float_as_uint(fabsf(v.x)), b1 = __float_as_uint(fabsf(v.y));
+        const uint32_t b2 = __float_as_uint(fabsf(v.z)), b3 = __float_as_uint(fabsf(v.w));
+        const uint32_t lo = b0 > b1 ? b0 : b1, hi = b2 > b3 ? b2 : b3;
+        atomicMax(&sh.slot_max[slot], lo > hi ? lo : hi);  // a NaN is above every number
+      } else if (c < q.R8) {
+        // one rounding to fp16: the tensor cores take y's second product in fp16
+        const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(f.out16 + (m0 + row) * q.R8 + c) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      }
     }
+    if (C > 1) cluster_sync();  // the peers' sums are read before they change or go
+    else __syncthreads();
   }
-  cp_async_wait<0>();
-  __syncthreads();
-  float* sums = reinterpret_cast<float*>(smem);  // [BR][RP]
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(sums + (warp * 16 * MT + t * 16 + lane / 4 + 8 * h) * RP + r * 8 + (lane % 4) * 2) =
-            make_float2(acc[t][r][2 * h], acc[t][r][2 * h + 1]);
-  if (C > 1) cluster_sync();
-  else __syncthreads();
-  pdl_wait();  // the maxima's start values are the plan's (at the forward: nothing to wait for any more)
-  for (int i = (int)rank * kProdThreads + tid; i < BR * RP / 4; i += (int)C * kProdThreads) {
-    const int row = i * 4 / RP, c = i * 4 % RP;
-    const uint32_t a = row_id[row];
-    if (a == 0xFFFFFFFFu) continue;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t k = 0; k < C; ++k) {
-      const float4 t = ld_cluster_f32x4(sums + i * 4, k);
-      v.x += t.x;
-      v.y += t.y;
-      v.z += t.z;
-      v.w += t.w;
-    }
-    const float s = p.scales ? p.scales[a] : 1.f;
-    v.x *= s;
-    v.y *= s;
-    v.z *= s;
-    v.w *= s;
-    if (f.out32) {
-      *reinterpret_cast<float4*>(f.out32 + (m0 + row) * RP + c) = v;
-      const uint32_t b0 = __float_as_uint(fabsf(v.x)), b1 = __float_as_uint(fabsf(v.y));
-      const uint32_t b2 = __float_as_uint(fabsf(v.z)), b3 = __float_as_uint(fabsf(v.w));
-      const uint32_t lo = b0 > b1 ? b0 : b1, hi = b2 > b3 ? b2 : b3;
-      atomicMax(&slot_max[row_slot[row]], lo > hi ? lo : hi);  // a NaN is above every number
-    } else if (c < q.R8) {
-      // one rounding to fp16: the tensor cores take y's second product in fp16
-      const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
-      *reinterpret_cast<uint2*>(f.out16 + (m0 + row) * q.R8 + c) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    }
-  }
-  if (f.out32) {
-    __syncthreads();
+  if (f.out32)
     for (int i = tid; i < n; i += kProdThreads)
-      if (slot_max[i]) atomicMax(f.amax + list[i], slot_max[i]);
-  }
-  if (C > 1) cluster_sync();  // the peers' sums are read before they go
+      if (sh.slot_max[i]) atomicMax(f.amax + sh.list[i], sh.slot_max[i]);
 }
 
-template <int RT, int MT>
+template <int RP>
 __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Products q) {
-  constexpr int BR = ProdCfg<RT, MT>::BR;
-  extern __shared__ __align__(128) uint8_t prod_smem[];
-  __shared__ uint32_t row_id[BR], row_slot[BR], list[2 * BR], slot_max[BR];
-  __shared__ int list_n;
+  extern __shared__ uint8_t prod_smem[];
+  __shared__ __align__(16) ProdShared sh;
+  uint8_t* smem = prod_smem + ((1024u - (smem_u32(prod_smem) & 1023u)) & 1023u);
   const uint32_t rank = cluster_rank(), C = cluster_size();
   const int unit = (int)(blockIdx.x / C);
   // The operands were there before the kernel that this launch may overlap (the
   // plan started its dependents only once they were); a forward waits.
   if (q.lists.tile) pdl_wait();
   pdl_launch_dependents();
-  if (unit < q.tiles) {
-    product_tile<RT, MT, false>(q, q.a, unit, rank, C, prod_smem, row_id, row_slot, list, slot_max, &list_n);
-  } else if (q.b.v && unit < 2 * q.tiles) {
-    product_tile<RT, MT, true>(q, q.b, unit - q.tiles, rank, C, prod_smem, row_id, row_slot, list, slot_max, &list_n);
-  } else if (rank == 0) {
-    token_list(q.p, q.lists, unit - q.tiles);
+  const bool first = unit < q.tiles, second = !first && q.b.v && unit < 2 * q.tiles;
+  if (!first && !second) {
+    if (rank == 0) token_list(q.p, q.lists, unit - q.tiles);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&sh.done[i], 1);
+    fence_barrier_init();
+  }
+  if (threadIdx.x < 32) {
+    tmem_alloc(&sh.tmem, ProdCfg<RP>::COLUMNS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (first) product_tile<RP, false>(q, q.a, unit, rank, C, smem, sh);
+  else product_tile<RP, true>(q, q.b, unit - q.tiles, rank, C, smem, sh);
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    tc_fence_after();
+    tmem_dealloc(sh.tmem, ProdCfg<RP>::COLUMNS);
   }
 }
 
-template <int RT, int MT>
+template <int RP>
 cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
-  using Cfg = ProdCfg<RT, MT>;
+  using Cfg = ProdCfg<RP>;
   static thread_local int configured_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev != dev) {
-    const cudaError_t e = cudaFuncSetAttribute(lora_products_kernel<RT, MT>,
+    const cudaError_t e = cudaFuncSetAttribute(lora_products_kernel<RP>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
     if (e != cudaSuccess) return e;
     configured_dev = dev;
   }
-  q.tiles = (int)((q.p.M + Cfg::BR - 1) / Cfg::BR);
+  q.tiles = (int)((q.p.M + kTileRows - 1) / kTileRows);
   const int products = q.b.v ? 2 : 1;
   int64_t most = (q.a.len + kChunk - 1) / kChunk;
   if (q.b.v && (q.b.len + kChunk - 1) / kChunk > most) most = (q.b.len + kChunk - 1) / kChunk;
@@ -384,17 +397,14 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, lora_products_kernel<RT, MT>, q);
+  return cudaLaunchKernelEx(&cfg, lora_products_kernel<RP>, q);
 }
 
-// 128-row tiles (a W fragment serves two m tiles) once they fill the GPU; ranks
-// above 64 keep 64 rows, whose accumulators fit the registers.
 cudaError_t dispatch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
-  const bool wide = q.p.M >= 1024;
-  if (q.p.R <= 16) return wide ? launch_products<2, 2>(q, sm_count, pdl, stream) : launch_products<2, 1>(q, sm_count, pdl, stream);
-  if (q.p.R <= 32) return wide ? launch_products<4, 2>(q, sm_count, pdl, stream) : launch_products<4, 1>(q, sm_count, pdl, stream);
-  if (q.p.R <= 64) return wide ? launch_products<8, 2>(q, sm_count, pdl, stream) : launch_products<8, 1>(q, sm_count, pdl, stream);
-  return launch_products<16, 1>(q, sm_count, pdl, stream);
+  if (q.p.R <= 16) return launch_products<16>(q, sm_count, pdl, stream);
+  if (q.p.R <= 32) return launch_products<32>(q, sm_count, pdl, stream);
+  if (q.p.R <= 64) return launch_products<64>(q, sm_count, pdl, stream);
+  return launch_products<128>(q, sm_count, pdl, stream);
 }
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
@@ -871,8 +881,8 @@ cudaError_t launch_sums(const Sums& q, int64_t items, int sm_count, bool pdl, cu
 
 }  // namespace
 
-cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, int sm_count, bool pdl,
-                                 cudaStream_t stream) {
+cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, unsigned int* status,
+                                 int sm_count, bool pdl, cudaStream_t stream) {
   Products q{};
   q.p = p;
   q.R8 = (p.R + 7) / 8 * 8;
@@ -882,6 +892,7 @@ cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, voi
   q.a.w = static_cast<const __half*>(p.a);
   q.a.out16 = static_cast<__half*>(h16);
   q.lists = lists;
+  q.status = status;
   return dispatch_products(q, sm_count, pdl, stream);
 }
 
@@ -936,6 +947,7 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
     q.b.w = static_cast<const __half*>(p.b);
     q.b.out32 = reinterpret_cast<float*>(base + s.g);
     q.b.amax = plan.amax + p.L;
+    q.status = g.status;
     q.dx_zero = g.add_dx ? nullptr : static_cast<__half*>(g.dx);
     if ((e = dispatch_products(q, sm_count, pdl, stream)) != cudaSuccess) return e;
   }
