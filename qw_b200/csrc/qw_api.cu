@@ -1266,8 +1266,8 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
   sa.status = res->status;
   // The decode kernel's counters are cleared by the first launch.
   ce = launch_lora_rank(la, token_tile, lws, workspace, skinny ? skinny_zeroed_bytes(sa) : 0, res->status,
-                        device_info(dev).sm_count, pdl, stream);
-  if (ce != cudaSuccess) return cuda_fail(ce, "adapter launch");
+                        device_info(dev).sm_count, pdl, stream, &err);
+  if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "adapter launch") : fail(QW_ECUDA, err);
   if (sa.M <= 16) {
     sa.y = lora_forward_product(la, lws);
     sa.y_f32 = true;
@@ -1358,8 +1358,9 @@ int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora
   g.add_dx = accumulate_dx != 0;
   g.da = da ? static_cast<float*>(da->data) : nullptr;
   g.db = db ? static_cast<float*>(db->data) : nullptr;
-  const cudaError_t ce = launch_lora_backward(la, g, workspace, sms, pdl_enabled(), as_stream(stream_v));
-  return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter gradient launch");
+  const cudaError_t ce = launch_lora_backward(la, g, workspace, sms, pdl_enabled(), as_stream(stream_v), &err);
+  if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "adapter gradient launch") : fail(QW_ECUDA, err);
+  return QW_OK;
 }
 
 // ------------------------------------------------------ distillation

@@ -219,7 +219,7 @@ size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile);
 // h = s x A^T into the workspace, with the token tiles' adapter lists where
 // token_tile != 0, and `zero_bytes` (rounded up to 16) at `zero` cleared.
 cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes,
-                             unsigned int* status, int sm_count, bool pdl, cudaStream_t stream);
+                             unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err);
 // fp32 [M][N] within the workspace of at most 16 rows: the projection's product.
 float* lora_forward_product(const LoraArgs& p, void* ws);
 cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, bool pdl, cudaStream_t stream);
@@ -227,10 +227,10 @@ cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, vo
 PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias);
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);
 cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
-                                 cudaStream_t stream);
+                                 cudaStream_t stream, std::string* err);
 // h = s x A^T in fp16 [M][R8] and the token tiles' lists, for a long forward.
 cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, unsigned int* status,
-                                 int sm_count, bool pdl, cudaStream_t stream);
+                                 int sm_count, bool pdl, cudaStream_t stream, std::string* err);
 
 // Distillation from a teacher's top logits (qw_distill.cu).
 struct DistillArgs {

@@ -281,7 +281,7 @@ cudaError_t launch_rank_rows(RankRows& q, int sm_count, bool pdl, cudaStream_t s
 size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile) { return forward_space(M, N, R, token_tile).end; }
 
 cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes,
-                             unsigned int* status, int sm_count, bool pdl, cudaStream_t stream) {
+                             unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
   const ForwardSpace f = forward_space(p.M, p.N, p.R, token_tile);
   uint8_t* base = static_cast<uint8_t*>(ws);
   RankRows q{};
@@ -299,7 +299,7 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
 #ifndef TILE_M
 #define TILE_M 512
 #endif
-    if (p.M >= TILE_M) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream);
+    if (p.M >= TILE_M) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);

@@ -12,6 +12,8 @@
 // everything else is rank-sized.
 #include <cuda_fp16.h>
 
+#include <cstring>
+
 #include "qw_internal.h"
 #include "qw_lora.cuh"
 #include "qw_ptx.cuh"
@@ -76,8 +78,11 @@ constexpr uint32_t mma_desc(int m, int n, bool a_mn, bool b_mn) {
 // v[m][i] W[i][r].  HBM-bound by v, which is read once.
 //
 // A cluster takes a tile and its CTAs split the reduction; a CTA walks 64 values
-// of it at a time, four copies deep (cp.async), and within those the adapters
-// that the tile's rows name, so v is staged once however mixed the rows are.
+// of it at a time, four TMA loads deep, and within those the adapters that the
+// tile's rows name, so v is staged once however mixed the rows are.  Rows or
+// weights that TMA cannot take (dy of a width, or lora_b of a rank, that is no
+// multiple of 8) are copied by the threads instead; that path pays a proxy fence
+// a step, which waits for every copy in flight.
 // Every adapter has columns of its own in TMEM (four adapters at a time, two
 // above rank 64) and a row reads those of its own adapter: no row's sum ever
 // meets another adapter's values.  Sums over the cluster go through distributed
@@ -101,6 +106,7 @@ struct Products {
   __half* dx_zero;   // [M][K]: rows without an adapter are cleared (nullable)
   int R8;
   int tiles;         // row tiles
+  int b_tma;         // TMA can take the second product's operands
   TokenLists lists;  // forward
   unsigned int* status;
 };
@@ -119,16 +125,19 @@ struct ProdCfg {
   static_assert(SMEM <= (RP > 64 ? 224 : 112) * 1024, "two CTAs an SM up to rank 64");
 };
 
+struct ProductMaps {
+  CUtensorMap av, aw, bv, bw;  // operands of the two products: v [M][len], w 3-D
+};
 struct ProdShared {
   uint32_t row_id[kTileRows], row_slot[kTileRows], list[2 * kTileRows], slot_max[kTileRows];
-  uint64_t done[kStages];
+  uint64_t full[kStages], done[kStages];
   int list_n;
   uint32_t tmem;
 };
 
-template <int RP, bool TRANS>
-__device__ void product_tile(const Products& q, const Product& f, int tile, uint32_t rank, uint32_t C, uint8_t* smem,
-                             ProdShared& sh) {
+template <int RP, bool TRANS, bool TMA>
+__device__ void product_tile(const Products& q, const Product& f, const CUtensorMap* map_v, const CUtensorMap* map_w,
+                             int tile, uint32_t rank, uint32_t C, uint8_t* smem, ProdShared& sh) {
   using Cfg = ProdCfg<RP>;
   const LoraArgs& p = q.p;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -183,7 +192,16 @@ __device__ void product_tile(const Products& q, const Product& f, int tile, uint
   const bool v16 = f.ld % 8 == 0 && f.len % 8 == 0 && (reinterpret_cast<uintptr_t>(f.v) & 15) == 0;
   const bool w16 = !TRANS || p.R % 8 == 0;
   bool ok = true;        // a bounded wait that ran out: go on without waiting
-  uint32_t parities = 0; // of done[i], a bit each: flips with every use waited for
+  uint32_t it0 = 0, vit0 = 0;  // TMA: steps and chunks of earlier rounds
+  constexpr uint32_t kDesc = mma_desc(kTileRows, TRANS ? Cfg::BLOCK : RP, false, TRANS);
+  auto multiply = [&](int chunk, int j, uint32_t vs, uint32_t ws) {
+    const uint64_t a = operand_k(vs), b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
+#pragma unroll
+    for (int kk = 0; kk < kChunk / 16; ++kk)
+      tc_mma_ss(sh.tmem + j * Cfg::BLOCK, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
+                chunk > 0 || kk > 0);
+  };
+  uint32_t parities = 0; // copies: of done[i], a bit each: flips with every use waited for
   auto wait_step = [&](int step) {
     const int i = step % kStages;
     ok = ok && mbar_wait(&sh.done[i], (parities >> i) & 1u, q.status, kDevTimeoutAccum);
@@ -193,71 +211,109 @@ __device__ void product_tile(const Products& q, const Product& f, int tile, uint
   for (int j0 = 0; j0 < n; j0 += Cfg::GROUP) {
     const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
     const int steps = (c1 - c0) * nj;
-    auto load = [&](int step) {
-      const int64_t i0 = (int64_t)(c0 + step / nj) * kChunk;
-      const int j = step % nj;
-      if (j == 0) {
-        const uint32_t dst = base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE;
-#pragma unroll
-        for (int k = 0; k < kTileRows * 8 / kProdThreads; ++k) {
-          const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
-          const int64_t i = i0 + piece * 8;
-          const bool in = m0 + row < p.M && i < f.len;
-          const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
-          const uint32_t at = dst + swizzled(row, piece);
-          if (v16) cp_async16(at, src, in);
-          else sts16(at, load_halves(src, in ? f.len - i : 0));
+    if constexpr (TMA) {
+      if (warp == 1 && lane == 0) {  // loads
+        uint32_t it = it0, vit = vit0;
+        for (int c = c0; c < c1; ++c, ++vit) {
+          for (int j = 0; j < nj; ++j, ++it) {
+            const uint32_t s = it % kStages;
+            if (it >= kStages)
+              ok = ok && mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
+            mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) + (TRANS ? Cfg::W_STAGE : RP * 128)));
+            if (j == 0)
+              tma_load_2d(smem + (vit % kStages) * Cfg::STAGE, map_v, &sh.full[s], c * kChunk, (int)m0);
+            uint8_t* dst = smem + s * Cfg::STAGE + Cfg::V_STAGE;
+            const int a = (int)sh.list[j0 + j];
+            if (TRANS) {
+              for (int b = 0; b < Cfg::BLOCK / 64; ++b)
+                tma_load_3d(dst + b * 8192, map_w, &sh.full[s], b * 64, c * kChunk, a);
+            } else {
+              tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
+            }
+          }
+        }
+      } else if (warp == 0 && lane == 0) {  // products
+        uint32_t it = it0, vit = vit0;
+        for (int c = c0; c < c1; ++c, ++vit) {
+          for (int j = 0; j < nj; ++j, ++it) {
+            const uint32_t s = it % kStages;
+            ok = ok && mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
+            tc_fence_after();
+            multiply(c - c0, j, base + (vit % kStages) * Cfg::STAGE, base + s * Cfg::STAGE + Cfg::V_STAGE);
+            tc_commit(&sh.done[s]);
+          }
         }
       }
-      const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
-      const __half* w = f.w + (int64_t)sh.list[j0 + j] * p.R * f.len;
-      constexpr int kPieces = 8 * RP;
+      it0 += (uint32_t)steps;
+      vit0 += (uint32_t)(c1 - c0);
+      __syncwarp();
+      // The last step's barrier has seen every earlier use waited for by the
+      // thread that loads, but for those of the last turn of the ring, which
+      // complete in order.
+      if (steps > 0) {
+        __syncthreads();
+        ok = ok && mbar_wait(&sh.done[(it0 - 1) % kStages], ((it0 - 1) / kStages) & 1, q.status, kDevTimeoutAccum);
+      }
+    } else {
+      auto load = [&](int step) {
+        const int64_t i0 = (int64_t)(c0 + step / nj) * kChunk;
+        const int j = step % nj;
+        if (j == 0) {
+          const uint32_t dst = base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE;
 #pragma unroll
-      for (int k = 0; k < kPieces / kProdThreads; ++k) {
-        const int e = k * kProdThreads + tid;
-        if (TRANS) {
-          const int row = e / (RP / 8), r = e % (RP / 8) * 8;
-          const bool in = i0 + row < f.len && r < p.R;
-          const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
-          const uint32_t at = dst + (r / 64) * 8192 + swizzled(row, r % 64 / 8);
-          if (w16) cp_async16(at, src, in);
-          else sts16(at, load_halves(src, in ? p.R - r : 0));
-        } else {
-          const int r = e / 8, piece = e % 8;
-          const bool in = r < p.R && i0 + piece * 8 < f.len;
-          cp_async16(dst + swizzled(r, piece), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
+          for (int k = 0; k < kTileRows * 8 / kProdThreads; ++k) {
+            const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
+            const int64_t i = i0 + piece * 8;
+            const bool in = m0 + row < p.M && i < f.len;
+            const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
+            const uint32_t at = dst + swizzled(row, piece);
+            if (v16) cp_async16(at, src, in);
+            else sts16(at, load_halves(src, in ? f.len - i : 0));
+          }
         }
-      }
-    };
+        const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
+        const __half* w = f.w + (int64_t)sh.list[j0 + j] * p.R * f.len;
+        constexpr int kPieces = 8 * RP;
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      if (s < steps) load(s);
-      cp_async_commit();
-    }
-    for (int step = 0; step < steps; ++step) {
-      cp_async_wait<kStages - 2>();
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tc_fence_after();
-        const int chunk = step / nj, j = step % nj;
-        const uint64_t a = operand_k(base + (uint32_t)(chunk % kStages) * Cfg::STAGE);
-        const uint32_t ws = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
-        const uint64_t b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
-        constexpr uint32_t kDesc = mma_desc(kTileRows, TRANS ? Cfg::BLOCK : RP, false, TRANS);
+        for (int k = 0; k < kPieces / kProdThreads; ++k) {
+          const int e = k * kProdThreads + tid;
+          if (TRANS) {
+            const int row = e / (RP / 8), r = e % (RP / 8) * 8;
+            const bool in = i0 + row < f.len && r < p.R;
+            const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
+            const uint32_t at = dst + (r / 64) * 8192 + swizzled(row, r % 64 / 8);
+            if (w16) cp_async16(at, src, in);
+            else sts16(at, load_halves(src, in ? p.R - r : 0));
+          } else {
+            const int r = e / 8, piece = e % 8;
+            const bool in = r < p.R && i0 + piece * 8 < f.len;
+            cp_async16(dst + swizzled(r, piece), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
+          }
+        }
+      };
 #pragma unroll
-        for (int kk = 0; kk < kChunk / 16; ++kk)
-          tc_mma_ss(sh.tmem + j * Cfg::BLOCK, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
-                    chunk > 0 || kk > 0);
-        tc_commit(&sh.done[step % kStages]);
+      for (int s = 0; s < kStages - 1; ++s) {
+        if (s < steps) load(s);
+        cp_async_commit();
       }
-      // the products that read the stage loaded next are the previous step's
-      if (step > 0) wait_step(step - 1);
-      if (step + kStages - 1 < steps) load(step + kStages - 1);
-      cp_async_commit();
+      for (int step = 0; step < steps; ++step) {
+        cp_async_wait<kStages - 2>();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          multiply(step / nj, step % nj, base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE,
+                   base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE);
+          tc_commit(&sh.done[step % kStages]);
+        }
+        // the products that read the stage loaded next are the previous step's
+        if (step > 0) wait_step(step - 1);
+        if (step + kStages - 1 < steps) load(step + kStages - 1);
+        cp_async_commit();
+      }
+      if (steps > 0) wait_step(steps - 1);
     }
-    if (steps > 0) wait_step(steps - 1);
     tc_fence_after();
     cp_async_wait<0>();
     __syncthreads();
@@ -318,6 +374,7 @@ __device__ void product_tile(const Products& q, const Product& f, int tile, uint
             make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
       }
     }
+    fence_proxy_async_smem();   // TMA writes there next
     if (C > 1) cluster_sync();  // the peers' sums are read before they change or go
     else __syncthreads();
   }
@@ -327,7 +384,8 @@ __device__ void product_tile(const Products& q, const Product& f, int tile, uint
 }
 
 template <int RP>
-__global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Products q) {
+__global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const __grid_constant__ Products q,
+                                                                     const __grid_constant__ ProductMaps maps) {
   extern __shared__ uint8_t prod_smem[];
   __shared__ __align__(16) ProdShared sh;
   uint8_t* smem = prod_smem + ((1024u - (smem_u32(prod_smem) & 1023u)) & 1023u);
@@ -343,7 +401,10 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Produ
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&sh.done[i], 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.done[i], 1);
+    }
     fence_barrier_init();
   }
   if (threadIdx.x < 32) {
@@ -353,8 +414,13 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Produ
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (first) product_tile<RP, false>(q, q.a, unit, rank, C, smem, sh);
-  else product_tile<RP, true>(q, q.b, unit - q.tiles, rank, C, smem, sh);
+  if (first) {
+    product_tile<RP, false, true>(q, q.a, &maps.av, &maps.aw, unit, rank, C, smem, sh);
+  } else if (q.b_tma) {
+    product_tile<RP, true, true>(q, q.b, &maps.bv, &maps.bw, unit - q.tiles, rank, C, smem, sh);
+  } else {
+    product_tile<RP, true, false>(q, q.b, nullptr, nullptr, unit - q.tiles, rank, C, smem, sh);
+  }
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -364,7 +430,7 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const Produ
 }
 
 template <int RP>
-cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
+cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
   using Cfg = ProdCfg<RP>;
   static thread_local int configured_dev = -1;
   int dev = 0;
@@ -376,6 +442,30 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
     configured_dev = dev;
   }
   q.tiles = (int)((q.p.M + kTileRows - 1) / kTileRows);
+  const LoraArgs& p = q.p;
+  ProductMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  {
+    const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.R, (uint64_t)p.L};
+    const uint64_t strides[2] = {(uint64_t)p.K * 2, (uint64_t)p.K * p.R * 2};
+    const uint32_t box[3] = {kChunk, RP, 1};
+    if (!encode_tmap_2d(&maps.av, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, q.a.v, (uint64_t)p.K, (uint64_t)p.M,
+                        (uint64_t)q.a.ld * 2, kChunk, kTileRows, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
+        !encode_tmap_3d(&maps.aw, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, q.a.w, dims, strides, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B, err))
+      return cudaErrorInvalidValue;
+  }
+  q.b_tma = q.b.v && q.b.ld % 8 == 0 && reinterpret_cast<uintptr_t>(q.b.v) % 16 == 0 && p.R % 8 == 0;
+  if (q.b_tma) {
+    const uint64_t dims[3] = {(uint64_t)p.R, (uint64_t)p.N, (uint64_t)p.L};
+    const uint64_t strides[2] = {(uint64_t)p.R * 2, (uint64_t)p.R * p.N * 2};
+    const uint32_t box[3] = {64, kChunk, 1};
+    if (!encode_tmap_2d(&maps.bv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, q.b.v, (uint64_t)p.N, (uint64_t)p.M,
+                        (uint64_t)q.b.ld * 2, kChunk, kTileRows, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
+        !encode_tmap_3d(&maps.bw, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, q.b.w, dims, strides, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B, err))
+      return cudaErrorInvalidValue;
+  }
   const int products = q.b.v ? 2 : 1;
   int64_t most = (q.a.len + kChunk - 1) / kChunk;
   if (q.b.v && (q.b.len + kChunk - 1) / kChunk > most) most = (q.b.len + kChunk - 1) / kChunk;
@@ -397,14 +487,14 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, lora_products_kernel<RP>, q);
+  return cudaLaunchKernelEx(&cfg, lora_products_kernel<RP>, q, maps);
 }
 
-cudaError_t dispatch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream) {
-  if (q.p.R <= 16) return launch_products<16>(q, sm_count, pdl, stream);
-  if (q.p.R <= 32) return launch_products<32>(q, sm_count, pdl, stream);
-  if (q.p.R <= 64) return launch_products<64>(q, sm_count, pdl, stream);
-  return launch_products<128>(q, sm_count, pdl, stream);
+cudaError_t dispatch_products(Products& q, int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
+  if (q.p.R <= 16) return launch_products<16>(q, sm_count, pdl, stream, err);
+  if (q.p.R <= 32) return launch_products<32>(q, sm_count, pdl, stream, err);
+  if (q.p.R <= 64) return launch_products<64>(q, sm_count, pdl, stream, err);
+  return launch_products<128>(q, sm_count, pdl, stream, err);
 }
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
@@ -882,7 +972,7 @@ cudaError_t launch_sums(const Sums& q, int64_t items, int sm_count, bool pdl, cu
 }  // namespace
 
 cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, unsigned int* status,
-                                 int sm_count, bool pdl, cudaStream_t stream) {
+                                 int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
   Products q{};
   q.p = p;
   q.R8 = (p.R + 7) / 8 * 8;
@@ -893,7 +983,7 @@ cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, voi
   q.a.out16 = static_cast<__half*>(h16);
   q.lists = lists;
   q.status = status;
-  return dispatch_products(q, sm_count, pdl, stream);
+  return dispatch_products(q, sm_count, pdl, stream, err);
 }
 
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count) {
@@ -901,7 +991,7 @@ size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L
 }
 
 cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
-                                 cudaStream_t stream) {
+                                 cudaStream_t stream, std::string* err) {
   cudaError_t e;
   const GradSpace s = grad_space(p.M, p.N, p.K, p.R, p.L, sm_count);
   uint8_t* base = static_cast<uint8_t*>(ws);
@@ -949,7 +1039,7 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
     q.b.amax = plan.amax + p.L;
     q.status = g.status;
     q.dx_zero = g.add_dx ? nullptr : static_cast<__half*>(g.dx);
-    if ((e = dispatch_products(q, sm_count, pdl, stream)) != cudaSuccess) return e;
+    if ((e = dispatch_products(q, sm_count, pdl, stream, err)) != cudaSuccess) return e;
   }
   Sums q{};
   q.p = p;
