@@ -7,7 +7,7 @@
 //   plan     sorts the rows by adapter and cuts each adapter's rows into chunks;
 //   products h and g, fp32, and the largest magnitude of each per adapter
 //            (runs beside the plan until its results);
-//   sums     dA, dB and dx, a chunk of rows and 256 columns at a time.
+//   sums     dA, dB and dx, a chunk of rows and 128 columns at a time.
 // x and dy are read twice, once across their width and once along their rows;
 // everything else is rank-sized.
 #include <cuda_fp16.h>
@@ -30,13 +30,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                                  uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr)
-               : "memory");
 }
 __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
@@ -606,10 +599,16 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
 }
 
 // -------------------------------------------------------------------- sums
-// A chunk of an adapter's rows and 256 columns of x (dA, and dx of those rows)
-// or of dy (dB) at a time, by a persistent grid.  Rows come 64 a step by
-// cp.async, three steps deep, their h or g beside them.  Products run over rows,
-// so both operands are read through transposing ldmatrix; D is [columns][ranks].
+// A chunk of an adapter's rows and 128 columns of x (dA, and dx of those rows)
+// or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step:
+//   warp 8      gathers the step's rows of x or dy (TMA, four rows an instruction),
+//               and an item's lora_a columns;
+//   warps 0-7   split the step's h or g for the tensor cores (below), and while
+//               those multiply take the step before's dx from TMEM to memory;
+//   warp 9      issues tcgen05.mma: D[columns][ranks] += v^T (h or g), both
+//               operands along MN since the rows are the reduction, and
+//               dx[rows][columns] = g A into one of two TMEM buffers.
+// HBM-bound by x and dy; at rank 64 the products take about half that time.
 //
 // The tensor cores take fp16, h and g are fp32: scaled by a power of two that
 // puts the adapter's largest magnitude below 2^15, each is split into the nearest
@@ -618,8 +617,11 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
 //
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
-constexpr int kCols(int rp) { return rp > 64 ? 128 : 256; }  // columns of an item, 32 a warp
-constexpr int kRows = 64;  // rows per step
+constexpr int kCols = 128;
+constexpr int kStepRows = 128;
+constexpr int kWorkers = 256;
+constexpr int kSumThreads = kWorkers + 64;
+constexpr int kVStages = 3;
 
 struct Sums {
   LoraArgs p;
@@ -629,272 +631,411 @@ struct Sums {
   Plan plan;
   __half* dx;
   float *da, *db;
-  float* part;         // [chunk of a joint sum][tiles][columns][RP]
+  float* part;         // [chunk of a joint sum][tiles][RP][kCols]
   bool add_dx;
   int x_tiles, tiles;  // column tiles of x, and of x and dy together
+  int dy_tma;          // TMA can take dy's rows
+  unsigned int* status;
+};
+struct SumMaps {
+  CUtensorMap x, dy, a;  // rows of x and dy (one row of 64 columns a box), lora_a 3-D
 };
 
-template <int RT>
+template <int RP>
 struct SumCfg {
-  static constexpr int RP = 8 * RT;
-  static constexpr int COLS = kCols(RP);
-  static constexpr int THREADS = COLS;
-  static constexpr int STAGES = 3;
-  static constexpr int ROW = COLS * 2;              // bytes of a V or lora_a row, 16-byte pieces swizzled by row
-  static constexpr int V_STAGE = kRows * ROW;
-  static constexpr int G_STAGE = kRows * RP * 4;
-  static constexpr int PITCH = RP * 2 + 16;          // of the split h or g, [64][RP] fp16
-  static constexpr int OFF_G = STAGES * V_STAGE;
-  static constexpr int OFF_HI = OFF_G + 2 * G_STAGE;  // a step's is free once it is split
-  static constexpr int OFF_LO = OFF_HI + kRows * PITCH;
-  static constexpr int OFF_A = OFF_LO + kRows * PITCH;  // lora_a [RP][columns]
-  static constexpr int OFF_DX = OFF_A + RP * ROW;      // dx, [16 rows][32 columns] fp32 a warp
-  static constexpr int SMEM = OFF_DX + THREADS / 32 * 16 * 32 * 4;
-  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  static constexpr int NRANK = RP > 64 ? 128 : 64;               // ranks of a D, whole 128-byte rows
+  static constexpr int V_STAGE = kStepRows * kCols * 2;          // two blocks of 64 columns
+  static constexpr int G_HALF = kStepRows * NRANK * 2;           // high or low halves, blocks of 64 ranks
+  static constexpr int G_BUFS = RP > 64 ? 1 : 2;
+  static constexpr int OFF_G = kVStages * V_STAGE;
+  static constexpr int OFF_A = OFF_G + G_BUFS * 2 * G_HALF;      // lora_a: two blocks of [RP][64 columns]
+  static constexpr int SMEM = OFF_A + RP * kCols * 2 + 1024;
+  static constexpr int PER = RP / 8;                             // float4 of h or g per worker and step
+  static_assert(SMEM <= 226 * 1024, "shared memory budget");
 };
 
-template <int RT>
-__global__ void __launch_bounds__(SumCfg<RT>::THREADS) lora_sums_kernel(const Sums q) {
-  using Cfg = SumCfg<RT>;
-  constexpr int RP = Cfg::RP, STAGES = Cfg::STAGES, COLS = Cfg::COLS, THREADS = Cfg::THREADS, PIECES = COLS / 8;
-  extern __shared__ __align__(128) uint8_t sum_smem[];
-  __shared__ int last;
-  const LoraArgs& p = q.p;
-  const uint32_t base = smem_u32(sum_smem);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  pdl_wait();
-  const int total = *q.plan.total;
-  const int64_t items = (int64_t)total * q.tiles;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Chunk ck = q.plan.chunks[item / q.tiles];
-    const int tile = (int)(item % q.tiles);
-    const bool is_x = tile < q.x_tiles;
-    const int64_t col0 = (int64_t)(is_x ? tile : tile - q.x_tiles) * COLS;
-    const int64_t width = is_x ? p.K : p.N;
-    const __half* v = is_x ? reinterpret_cast<const __half*>(p.x) : q.dy;
-    const int64_t ld = is_x ? p.x_ld : q.dy_ld;
-    const float* t = is_x ? q.g : q.h;
-    float* out = is_x ? q.da : q.db;
-    const bool want_dx = is_x && q.dx;
-    if (!out && !want_dx) continue;
-    const bool v16 = ld % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(v) & 15) == 0;
-    // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
-    const uint32_t top = q.plan.amax[(is_x ? p.L : 0) + ck.adapter];
-    int e = top == 0u || top >= 0x7F800000u ? 0 : 14 - ((int)(top >> 23) - 127);
-    e = e > 126 ? 126 : (e < -126 ? -126 : e);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+struct SumShared {
+  uint64_t vfull[kVStages], vempty[kVStages], gfull[2], gempty[2], dxfull[2], dxempty[2];
+  uint64_t accfull, accempty, afull, aempty;
+  uint32_t tmem;
+  int last;
+};
 
-    auto load = [&](int step) {
-      const int s = step % STAGES;
-#pragma unroll
-      for (int k = 0; k < kRows * PIECES / THREADS; ++k) {
-        const int row = (k * THREADS + tid) / PIECES, piece = tid % PIECES;
-        const int64_t c = col0 + piece * 8;
-        const bool in = step * kRows + row < ck.count && c < width;
-        const __half* src = v + (in ? q.plan.order[ck.start + step * kRows + row] * ld + c : 0);
-        const uint32_t at = base + s * Cfg::V_STAGE + row * Cfg::ROW + ((piece ^ (row & 7)) << 4);
-        if (v16) cp_async16(at, src, in);
-        else sts16(at, load_halves(src, in ? width - c : 0));
-      }
-#pragma unroll
-      for (int k = 0; k < kRows * RP / 4 / THREADS; ++k) {
-        const int i = k * THREADS + tid, row = i / (RP / 4), piece = i % (RP / 4);
-        const bool in = step * kRows + row < ck.count;
-        const float* src = t + (in ? (int64_t)q.plan.order[ck.start + step * kRows + row] * RP + piece * 4 : 0);
-        cp_async16(base + Cfg::OFF_G + (step % 2) * Cfg::G_STAGE + i * 16, src, in);
-      }
-    };
-    const int steps = (ck.count + kRows - 1) / kRows;
-    __syncthreads();  // the item before has left shared memory
-    if (want_dx) {    // with the first step's group
-#pragma unroll
-      for (int k = 0; k < RP * PIECES / THREADS; ++k) {
-        const int i = k * THREADS + tid, r = i / PIECES, piece = i % PIECES;
-        const bool in = r < p.R && col0 + piece * 8 < width;
-        const __half* src = reinterpret_cast<const __half*>(p.a) +
-                            (in ? ((int64_t)ck.adapter * p.R + r) * p.K + col0 + piece * 8 : 0);
-        cp_async16(base + Cfg::OFF_A + r * Cfg::ROW + ((piece ^ (r & 7)) << 4), src, in);
-      }
+// Four rows of 64 columns from column c, one under the other.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c, const int (&r)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
+      "%6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      : "memory");
+}
+__device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
+
+// One item of the persistent loop.
+struct Item {
+  Chunk ck;
+  int tile, steps;
+  bool is_x, sum, dx;  // columns of x; dA or dB wanted; dx wanted
+  int64_t col0, width;
+};
+__device__ __forceinline__ Item item_at(const Sums& q, int64_t i) {
+  Item t;
+  t.ck = q.plan.chunks[i / q.tiles];
+  t.tile = (int)(i % q.tiles);
+  t.is_x = t.tile < q.x_tiles;
+  t.col0 = (int64_t)(t.is_x ? t.tile : t.tile - q.x_tiles) * kCols;
+  t.width = t.is_x ? q.p.K : q.p.N;
+  t.sum = t.is_x ? q.da != nullptr : q.db != nullptr;
+  t.dx = t.is_x && q.dx != nullptr;
+  t.steps = t.sum || t.dx ? (t.ck.count + kStepRows - 1) / kStepRows : 0;
+  return t;
+}
+
+template <int RP>
+__global__ void __launch_bounds__(kSumThreads, 1)
+    lora_sums_kernel(const __grid_constant__ Sums q, const __grid_constant__ SumMaps maps) {
+  using Cfg = SumCfg<RP>;
+  extern __shared__ uint8_t sum_smem[];
+  __shared__ SumShared sh;
+  uint8_t* smem = sum_smem + ((1024u - (smem_u32(sum_smem) & 1023u)) & 1023u);
+  const uint32_t base = smem_u32(smem);
+  const LoraArgs& p = q.p;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  if (tid == 0) {
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(&sh.vfull[i], 1);
+      mbar_init(&sh.vempty[i], 1);
     }
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-      if (s < steps) load(s);
-      cp_async_commit();
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.gfull[i], kWorkers / 32);
+      mbar_init(&sh.gempty[i], 1);
+      mbar_init(&sh.dxfull[i], 1);
+      mbar_init(&sh.dxempty[i], kWorkers / 32);
     }
-    float acc[2][RT][4];  // columns 32 warp + 16 i + .., ranks
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.f;
-    for (int step = 0; step < steps; ++step) {
-      cp_async_wait<STAGES - 2>();
-      __syncthreads();
-      // split h or g
-      const uint32_t gs = base + Cfg::OFF_G + (step % 2) * Cfg::G_STAGE;
-#pragma unroll
-      for (int k = 0; k < kRows * RP / 4 / THREADS; ++k) {
-        const int i = k * THREADS + tid, row = i / (RP / 4), c = i % (RP / 4) * 4;
-        float f[4];
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
-                     : "r"(gs + i * 16)
-                     : "memory");
-        __half hi[4], lo[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          f[x] *= up;
-          hi[x] = __float2half_rn(f[x]);
-          lo[x] = __float2half_rn(f[x] - __half2float(hi[x]));
+    mbar_init(&sh.accfull, 1);
+    mbar_init(&sh.accempty, kWorkers / 32);
+    mbar_init(&sh.afull, 1);
+    mbar_init(&sh.aempty, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  // ranks past RP of the split h and g stay zero
+  if (RP < 64 && warp < 8)
+    for (int i = tid; i < Cfg::G_BUFS * 2 * Cfg::G_HALF / 16; i += kWorkers)
+      sts16(base + Cfg::OFF_G + i * 16, make_uint4(0u, 0u, 0u, 0u));
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  constexpr uint32_t kDx = 128;  // TMEM columns of the two dx buffers
+  pdl_wait();
+  const int64_t items = (int64_t)*q.plan.total * q.tiles;
+  bool ok = true;  // a bounded wait that ran out: go on without waiting
+
+  if (warp == 8) {
+    // -------------------------------------------------------------- loads
+    uint32_t it = 0, ai = 0;
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+      const Item t = item_at(q, i);
+      if (t.steps == 0) continue;
+      if (t.dx) {
+        if (lane == 0) {
+          if (ai > 0) ok = ok && mbar_wait(&sh.aempty, (ai - 1) & 1, q.status, kDevTimeoutEmpty);
+          mbar_arrive_expect_tx(&sh.afull, RP * kCols * 2);
+          for (int b = 0; b < 2; ++b)
+            tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &maps.a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
         }
-        auto pack = [](const __half (&h)[4]) {
-          return make_uint2((uint32_t)__half_as_ushort(h[0]) | ((uint32_t)__half_as_ushort(h[1]) << 16),
-                            (uint32_t)__half_as_ushort(h[2]) | ((uint32_t)__half_as_ushort(h[3]) << 16));
-        };
-        const uint2 a = pack(hi), b = pack(lo);
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + Cfg::OFF_HI + row * Cfg::PITCH + c * 2), "r"(a.x),
-                     "r"(a.y)
-                     : "memory");
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + Cfg::OFF_LO + row * Cfg::PITCH + c * 2), "r"(b.x),
-                     "r"(b.y)
-                     : "memory");
+        ++ai;
       }
-      __syncthreads();
-      if (step + STAGES - 1 < steps) load(step + STAGES - 1);
-      cp_async_commit();
-      const uint32_t vs = base + (step % STAGES) * Cfg::V_STAGE;
-      if (out) {
+      const bool tma = t.is_x || q.dy_tma;
+      for (int step = 0; step < t.steps; ++step, ++it) {
+        const uint32_t s = it % kVStages;
+        int r[4];  // a lane's four rows; past the end, the chunk's last row (its h or g is taken as zero)
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk) {
-          uint32_t a[2][4];
+        for (int k = 0; k < 4; ++k) {
+          const int at = step * kStepRows + lane * 4 + k;
+          r[k] = __ldcg(q.plan.order + t.ck.start + (at < t.ck.count ? at : t.ck.count - 1));
+        }
+        if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[s], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
+        if (lane == 0) {
+          if (tma) mbar_arrive_expect_tx(&sh.vfull[s], Cfg::V_STAGE);
+          else mbar_arrive(&sh.vfull[s]);  // the workers copy
+        }
+        __syncwarp();
+        if (tma) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {  // V^T: [16 columns][16 rows]
-            const int row = kk * 16 + (lane >> 4) * 8 + (lane & 7);
-            const int piece = warp * 4 + i * 2 + ((lane >> 3) & 1);
-            ldmatrix_x4_trans(vs + row * Cfg::ROW + ((piece ^ (row & 7)) << 4), a[i][0], a[i][1], a[i][2], a[i][3]);
-          }
-          const int row = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+          for (int b = 0; b < 2; ++b)
+            tma_gather4(base + s * Cfg::V_STAGE + b * (kStepRows * 128) + lane * 512, t.is_x ? &maps.x : &maps.dy,
+                        &sh.vfull[s], (int)t.col0 + b * 64, r);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ----------------------------------------------------------- products
+    uint32_t it = 0, dxs = 0, sums = 0, ai = 0;
+    if (lane == 0) {
+      constexpr uint32_t kSumDesc = mma_desc(kCols, Cfg::NRANK, true, true);
+      constexpr uint32_t kDxDesc = mma_desc(kStepRows, kCols, false, true);
+      for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const Item t = item_at(q, i);
+        if (t.steps == 0) continue;
+        if (t.dx) ok = ok && mbar_wait(&sh.afull, ai & 1, q.status, kDevTimeoutFull);
+        if (t.sum && sums > 0) ok = ok && mbar_wait(&sh.accempty, (sums - 1) & 1, q.status, kDevTimeoutAccum);
+        for (int step = 0; step < t.steps; ++step, ++it) {
+          const uint32_t s = it % kVStages, gb = it % Cfg::G_BUFS;
+          ok = ok && mbar_wait(&sh.vfull[s], (it / kVStages) & 1, q.status, kDevTimeoutFull);
+          ok = ok && mbar_wait(&sh.gfull[gb], (it / Cfg::G_BUFS) & 1, q.status, kDevTimeoutFull);
+          if (t.dx && dxs >= 2) ok = ok && mbar_wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, q.status, kDevTimeoutAccum);
+          tc_fence_after();
+          const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * 2 * Cfg::G_HALF;
+          if (t.sum) {
+            const uint64_t a = operand_mn(vs, kStepRows * 128);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t ts = base + (half ? Cfg::OFF_LO : Cfg::OFF_HI) + row * Cfg::PITCH + (lane >> 4) * 16;
+            for (int half = 0; half < 2; ++half) {
+              const uint64_t b = operand_mn(gs + half * Cfg::G_HALF, kStepRows * 128);
 #pragma unroll
-            for (int r = 0; r < RT; r += 2) {
-              uint32_t b[4];
-              ldmatrix_x4_trans(ts + r * 16, b[0], b[1], b[2], b[3]);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                mma_16816(acc[i][r], a[i][0], a[i][1], a[i][2], a[i][3], b[0], b[1]);
-                mma_16816(acc[i][r + 1], a[i][0], a[i][1], a[i][2], a[i][3], b[2], b[3]);
-              }
+              for (int kk = 0; kk < kStepRows / 16; ++kk)
+                tc_mma_ss(tmem, a + (uint64_t)(128 * kk), b + (uint64_t)(128 * kk), kSumDesc,
+                          step > 0 || half > 0 || kk > 0);
             }
           }
+          if (t.dx) {
+            const uint64_t b = operand_mn(base + Cfg::OFF_A, RP * 128);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+              for (int kk = 0; kk < RP / 16; ++kk) {
+                const uint64_t a = operand_k(gs + half * Cfg::G_HALF + kk / 4 * (kStepRows * 128)) + (uint64_t)(2 * (kk % 4));
+                tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, half > 0 || kk > 0);
+              }
+            }
+            tc_commit(&sh.dxfull[dxs & 1]);
+            ++dxs;
+          }
+          tc_commit(&sh.vempty[s]);
+          tc_commit(&sh.gempty[gb]);
+        }
+        if (t.sum) {
+          tc_commit(&sh.accfull);
+          ++sums;
+        }
+        if (t.dx) {
+          tc_commit(&sh.aempty);
+          ++ai;
         }
       }
-      if (want_dx) {
-        // dx of the step's rows: [64 rows][32 columns] a warp, ranks the reduction
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ workers
+    const int quarter = warp % 4, upper = warp / 4;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const bool dx32 = (reinterpret_cast<uintptr_t>(q.dx) & 31) == 0;
+    uint32_t it = 0, dxs = 0, sums = 0;
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+      const Item t = item_at(q, i);
+      const Chunk& ck = t.ck;
+      const int* order = q.plan.order + ck.start;
+      float* out = t.is_x ? q.da : q.db;
+      // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
+      const uint32_t top = q.plan.amax[(t.is_x ? p.L : 0) + ck.adapter];
+      int e = top == 0u || top >= 0x7F800000u ? 0 : 14 - ((int)(top >> 23) - 127);
+      e = e > 126 ? 126 : (e < -126 ? -126 : e);
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+      const float* src = t.is_x ? q.g : q.h;
+      const int piece = tid % (RP / 4), row0 = tid / (RP / 4);
+      constexpr int kRowStep = kWorkers / (RP / 4);
+      float4 v[Cfg::PER];
+      auto fetch = [&](int step) {
+#pragma unroll
+        for (int k = 0; k < Cfg::PER; ++k) {
+          const int at = step * kStepRows + row0 + k * kRowStep;
+          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at < ck.count) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)__ldcg(order + at) * RP) + piece);
+        }
+      };
+      // dx of a step whose products are done: a row a lane, 64 columns a warp
+      auto store_dx = [&](int step) {
+        const uint32_t b = dxs & 1;
+        ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
+        tc_fence_after();
+        const int at = step * kStepRows + quarter * 32 + lane;
+        const bool in = at < ck.count;
+        __half* row = q.dx + (int64_t)(in ? __ldcg(order + at) : 0) * p.K;
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) {
+          const int64_t col = t.col0 + upper * 64 + c;
+          uint32_t d[16];
+          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c, d);
+          tmem_wait_ld();
+          if (!in || col >= t.width) continue;
+          uint32_t o[8];
+          if (q.add_dx) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              *reinterpret_cast<uint4*>(o + 4 * x) = *reinterpret_cast<const uint4*>(row + col + 8 * x);
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            float2 f = make_float2(__uint_as_float(d[2 * x]) * down, __uint_as_float(d[2 * x + 1]) * down);
+            if (q.add_dx) {
+              const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&o[x]));
+              f.x += w.x;
+              f.y += w.y;
+            }
+            const __half2 r = __floats2half2_rn(f.x, f.y);
+            o[x] = *reinterpret_cast<const uint32_t*>(&r);
+          }
+          if (dx32) {  // a whole 32-byte sector a lane
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + col), "r"(o[0]), "r"(o[1]),
+                         "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                         : "memory");
+          } else {
+            *reinterpret_cast<uint4*>(row + col) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row + col + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.dxempty[b]);
+        ++dxs;
+      };
+      if (t.steps > 0) fetch(0);
+      for (int step = 0; step < t.steps; ++step, ++it) {
+        const uint32_t gb = it % Cfg::G_BUFS;
+        // the products that read this buffer last are done
+        if (it >= Cfg::G_BUFS)
+          ok = ok && mbar_wait(&sh.gempty[gb], (it / Cfg::G_BUFS - 1) & 1, q.status, kDevTimeoutEmpty);
+        const uint32_t gs = base + Cfg::OFF_G + gb * 2 * Cfg::G_HALF;
+#pragma unroll
+        for (int k = 0; k < Cfg::PER; ++k) {
+          const int row = row0 + k * kRowStep, c = piece * 4;
+          const float f[4] = {v[k].x * up, v[k].y * up, v[k].z * up, v[k].w * up};
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const __half2 h = __floats2half2_rn(f[2 * x], f[2 * x + 1]);
+            const float2 back = __half22float2(h);
+            const __half2 l = __floats2half2_rn(f[2 * x] - back.x, f[2 * x + 1] - back.y);
+            hi[x] = *reinterpret_cast<const uint32_t*>(&h);
+            lo[x] = *reinterpret_cast<const uint32_t*>(&l);
+          }
+          const uint32_t at = gs + c / 64 * (kStepRows * 128) + swizzled(row, c % 64 / 8) + (c % 8) * 2;
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + Cfg::G_HALF), "r"(lo[0]), "r"(lo[1]) : "memory");
+        }
+        if (!t.is_x && !q.dy_tma) {
+          // Rows that TMA cannot take.  The slot's last products are three steps
+          // back, done by the wait above (for those of at most two steps back).
+          for (int x = tid; x < kStepRows * kCols / 8; x += kWorkers) {
+            const int row = x / (kCols / 8), pc = x % (kCols / 8);
+            const int at = step * kStepRows + row;
+            const int64_t col = t.col0 + pc * 8;
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (at < ck.count && col < t.width)
+              w = load_halves(q.dy + (int64_t)__ldcg(order + at) * q.dy_ld + col, t.width - col);
+            sts16(base + it % kVStages * Cfg::V_STAGE + pc / 8 * (kStepRows * 128) + swizzled(row, pc % 8), w);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.gfull[gb]);
+        if (step + 1 < t.steps) fetch(step + 1);
+        if (t.dx && step > 0) store_dx(step - 1);
+      }
+      if (t.dx && t.steps > 0) store_dx(t.steps - 1);
+      if (!t.sum) continue;
+
+      // D[column][rank] of this chunk (a column a lane, 16 ranks at a time over two warps), then the sum's
+      if (t.steps > 0) {
+        ok = ok && mbar_wait(&sh.accfull, sums & 1, q.status, kDevTimeoutAccum);
+        ++sums;
+        tc_fence_after();
+      }
+      const int c = quarter * 32 + lane;
+      float* slots = q.part + ((int64_t)ck.slot0 * q.tiles + t.tile) * kCols * RP + c;
+      const int64_t apart = (int64_t)q.tiles * kCols * RP;
+      auto write = [&](int r0, const float (&f)[16]) {
+        const int64_t col = t.col0 + c;
+        if (col >= t.width) return;
+        if (t.is_x) {
+          float* o = out + ((int64_t)ck.adapter * p.R + r0) * t.width + col;
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (r0 + x < p.R) o[x * t.width] = f[x] * down;
+        } else {
+          float* o = out + ((int64_t)ck.adapter * t.width + col) * p.R + r0;
+          if (p.R % 4 == 0) {
+#pragma unroll
+            for (int x = 0; x < 16; x += 4)
+              if (r0 + x < p.R)
+                *reinterpret_cast<float4*>(o + x) =
+                    make_float4(f[x] * down, f[x + 1] * down, f[x + 2] * down, f[x + 3] * down);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              if (r0 + x < p.R) o[x] = f[x] * down;
+          }
+        }
+      };
 #pragma unroll 1
-        for (int mt = 0; mt < kRows / 16; ++mt) {
-          if (step * kRows + mt * 16 >= ck.count) break;
-          float d[4][4];
+      for (int r0 = upper * 16; r0 < RP; r0 += 32) {
+        uint32_t d[16];
+        if (t.steps > 0) {
+          tmem_ld_32x32b_x16(tmem + lanes + r0, d);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) d[c][0] = d[c][1] = d[c][2] = d[c][3] = 0.f;
+          for (int x = 0; x < 16; ++x) d[x] = 0u;
+        }
+        if (ck.of == 1) {
+          float f[16];
 #pragma unroll
-          for (int kk = 0; kk < RP / 16; ++kk) {
-            uint32_t hi[4], lo[4];
-            const uint32_t at = (uint32_t)((mt * 16 + (lane & 15)) * Cfg::PITCH + kk * 32 + (lane >> 4) * 16);
-            ldmatrix_x4(base + Cfg::OFF_HI + at, hi[0], hi[1], hi[2], hi[3]);
-            ldmatrix_x4(base + Cfg::OFF_LO + at, lo[0], lo[1], lo[2], lo[3]);
+          for (int x = 0; x < 16; ++x) f[x] = __uint_as_float(d[x]);
+          write(r0, f);
+        } else {
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-              uint32_t b[4];
-              const int r = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), piece = warp * 4 + c + (lane >> 4);
-              ldmatrix_x4_trans(base + Cfg::OFF_A + r * Cfg::ROW + ((piece ^ (r & 7)) << 4), b[0], b[1], b[2], b[3]);
-              mma_16816(d[c], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
-              mma_16816(d[c + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
-              mma_16816(d[c], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
-              mma_16816(d[c + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
-            }
-          }
-          // through shared memory (this warp's 64 bytes of each row) into rows of 16-byte stores
-          float* stage = reinterpret_cast<float*>(sum_smem + Cfg::OFF_DX) + warp * 16 * 32;  // [16][32] fp32
-          __syncwarp();
+          for (int x = 0; x < 16; ++x) __stcg(slots + ck.index * apart + (r0 + x) * kCols, __uint_as_float(d[x]));
+        }
+      }
+      if (t.steps > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.accempty);
+      }
+      if (ck.of > 1) {
+        __threadfence();
+        worker_sync();
+        if (tid == 0)
+          sh.last = atomicAdd(q.plan.count + (int64_t)ck.joint * q.tiles + t.tile, 1u) == (uint32_t)ck.of - 1;
+        worker_sync();
+        const bool last = sh.last != 0;
+        worker_sync();
+        if (!last) continue;
+        __threadfence();
+#pragma unroll 1
+        for (int r0 = upper * 16; r0 < RP; r0 += 32) {
+          float f[16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int x = 0; x < 16; ++x) f[x] = 0.f;
+          for (int k = 0; k < ck.of; ++k)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int row = lane / 4 + 8 * h, col = c * 8 + (lane % 4) * 2;
-              *reinterpret_cast<float2*>(stage + row * 32 + (col ^ ((row & 7) << 2))) =
-                  make_float2(d[c][2 * h] * down, d[c][2 * h + 1] * down);
-            }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int i = k * 32 + lane, row = i / 4, col = i % 4 * 8;  // 8 columns a lane
-            const int at = step * kRows + mt * 16 + row;
-            const int64_t cg = col0 + warp * 32 + col;
-            if (at < ck.count && cg < width) {
-              uint4* dst = reinterpret_cast<uint4*>(q.dx + q.plan.order[ck.start + at] * p.K + cg);
-              uint4 old = make_uint4(0u, 0u, 0u, 0u);
-              if (q.add_dx) old = *dst;
-              uint32_t* o = &old.x;
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float2 f = *reinterpret_cast<const float2*>(stage + row * 32 + ((col + 2 * x) ^ ((row & 7) << 2)));
-                float2 s = __half22float2(*reinterpret_cast<const __half2*>(&o[x]));
-                s.x += f.x;
-                s.y += f.y;
-                const __half2 r = __floats2half2_rn(s.x, s.y);
-                o[x] = *reinterpret_cast<const uint32_t*>(&r);
-              }
-              *dst = old;
-            }
-          }
+            for (int x = 0; x < 16; ++x) f[x] += __ldcg(slots + k * apart + (r0 + x) * kCols);
+          write(r0, f);
         }
       }
     }
-    cp_async_wait<0>();
-    if (!out) continue;
-    // D[column][rank] of this chunk, then the sum's
-    auto put = [&](auto&& f) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) f(warp * 32 + i * 16 + lane / 4 + 8 * h, r * 8 + (lane % 4) * 2, acc[i][r] + 2 * h);
-    };
-    if (ck.of > 1) {
-      const int64_t sum = (int64_t)ck.joint * q.tiles + tile;
-      // slot of the adapter's first chunk; its next ones follow, q.tiles apart
-      float* slots = q.part + ((int64_t)ck.slot0 * q.tiles + tile) * COLS * RP;
-      const int64_t apart = (int64_t)q.tiles * COLS * RP;
-      put([&](int c, int r, float* a) {
-        __stcg(reinterpret_cast<float2*>(slots + ck.index * apart + c * RP + r), make_float2(a[0], a[1]));
-      });
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) last = atomicAdd(q.plan.count + sum, 1u) == (uint32_t)ck.of - 1;
-      __syncthreads();
-      if (!last) continue;
-      __threadfence();
-      put([&](int c, int r, float* a) {
-        float2 s = make_float2(0.f, 0.f);
-        for (int k = 0; k < ck.of; ++k) {
-          const float2 x = __ldcg(reinterpret_cast<const float2*>(slots + k * apart + c * RP + r));
-          s.x += x.x;
-          s.y += x.y;
-        }
-        a[0] = s.x;
-        a[1] = s.y;
-      });
-    }
-    const int64_t a0 = (int64_t)ck.adapter * p.R * width;
-    put([&](int c, int r, float* a) {
-      if (col0 + c >= width) return;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (r + x < p.R)
-          out[is_x ? a0 + (int64_t)(r + x) * width + col0 + c : a0 + (col0 + c) * p.R + r + x] = a[x] * down;
-    });
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -910,16 +1051,15 @@ struct GradSpace {
 GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_count) {
   GradSpace s;
   s.RP = padded_rank(R);
-  const int cols = kCols(s.RP);
-  s.x_tiles = (int)((K + cols - 1) / cols);
-  s.tiles = s.x_tiles + (int)((N + cols - 1) / cols);
+  s.x_tiles = (int)((K + kCols - 1) / kCols);
+  s.tiles = s.x_tiles + (int)((N + kCols - 1) / kCols);
   // about two items an SM
   int64_t cuts = (2 * (int64_t)sm_count + s.tiles - 1) / s.tiles;
-  const int64_t most = (M + kRows - 1) / kRows;
+  const int64_t most = (M + kStepRows - 1) / kStepRows;
   cuts = cuts > most ? most : cuts;
   cuts = cuts < 1 ? 1 : cuts;
-  s.chunk_rows = (int)(((M + cuts - 1) / cuts + kRows - 1) / kRows * kRows);
-  if (s.chunk_rows < kRows) s.chunk_rows = kRows;
+  s.chunk_rows = (int)(((M + cuts - 1) / cuts + kStepRows - 1) / kStepRows * kStepRows);
+  if (s.chunk_rows < kStepRows) s.chunk_rows = kStepRows;
   s.max_chunks = M / s.chunk_rows + L;
   s.joints = M / (s.chunk_rows + 1);  // adapters of more than chunk_rows rows
   if (s.joints > L) s.joints = L;
@@ -936,29 +1076,26 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.order = take((size_t)M * sizeof(int));
   s.amax = take((size_t)2 * L * sizeof(uint32_t));
   s.count = take((size_t)s.joints * s.tiles * sizeof(uint32_t));
-  s.part = take((size_t)parts * s.tiles * cols * s.RP * sizeof(float));
+  s.part = take((size_t)parts * s.tiles * kCols * s.RP * sizeof(float));
   s.end = at;
   return s;
 }
 
-template <int RT>
-cudaError_t launch_sums(const Sums& q, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
-  using Cfg = SumCfg<RT>;
-  static thread_local int configured_dev = -1, per_sm = 1;
+template <int RP>
+cudaError_t launch_sums(const Sums& q, const SumMaps& maps, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
+  using Cfg = SumCfg<RP>;
+  static thread_local int configured_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev != dev) {
-    cudaError_t e = cudaFuncSetAttribute(lora_sums_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-    if (e == cudaSuccess)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, lora_sums_kernel<RT>, Cfg::THREADS, Cfg::SMEM);
+    const cudaError_t e =
+        cudaFuncSetAttribute(lora_sums_kernel<RP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
     if (e != cudaSuccess) return e;
-    if (per_sm < 1) return cudaErrorInvalidConfiguration;
     configured_dev = dev;
   }
-  const int64_t grid = items < (int64_t)sm_count * per_sm ? items : (int64_t)sm_count * per_sm;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.gridDim = dim3((unsigned)(items < sm_count ? items : sm_count));
+  cfg.blockDim = dim3(kSumThreads);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -966,7 +1103,7 @@ cudaError_t launch_sums(const Sums& q, int64_t items, int sm_count, bool pdl, cu
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RT>, q);
+  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RP>, q, maps);
 }
 
 }  // namespace
@@ -1055,11 +1192,31 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
   q.add_dx = g.add_dx;
   q.x_tiles = s.x_tiles;
   q.tiles = s.tiles;
+  q.status = g.status;
+  SumMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  {
+    const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.R, (uint64_t)p.L};
+    const uint64_t strides[2] = {(uint64_t)p.K * 2, (uint64_t)p.K * p.R * 2};
+    const uint32_t box[3] = {64, (uint32_t)s.RP, 1};
+    if (!encode_tmap_3d(&maps.a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                        err))
+      return cudaErrorInvalidValue;
+  }
+  if (p.M) {  // a gathered box is one row
+    if (!encode_tmap_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, (uint64_t)p.K, (uint64_t)p.M,
+                        (uint64_t)p.x_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
+      return cudaErrorInvalidValue;
+    q.dy_tma = g.dy_ld % 8 == 0 && reinterpret_cast<uintptr_t>(g.dy) % 16 == 0;
+    if (q.dy_tma && !encode_tmap_2d(&maps.dy, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.dy, (uint64_t)p.N, (uint64_t)p.M,
+                                    (uint64_t)g.dy_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
+      return cudaErrorInvalidValue;
+  }
   const int64_t items = s.max_chunks * s.tiles;
-  if (p.R <= 16) return launch_sums<2>(q, items, sm_count, pdl, stream);
-  if (p.R <= 32) return launch_sums<4>(q, items, sm_count, pdl, stream);
-  if (p.R <= 64) return launch_sums<8>(q, items, sm_count, pdl, stream);
-  return launch_sums<16>(q, items, sm_count, pdl, stream);
+  if (p.R <= 16) return launch_sums<16>(q, maps, items, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_sums<32>(q, maps, items, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_sums<64>(q, maps, items, sm_count, pdl, stream);
+  return launch_sums<128>(q, maps, items, sm_count, pdl, stream);
 }
 
 }  // namespace qw
