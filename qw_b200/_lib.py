@@ -70,12 +70,12 @@ SIGNATURES = {
     "qw_quantized_linear_forward": ([_PA, _PA, _PA, _PA, _PA, _I, _I, ctypes.c_char_p, _PA, _P], _I),
     "qw_quantized_linear_forward_global_scale": (
         [_PA, _PA, _PA, _PA, _PA, _PA, _I, _I, ctypes.c_char_p, _PA, _P], _I),
-    "qw_quantized_linear_lora": (
-        [_PA, _PA, _PA, _PA, _PA, _PA, _PA, _PA, _PA, _I, _I, ctypes.c_char_p, _PA, _P, ctypes.c_int64, _P], _I),
+    # (descriptors of these as void pointers: ops.py passes them packed as bytes)
+    "qw_quantized_linear_lora": ([_P] * 9 + [_I, _I, ctypes.c_char_p, _P, _P, ctypes.c_int64, _P], _I),
     "qw_quantized_linear_lora_workspace": ([ctypes.c_int64] * 3 + [ctypes.POINTER(ctypes.c_int64)], _I),
-    "qw_lora_backward": ([_PA, _PA, _PA, _PA, _PA, _PA, _I, _PA, _PA, _PA, _P, ctypes.c_int64, _P], _I),
+    "qw_lora_backward": ([_P] * 6 + [_I, _P, _P, _P, _P, ctypes.c_int64, _P], _I),
     "qw_lora_backward_workspace": ([ctypes.c_int64] * 5 + [ctypes.POINTER(ctypes.c_int64)], _I),
-    "qw_topk_distill": ([_PA, _PA, _PA, _PA, _PA, _PA, _PA, _P], _I),
+    "qw_topk_distill": ([_P] * 8, _I),
     "qw_dequantize": ([_PA, _PA, _PA, _I, _I, ctypes.c_char_p, _PA, _P], _I),
     "qw_dequantize_rounding": ([_PA, _PA, _PA, _I, _I, ctypes.c_char_p, _I, _PA, _P], _I),
     "qw_quantize": ([_PA, _I, _I, ctypes.c_char_p, _PA, _PA, _PA, _P], _I),

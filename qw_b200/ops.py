@@ -8,7 +8,9 @@ supplies device memory and the current stream only.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -64,6 +66,29 @@ def _stream(t: torch.Tensor) -> int:
 
 def _mode(mode: str) -> bytes:
     return mode.encode()
+
+
+# A qw_array packed as bytes (the layout of _lib.QwArray), for operands that
+# change from call to call: one pack costs a third of a ctypes structure, and
+# nothing is kept.  Zero strides mean row-contiguous.
+_PACK = struct.Struct("=Qii8q").pack
+_PAD = [None] + [(0,) * (4 - n) for n in range(1, 5)]
+
+
+def _desc(t: Optional[torch.Tensor]) -> Optional[bytes]:
+    if t is None:
+        return None
+    dt = _DT.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    shape = t.shape
+    n = len(shape)
+    if n < 1 or n > 4:
+        raise ValueError("qw arrays have 1 to 4 dimensions")
+    pad = _PAD[n]
+    if t.is_contiguous():
+        return _PACK(t.data_ptr(), dt, n, *shape, *pad, 0, 0, 0, 0)
+    return _PACK(t.data_ptr(), dt, n, *shape, *pad, *t.stride(), *pad)
 
 
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: Optional[torch.Tensor],
@@ -212,19 +237,42 @@ def quantized_linear_forward_global_scale(x, w, scales, biases, global_scale=Non
     return out
 
 
-def _one_device(x: torch.Tensor, *tensors):
-    """Every operand on x's device (the library is given bare addresses)."""
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(x: torch.Tensor, *tensors):
+    """Context of a call on x's device; every operand must be there (the
+    library is given bare addresses)."""
+    dev = x.get_device()
     for t in tensors:
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"operands on {x.device} and {t.device}")
-    return torch.cuda.device(x.device)
+    if dev < 0:
+        raise ValueError("operands must be CUDA tensors")
+    return _SAME_DEVICE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _workspace(query, x: torch.Tensor, *sizes) -> torch.Tensor:
-    """Scratch of one call, of the current stream (inside a capture: of the graph's own pool)."""
-    n = ctypes.c_int64(0)
-    _lib.check(query(*[int(s) for s in sizes], ctypes.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=x.device)
+def _raw_stream(x: torch.Tensor) -> int:
+    """Handle of x's device's current stream (without the Stream object, which costs more than a launch's checks)."""
+    return torch._C._cuda_getCurrentRawStream(x.get_device())
+
+
+# Workspace bytes by query and sizes (and device: they depend on its SM count).
+_WORKSPACE_BYTES: dict = {}
+
+
+def _workspace(query: str, x: torch.Tensor, *sizes) -> torch.Tensor:
+    """Scratch of one call, of the current stream (inside a capture: of the graph's own pool), as fp16 for
+    ``x.new_empty`` (the cheapest allocation call); the library reads bytes."""
+    key = (query, x.get_device(), sizes)
+    n = _WORKSPACE_BYTES.get(key)
+    if n is None:
+        out = ctypes.c_int64(0)
+        _lib.check(getattr(_lib.load(), query)(*sizes, ctypes.byref(out)))
+        if len(_WORKSPACE_BYTES) >= 4096:
+            _WORKSPACE_BYTES.clear()
+        n = _WORKSPACE_BYTES[key] = (out.value + 1) // 2
+    return x.new_empty((n,))
 
 
 def quantized_linear_lora(x: torch.Tensor, w, scales, biases, lora_a: torch.Tensor, lora_b: torch.Tensor,
@@ -237,15 +285,15 @@ def quantized_linear_lora(x: torch.Tensor, w, scales, biases, lora_a: torch.Tens
     ``adapter_idx`` int32, one per row in any order, -1 for none (None: adapter
     0 for every row)."""
     if out is None:
-        out = torch.empty(*x.shape[:-1], w.shape[0], dtype=torch.float16, device=x.device)
+        out = x.new_empty((*x.shape[:-1], w.shape[0]), dtype=torch.float16)
     L = _lib.load()
-    with _one_device(x, w, scales, biases, lora_a, lora_b, lora_scales, adapter_idx, linear_bias, out):
+    with _on_device(x, w, scales, biases, lora_a, lora_b, lora_scales, adapter_idx, linear_bias, out):
         rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        ws = _workspace(L.qw_quantized_linear_lora_workspace, x, rows, w.shape[0], lora_a.shape[1])
+        ws = _workspace("qw_quantized_linear_lora_workspace", x, rows, w.shape[0], lora_a.shape[1])
         _lib.check(L.qw_quantized_linear_lora(
-            _arr(x), _arr(w), _arr(scales), _arr(biases), _arr(linear_bias), _arr(lora_a), _arr(lora_b),
-            _arr(lora_scales), _arr(adapter_idx), group_size, bits, _mode(mode), _arr(out), ws.data_ptr(),
-            ws.numel(), _stream(x)))
+            _desc(x), _desc(w), _desc(scales), _desc(biases), _desc(linear_bias), _desc(lora_a), _desc(lora_b),
+            _desc(lora_scales), _desc(adapter_idx), group_size, bits, _mode(mode), _desc(out), ws.data_ptr(),
+            ws.nbytes, _raw_stream(x)))
     return out
 
 
@@ -258,17 +306,17 @@ def lora_backward(x: torch.Tensor, dy: torch.Tensor, lora_a: torch.Tensor, lora_
     a new tensor holds that part alone."""
     accumulate = dx is not None
     if dx is None:
-        dx = torch.empty(x.shape, dtype=torch.float16, device=x.device)
-    da = torch.empty(lora_a.shape, dtype=torch.float32, device=x.device)
-    db = torch.empty(lora_b.shape, dtype=torch.float32, device=x.device)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    da = torch.empty_like(lora_a, dtype=torch.float32)
+    db = torch.empty_like(lora_b, dtype=torch.float32)
     L = _lib.load()
-    with _one_device(x, dy, lora_a, lora_b, lora_scales, adapter_idx, dx):
+    with _on_device(x, dy, lora_a, lora_b, lora_scales, adapter_idx, dx):
         rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        ws = _workspace(L.qw_lora_backward_workspace, x, rows, dy.shape[-1], x.shape[-1], lora_a.shape[1],
+        ws = _workspace("qw_lora_backward_workspace", x, rows, dy.shape[-1], x.shape[-1], lora_a.shape[1],
                         lora_a.shape[0])
-        _lib.check(L.qw_lora_backward(_arr(x), _arr(dy), _arr(lora_a), _arr(lora_b), _arr(lora_scales),
-                                      _arr(adapter_idx), int(accumulate), _arr(dx), _arr(da), _arr(db),
-                                      ws.data_ptr(), ws.numel(), _stream(x)))
+        _lib.check(L.qw_lora_backward(_desc(x), _desc(dy), _desc(lora_a), _desc(lora_b), _desc(lora_scales),
+                                      _desc(adapter_idx), accumulate, _desc(dx), _desc(da), _desc(db),
+                                      ws.data_ptr(), ws.nbytes, _raw_stream(x)))
     return dx, da, db
 
 
@@ -284,12 +332,12 @@ def topk_distillation(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_v
     if teacher_idx.dtype == torch.int64:
         teacher_idx = teacher_idx.to(torch.int32)
     if dlogits is None and grad:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    loss = torch.empty(logits.shape[:-1] or (1,), dtype=torch.float32, device=logits.device)
-    with _one_device(logits, teacher_idx, teacher_values, temperature, row_weights, dlogits):
-        _lib.check(_lib.load().qw_topk_distill(_arr(logits), _arr(teacher_idx), _arr(teacher_values),
-                                               _arr(temperature), _arr(row_weights), _arr(loss), _arr(dlogits),
-                                               _stream(logits)))
+        dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    loss = logits.new_empty(logits.shape[:-1] or (1,), dtype=torch.float32)
+    with _on_device(logits, teacher_idx, teacher_values, temperature, row_weights, dlogits):
+        _lib.check(_lib.load().qw_topk_distill(_desc(logits), _desc(teacher_idx), _desc(teacher_values),
+                                               _desc(temperature), _desc(row_weights), _desc(loss), _desc(dlogits),
+                                               _raw_stream(logits)))
     return loss, dlogits
 
 

@@ -245,9 +245,9 @@ def test_partial_outputs_and_non_finite_gradients(cuda_dev):
     from qw_b200.ops import _arr, _stream, _workspace
     for keep in range(3):
         outs = [torch.empty_like(t) if i == keep else None for i, t in enumerate(full)]
-        ws = _workspace(lib.qw_lora_backward_workspace, x, M, N, K, R, L)
+        ws = _workspace("qw_lora_backward_workspace", x, M, N, K, R, L)
         _lib.check(lib.qw_lora_backward(_arr(x), _arr(dy), _arr(a), _arr(b), _arr(s), _arr(idx), 0, _arr(outs[0]),
-                                        _arr(outs[1]), _arr(outs[2]), ws.data_ptr(), ws.numel(), _stream(x)))
+                                        _arr(outs[1]), _arr(outs[2]), ws.data_ptr(), ws.nbytes, _stream(x)))
         assert torch.equal(outs[keep], full[keep])
     dy[2] = float("inf")  # a row of adapter 2
     dx, da, db = qw_b200.lora_backward(x, dy, a, b, s, idx)
