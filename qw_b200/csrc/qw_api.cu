@@ -1224,7 +1224,7 @@ int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64
   const cudaError_t ce = cudaGetDevice(&dev);
   if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
   *bytes = (int64_t)(lora_skinny_bytes(m, n, 0, dev) +
-                     lora_forward_bytes(m, n, (int)rank, m > 16 ? prefill_token_tile(m) : 0));
+                     lora_forward_bytes(m, (int)rank, m > 16 ? prefill_token_tile(m) : 0));
   return QW_OK;
 }
 
@@ -1254,7 +1254,7 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
   if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
   const size_t skinny = lora_skinny_bytes(sa.M, sa.N, sa.K, dev);
   const int token_tile = sa.M > 16 ? prefill_token_tile(sa.M) : 0;
-  if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, sa.N, la.R, token_tile))))
+  if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, la.R, token_tile))))
     return rc;
   DeviceRes* res = nullptr;
   std::string err;
@@ -1269,13 +1269,12 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
                         device_info(dev).sm_count, pdl, stream, &err);
   if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "adapter launch") : fail(QW_ECUDA, err);
   if (sa.M <= 16) {
-    sa.y = lora_forward_product(la, lws);
-    sa.y_f32 = true;
+    const SkinnyLora lora = lora_skinny_operands(la, lws, bias);
+    sa.lora = &lora;
     Scratch sc{workspace, skinny};
     ce = launch_skinny(sa, sc, stream, pdl, &err);
     if (ce != cudaSuccess) return err.empty() ? cuda_fail(ce, "skinny launch") : fail(QW_ECUDA, err);
-    ce = launch_lora_expand(la, lws, bias, y->data, pdl, stream);
-    return ce == cudaSuccess ? QW_OK : cuda_fail(ce, "adapter launch");
+    return QW_OK;
   }
   const PrefillLora lora = lora_prefill_operands(la, token_tile, lws, bias);
   PrefillArgs pa{sa.x, sa.w, sa.scales, sa.biases, y->data, false, sa.M, sa.N, sa.K, res->status};

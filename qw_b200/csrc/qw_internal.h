@@ -41,6 +41,15 @@ struct Scratch {
 // Skinny path (M <= 16): stream-K over (row tile, 512-wide k chunk) units.
 struct ArComm;
 
+// Adapters of a decode call, added in its epilogue.
+struct SkinnyLora {
+  const float* h;       // fp32 [M][R], 16-byte aligned rows where R is a multiple of 8
+  const void* b;        // fp16 [L][N][R]
+  const uint32_t* idx;  // [M] or null (adapter 0)
+  const void* bias;     // fp16 [N] or null
+  int R, L;
+};
+
 struct SkinnyArgs {
   const void* x;         // fp16 [M][K], rows x_ld apart
   const uint32_t* w;     // [N][K/8]
@@ -67,6 +76,9 @@ struct SkinnyArgs {
   // rank's x W^T, exchanged through the communicator's buffers in the
   // kernel's epilogue.  Null: y is this rank's product alone.
   const ArComm* ar = nullptr;
+  // Adapters and a bias added to the product (not SwiGLU, no exchange or
+  // greedy keys; y fp16).
+  const SkinnyLora* lora = nullptr;
 };
 // The decode kernel's configuration and schedule for a matmul (the choice
 // launch_skinny makes, computed without touching a device).
@@ -215,14 +227,13 @@ constexpr int kLoraMaxRank = 128;
 constexpr int64_t kLoraMaxAdapters = 4096;
 // Forward workspace (after the decode kernel's scratch): token_tile 0 for at
 // most 16 rows, else prefill_token_tile(M).
-size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile);
+size_t lora_forward_bytes(int64_t M, int R, int token_tile);
 // h = s x A^T into the workspace, with the token tiles' adapter lists where
 // token_tile != 0, and `zero_bytes` (rounded up to 16) at `zero` cleared.
 cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes,
                              unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err);
-// fp32 [M][N] within the workspace of at most 16 rows: the projection's product.
-float* lora_forward_product(const LoraArgs& p, void* ws);
-cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, bool pdl, cudaStream_t stream);
+// What the decode kernel adds to its products, from the workspace.
+SkinnyLora lora_skinny_operands(const LoraArgs& p, void* ws, const void* bias);
 // What the tcgen05 kernel adds to its products, from the workspace.
 PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias);
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);

@@ -5,12 +5,11 @@
 //   h = s x A^T, g = s dy B, dA = g^T x, dB = dy^T h, dx = g A
 // with the sums over the rows of each adapter.
 //
-// Forward, three launches chained by programmatic dependent launch:
-//   rank_rows     h = s x A^T (below);
-//   the projection's own kernel: the decode kernel (at most 16 rows) into an
-//                 fp32 product, or the tcgen05 kernel, which takes h and B as
-//                 further columns of its reduction and writes y itself;
-//   expand_rows   (at most 16 rows) y = fp16(product + h B^T + bias).
+// Forward, two launches chained by programmatic dependent launch:
+//   rank_rows     h = s x A^T (below; a long forward: lora_products);
+//   the projection's own kernel: the decode kernel (at most 16 rows) adds h B^T
+//                 in its epilogue, the tcgen05 kernel takes h and B as further
+//                 columns of its reduction.
 #include <cuda_fp16.h>
 
 #include "qw_internal.h"
@@ -46,6 +45,7 @@ struct RankRows {
   TokenLists lists;
   uint4* zero;        // cleared by the blocks behind the lists
   int zero_vecs;
+  int prefetch;       // bring B of the adapters present to L2 (for the decode kernel's epilogue)
 };
 
 template <int RT, int WARPS, int U>
@@ -86,6 +86,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows
   }
   __syncthreads();
   const int n = list_n;
+  if (q.prefetch) {  // each group's adapters, split over the cluster
+    for (int j = group; j < n; j += q.groups) {
+      const char* b = reinterpret_cast<const char*>(p.b) + (int64_t)list[j] * p.N * p.R * 2;
+      const int64_t lines = (p.N * p.R * 2 + 127) / 128;
+      for (int64_t i = rank * WARPS * 32 + tid; i < lines; i += (int64_t)C * WARPS * 32)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(b + (i * 128 < p.N * p.R * 2 ? i * 128 : 0)));
+    }
+  }
   const int steps = (int)(p.K / 32);
   const int s0 = (int)((int64_t)steps * rank / C), s1 = (int)((int64_t)steps * (rank + 1) / C);
   const int r = lane / 4, kq = (lane % 4) * 8;
@@ -156,75 +164,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows
   }
 }
 
-// y = fp16(product + h B^T + bias) for at most 16 rows.  Bound by the launch and
-// one trip to memory: a thread has a column and every fourth row; B's lines are
-// asked for before the wait for the projection.
-template <int RV>  // R = 8 RV (0: any rank)
-__global__ void __launch_bounds__(256) expand_rows_kernel(const LoraArgs p, const float* y32, const float* h,
-                                                          const __half* bias, __half* y, int row_groups) {
-  extern __shared__ float hs[];  // [M][R]
-  const int cols = 256 / row_groups;
-  const int64_t n = (int64_t)blockIdx.x * cols + threadIdx.x % cols;
-  const int rg = threadIdx.x / cols;
-  const __half* b0 = reinterpret_cast<const __half*>(p.b);
-  if (n < p.N) {
-    for (int m = rg; m < p.M; m += row_groups) {
-      const int64_t a = adapter_of(p, m);
-      if (a < 0) continue;
-      const char* line = reinterpret_cast<const char*>(b0 + (a * p.N + n) * p.R);
-      for (int i = 0; i < p.R * 2; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + i));
-    }
-  }
-  pdl_wait();
-  for (int i = threadIdx.x; i < (int)p.M * p.R; i += 256) hs[i] = __ldcg(h + i);
-  __syncthreads();
-  if (n >= p.N) return;
-  const float bn = bias ? __half2float(bias[n]) : 0.f;
-#pragma unroll 4
-  for (int m = rg; m < p.M; m += row_groups) {
-    const int64_t a = adapter_of(p, m);
-    float acc = __ldcg(y32 + m * p.N + n) + bn;
-    if (a >= 0) {
-      const __half* b = b0 + (a * p.N + n) * p.R;
-      float part = 0.f;
-      if constexpr (RV > 0) {
-#pragma unroll
-        for (int v = 0; v < RV; ++v) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(b) + v);
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ws[i]));
-            part = fmaf(hs[m * 8 * RV + 8 * v + 2 * i], f.x, part);
-            part = fmaf(hs[m * 8 * RV + 8 * v + 2 * i + 1], f.y, part);
-          }
-        }
-      } else {
-        for (int i = 0; i < p.R; ++i) part = fmaf(hs[m * p.R + i], __half2float(b[i]), part);
-      }
-      acc += part;
-    }
-    y[m * p.N + n] = __float2half_rn(acc);
-  }
-}
-
-}  // namespace
-
-namespace {
-
 constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int round8(int r) { return (r + 7) / 8 * 8; }
 
-// Forward workspace: at most 16 rows, h fp32 then the projection's fp32
-// product; above, h fp16 (zero-padded rank) and the token tiles' lists.
+// Forward workspace: at most 16 rows, h fp32; above, h fp16 (zero-padded rank)
+// and the token tiles' lists.
 struct ForwardSpace {
   size_t second, third, fourth, end;
 };
-ForwardSpace forward_space(int64_t M, int64_t N, int R, int token_tile) {
+ForwardSpace forward_space(int64_t M, int R, int token_tile) {
   ForwardSpace f;
   if (token_tile == 0) {
-    f.second = align256((size_t)M * R * sizeof(float));
-    f.third = f.fourth = f.end = f.second + align256((size_t)M * N * sizeof(float));
+    f.second = f.third = f.fourth = f.end = align256((size_t)M * R * sizeof(float));
   } else {
     const size_t tiles = (size_t)((M + token_tile - 1) / token_tile);
     f.second = align256((size_t)M * round8(R) * sizeof(__half));
@@ -278,17 +229,18 @@ cudaError_t launch_rank_rows(RankRows& q, int sm_count, bool pdl, cudaStream_t s
 
 }  // namespace
 
-size_t lora_forward_bytes(int64_t M, int64_t N, int R, int token_tile) { return forward_space(M, N, R, token_tile).end; }
+size_t lora_forward_bytes(int64_t M, int R, int token_tile) { return forward_space(M, R, token_tile).end; }
 
 cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* zero, size_t zero_bytes,
                              unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
-  const ForwardSpace f = forward_space(p.M, p.N, p.R, token_tile);
+  const ForwardSpace f = forward_space(p.M, p.R, token_tile);
   uint8_t* base = static_cast<uint8_t*>(ws);
   RankRows q{};
   q.p = p;
   q.R8 = round8(p.R);
   if (token_tile == 0) {
     q.h32 = reinterpret_cast<float*>(base);
+    q.prefetch = 1;
   } else {
     q.h16 = reinterpret_cast<__half*>(base);
     q.lists.tile = token_tile;
@@ -311,12 +263,12 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
   return launch_rank_rows<16, 8, 1>(q, sm_count, pdl, stream);
 }
 
-float* lora_forward_product(const LoraArgs& p, void* ws) {
-  return reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + forward_space(p.M, p.N, p.R, 0).second);
+SkinnyLora lora_skinny_operands(const LoraArgs& p, void* ws, const void* bias) {
+  return SkinnyLora{static_cast<const float*>(ws), p.b, p.idx, bias, p.R, (int)p.L};
 }
 
 PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, const void* bias) {
-  const ForwardSpace f = forward_space(p.M, p.N, p.R, token_tile);
+  const ForwardSpace f = forward_space(p.M, p.R, token_tile);
   uint8_t* base = static_cast<uint8_t*>(ws);
   PrefillLora l{};
   l.h = base;
@@ -329,32 +281,6 @@ PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, c
   l.R = p.R;
   l.L = (int)p.L;
   return l;
-}
-
-cudaError_t launch_lora_expand(const LoraArgs& p, void* ws, const void* bias, void* y, bool pdl, cudaStream_t stream) {
-  const int row_groups = p.M >= 4 ? 4 : 1;
-  const int cols = 256 / row_groups;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.N + cols - 1) / cols));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = (size_t)p.M * p.R * sizeof(float);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  const float* y32 = lora_forward_product(p, ws);
-  const float* h = static_cast<const float*>(ws);
-  const __half* bi = static_cast<const __half*>(bias);
-  __half* yo = static_cast<__half*>(y);
-  switch (p.R) {
-    case 8: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<1>, p, y32, h, bi, yo, row_groups);
-    case 16: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<2>, p, y32, h, bi, yo, row_groups);
-    case 32: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<4>, p, y32, h, bi, yo, row_groups);
-    case 64: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<8>, p, y32, h, bi, yo, row_groups);
-    default: return cudaLaunchKernelEx(&cfg, expand_rows_kernel<0>, p, y32, h, bi, yo, row_groups);
-  }
 }
 
 }  // namespace qw

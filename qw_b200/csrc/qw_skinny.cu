@@ -42,7 +42,7 @@
 // 512 contiguous bytes per weight row per stage and half the units, chosen
 // per shape by the host.
 //
-// Row-parallel exchange (a separate instantiation, XCHG): the launch is one
+// Row-parallel exchange (a separate instantiation): the launch is one
 // rank's K-slice of a tensor-parallel projection, and y is the sum over the
 // ranks.  Finished tiles go to this rank's slot of the communicator's buffer
 // (qw_exchange.cuh); after its last unit a CTA copies its tiles into every
@@ -213,6 +213,7 @@ struct SkinnyLaunch {
   unsigned long long* amax;  // one matmul only, may be null: [M] greedy-token keys (atomicMax)
   unsigned int* status;   // device status word
   ArParams ar;            // one matmul only: ar.P > 0 sums y over the ranks in the epilogue
+  SkinnyLora lora;        // one matmul only: adapters added in the epilogue (kEpiLora)
 };
 
 __device__ __forceinline__ long long unit_begin(long long i, long long U, int G) { return (i * U) / G; }
@@ -283,14 +284,24 @@ __device__ __forceinline__ bool wait_matmuls_done(const unsigned int* gbar, unsi
   return true;
 }
 
-// XCHG: the row-parallel exchange in the epilogue (p.ar); a separate
-// instantiation, so the plain kernel carries none of its code.
-template <int MT, int OPS_MAX, int BITS, bool WIDE, bool XCHG>
+// EPI: what the epilogue does beyond writing y, a separate instantiation each,
+// so the plain kernel carries none of their code.
+//   kEpiExchange  the row-parallel exchange (p.ar)
+//   kEpiLora      adapters beside the projection (p.lora): y + bias + h B^T of
+//                 each token's adapter, in fp32, rounded once.  A lane reads its
+//                 outputs' B rows (prefetched to L2 by the kernel that makes h)
+//                 and h, 8 ranks of all of them at a time; against a kernel of
+//                 its own behind the projection this saves a launch and the
+//                 product's trip through memory (16 rows of 16 adapters, 8192 x
+//                 5120: 24.3 us with that kernel).
+constexpr int kEpiPlain = 0, kEpiExchange = 1, kEpiLora = 2;
+template <int MT, int OPS_MAX, int BITS, bool WIDE, int EPI>
 __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
     __maxnreg__((SkinnyCfg<MT, BITS, WIDE>::MAXREG))
         qmm_skinny_kernel(const __grid_constant__ SkinnyLaunch<OPS_MAX> p) {
   using Cfg = SkinnyCfg<MT, BITS, WIDE>;
-  static_assert(!XCHG || OPS_MAX == 1, "the exchange takes single-matmul launches");
+  constexpr bool XCHG = EPI == kEpiExchange, LORA = EPI == kEpiLora;
+  static_assert(EPI == kEpiPlain || OPS_MAX == 1, "the exchange and adapters take single-matmul launches");
   constexpr int NT = Cfg::NT;
   constexpr int WST = Cfg::WST;
   constexpr int SST = Cfg::SST;
@@ -716,6 +727,82 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
             if (op.y_f32) reinterpret_cast<float*>(op.y)[idx] = h;
             else reinterpret_cast<__half*>(op.y)[idx] = __float2half_rn(h);
           }
+        }
+      return;
+    }
+    if constexpr (LORA) {
+      const SkinnyLora& l = p.lora;
+      float d[NT][4];  // tokens tt*8 + 2*s4 + (e & 1), rows wrow + r (+ 64 where e & 2)
+      const __half* b[NT][4];
+      uint32_t a[NT][2];
+      const int row0 = tile * Cfg::BN + wrow + r;
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = tt * 8 + 2 * s4 + (e & 1), row = row0 + ((e & 2) ? Cfg::BN / 2 : 0);
+          if (e < 2) {
+            a[tt][e] = n < p.M ? (l.idx ? l.idx[n] : 0u) : 0xFFFFFFFFu;
+            if (a[tt][e] >= (uint32_t)l.L) a[tt][e] = 0xFFFFFFFFu;
+          }
+          const bool in = a[tt][e & 1] != 0xFFFFFFFFu && row < op.N;
+          b[tt][e] = in ? reinterpret_cast<const __half*>(l.b) + ((size_t)a[tt][e & 1] * op.N + row) * l.R : nullptr;
+          d[tt][e] = v[tt][e];
+          if (l.bias && row < op.N) d[tt][e] += __half2float(reinterpret_cast<const __half*>(l.bias)[row]);
+        }
+      if (l.R % 8 == 0) {
+#pragma unroll 1
+        for (int q = 0; q < l.R; q += 8) {
+          uint4 w[NT][4];
+          float4 h[NT][2][2];
+#pragma unroll
+          for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[tt][e] = make_uint4(0u, 0u, 0u, 0u);
+              if (b[tt][e]) w[tt][e] = __ldg(reinterpret_cast<const uint4*>(b[tt][e] + q));
+              if (e < 2) {
+                h[tt][e][0] = h[tt][e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (a[tt][e] != 0xFFFFFFFFu) {
+                  const float4* src = reinterpret_cast<const float4*>(l.h + (size_t)(tt * 8 + 2 * s4 + e) * l.R + q);
+                  h[tt][e][0] = src[0];
+                  h[tt][e][1] = src[1];
+                }
+              }
+            }
+#pragma unroll
+          for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 h0 = h[tt][e & 1][0], h1 = h[tt][e & 1][1];
+              const uint4 x = w[tt][e];
+              float s = half_lo(x.x) * h0.x;
+              s = fmaf(half_hi(x.x), h0.y, s);
+              s = fmaf(half_lo(x.y), h0.z, s);
+              s = fmaf(half_hi(x.y), h0.w, s);
+              s = fmaf(half_lo(x.z), h1.x, s);
+              s = fmaf(half_hi(x.z), h1.y, s);
+              s = fmaf(half_lo(x.w), h1.z, s);
+              s = fmaf(half_hi(x.w), h1.w, s);
+              d[tt][e] += s;
+            }
+        }
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < l.R; ++q)
+#pragma unroll
+          for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (b[tt][e])
+                d[tt][e] = fmaf(__half2float(b[tt][e][q]), l.h[(size_t)(tt * 8 + 2 * s4 + (e & 1)) * l.R + q], d[tt][e]);
+      }
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = tt * 8 + 2 * s4 + (e & 1), row = row0 + ((e & 2) ? Cfg::BN / 2 : 0);
+          if (n < p.M && row < op.N) reinterpret_cast<__half*>(op.y)[(size_t)n * op.N + row] = __float2half_rn(d[tt][e]);
         }
       return;
     }
@@ -1329,12 +1416,12 @@ bool make_op(const SkinnyArgs& a, SkinnyOp* op, std::string* err) {
   return true;
 }
 
-template <int MT, int OPS_MAX, int BITS, bool WIDE, bool XCHG>
+template <int MT, int OPS_MAX, int BITS, bool WIDE, int EPI>
 cudaError_t set_smem_attr(int dev) {
   static thread_local int configured_dev = -1;
   // cudaFuncSetAttribute is per device; cheap enough to repeat on change.
   if (configured_dev != dev) {
-    cudaError_t e = cudaFuncSetAttribute(qmm_skinny_kernel<MT, OPS_MAX, BITS, WIDE, XCHG>,
+    cudaError_t e = cudaFuncSetAttribute(qmm_skinny_kernel<MT, OPS_MAX, BITS, WIDE, EPI>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          SkinnyCfg<MT, BITS, WIDE>::SMEM);
     if (e != cudaSuccess) return e;
@@ -1403,7 +1490,9 @@ cudaError_t launch_cfg(const SkinnyArgs& a, const Scratch& scratch, cudaStream_t
   cudaGetDevice(&dev);
   const DeviceInfo& di = device_info(dev);
   const bool xchg = a.ar != nullptr;
-  cudaError_t e = xchg ? set_smem_attr<MT, 1, BITS, WIDE, true>(dev) : set_smem_attr<MT, 1, BITS, WIDE, false>(dev);
+  cudaError_t e = xchg     ? set_smem_attr<MT, 1, BITS, WIDE, kEpiExchange>(dev)
+                  : a.lora ? set_smem_attr<MT, 1, BITS, WIDE, kEpiLora>(dev)
+                           : set_smem_attr<MT, 1, BITS, WIDE, kEpiPlain>(dev);
   if (e != cudaSuccess) return e;
   SkinnyLaunch<1> p{};
   if (!make_op<MT, BITS, WIDE>(a, &p.op[0], err)) return cudaErrorInvalidValue;
@@ -1425,6 +1514,7 @@ cudaError_t launch_cfg(const SkinnyArgs& a, const Scratch& scratch, cudaStream_t
   p.part = reinterpret_cast<float*>(base + kGbarBytes + kCounterBytes);
   p.status = a.status;
   p.amax = a.amax;
+  if (a.lora) p.lora = *a.lora;
   if (xchg) {
     if (!skinny_exchange_fits(a) || a.M * a.N > ar_ll_elems(a.ar->n_max) || a.ar->P < 1 ||
         a.ar->P > kArMaxRanks) {
@@ -1468,8 +1558,9 @@ cudaError_t launch_cfg(const SkinnyArgs& a, const Scratch& scratch, cudaStream_t
   }
   cfg.attrs = attr;
   cfg.numAttrs = nattr;
-  return xchg ? cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, 1, BITS, WIDE, true>, p)
-              : cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, 1, BITS, WIDE, false>, p);
+  if (xchg) return cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, 1, BITS, WIDE, kEpiExchange>, p);
+  if (a.lora) return cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, 1, BITS, WIDE, kEpiLora>, p);
+  return cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, 1, BITS, WIDE, kEpiPlain>, p);
 }
 
 // A chain of up to kSkinnyChainMax matmuls in one cooperative launch of one
@@ -1481,7 +1572,7 @@ cudaError_t launch_chain_cfg(const SkinnyArgs* ops, int n, const Scratch& scratc
   int dev = 0;
   cudaGetDevice(&dev);
   const DeviceInfo& di = device_info(dev);
-  cudaError_t e = set_smem_attr<MT, kSkinnyChainMax, 4, false, false>(dev);
+  cudaError_t e = set_smem_attr<MT, kSkinnyChainMax, 4, false, kEpiPlain>(dev);
   if (e != cudaSuccess) return e;
   static SkinnyLaunch<kSkinnyChainMax> p;  // large: build it outside the stack (copied at launch)
   static std::mutex mu;
@@ -1519,7 +1610,7 @@ cudaError_t launch_chain_cfg(const SkinnyArgs* ops, int n, const Scratch& scratc
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, kSkinnyChainMax, 4, false, false>, p);
+  return cudaLaunchKernelEx(&cfg, qmm_skinny_kernel<MT, kSkinnyChainMax, 4, false, kEpiPlain>, p);
 }
 
 }  // namespace
