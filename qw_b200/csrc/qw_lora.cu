@@ -30,7 +30,8 @@ namespace {
 // consecutive k for two products' slots, the order of k within a sum being
 // free as long as x and A agree, so no shared memory, no barrier and no copy
 // stands between the loads and the products, and a warp keeps U steps of 32 k
-// in flight.  Each adapter has its own accumulators: what a row that is not its
+// in flight.  CTAs of 128 threads fit beside the decode kernel's, which starts
+// while this one runs.  Each adapter has its own accumulators: what a row that is not its
 // own, or A of another, holds never meets it.  Sums over warps and CTAs go
 // through (distributed) shared memory in a fixed order.
 //
@@ -48,8 +49,10 @@ struct RankRows {
   int prefetch;       // bring B of the adapters present to L2 (for the decode kernel's epilogue)
 };
 
+// The second bound keeps a CTA up to rank 16 within the registers that the decode
+// kernel leaves of an SM (12 thousand at 9 to 16 rows).
 template <int RT, int WARPS, int U>
-__global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows q) {
+__global__ void __launch_bounds__(WARPS * 32, RT <= 2 ? 5 : (RT <= 4 ? 4 : 2)) rank_rows_kernel(const RankRows q) {
   constexpr int RP = 8 * RT;
   extern __shared__ float red[];  // [WARPS][16][RP], then the CTA's sum [16][RP]
   __shared__ uint32_t row_id[16];
@@ -86,14 +89,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows
   }
   __syncthreads();
   const int n = list_n;
-  if (q.prefetch) {  // each group's adapters, split over the cluster
-    for (int j = group; j < n; j += q.groups) {
-      const char* b = reinterpret_cast<const char*>(p.b) + (int64_t)list[j] * p.N * p.R * 2;
-      const int64_t lines = (p.N * p.R * 2 + 127) / 128;
-      for (int64_t i = rank * WARPS * 32 + tid; i < lines; i += (int64_t)C * WARPS * 32)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(b + (i * 128 < p.N * p.R * 2 ? i * 128 : 0)));
-    }
-  }
   const int steps = (int)(p.K / 32);
   const int s0 = (int)((int64_t)steps * rank / C), s1 = (int)((int64_t)steps * (rank + 1) / C);
   const int r = lane / 4, kq = (lane % 4) * 8;
@@ -128,6 +123,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rank_rows_kernel(const RankRows
           mma_16816(acc[t], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][t].x, w[u][t].y);
           mma_16816(acc[t], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][t].z, w[u][t].w);
         }
+    }
+    if (q.prefetch) {  // this adapter's B, split over the cluster
+      const char* b = reinterpret_cast<const char*>(p.b) + (int64_t)a * p.N * p.R * 2;
+      for (int64_t i = ((int64_t)rank * WARPS * 32 + tid) * 128; i < p.N * p.R * 2; i += (int64_t)C * WARPS * 32 * 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(b + i));
     }
     __syncthreads();  // the sums of the adapter before are read
 #pragma unroll
@@ -193,8 +193,8 @@ cudaError_t launch_rank_rows(RankRows& q, int sm_count, bool pdl, cudaStream_t s
   const int steps = (int)(q.p.K / 32);
   int C = (steps + WARPS * U - 1) / (WARPS * U);
   C = C > 8 ? 8 : C;
-  while (C > 1 && (int64_t)q.tiles * C > 2 * sm_count) --C;
-  int64_t groups = 2 * sm_count / ((int64_t)q.tiles * C);
+  while (C > 1 && (int64_t)q.tiles * C > 4 * sm_count) --C;
+  int64_t groups = 4 * sm_count / ((int64_t)q.tiles * C);
   const int64_t most = q.p.L < 16 ? q.p.L : 16;
   groups = groups > most ? most : groups;
   groups = groups < 1 ? 1 : groups;
@@ -256,11 +256,11 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);
   q.zero_vecs = (int)((zero_bytes + 15) / 16);
-  if (p.R <= 8) return launch_rank_rows<1, 16, 6>(q, sm_count, pdl, stream);
-  if (p.R <= 16) return launch_rank_rows<2, 16, 4>(q, sm_count, pdl, stream);
-  if (p.R <= 32) return launch_rank_rows<4, 16, 3>(q, sm_count, pdl, stream);
-  if (p.R <= 64) return launch_rank_rows<8, 8, 3>(q, sm_count, pdl, stream);
-  return launch_rank_rows<16, 8, 1>(q, sm_count, pdl, stream);
+  if (p.R <= 8) return launch_rank_rows<1, 4, 4>(q, sm_count, pdl, stream);
+  if (p.R <= 16) return launch_rank_rows<2, 4, 3>(q, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_rank_rows<4, 4, 2>(q, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_rank_rows<8, 4, 1>(q, sm_count, pdl, stream);
+  return launch_rank_rows<16, 4, 1>(q, sm_count, pdl, stream);
 }
 
 SkinnyLora lora_skinny_operands(const LoraArgs& p, void* ws, const void* bias) {

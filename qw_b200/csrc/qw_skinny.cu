@@ -540,7 +540,9 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
     // ------------------------------------------------------- x producer
     if (lane == 0) {
       const uint32_t x_bytes = Cfg::GPS * 128 * p.M;
-      pdl_wait();  // x is the previous kernel's output
+      // x is the previous kernel's output.  With adapters the previous kernel makes
+      // h, and started this one only once x was there: the products run beside it.
+      if (!LORA) pdl_wait();
       int slot = 0, issued = 0;
       uint32_t phase = 0;
       for (int o = 0; o < (OPS_MAX == 1 ? 1 : p.n_ops) && !*abort_flag; ++o) {
@@ -575,7 +577,7 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
   if (warp < 2 + Cfg::HW) {
     // ------------------------------------------------------------- helpers
     const int h = warp - 2;
-    pdl_wait();
+    if (!LORA) pdl_wait();
     // COLS: the B blocks are zero outside the lanes of their own group's
     // column, for the whole launch; only those lanes are written per unit.
     if (Cfg::COLS) {
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
   // SwiGLU tile a lane holds a gate row and its up row.
   const int wrow = cw * 8;
   const int r = lane / 4, s4 = lane % 4;
-  pdl_wait();
+  if (!LORA) pdl_wait();
   // Row-parallel exchange: this call's epoch, read once the previous kernel
   // of the stream (the previous call's last CTA included) has completed;
   // kept in shared memory, not in registers across the main loop.
@@ -1117,6 +1119,7 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
         ++t;
       }
       if (!seg_end) continue;
+      if (LORA) pdl_wait();  // h is there, and the counters of split tiles are cleared
       if constexpr (Cfg::COLS) {
         // a row's groups were folded in the lanes that hold the same tokens:
         // every one of them gets the sum
