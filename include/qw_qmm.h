@@ -315,7 +315,8 @@ int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64
  * put the frozen projection's dy @ dequantize(w) there), and rows without an
  * adapter are left as they are.  x f16 [..., K] (rows may be strided as in
  * qw_quantized_matmul), K a multiple of 64; dy f16 [..., N] row-contiguous; dx
- * must not overlap x or dy.  Products are accumulated in fp32; h and g enter
+ * must not overlap x or dy; x, dx, da, db and, where N is a multiple of 8, dy
+ * are 16-byte aligned.  Products are accumulated in fp32; h and g enter
  * the sums over rows with 22 significant bits relative to their largest
  * magnitude in the adapter.  Results do not depend on scheduling: the same
  * inputs give the same bits.  Non-finite values in dy or x of an adapter's

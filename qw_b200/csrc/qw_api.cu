@@ -1337,7 +1337,8 @@ int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora
   if ((M && !aligned(x->data, 16)) || (dx && !aligned(dx->data, 16)) || (da && !aligned(da->data, 16)) ||
       (db && !aligned(db->data, 16)))
     return fail(QW_EINVAL, "x, dx, da and db must be 16-byte aligned");
-  if (M && !aligned(dy->data, 2)) return fail(QW_EINVAL, "dy is misaligned");
+  if (M && !aligned(dy->data, N % 8 ? 2 : 16))
+    return fail(QW_EINVAL, "dy must be 16-byte aligned (2-byte where N is no multiple of 8)");
   if (dx && (overlap(dx, x, 0, la.x_ld) || overlap(dx, dy)))
     return fail(QW_EINVAL, "dx must not overlap x or dy");
   int dev = 0;

@@ -22,15 +22,6 @@ namespace qw {
 
 namespace {
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;  // 0 bytes read: 16 zeros written
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
@@ -72,10 +63,7 @@ constexpr uint32_t mma_desc(int m, int n, bool a_mn, bool b_mn) {
 //
 // A cluster takes a tile and its CTAs split the reduction; a CTA walks 64 values
 // of it at a time, four TMA loads deep, and within those the adapters that the
-// tile's rows name, so v is staged once however mixed the rows are.  Rows or
-// weights that TMA cannot take (dy of a width, or lora_b of a rank, that is no
-// multiple of 8) are copied by the threads instead; that path pays a proxy fence
-// a step, which waits for every copy in flight.
+// tile's rows name, so v is staged once however mixed the rows are.
 // Every adapter has columns of its own in TMEM (four adapters at a time, two
 // above rank 64) and a row reads those of its own adapter: no row's sum ever
 // meets another adapter's values.  Sums over the cluster go through distributed
@@ -88,7 +76,7 @@ constexpr int kTileRows = 128;
 struct Product {
   const __half* v;  // [M][len], rows ld apart
   int64_t ld, len;
-  const __half* w;  // [L][R][len], or for the second product [L][len][R]
+  const __half* w;  // [L][R][len], or for the second product [L][len][R8]
   float* out32;     // [M][RP] fp32, RP the kernel's padded rank (null: out16)
   __half* out16;    // [M][R8] fp16
   uint32_t* amax;   // [L] largest magnitude of out32, as fp32 bits
@@ -99,7 +87,7 @@ struct Products {
   __half* dx_zero;   // [M][K]: rows without an adapter are cleared (nullable)
   int R8;
   int tiles;         // row tiles
-  int b_tma;         // TMA can take the second product's operands
+  bool wait;         // operands come from the kernel before
   TokenLists lists;  // forward
   unsigned int* status;
 };
@@ -128,7 +116,7 @@ struct ProdShared {
   uint32_t tmem;
 };
 
-template <int RP, bool TRANS, bool TMA>
+template <int RP, bool TRANS>
 __device__ void product_tile(const Products& q, const Product& f, const CUtensorMap* map_v, const CUtensorMap* map_w,
                              int tile, uint32_t rank, uint32_t C, uint8_t* smem, ProdShared& sh) {
   using Cfg = ProdCfg<RP>;
@@ -182,10 +170,8 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   const int chunks = (int)((f.len + kChunk - 1) / kChunk);
   const int c0 = (int)((int64_t)chunks * rank / C), c1 = (int)((int64_t)chunks * (rank + 1) / C);
   const uint32_t base = smem_u32(smem);
-  const bool v16 = f.ld % 8 == 0 && f.len % 8 == 0 && (reinterpret_cast<uintptr_t>(f.v) & 15) == 0;
-  const bool w16 = !TRANS || p.R % 8 == 0;
   bool ok = true;        // a bounded wait that ran out: go on without waiting
-  uint32_t it0 = 0, vit0 = 0;  // TMA: steps and chunks of earlier rounds
+  uint32_t it0 = 0, vit0 = 0;  // steps and chunks of earlier rounds
   constexpr uint32_t kDesc = mma_desc(kTileRows, TRANS ? Cfg::BLOCK : RP, false, TRANS);
   auto multiply = [&](int chunk, int j, uint32_t vs, uint32_t ws) {
     const uint64_t a = operand_k(vs), b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
@@ -194,121 +180,53 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       tc_mma_ss(sh.tmem + j * Cfg::BLOCK, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
                 chunk > 0 || kk > 0);
   };
-  uint32_t parities = 0; // copies: of done[i], a bit each: flips with every use waited for
-  auto wait_step = [&](int step) {
-    const int i = step % kStages;
-    ok = ok && mbar_wait(&sh.done[i], (parities >> i) & 1u, q.status, kDevTimeoutAccum);
-    parities ^= 1u << i;
-  };
 
   for (int j0 = 0; j0 < n; j0 += Cfg::GROUP) {
     const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
     const int steps = (c1 - c0) * nj;
-    if constexpr (TMA) {
-      if (warp == 1 && lane == 0) {  // loads
-        uint32_t it = it0, vit = vit0;
-        for (int c = c0; c < c1; ++c, ++vit) {
-          for (int j = 0; j < nj; ++j, ++it) {
-            const uint32_t s = it % kStages;
-            if (it >= kStages)
-              ok = ok && mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
-            mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) + (TRANS ? Cfg::W_STAGE : RP * 128)));
-            if (j == 0)
-              tma_load_2d(smem + (vit % kStages) * Cfg::STAGE, map_v, &sh.full[s], c * kChunk, (int)m0);
-            uint8_t* dst = smem + s * Cfg::STAGE + Cfg::V_STAGE;
-            const int a = (int)sh.list[j0 + j];
-            if (TRANS) {
-              for (int b = 0; b < Cfg::BLOCK / 64; ++b)
-                tma_load_3d(dst + b * 8192, map_w, &sh.full[s], b * 64, c * kChunk, a);
-            } else {
-              tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
-            }
-          }
-        }
-      } else if (warp == 0 && lane == 0) {  // products
-        uint32_t it = it0, vit = vit0;
-        for (int c = c0; c < c1; ++c, ++vit) {
-          for (int j = 0; j < nj; ++j, ++it) {
-            const uint32_t s = it % kStages;
-            ok = ok && mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
-            tc_fence_after();
-            multiply(c - c0, j, base + (vit % kStages) * Cfg::STAGE, base + s * Cfg::STAGE + Cfg::V_STAGE);
-            tc_commit(&sh.done[s]);
-          }
-        }
-      }
-      it0 += (uint32_t)steps;
-      vit0 += (uint32_t)(c1 - c0);
-      __syncwarp();
-      // The last step's barrier has seen every earlier use waited for by the
-      // thread that loads, but for those of the last turn of the ring, which
-      // complete in order.
-      if (steps > 0) {
-        __syncthreads();
-        ok = ok && mbar_wait(&sh.done[(it0 - 1) % kStages], ((it0 - 1) / kStages) & 1, q.status, kDevTimeoutAccum);
-      }
-    } else {
-      auto load = [&](int step) {
-        const int64_t i0 = (int64_t)(c0 + step / nj) * kChunk;
-        const int j = step % nj;
-        if (j == 0) {
-          const uint32_t dst = base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE;
-#pragma unroll
-          for (int k = 0; k < kTileRows * 8 / kProdThreads; ++k) {
-            const int row = (k * kProdThreads + tid) / 8, piece = tid % 8;
-            const int64_t i = i0 + piece * 8;
-            const bool in = m0 + row < p.M && i < f.len;
-            const __half* src = f.v + (in ? (m0 + row) * f.ld + i : 0);
-            const uint32_t at = dst + swizzled(row, piece);
-            if (v16) cp_async16(at, src, in);
-            else sts16(at, load_halves(src, in ? f.len - i : 0));
-          }
-        }
-        const uint32_t dst = base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE;
-        const __half* w = f.w + (int64_t)sh.list[j0 + j] * p.R * f.len;
-        constexpr int kPieces = 8 * RP;
-#pragma unroll
-        for (int k = 0; k < kPieces / kProdThreads; ++k) {
-          const int e = k * kProdThreads + tid;
+    if (warp == 1 && lane == 0) {  // loads
+      uint32_t it = it0, vit = vit0;
+      for (int c = c0; c < c1; ++c, ++vit) {
+        for (int j = 0; j < nj; ++j, ++it) {
+          const uint32_t s = it % kStages;
+          if (it >= kStages)
+            ok = ok && mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
+          mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) + (TRANS ? Cfg::W_STAGE : RP * 128)));
+          if (j == 0)
+            tma_load_2d(smem + (vit % kStages) * Cfg::STAGE, map_v, &sh.full[s], c * kChunk, (int)m0);
+          uint8_t* dst = smem + s * Cfg::STAGE + Cfg::V_STAGE;
+          const int a = (int)sh.list[j0 + j];
           if (TRANS) {
-            const int row = e / (RP / 8), r = e % (RP / 8) * 8;
-            const bool in = i0 + row < f.len && r < p.R;
-            const __half* src = w + (in ? (i0 + row) * p.R + r : 0);
-            const uint32_t at = dst + (r / 64) * 8192 + swizzled(row, r % 64 / 8);
-            if (w16) cp_async16(at, src, in);
-            else sts16(at, load_halves(src, in ? p.R - r : 0));
+            for (int b = 0; b < Cfg::BLOCK / 64; ++b)
+              tma_load_3d(dst + b * 8192, map_w, &sh.full[s], b * 64, c * kChunk, a);
           } else {
-            const int r = e / 8, piece = e % 8;
-            const bool in = r < p.R && i0 + piece * 8 < f.len;
-            cp_async16(dst + swizzled(r, piece), w + (in ? (int64_t)r * f.len + i0 + piece * 8 : 0), in);
+            tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
           }
         }
-      };
-#pragma unroll
-      for (int s = 0; s < kStages - 1; ++s) {
-        if (s < steps) load(s);
-        cp_async_commit();
       }
-      for (int step = 0; step < steps; ++step) {
-        cp_async_wait<kStages - 2>();
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncthreads();
-        if (tid == 0) {
+    } else if (warp == 0 && lane == 0) {  // products
+      uint32_t it = it0, vit = vit0;
+      for (int c = c0; c < c1; ++c, ++vit) {
+        for (int j = 0; j < nj; ++j, ++it) {
+          const uint32_t s = it % kStages;
+          ok = ok && mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
           tc_fence_after();
-          multiply(step / nj, step % nj, base + (uint32_t)((step / nj) % kStages) * Cfg::STAGE,
-                   base + (uint32_t)(step % kStages) * Cfg::STAGE + Cfg::V_STAGE);
-          tc_commit(&sh.done[step % kStages]);
+          multiply(c - c0, j, base + (vit % kStages) * Cfg::STAGE, base + s * Cfg::STAGE + Cfg::V_STAGE);
+          tc_commit(&sh.done[s]);
         }
-        // the products that read the stage loaded next are the previous step's
-        if (step > 0) wait_step(step - 1);
-        if (step + kStages - 1 < steps) load(step + kStages - 1);
-        cp_async_commit();
       }
-      if (steps > 0) wait_step(steps - 1);
+    }
+    it0 += (uint32_t)steps;
+    vit0 += (uint32_t)(c1 - c0);
+    __syncwarp();
+    // The last step's barrier has seen every earlier use waited for by the
+    // thread that loads, but for those of the last turn of the ring, which
+    // complete in order.
+    if (steps > 0) {
+      __syncthreads();
+      ok = ok && mbar_wait(&sh.done[(it0 - 1) % kStages], ((it0 - 1) / kStages) & 1, q.status, kDevTimeoutAccum);
     }
     tc_fence_after();
-    cp_async_wait<0>();
     __syncthreads();
 
     // each row's own columns, to shared memory
@@ -384,9 +302,9 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const __gri
   uint8_t* smem = prod_smem + ((1024u - (smem_u32(prod_smem) & 1023u)) & 1023u);
   const uint32_t rank = cluster_rank(), C = cluster_size();
   const int unit = (int)(blockIdx.x / C);
-  // The operands were there before the kernel that this launch may overlap (the
-  // plan started its dependents only once they were); a forward waits.
-  if (q.lists.tile) pdl_wait();
+  // A gradient's operands were there before the plan started this launch, unless
+  // it lays dy or lora_b out anew; a forward waits for the kernel before it.
+  if (q.wait) pdl_wait();
   pdl_launch_dependents();
   const bool first = unit < q.tiles, second = !first && q.b.v && unit < 2 * q.tiles;
   if (!first && !second) {
@@ -407,13 +325,8 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (first) {
-    product_tile<RP, false, true>(q, q.a, &maps.av, &maps.aw, unit, rank, C, smem, sh);
-  } else if (q.b_tma) {
-    product_tile<RP, true, true>(q, q.b, &maps.bv, &maps.bw, unit - q.tiles, rank, C, smem, sh);
-  } else {
-    product_tile<RP, true, false>(q, q.b, nullptr, nullptr, unit - q.tiles, rank, C, smem, sh);
-  }
+  if (first) product_tile<RP, false>(q, q.a, &maps.av, &maps.aw, unit, rank, C, smem, sh);
+  else product_tile<RP, true>(q, q.b, &maps.bv, &maps.bw, unit - q.tiles, rank, C, smem, sh);
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -448,10 +361,9 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
                         CU_TENSOR_MAP_SWIZZLE_128B, err))
       return cudaErrorInvalidValue;
   }
-  q.b_tma = q.b.v && q.b.ld % 8 == 0 && reinterpret_cast<uintptr_t>(q.b.v) % 16 == 0 && p.R % 8 == 0;
-  if (q.b_tma) {
-    const uint64_t dims[3] = {(uint64_t)p.R, (uint64_t)p.N, (uint64_t)p.L};
-    const uint64_t strides[2] = {(uint64_t)p.R * 2, (uint64_t)p.R * p.N * 2};
+  if (q.b.v) {
+    const uint64_t dims[3] = {(uint64_t)q.R8, (uint64_t)p.N, (uint64_t)p.L};
+    const uint64_t strides[2] = {(uint64_t)q.R8 * 2, (uint64_t)q.R8 * p.N * 2};
     const uint32_t box[3] = {64, kChunk, 1};
     if (!encode_tmap_2d(&maps.bv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, q.b.v, (uint64_t)p.N, (uint64_t)p.M,
                         (uint64_t)q.b.ld * 2, kChunk, kTileRows, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
@@ -526,12 +438,36 @@ __device__ int block_scan(int v, int* warp_tot) {  // exclusive prefix over the 
   return before + incl - v;
 }
 
+// Rows of `width` halves, laid out anew `pitch` apart (a multiple of 8, zero
+// behind the width): what TMA cannot take as it is.
+struct Repack {
+  const __half* src;
+  __half* dst;  // null: nothing to do
+  int64_t rows, width, ld, pitch;
+};
+__device__ __forceinline__ void repack(const Repack& r, int64_t first, int64_t step) {
+  const int64_t pieces = r.pitch / 8;
+  for (int64_t i = first; i < r.rows * pieces; i += step) {
+    const int64_t row = i / pieces, c = i % pieces * 8;
+    *reinterpret_cast<uint4*>(r.dst + row * r.pitch + c) = load_halves(r.src + row * r.ld + c, r.width - c);
+  }
+}
+
+// Block 0 plans, the others lay out dy and lora_b anew where that is needed.
 __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs p, const Plan plan, int warps,
-                                                                 int chunk_rows, int64_t counters) {
+                                                                 int chunk_rows, int64_t counters, const Repack dy,
+                                                                 const Repack b) {
   extern __shared__ int hist[];  // [warps][L]
   __shared__ int warp_tot[32];
   pdl_wait();
   pdl_launch_dependents();
+  if (blockIdx.x > 0) {
+    const int64_t first = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x;
+    const int64_t step = (int64_t)(gridDim.x - 1) * kPlanThreads;
+    if (dy.dst) repack(dy, first, step);
+    if (b.dst) repack(b, first, step);
+    return;
+  }
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int L = (int)p.L;
   for (int i = tid; i < 2 * L; i += kPlanThreads) plan.amax[i] = 0u;
@@ -625,8 +561,6 @@ constexpr int kVStages = 3;
 
 struct Sums {
   LoraArgs p;
-  const __half* dy;
-  int64_t dy_ld;
   const float *h, *g;  // [M][RP]
   Plan plan;
   __half* dx;
@@ -634,7 +568,6 @@ struct Sums {
   float* part;         // [chunk of a joint sum][tiles][RP][kCols]
   bool add_dx;
   int x_tiles, tiles;  // column tiles of x, and of x and dy together
-  int dy_tma;          // TMA can take dy's rows
   unsigned int* status;
 };
 struct SumMaps {
@@ -752,7 +685,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         }
         ++ai;
       }
-      const bool tma = t.is_x || q.dy_tma;
       for (int step = 0; step < t.steps; ++step, ++it) {
         const uint32_t s = it % kVStages;
         int r[4];  // a lane's four rows; past the end, the chunk's last row (its h or g is taken as zero)
@@ -762,17 +694,12 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           r[k] = __ldcg(q.plan.order + t.ck.start + (at < t.ck.count ? at : t.ck.count - 1));
         }
         if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[s], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
-        if (lane == 0) {
-          if (tma) mbar_arrive_expect_tx(&sh.vfull[s], Cfg::V_STAGE);
-          else mbar_arrive(&sh.vfull[s]);  // the workers copy
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&sh.vfull[s], Cfg::V_STAGE);
         __syncwarp();
-        if (tma) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-            tma_gather4(base + s * Cfg::V_STAGE + b * (kStepRows * 128) + lane * 512, t.is_x ? &maps.x : &maps.dy,
-                        &sh.vfull[s], (int)t.col0 + b * 64, r);
-        }
+        for (int b = 0; b < 2; ++b)
+          tma_gather4(base + s * Cfg::V_STAGE + b * (kStepRows * 128) + lane * 512, t.is_x ? &maps.x : &maps.dy,
+                      &sh.vfull[s], (int)t.col0 + b * 64, r);
       }
     }
   } else if (warp == 9) {
@@ -929,19 +856,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
           asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + Cfg::G_HALF), "r"(lo[0]), "r"(lo[1]) : "memory");
         }
-        if (!t.is_x && !q.dy_tma) {
-          // Rows that TMA cannot take.  The slot's last products are three steps
-          // back, done by the wait above (for those of at most two steps back).
-          for (int x = tid; x < kStepRows * kCols / 8; x += kWorkers) {
-            const int row = x / (kCols / 8), pc = x % (kCols / 8);
-            const int at = step * kStepRows + row;
-            const int64_t col = t.col0 + pc * 8;
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (at < ck.count && col < t.width)
-              w = load_halves(q.dy + (int64_t)__ldcg(order + at) * q.dy_ld + col, t.width - col);
-            sts16(base + it % kVStages * Cfg::V_STAGE + pc / 8 * (kStepRows * 128) + swizzled(row, pc % 8), w);
-          }
-        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.gfull[gb]);
@@ -1046,7 +960,8 @@ constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct GradSpace {
   int RP, x_tiles, tiles, chunk_rows;
   int64_t max_chunks, joints;
-  size_t h, g, chunks, order, amax, count, part, end;
+  int64_t dy_pitch, b_pitch;  // of dy and lora_b laid out anew (0: as they are)
+  size_t h, g, chunks, order, amax, count, part, dy, b, end;
 };
 GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_count) {
   GradSpace s;
@@ -1077,6 +992,10 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.amax = take((size_t)2 * L * sizeof(uint32_t));
   s.count = take((size_t)s.joints * s.tiles * sizeof(uint32_t));
   s.part = take((size_t)parts * s.tiles * kCols * s.RP * sizeof(float));
+  s.dy_pitch = N % 8 ? (N + 7) / 8 * 8 : 0;
+  s.b_pitch = R % 8 ? (R + 7) / 8 * 8 : 0;
+  s.dy = take((size_t)M * s.dy_pitch * sizeof(__half));
+  s.b = take((size_t)L * N * s.b_pitch * sizeof(__half));
   s.end = at;
   return s;
 }
@@ -1119,6 +1038,7 @@ cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, voi
   q.a.w = static_cast<const __half*>(p.a);
   q.a.out16 = static_cast<__half*>(h16);
   q.lists = lists;
+  q.wait = true;
   q.status = status;
   return dispatch_products(q, sm_count, pdl, stream, err);
 }
@@ -1142,6 +1062,9 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
   plan.order = reinterpret_cast<int*>(base + s.order);
   plan.amax = reinterpret_cast<uint32_t*>(base + s.amax);
   plan.count = reinterpret_cast<uint32_t*>(base + s.count);
+  const __half *dy = static_cast<const __half*>(g.dy), *lora_b = static_cast<const __half*>(p.b);
+  int64_t dy_ld = g.dy_ld;
+  bool anew = false;
   {
     // a warp's counters for every adapter; as many warps as fit 192 KB
     int warps = (int)(192 * 1024 / (p.L * 4));
@@ -1154,8 +1077,20 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
       if (e != cudaSuccess) return e;
       configured_dev = dev;
     }
-    lora_plan_kernel<<<1, kPlanThreads, (size_t)warps * p.L * 4, stream>>>(p, plan, warps, s.chunk_rows,
-                                                                          s.joints * s.tiles);
+    Repack rdy{}, rb{};
+    if (s.dy_pitch && p.M)
+      rdy = Repack{dy, reinterpret_cast<__half*>(base + s.dy), p.M, p.N, p.N, s.dy_pitch};
+    if (s.b_pitch) rb = Repack{lora_b, reinterpret_cast<__half*>(base + s.b), p.L * p.N, p.R, p.R, s.b_pitch};
+    const int64_t pieces = (rdy.dst ? p.M * (s.dy_pitch / 8) : 0) + (rb.dst ? p.L * p.N * (s.b_pitch / 8) : 0);
+    const int64_t blocks = (pieces + kPlanThreads - 1) / kPlanThreads;
+    lora_plan_kernel<<<1 + (unsigned)(blocks < 2 * sm_count ? blocks : 2 * sm_count), kPlanThreads,
+                       (size_t)warps * p.L * 4, stream>>>(p, plan, warps, s.chunk_rows, s.joints * s.tiles, rdy, rb);
+    if (rdy.dst) {
+      dy = rdy.dst;
+      dy_ld = s.dy_pitch;
+    }
+    if (rb.dst) lora_b = rb.dst;
+    anew = rdy.dst || rb.dst;
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (p.M) {
@@ -1168,10 +1103,11 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
     q.a.w = static_cast<const __half*>(p.a);
     q.a.out32 = reinterpret_cast<float*>(base + s.h);
     q.a.amax = plan.amax;
-    q.b.v = static_cast<const __half*>(g.dy);
-    q.b.ld = g.dy_ld;
+    q.b.v = dy;
+    q.b.ld = dy_ld;
     q.b.len = p.N;
-    q.b.w = static_cast<const __half*>(p.b);
+    q.b.w = lora_b;
+    q.wait = anew;
     q.b.out32 = reinterpret_cast<float*>(base + s.g);
     q.b.amax = plan.amax + p.L;
     q.status = g.status;
@@ -1180,8 +1116,6 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
   }
   Sums q{};
   q.p = p;
-  q.dy = static_cast<const __half*>(g.dy);
-  q.dy_ld = g.dy_ld;
   q.h = reinterpret_cast<const float*>(base + s.h);
   q.g = reinterpret_cast<const float*>(base + s.g);
   q.plan = plan;
@@ -1207,9 +1141,8 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
     if (!encode_tmap_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, (uint64_t)p.K, (uint64_t)p.M,
                         (uint64_t)p.x_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
       return cudaErrorInvalidValue;
-    q.dy_tma = g.dy_ld % 8 == 0 && reinterpret_cast<uintptr_t>(g.dy) % 16 == 0;
-    if (q.dy_tma && !encode_tmap_2d(&maps.dy, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, g.dy, (uint64_t)p.N, (uint64_t)p.M,
-                                    (uint64_t)g.dy_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
+    if (!encode_tmap_2d(&maps.dy, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy, (uint64_t)p.N, (uint64_t)p.M,
+                        (uint64_t)dy_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
       return cudaErrorInvalidValue;
   }
   const int64_t items = s.max_chunks * s.tiles;

@@ -107,12 +107,22 @@ struct PrefillParams {
 // 8 consecutive ranks of one lora_b row from rank r0 on, zero past the rank.
 __device__ __forceinline__ uint4 lora_chunk(const __half* row, int r0, int R) {
   if (R % 8 == 0) return __ldg(reinterpret_cast<const uint4*>(row + r0));
-  uint32_t w[4];
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  if (R % 4 == 0) {  // rows of 8-byte alignment
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = r0 + 2 * i < R ? __half_as_ushort(row[r0 + 2 * i]) : 0;
-    const uint32_t hi = r0 + 2 * i + 1 < R ? __half_as_ushort(row[r0 + 2 * i + 1]) : 0;
-    w[i] = lo | (hi << 16);
+    for (int i = 0; i < 4; i += 2)
+      if (r0 + 2 * i < R) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + r0 + 2 * i));
+        w[i] = v.x;
+        w[i + 1] = v.y;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = r0 + 2 * i < R ? __half_as_ushort(row[r0 + 2 * i]) : 0;
+      const uint32_t hi = r0 + 2 * i + 1 < R ? __half_as_ushort(row[r0 + 2 * i + 1]) : 0;
+      w[i] = lo | (hi << 16);
+    }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
