@@ -129,7 +129,22 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   sh.slot_max[tid] = 0u;
   __syncthreads();
   const uint32_t my_id = sh.row_id[tid];
-  {
+  const bool none = my_id == 0xFFFFFFFFu;
+  const bool some_none = __syncthreads_or(none && m0 + tid < p.M);
+  {  // one adapter in the whole tile, mostly
+    const uint32_t low = __reduce_min_sync(0xffffffffu, my_id);
+    if (lane == 0) sh.list[warp] = low;
+  }
+  __syncthreads();
+  const uint32_t low = min(min(sh.list[0], sh.list[1]), min(sh.list[2], sh.list[3]));
+  if (__syncthreads_and(none || my_id == low)) {
+    sh.row_slot[tid] = none ? my_id : 0u;
+    if (tid == 0) {
+      sh.list[0] = low;
+      sh.list_n = low != 0xFFFFFFFFu;
+    }
+    __syncthreads();
+  } else {
     const uint4* ids = reinterpret_cast<const uint4*>(sh.row_id);
     int first = tid;
     for (int k = tid / 4; k >= 0; --k) {  // four rows at a time, downwards
@@ -155,7 +170,7 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   }
   const int n = sh.list_n;
   const int my_slot = (int)sh.row_slot[tid];  // -1: none
-  if (!TRANS && q.dx_zero) {  // rows without an adapter
+  if (!TRANS && q.dx_zero && some_none) {  // rows without an adapter
     for (int row = warp; row < kTileRows && m0 + row < p.M; row += kProdThreads / 32) {
       if (sh.row_id[row] != 0xFFFFFFFFu) continue;
       uint4* dst = reinterpret_cast<uint4*>(q.dx_zero + (m0 + row) * p.K);
@@ -260,12 +275,18 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       const int slot = (int)sh.row_slot[row];
       if (slot < j0 || slot >= j0 + nj) continue;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t k = 0; k < C; ++k) {
-        const float4 t = ld_cluster_f32x4(sums + row * Cfg::PITCH + c, k);
-        v.x += t.x;
-        v.y += t.y;
-        v.z += t.z;
-        v.w += t.w;
+      for (uint32_t k0 = 0; k0 < C; k0 += 8) {  // in rank order, eight reads in flight
+        float4 t[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+          t[k] = k0 + k < C ? ld_cluster_f32x4(sums + row * Cfg::PITCH + c, k0 + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          v.x += t[k].x;
+          v.y += t[k].y;
+          v.z += t[k].z;
+          v.w += t[k].w;
+        }
       }
       const float s = p.scales ? p.scales[sh.row_id[row]] : 1.f;
       v.x *= s;
@@ -342,8 +363,10 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev != dev) {
-    const cudaError_t e = cudaFuncSetAttribute(lora_products_kernel<RP>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(lora_products_kernel<RP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Cfg::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(lora_products_kernel<RP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     configured_dev = dev;
   }
@@ -374,9 +397,11 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   const int products = q.b.v ? 2 : 1;
   int64_t most = (q.a.len + kChunk - 1) / kChunk;
   if (q.b.v && (q.b.len + kChunk - 1) / kChunk > most) most = (q.b.len + kChunk - 1) / kChunk;
-  // two CTAs an SM from the clusters' splits
-  int C = most < 8 ? (int)most : 8;
-  while (C > 1 && (int64_t)products * q.tiles * C > 2 * sm_count) --C;
+  // Splits for about four CTAs an SM, each two SM's worth in flight: the loads of
+  // an SM run at 46 GB/s (a 128-byte row in 5 cycles), so all of them are needed.
+  // 16 CTAs to a cluster, twice the portable size, where the tiles are few.
+  int C = most < 16 ? (int)most : 16;
+  while (C > 1 && (int64_t)products * q.tiles * C > (C > 8 ? 1 : 4) * sm_count) --C;
   const int64_t units = (int64_t)products * q.tiles + q.lists.tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * C));
@@ -537,11 +562,13 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
 // -------------------------------------------------------------------- sums
 // A chunk of an adapter's rows and 128 columns of x (dA, and dx of those rows)
 // or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step:
-//   warp 8      gathers the step's rows of x or dy (TMA, four rows an instruction),
-//               and an item's lora_a columns;
+//   warps 8-10  copy the rows of x or dy (cp.async), a step each in turn, so that
+//               a warp's proxy fence waits for its own step's copies alone and
+//               three steps are in flight (TMA's four-row gathers were issued at
+//               one in 80 cycles: 12 GB/s an SM); warp 8 also an item's lora_a;
 //   warps 0-7   split the step's h or g for the tensor cores (below), and while
 //               those multiply take the step before's dx from TMEM to memory;
-//   warp 9      issues tcgen05.mma: D[columns][ranks] += v^T (h or g), both
+//   warp 11     issues tcgen05.mma: D[columns][ranks] += v^T (h or g), both
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers.
 // HBM-bound by x and dy; at rank 64 the products take about half that time.
@@ -556,11 +583,14 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
 constexpr int kCols = 128;
 constexpr int kStepRows = 128;
 constexpr int kWorkers = 256;
-constexpr int kSumThreads = kWorkers + 64;
-constexpr int kVStages = 3;
+constexpr int kVStages = 3;  // and as many warps that copy
+constexpr int kMmaWarp = kWorkers / 32 + kVStages;
+constexpr int kSumThreads = (kMmaWarp + 1) * 32;
 
 struct Sums {
   LoraArgs p;
+  const __half* dy;
+  int64_t dy_ld;
   const float *h, *g;  // [M][RP]
   Plan plan;
   __half* dx;
@@ -570,10 +600,6 @@ struct Sums {
   int x_tiles, tiles;  // column tiles of x, and of x and dy together
   unsigned int* status;
 };
-struct SumMaps {
-  CUtensorMap x, dy, a;  // rows of x and dy (one row of 64 columns a box), lora_a 3-D
-};
-
 template <int RP>
 struct SumCfg {
   static constexpr int NRANK = RP > 64 ? 128 : 64;               // ranks of a D, whole 128-byte rows
@@ -594,13 +620,10 @@ struct SumShared {
   int last;
 };
 
-// Four rows of 64 columns from column c, one under the other.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c, const int (&r)[4]) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
-      "%6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-      : "memory");
+// 16 bytes from src (zeros where !valid)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
@@ -626,7 +649,7 @@ __device__ __forceinline__ Item item_at(const Sums& q, int64_t i) {
 
 template <int RP>
 __global__ void __launch_bounds__(kSumThreads, 1)
-    lora_sums_kernel(const __grid_constant__ Sums q, const __grid_constant__ SumMaps maps) {
+    lora_sums_kernel(const __grid_constant__ Sums q, const __grid_constant__ CUtensorMap map_a) {
   using Cfg = SumCfg<RP>;
   extern __shared__ uint8_t sum_smem[];
   __shared__ SumShared sh;
@@ -652,7 +675,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     mbar_init(&sh.aempty, 1);
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
@@ -670,39 +693,54 @@ __global__ void __launch_bounds__(kSumThreads, 1)
   const int64_t items = (int64_t)*q.plan.total * q.tiles;
   bool ok = true;  // a bounded wait that ran out: go on without waiting
 
-  if (warp == 8) {
-    // -------------------------------------------------------------- loads
-    uint32_t it = 0, ai = 0;
+  if (warp >= kWorkers / 32 && warp < kMmaWarp) {
+    // ------------------------------------------------------------- copies
+    const int slot = warp - kWorkers / 32;
+    uint32_t it = 0, ai = 0, uses = 0;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
       const Item t = item_at(q, i);
       if (t.steps == 0) continue;
-      if (t.dx) {
+      if (t.dx && slot == 0) {
         if (lane == 0) {
           if (ai > 0) ok = ok && mbar_wait(&sh.aempty, (ai - 1) & 1, q.status, kDevTimeoutEmpty);
           mbar_arrive_expect_tx(&sh.afull, RP * kCols * 2);
           for (int b = 0; b < 2; ++b)
-            tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &maps.a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
+            tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &map_a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
         }
+        __syncwarp();
         ++ai;
       }
+      const __half* v = t.is_x ? reinterpret_cast<const __half*>(p.x) : q.dy;
+      const int64_t ld = t.is_x ? p.x_ld : q.dy_ld;
+      const int64_t c = t.col0 + lane % 16 * 8;
+      const bool in_c = c < t.width;
       for (int step = 0; step < t.steps; ++step, ++it) {
-        const uint32_t s = it % kVStages;
-        int r[4];  // a lane's four rows; past the end, the chunk's last row (its h or g is taken as zero)
+        if (it % kVStages != (uint32_t)slot) continue;
+        int at[4];  // the step's rows, 32 k + lane
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int at = step * kStepRows + lane * 4 + k;
-          r[k] = __ldcg(q.plan.order + t.ck.start + (at < t.ck.count ? at : t.ck.count - 1));
+          const int r = step * kStepRows + 32 * k + lane;
+          at[k] = r < t.ck.count ? __ldcg(q.plan.order + t.ck.start + r) : -1;
         }
-        if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[s], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
-        if (lane == 0) mbar_arrive_expect_tx(&sh.vfull[s], Cfg::V_STAGE);
-        __syncwarp();
+        if (uses > 0) ok = ok && mbar_wait(&sh.vempty[slot], (uses - 1) & 1, q.status, kDevTimeoutEmpty);
+        ++uses;
+        const uint32_t dst = base + slot * Cfg::V_STAGE + lane % 16 / 8 * (kStepRows * 128);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          tma_gather4(base + s * Cfg::V_STAGE + b * (kStepRows * 128) + lane * 512, t.is_x ? &maps.x : &maps.dy,
-                      &sh.vfull[s], (int)t.col0 + b * 64, r);
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {  // two rows of 256 bytes
+            const int row = 32 * k + 2 * j + lane / 16;
+            const int m = __shfl_sync(0xffffffffu, at[k], 2 * j + lane / 16);
+            const bool in = in_c && m >= 0;
+            cp_async16(dst + swizzled(row, lane % 8), v + (in ? m * ld + c : 0), in);
+          }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.vfull[slot]);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------- products
     uint32_t it = 0, dxs = 0, sums = 0, ai = 0;
     if (lane == 0) {
@@ -777,23 +815,37 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       const float* src = t.is_x ? q.g : q.h;
       const int piece = tid % (RP / 4), row0 = tid / (RP / 4);
       constexpr int kRowStep = kWorkers / (RP / 4);
+      // A worker's rows of a step, and their h or g a step later: the row numbers
+      // are read a step before they are needed.
       float4 v[Cfg::PER];
-      auto fetch = [&](int step) {
+      int at[Cfg::PER];
+      auto fetch_rows = [&](int step) {
 #pragma unroll
         for (int k = 0; k < Cfg::PER; ++k) {
-          const int at = step * kStepRows + row0 + k * kRowStep;
-          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (at < ck.count) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)__ldcg(order + at) * RP) + piece);
+          const int r = step * kStepRows + row0 + k * kRowStep;
+          at[k] = r < ck.count ? __ldcg(order + r) : -1;
         }
       };
+      auto fetch = [&]() {
+#pragma unroll
+        for (int k = 0; k < Cfg::PER; ++k) {
+          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at[k] >= 0) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)at[k] * RP) + piece);
+        }
+      };
+      int dx_row = -1;  // the row of dx that this lane writes next
+      auto fetch_dx_row = [&](int step) {
+        const int r = step * kStepRows + quarter * 32 + lane;
+        dx_row = r < ck.count ? __ldcg(order + r) : -1;
+      };
       // dx of a step whose products are done: a row a lane, 64 columns a warp
-      auto store_dx = [&](int step) {
+      auto store_dx = [&](int next) {
         const uint32_t b = dxs & 1;
+        const bool in = dx_row >= 0;
+        __half* row = q.dx + (int64_t)(in ? dx_row : 0) * p.K;
+        if (next < t.steps) fetch_dx_row(next);
         ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
         tc_fence_after();
-        const int at = step * kStepRows + quarter * 32 + lane;
-        const bool in = at < ck.count;
-        __half* row = q.dx + (int64_t)(in ? __ldcg(order + at) : 0) * p.K;
 #pragma unroll
         for (int c = 0; c < 64; c += 16) {
           const int64_t col = t.col0 + upper * 64 + c;
@@ -832,7 +884,12 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         if (lane == 0) mbar_arrive(&sh.dxempty[b]);
         ++dxs;
       };
-      if (t.steps > 0) fetch(0);
+      if (t.steps > 0) {
+        fetch_rows(0);
+        if (t.dx) fetch_dx_row(0);
+        fetch();
+        if (t.steps > 1) fetch_rows(1);
+      }
       for (int step = 0; step < t.steps; ++step, ++it) {
         const uint32_t gb = it % Cfg::G_BUFS;
         // the products that read this buffer last are done
@@ -859,10 +916,11 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.gfull[gb]);
-        if (step + 1 < t.steps) fetch(step + 1);
-        if (t.dx && step > 0) store_dx(step - 1);
+        if (step + 1 < t.steps) fetch();
+        if (step + 2 < t.steps) fetch_rows(step + 2);
+        if (t.dx && step > 0) store_dx(step);
       }
-      if (t.dx && t.steps > 0) store_dx(t.steps - 1);
+      if (t.dx && t.steps > 0) store_dx(t.steps);
       if (!t.sum) continue;
 
       // D[column][rank] of this chunk (a column a lane, 16 ranks at a time over two warps), then the sum's
@@ -947,7 +1005,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1001,7 +1059,7 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
 }
 
 template <int RP>
-cudaError_t launch_sums(const Sums& q, const SumMaps& maps, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
+cudaError_t launch_sums(const Sums& q, const CUtensorMap& map_a, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
   using Cfg = SumCfg<RP>;
   static thread_local int configured_dev = -1;
   int dev = 0;
@@ -1022,7 +1080,7 @@ cudaError_t launch_sums(const Sums& q, const SumMaps& maps, int64_t items, int s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RP>, q, maps);
+  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RP>, q, map_a);
 }
 
 }  // namespace
@@ -1127,29 +1185,23 @@ cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws
   q.x_tiles = s.x_tiles;
   q.tiles = s.tiles;
   q.status = g.status;
-  SumMaps maps;
-  std::memset(&maps, 0, sizeof(maps));
+  q.dy = dy;
+  q.dy_ld = dy_ld;
+  CUtensorMap map_a;
+  std::memset(&map_a, 0, sizeof(map_a));
   {
     const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.R, (uint64_t)p.L};
     const uint64_t strides[2] = {(uint64_t)p.K * 2, (uint64_t)p.K * p.R * 2};
     const uint32_t box[3] = {64, (uint32_t)s.RP, 1};
-    if (!encode_tmap_3d(&maps.a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (!encode_tmap_3d(&map_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
                         err))
       return cudaErrorInvalidValue;
   }
-  if (p.M) {  // a gathered box is one row
-    if (!encode_tmap_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, (uint64_t)p.K, (uint64_t)p.M,
-                        (uint64_t)p.x_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
-      return cudaErrorInvalidValue;
-    if (!encode_tmap_2d(&maps.dy, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy, (uint64_t)p.N, (uint64_t)p.M,
-                        (uint64_t)dy_ld * 2, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, err))
-      return cudaErrorInvalidValue;
-  }
   const int64_t items = s.max_chunks * s.tiles;
-  if (p.R <= 16) return launch_sums<16>(q, maps, items, sm_count, pdl, stream);
-  if (p.R <= 32) return launch_sums<32>(q, maps, items, sm_count, pdl, stream);
-  if (p.R <= 64) return launch_sums<64>(q, maps, items, sm_count, pdl, stream);
-  return launch_sums<128>(q, maps, items, sm_count, pdl, stream);
+  if (p.R <= 16) return launch_sums<16>(q, map_a, items, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_sums<32>(q, map_a, items, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_sums<64>(q, map_a, items, sm_count, pdl, stream);
+  return launch_sums<128>(q, map_a, items, sm_count, pdl, stream);
 }
 
 }  // namespace qw
