@@ -318,7 +318,7 @@ int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64
  * must not overlap x or dy; x, dx, da, db and, where N is a multiple of 8, dy
  * are 16-byte aligned.  Products are accumulated in fp32; h and g enter
  * the sums over rows with 22 significant bits relative to their largest
- * magnitude in the adapter.  Results do not depend on scheduling: the same
+ * magnitude in the adapter, g enters dx rounded to fp16 at that scale.  Results do not depend on scheduling: the same
  * inputs give the same bits.  Non-finite values in dy or x of an adapter's
  * rows make that adapter's gradients non-finite. */
 int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora_a, const qw_array* lora_b,

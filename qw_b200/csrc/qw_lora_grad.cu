@@ -568,15 +568,18 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
 //               one in 80 cycles: 12 GB/s an SM); warp 8 also an item's lora_a;
 //   warps 0-7   split the step's h or g for the tensor cores (below), and while
 //               those multiply take the step before's dx from TMEM to memory;
-//   warp 11     issues tcgen05.mma: D[columns][ranks] += v^T (h or g), both
+//   warp 11     issues tcgen05.mma: D[ranks][columns] += (h or g)^T v, both
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers.
-// HBM-bound by x and dy; at rank 64 the products take about half that time.
+// HBM-bound by x and dy; operands along MN run at about half the tensor cores'
+// rate, so at rank 64 the products take as long as the copies.
 //
 // The tensor cores take fp16, h and g are fp32: scaled by a power of two that
 // puts the adapter's largest magnitude below 2^15, each is split into the nearest
-// fp16 and the nearest fp16 of the rest (22 bits together) and both halves are
-// multiplied, so dA and dB keep what an fp32 product would.
+// fp16 and the nearest fp16 of the rest (22 bits together), so dA and dB keep what
+// an fp32 product would.  Up to rank 64 both halves are rows of one D (64 of
+// each) and are added when it is read.  dx, an fp16 result, takes the nearest
+// fp16 of g alone: its error stays below the result's own rounding.
 //
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
@@ -595,20 +598,24 @@ struct Sums {
   Plan plan;
   __half* dx;
   float *da, *db;
-  float* part;         // [chunk of a joint sum][tiles][RP][kCols]
+  float* part;         // [chunk of a joint sum][tiles][kCols][RP]
   bool add_dx;
   int x_tiles, tiles;  // column tiles of x, and of x and dy together
   unsigned int* status;
 };
 template <int RP>
 struct SumCfg {
-  static constexpr int NRANK = RP > 64 ? 128 : 64;               // ranks of a D, whole 128-byte rows
+  static constexpr bool STACK = RP <= 64;                        // a D's rows are 64 high and 64 low halves
+  static constexpr int NRANK = RP > 64 ? 128 : 64;               // ranks in whole 128-byte rows
   static constexpr int V_STAGE = kStepRows * kCols * 2;          // two blocks of 64 columns
+  static_assert(kStepRows * 128 == kStepRows * 64 * 2, "a block of 64 ranks or columns");
   static constexpr int G_HALF = kStepRows * NRANK * 2;           // high or low halves, blocks of 64 ranks
   static constexpr int G_BUFS = RP > 64 ? 1 : 2;
   static constexpr int OFF_G = kVStages * V_STAGE;
   static constexpr int OFF_A = OFF_G + G_BUFS * 2 * G_HALF;      // lora_a: two blocks of [RP][64 columns]
   static constexpr int SMEM = OFF_A + RP * kCols * 2 + 1024;
+  static constexpr int XPITCH = kCols + 4;                       // floats of a row of the low halves' sums
+  static_assert(64 * XPITCH * 4 <= G_BUFS * 2 * G_HALF, "they fit where h or g were");
   static constexpr int PER = RP / 8;                             // float4 of h or g per worker and step
   static_assert(SMEM <= 226 * 1024, "shared memory budget");
 };
@@ -679,11 +686,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
-  // ranks past RP of the split h and g stay zero
-  if (RP < 64 && warp < 8)
-    for (int i = tid; i < Cfg::G_BUFS * 2 * Cfg::G_HALF / 16; i += kWorkers)
-      sts16(base + Cfg::OFF_G + i * 16, make_uint4(0u, 0u, 0u, 0u));
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -744,7 +746,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     // ----------------------------------------------------------- products
     uint32_t it = 0, dxs = 0, sums = 0, ai = 0;
     if (lane == 0) {
-      constexpr uint32_t kSumDesc = mma_desc(kCols, Cfg::NRANK, true, true);
+      constexpr uint32_t kSumDesc = mma_desc(128, kCols, true, true);
       constexpr uint32_t kDxDesc = mma_desc(kStepRows, kCols, false, true);
       for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
         const Item t = item_at(q, i);
@@ -759,10 +761,11 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           tc_fence_after();
           const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * 2 * Cfg::G_HALF;
           if (t.sum) {
-            const uint64_t a = operand_mn(vs, kStepRows * 128);
+            const uint64_t b = operand_mn(vs, kStepRows * 128);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint64_t b = operand_mn(gs + half * Cfg::G_HALF, kStepRows * 128);
+            for (int half = 0; half < (Cfg::STACK ? 1 : 2); ++half) {
+              // both halves, 64 ranks of each, or one half's 128
+              const uint64_t a = operand_mn(gs + half * Cfg::G_HALF, kStepRows * 128);
 #pragma unroll
               for (int kk = 0; kk < kStepRows / 16; ++kk)
                 tc_mma_ss(tmem, a + (uint64_t)(128 * kk), b + (uint64_t)(128 * kk), kSumDesc,
@@ -772,12 +775,9 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           if (t.dx) {
             const uint64_t b = operand_mn(base + Cfg::OFF_A, RP * 128);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-              for (int kk = 0; kk < RP / 16; ++kk) {
-                const uint64_t a = operand_k(gs + half * Cfg::G_HALF + kk / 4 * (kStepRows * 128)) + (uint64_t)(2 * (kk % 4));
-                tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, half > 0 || kk > 0);
-              }
+            for (int kk = 0; kk < RP / 16; ++kk) {
+              const uint64_t a = operand_k(gs + kk / 4 * (kStepRows * 128)) + (uint64_t)(2 * (kk % 4));
+              tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, kk > 0);
             }
             tc_commit(&sh.dxfull[dxs & 1]);
             ++dxs;
@@ -846,12 +846,18 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         if (next < t.steps) fetch_dx_row(next);
         ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
         tc_fence_after();
+        uint32_t dall[4][16];
 #pragma unroll
-        for (int c = 0; c < 64; c += 16) {
-          const int64_t col = t.col0 + upper * 64 + c;
-          uint32_t d[16];
-          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c, d);
-          tmem_wait_ld();
+        for (int c = 0; c < 4; ++c)
+          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c * 16, dall[c]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.dxempty[b]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int64_t col = t.col0 + upper * 64 + c * 16;
+          const uint32_t(&d)[16] = dall[c];
           if (!in || col >= t.width) continue;
           uint32_t o[8];
           if (q.add_dx) {
@@ -879,9 +885,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
             *reinterpret_cast<uint4*>(row + col + 8) = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.dxempty[b]);
         ++dxs;
       };
       if (t.steps > 0) {
@@ -923,56 +926,79 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       if (t.dx && t.steps > 0) store_dx(t.steps);
       if (!t.sum) continue;
 
-      // D[column][rank] of this chunk (a column a lane, 16 ranks at a time over two warps), then the sum's
+      // D[rank][column] of this chunk: a rank a lane, 64 columns a warp; the low
+      // halves' sums go to the high halves' warps through shared memory.
       if (t.steps > 0) {
         ok = ok && mbar_wait(&sh.accfull, sums & 1, q.status, kDevTimeoutAccum);
         ++sums;
         tc_fence_after();
       }
-      const int c = quarter * 32 + lane;
-      float* slots = q.part + ((int64_t)ck.slot0 * q.tiles + t.tile) * kCols * RP + c;
-      const int64_t apart = (int64_t)q.tiles * kCols * RP;
-      auto write = [&](int r0, const float (&f)[16]) {
-        const int64_t col = t.col0 + c;
-        if (col >= t.width) return;
-        if (t.is_x) {
-          float* o = out + ((int64_t)ck.adapter * p.R + r0) * t.width + col;
+      const bool low = Cfg::STACK && quarter >= 2;
+      const int r = (Cfg::STACK ? quarter & 1 : quarter) * 32 + lane, c0 = upper * 64;
+      float* const exchange = reinterpret_cast<float*>(smem + Cfg::OFF_G) + r * Cfg::XPITCH + c0;
+      if (low && t.steps > 0) {
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t d[16];
+          tmem_ld_32x32b_x16(tmem + lanes + c0 + c, d);
+          tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if (r0 + x < p.R) o[x * t.width] = f[x] * down;
-        } else {
-          float* o = out + ((int64_t)ck.adapter * t.width + col) * p.R + r0;
-          if (p.R % 4 == 0) {
+          for (int x = 0; x < 16; x += 4)
+            *reinterpret_cast<uint4*>(exchange + c + x) = make_uint4(d[x], d[x + 1], d[x + 2], d[x + 3]);
+        }
+      }
+      if (Cfg::STACK) worker_sync();
+      // a chunk's sums lie [column][rank], those of the adapter's next chunk q.tiles further on
+      float* slots = q.part + (((int64_t)ck.slot0 * q.tiles + t.tile) * kCols + c0) * RP + r;
+      const int64_t apart = (int64_t)q.tiles * kCols * RP;
+      auto write = [&](int c, const float (&f)[16]) {
+        const int64_t col = t.col0 + c0 + c;
+        if (r >= p.R) return;
+        if (t.is_x) {
+          float* o = out + ((int64_t)ck.adapter * p.R + r) * t.width + col;
+          if (col < t.width) {  // the width is a multiple of 64
 #pragma unroll
             for (int x = 0; x < 16; x += 4)
-              if (r0 + x < p.R)
-                *reinterpret_cast<float4*>(o + x) =
-                    make_float4(f[x] * down, f[x + 1] * down, f[x + 2] * down, f[x + 3] * down);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              if (r0 + x < p.R) o[x] = f[x] * down;
+              *reinterpret_cast<float4*>(o + x) =
+                  make_float4(f[x] * down, f[x + 1] * down, f[x + 2] * down, f[x + 3] * down);
           }
+        } else {
+          float* o = out + ((int64_t)ck.adapter * t.width + col) * p.R + r;
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (col + x < t.width) o[x * p.R] = f[x] * down;
         }
       };
+      if (!low) {
 #pragma unroll 1
-      for (int r0 = upper * 16; r0 < RP; r0 += 32) {
-        uint32_t d[16];
-        if (t.steps > 0) {
-          tmem_ld_32x32b_x16(tmem + lanes + r0, d);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int x = 0; x < 16; ++x) d[x] = 0u;
-        }
-        if (ck.of == 1) {
+        for (int c = 0; c < 64; c += 16) {
           float f[16];
+          if (t.steps > 0) {
+            uint32_t d[16];
+            tmem_ld_32x32b_x16(tmem + lanes + c0 + c, d);
+            tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 16; ++x) f[x] = __uint_as_float(d[x]);
-          write(r0, f);
-        } else {
+            for (int x = 0; x < 16; ++x) f[x] = __uint_as_float(d[x]);
+            if (Cfg::STACK) {
 #pragma unroll
-          for (int x = 0; x < 16; ++x) __stcg(slots + ck.index * apart + (r0 + x) * kCols, __uint_as_float(d[x]));
+              for (int x = 0; x < 16; x += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(exchange + c + x);
+                f[x] += w.x;
+                f[x + 1] += w.y;
+                f[x + 2] += w.z;
+                f[x + 3] += w.w;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) f[x] = 0.f;
+          }
+          if (ck.of == 1) {
+            write(c, f);
+          } else if (r < RP) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) __stcg(slots + ck.index * apart + (c + x) * RP, f[x]);
+          }
         }
       }
       if (t.steps > 0) {
@@ -987,20 +1013,21 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           sh.last = atomicAdd(q.plan.count + (int64_t)ck.joint * q.tiles + t.tile, 1u) == (uint32_t)ck.of - 1;
         worker_sync();
         const bool last = sh.last != 0;
-        worker_sync();
-        if (!last) continue;
-        __threadfence();
+        if (last && !low && r < RP) {
+          __threadfence();
 #pragma unroll 1
-        for (int r0 = upper * 16; r0 < RP; r0 += 32) {
-          float f[16];
+          for (int c = 0; c < 64; c += 16) {
+            float f[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) f[x] = 0.f;
-          for (int k = 0; k < ck.of; ++k)
+            for (int x = 0; x < 16; ++x) f[x] = 0.f;
+            for (int k = 0; k < ck.of; ++k)
 #pragma unroll
-            for (int x = 0; x < 16; ++x) f[x] += __ldcg(slots + k * apart + (r0 + x) * kCols);
-          write(r0, f);
+              for (int x = 0; x < 16; ++x) f[x] += __ldcg(slots + k * apart + (c + x) * RP);
+            write(c, f);
+          }
         }
       }
+      worker_sync();  // the low halves' sums are read before h or g go there again
     }
   }
   tc_fence_before();
@@ -1026,11 +1053,19 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.RP = padded_rank(R);
   s.x_tiles = (int)((K + kCols - 1) / kCols);
   s.tiles = s.x_tiles + (int)((N + kCols - 1) / kCols);
-  // about two items an SM
-  int64_t cuts = (2 * (int64_t)sm_count + s.tiles - 1) / s.tiles;
-  const int64_t most = (M + kStepRows - 1) / kStepRows;
-  cuts = cuts > most ? most : cuts;
-  cuts = cuts < 1 ? 1 : cuts;
+  // The cuts of an adapter with all rows whose rounds of items take least, in
+  // steps: an item's beginning and end cost about two, joining its sum two more
+  // (256 rows, 6144 x 5120: 15.9 us in one cut of two steps, 20 in two of one).
+  int64_t cuts = 1, best = 0;
+  for (int64_t c = 1; c <= 8 && (c - 1) * kStepRows < M; ++c) {
+    const int64_t rounds = (c * s.tiles + sm_count - 1) / sm_count;
+    const int64_t steps = ((M + c - 1) / c + kStepRows - 1) / kStepRows;
+    const int64_t cost = rounds * (steps + (c > 1 ? 4 : 2));
+    if (c == 1 || cost < best) {
+      cuts = c;
+      best = cost;
+    }
+  }
   s.chunk_rows = (int)(((M + cuts - 1) / cuts + kStepRows - 1) / kStepRows * kStepRows);
   if (s.chunk_rows < kStepRows) s.chunk_rows = kStepRows;
   s.max_chunks = M / s.chunk_rows + L;

@@ -40,7 +40,10 @@ def lora_delta(x, a, b, s, idx, half_h):
 def lora_grads(x, dy, a, b, s, idx):
     """((dx, da, db), bounds): float64 gradients of the adapters' term.  The
     bounds count fp32 sums and h, g held as two fp16 terms relative to their
-    largest magnitude in the adapter (2^-21 of it covers both terms' rounding)."""
+    largest magnitude in the adapter (2^-21 of it covers both terms' rounding);
+    dx, an fp16 result, takes g rounded to one fp16 term (half a step of g, or of
+    the smallest fp16 where the largest magnitude is scaled to 2^14 at least:
+    2^-25 / 2^14 of it)."""
     x, dy, a, b = x.cpu().double(), dy.cpu().double(), a.cpu().double(), b.cpu().double()
     L, R, K = a.shape
     M, N = dy.shape
@@ -57,7 +60,8 @@ def lora_grads(x, dy, a, b, s, idx):
         dh, dg = dh + 2.0 ** -21 * h.abs().max(), dg + 2.0 ** -21 * g.abs().max()
         m = len(r) + 8
         dx[r] = g @ a[l]
-        ex[r] = dg @ a[l].abs() + (R + 8) * U * (g.abs() @ a[l].abs())
+        dgx = dg + half_step(torch.float16) * (g.abs() + dg) + 2.0 ** -39 * g.abs().max()
+        ex[r] = dgx @ a[l].abs() + (R + 8) * U * (g.abs() @ a[l].abs())
         da[l] = g.T @ x[r]
         ea[l] = dg.T @ x[r].abs() + m * U * (g.abs().T @ x[r].abs())
         db[l] = dy[r].T @ h
