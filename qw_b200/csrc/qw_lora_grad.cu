@@ -613,7 +613,8 @@ struct SumCfg {
   static constexpr int G_BUFS = RP > 64 ? 1 : 2;
   static constexpr int OFF_G = kVStages * V_STAGE;
   static constexpr int OFF_A = OFF_G + G_BUFS * 2 * G_HALF;      // lora_a: two blocks of [RP][64 columns]
-  static constexpr int SMEM = OFF_A + RP * kCols * 2 + 1024;
+  static constexpr int OFF_DX = OFF_A + RP * kCols * 2;          // dx of a step, [128 rows][128 columns] fp16
+  static constexpr int SMEM = OFF_DX + kStepRows * kCols * 2 + 1024;
   static constexpr int XPITCH = kCols + 4;                       // floats of a row of the low halves' sums
   static_assert(64 * XPITCH * 4 <= G_BUFS * 2 * G_HALF, "they fit where h or g were");
   static constexpr int PER = RP / 8;                             // float4 of h or g per worker and step
@@ -800,7 +801,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     // ------------------------------------------------------------ workers
     const int quarter = warp % 4, upper = warp / 4;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const bool dx32 = (reinterpret_cast<uintptr_t>(q.dx) & 31) == 0;
     uint32_t it = 0, dxs = 0, sums = 0;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
       const Item t = item_at(q, i);
@@ -838,54 +838,79 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         const int r = step * kStepRows + quarter * 32 + lane;
         dx_row = r < ck.count ? __ldcg(order + r) : -1;
       };
-      // dx of a step whose products are done: a row a lane, 64 columns a warp
+      // dx of a step whose products are done: a row a lane and 64 columns a warp
+      // out of TMEM, through shared memory into whole rows of 256 bytes (32 bytes
+      // of 32 rows an instruction cost 2200 cycles a step).  Added to what dx
+      // holds, it goes there directly, in fp32 up to its one rounding.
       auto store_dx = [&](int next) {
         const uint32_t b = dxs & 1;
-        const bool in = dx_row >= 0;
-        __half* row = q.dx + (int64_t)(in ? dx_row : 0) * p.K;
+        const int mine = dx_row;
         if (next < t.steps) fetch_dx_row(next);
         ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
         tc_fence_after();
-        uint32_t dall[4][16];
+        uint32_t d[4][16];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c * 16, dall[c]);
+          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c * 16, d[c]);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.dxempty[b]);
+        ++dxs;
+        if (q.add_dx) {
+          if (mine < 0) return;
+          __half* row = q.dx + (int64_t)mine * p.K + t.col0 + upper * 64;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int64_t col = t.col0 + upper * 64 + c * 16;
-          const uint32_t(&d)[16] = dall[c];
-          if (!in || col >= t.width) continue;
-          uint32_t o[8];
-          if (q.add_dx) {
+          for (int c = 0; c < 4; ++c) {
+            if (t.col0 + upper * 64 + c * 16 >= t.width) continue;
+            uint32_t o[8];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-              *reinterpret_cast<uint4*>(o + 4 * x) = *reinterpret_cast<const uint4*>(row + col + 8 * x);
-          }
+              *reinterpret_cast<uint4*>(o + 4 * x) = *reinterpret_cast<const uint4*>(row + c * 16 + 8 * x);
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            float2 f = make_float2(__uint_as_float(d[2 * x]) * down, __uint_as_float(d[2 * x + 1]) * down);
-            if (q.add_dx) {
+            for (int x = 0; x < 8; ++x) {
               const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&o[x]));
-              f.x += w.x;
-              f.y += w.y;
+              const __half2 r = __floats2half2_rn(fmaf(__uint_as_float(d[c][2 * x]), down, w.x),
+                                                  fmaf(__uint_as_float(d[c][2 * x + 1]), down, w.y));
+              o[x] = *reinterpret_cast<const uint32_t*>(&r);
             }
-            const __half2 r = __floats2half2_rn(f.x, f.y);
-            o[x] = *reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              *reinterpret_cast<uint4*>(row + c * 16 + 8 * x) =
+                  make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
-          if (dx32) {  // a whole 32-byte sector a lane
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + col), "r"(o[0]), "r"(o[1]),
-                         "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
-                         : "memory");
-          } else {
-            *reinterpret_cast<uint4*>(row + col) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(row + col + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-          }
+          return;
         }
-        ++dxs;
+        // the two warps of a lane quarter share its 32 rows
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");  // the step before's rows are read
+        const int row = quarter * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t o[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const __half2 r = __floats2half2_rn(__uint_as_float(d[c][8 * x + 2 * y]) * down,
+                                                  __uint_as_float(d[c][8 * x + 2 * y + 1]) * down);
+              o[y] = *reinterpret_cast<const uint32_t*>(&r);
+            }
+            sts16(base + Cfg::OFF_DX + row * 256 + (((upper * 8 + c * 2 + x) ^ (row & 7)) << 4),
+                  make_uint4(o[0], o[1], o[2], o[3]));
+          }
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
+        const int64_t col = t.col0 + lane % 16 * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int in_quarter = upper * 16 + 2 * k + lane / 16, r = quarter * 32 + in_quarter;
+          const int m = __shfl_sync(0xffffffffu, mine, in_quarter);
+          uint4 v4;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v4.x), "=r"(v4.y), "=r"(v4.z), "=r"(v4.w)
+                       : "r"(base + Cfg::OFF_DX + r * 256 + (((lane % 16) ^ (r & 7)) << 4))
+                       : "memory");
+          if (m >= 0 && col < t.width) *reinterpret_cast<uint4*>(q.dx + (int64_t)m * p.K + col) = v4;
+        }
       };
       if (t.steps > 0) {
         fetch_rows(0);
