@@ -4,12 +4,15 @@
 //   dA = g^T x, dB = dy^T h                    sums over the adapter's rows
 //   dx = g A (+ dx)
 // Three launches, chained by programmatic dependent launch:
-//   plan     sorts the rows by adapter and cuts each adapter's rows into chunks;
-//   products h and g, fp32, and the largest magnitude of each per adapter
-//            (runs beside the plan until its results);
+//   products h and g, fp32, and the largest magnitude of each by tile and adapter;
+//            one more CTA sorts the rows by adapter and cuts each adapter's rows
+//            into chunks (the plan);
+//   split    h and g of the sorted rows as two fp16 terms, laid out as the tensor
+//            cores take them from shared memory;
 //   sums     dA, dB and dx, a chunk of rows and 128 columns at a time.
-// x and dy are read twice, once across their width and once along their rows;
-// everything else is rank-sized.
+// (dy of odd width and lora_b of odd rank are first laid out anew.)  x and dy are
+// read twice, once across their width and once along their rows; everything else
+// is rank-sized.
 #include <cuda_fp16.h>
 
 #include <cstring>
@@ -57,6 +60,141 @@ constexpr uint32_t mma_desc(int m, int n, bool a_mn, bool b_mn) {
          ((uint32_t)(m >> 4) << 24);
 }
 
+// -------------------------------------------------------------------- plan
+// Rows sorted by adapter (stable) and cut into chunks of whole steps (128 rows).
+// One CTA: each warp counts the adapters of its share of the rows, the counts
+// become positions, and each warp places its rows; a warp owns its counters, so
+// nothing is atomic.
+constexpr int kStepRows = 128;
+struct Chunk {
+  int adapter, start, count;  // rows order[start .. start + count)
+  int step0;                  // first of its steps
+  int index, of;              // which of the adapter's chunks
+  int joint, slot0;           // of an adapter of several chunks: its place among those, and its first partial sum's
+};
+struct Step {
+  int adapter, start, rows;  // rows order[start .. start + rows)
+  int chunk;                 // whose first step it is, else -1
+};
+struct PlanArgs {
+  int* total;         // chunks, and steps
+  Chunk* chunks;
+  Step* steps;
+  int* order;         // [M] rows by adapter
+  uint32_t* count;    // [joint][tiles] chunks of a sum that are done
+  int64_t counters;
+  int chunk_rows;
+};
+constexpr int kPlanWarps = 4;
+
+// Exclusive prefix over the CTA's 128 threads, and their total.
+__device__ __forceinline__ int block_scan(int v, int* warp_tot, int* total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_tot[warp] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kPlanWarps; ++w) {
+    before += w < warp ? warp_tot[w] : 0;
+    all += warp_tot[w];
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+__device__ void make_plan(const LoraArgs& p, const PlanArgs& plan, int* hist) {  // hist [kPlanWarps][L]
+  __shared__ int warp_tot[kPlanWarps];
+  constexpr int kThreads = kPlanWarps * 32;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int L = (int)p.L;
+  for (int64_t i = tid; i < plan.counters; i += kThreads) plan.count[i] = 0u;
+  for (int i = tid; i < kPlanWarps * L; i += kThreads) hist[i] = 0;
+  __syncthreads();
+  const int64_t per = ((p.M + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+  const int64_t r0 = per * warp, r1 = r0 + per < p.M ? r0 + per : p.M;
+  int* const mine = hist + warp * L;
+  auto walk = [&](auto&& place) {
+    for (int64_t b = r0; b < r1; b += 32) {
+      const int64_t m = b + lane;
+      const int a = m < r1 ? (int)adapter_of(p, m) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int at = a >= 0 ? mine[a] : 0;
+      __syncwarp();
+      if (a >= 0 && rank == 0) mine[a] = at + __popc(same);
+      __syncwarp();
+      if (a >= 0) place(m, at + rank);
+    }
+  };
+  walk([](int64_t, int) {});
+  __syncthreads();
+  int start0 = 0, chunk0 = 0, step0 = 0, joint0 = 0, slot0 = 0;  // of the adapters before
+  for (int base = 0; base < L; base += kThreads) {
+    const int a = base + tid;
+    int rows = 0;
+    for (int w = 0; w < kPlanWarps && a < L; ++w) rows += hist[w * L + a];
+    // an adapter without rows has zeros to write
+    const int cuts = a < L ? (rows > 0 ? (rows + plan.chunk_rows - 1) / plan.chunk_rows : 1) : 0;
+    const int steps = (rows + kStepRows - 1) / kStepRows;  // chunks are whole steps
+    int total;
+    int start = start0 + block_scan(rows, warp_tot, &total);
+    start0 += total;
+    int chunk = chunk0 + block_scan(cuts, warp_tot, &total);
+    chunk0 += total;
+    int step = step0 + block_scan(steps, warp_tot, &total);
+    step0 += total;
+    const int joint = joint0 + block_scan(cuts > 1, warp_tot, &total);
+    joint0 += total;
+    const int slot = slot0 + block_scan(cuts > 1 ? cuts : 0, warp_tot, &total);
+    slot0 += total;
+    for (int k = 0; k < cuts; ++k) {
+      const int left = rows - k * plan.chunk_rows;
+      const int count = left < plan.chunk_rows ? left : plan.chunk_rows;
+      plan.chunks[chunk] = Chunk{a, start + k * plan.chunk_rows, count, step, k, cuts, joint, slot};
+      for (int i = 0; i < count; i += kStepRows)
+        plan.steps[step++] = Step{a, start + k * plan.chunk_rows + i, count - i < kStepRows ? count - i : kStepRows,
+                                  i == 0 ? chunk : -1};
+      ++chunk;
+    }
+    for (int w = 0; w < kPlanWarps && a < L; ++w) {  // counts to positions
+      const int c = hist[w * L + a];
+      hist[w * L + a] = start;
+      start += c;
+    }
+  }
+  if (tid == 0) {
+    plan.total[0] = chunk0;
+    plan.total[1] = step0;
+  }
+  __syncthreads();
+  walk([&](int64_t m, int at) { plan.order[at] = (int)m; });
+}
+
+// Rows of `width` halves, laid out anew `pitch` apart (a multiple of 8, zero
+// behind the width): what TMA cannot take as it is.
+struct Repack {
+  const __half* src;
+  __half* dst;  // null: nothing to do
+  int64_t rows, width, ld, pitch;
+};
+__device__ __forceinline__ void repack(const Repack& r) {
+  const int64_t pieces = r.pitch / 8;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < r.rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / pieces, c = i % pieces * 8;
+    *reinterpret_cast<uint4*>(r.dst + row * r.pitch + c) = load_halves(r.src + row * r.ld + c, r.width - c);
+  }
+}
+__global__ void __launch_bounds__(256) lora_repack_kernel(const Repack dy, const Repack b) {
+  if (dy.dst) repack(dy);
+  if (b.dst) repack(b);
+}
+
 // ---------------------------------------------------------------- products
 // v W of each row's adapter, a tile of 128 rows at a time: out[m][r] = s sum_i
 // v[m][i] W[i][r].  HBM-bound by v, which is read once.
@@ -72,6 +210,7 @@ constexpr int kStages = 4;
 constexpr int kProdThreads = 128;
 constexpr int kChunk = 64;  // reduction values per step
 constexpr int kTileRows = 128;
+constexpr int kMaxSplit = 16;  // CTAs of a cluster
 
 struct Product {
   const __half* v;  // [M][len], rows ld apart
@@ -79,15 +218,16 @@ struct Product {
   const __half* w;  // [L][R][len], or for the second product [L][len][R8]
   float* out32;     // [M][RP] fp32, RP the kernel's padded rank (null: out16)
   __half* out16;    // [M][R8] fp16
-  uint32_t* amax;   // [L] largest magnitude of out32, as fp32 bits
+  uint32_t* top;    // [tiles][kMaxSplit][kTileRows] largest magnitude of out32 by adapter, as fp32 bits
 };
 struct Products {
   LoraArgs p;
   Product a, b;      // b.v null: one product
   __half* dx_zero;   // [M][K]: rows without an adapter are cleared (nullable)
   int R8;
-  int tiles;         // row tiles
-  bool wait;         // operands come from the kernel before
+  int tiles, split;  // row tiles and CTAs of a tile's cluster, filled at the launch
+  uint32_t* tile_ids;  // gradient: adapters of each row tile (0xFFFFFFFF: no more), [tiles][kTileRows]
+  PlanArgs plan;     // gradient (plan.total null: none)
   TokenLists lists;  // forward
   unsigned int* status;
 };
@@ -177,10 +317,9 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       for (int64_t c = rank * 32 + lane; c < p.K / 8; c += C * 32) dst[c] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  if (n == 0) {  // the whole cluster: nobody's rows
-    pdl_wait();  // a kernel behind this one counts on the plan, too
-    return;
-  }
+  if (!TRANS && f.out32 && rank == 0)  // for the split
+    q.tile_ids[(int64_t)tile * kTileRows + tid] = tid < n ? sh.list[tid] : 0xFFFFFFFFu;
+  if (n == 0) return;  // the whole cluster: nobody's rows
 
   const int chunks = (int)((f.len + kChunk - 1) / kChunk);
   const int c0 = (int)((int64_t)chunks * rank / C), c1 = (int)((int64_t)chunks * (rank + 1) / C);
@@ -269,7 +408,6 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
     tc_fence_before();
     if (C > 1) cluster_sync();
     else __syncthreads();
-    pdl_wait();  // the maxima's start values are the plan's (a forward has waited)
     for (int i = (int)rank * kProdThreads + tid; i < kTileRows * RP / 4; i += (int)C * kProdThreads) {
       const int row = i / (RP / 4), c = i % (RP / 4) * 4;
       const int slot = (int)sh.row_slot[row];
@@ -312,7 +450,7 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   }
   if (f.out32)
     for (int i = tid; i < n; i += kProdThreads)
-      if (sh.slot_max[i]) atomicMax(f.amax + sh.list[i], sh.slot_max[i]);
+      f.top[((int64_t)tile * kMaxSplit + rank) * kTileRows + i] = sh.slot_max[i];
 }
 
 template <int RP>
@@ -322,11 +460,13 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const __gri
   __shared__ __align__(16) ProdShared sh;
   uint8_t* smem = prod_smem + ((1024u - (smem_u32(prod_smem) & 1023u)) & 1023u);
   const uint32_t rank = cluster_rank(), C = cluster_size();
-  const int unit = (int)(blockIdx.x / C);
-  // A gradient's operands were there before the plan started this launch, unless
-  // it lays dy or lora_b out anew; a forward waits for the kernel before it.
-  if (q.wait) pdl_wait();
+  const int unit = (int)(blockIdx.x / C) - (q.plan.total ? 1 : 0);
+  pdl_wait();
   pdl_launch_dependents();
+  if (unit < 0) {
+    if (rank == 0) make_plan(q.p, q.plan, reinterpret_cast<int*>(smem));
+    return;
+  }
   const bool first = unit < q.tiles, second = !first && q.b.v && unit < 2 * q.tiles;
   if (!first && !second) {
     if (rank == 0) token_list(q.p, q.lists, unit - q.tiles);
@@ -400,9 +540,10 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   // Splits for about four CTAs an SM, each two SM's worth in flight: the loads of
   // an SM run at 46 GB/s (a 128-byte row in 5 cycles), so all of them are needed.
   // 16 CTAs to a cluster, twice the portable size, where the tiles are few.
-  int C = most < 16 ? (int)most : 16;
+  int C = most < kMaxSplit ? (int)most : kMaxSplit;
   while (C > 1 && (int64_t)products * q.tiles * C > (C > 8 ? 1 : 4) * sm_count) --C;
-  const int64_t units = (int64_t)products * q.tiles + q.lists.tiles;
+  q.split = C;
+  const int64_t units = (int64_t)products * q.tiles + q.lists.tiles + (q.plan.total ? 1 : 0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * C));
   cfg.blockDim = dim3(kProdThreads);
@@ -428,165 +569,138 @@ cudaError_t dispatch_products(Products& q, int sm_count, bool pdl, cudaStream_t 
 }
 int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
-// -------------------------------------------------------------------- plan
-// Rows sorted by adapter (stable) and cut into chunks.  One CTA: each warp
-// counts the adapters of its share of the rows, the counts become positions, and
-// each warp places its rows; a warp owns its counters, so nothing is atomic.
-struct Chunk {
-  int adapter, start, count;  // rows order[start .. start + count)
-  int index, of;              // which of the adapter's chunks
-  int joint, slot0;           // of an adapter of several chunks: its place among those, and its first partial sum's
+// ------------------------------------------------------------------- split
+// The tensor cores take fp16, h and g are fp32: scaled by a power of two that
+// puts the adapter's largest magnitude below 2^15, each is split into the nearest
+// fp16 and the nearest fp16 of the rest (22 bits together), so dA and dB keep what
+// an fp32 product would.  A CTA lays out one step, 128 sorted rows of both, as the
+// sums' shared memory holds them: high halves then low halves, blocks of 64 ranks,
+// 128 rows of 128 swizzled bytes, so that a step is one bulk copy there however
+// many column tiles read it.
+template <int RP>
+struct SplitCfg {
+  static constexpr int NRANK = RP > 64 ? 128 : 64;          // ranks in whole 128-byte rows
+  static constexpr int HALF = kStepRows * NRANK * 2;        // high or low halves
+  static constexpr int IMAGE = 2 * HALF;                    // h or g of a step
 };
-struct Plan {
-  int* total;       // chunks
-  Chunk* chunks;
-  int* order;       // [M] rows by adapter
-  uint32_t* amax;   // [2][L] largest magnitude of h and g, as fp32 bits
-  uint32_t* count;  // [joint][tiles] chunks of a sum that are done
+struct Split {
+  LoraArgs p;
+  PlanArgs plan;
+  const float *h, *g;                 // [M][RP]
+  const uint32_t *top_h, *top_g;      // [tiles][kMaxSplit][kTileRows]
+  const uint32_t* tile_ids;
+  int tiles, split;                   // row tiles and cluster size of the products
+  uint8_t* images;                    // [steps][h, g][IMAGE]
+  float* down;                        // [chunks][h, g] 2^-e, the scale back
+  int2* runs;                         // [steps] first row of a whole step of consecutive rows, else -1, and bits of
+                                      // the groups of 8 rows that are consecutive
 };
+constexpr int kSplitThreads = 128, kSplitRows = 32;
 
-constexpr int kPlanThreads = 1024;
-
-__device__ int block_scan(int v, int* warp_tot) {  // exclusive prefix over the CTA
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
-  }
-  __syncthreads();
-  if (lane == 31) warp_tot[warp] = incl;
-  __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; ++w) before += warp_tot[w];
-  return before + incl - v;
-}
-
-// Rows of `width` halves, laid out anew `pitch` apart (a multiple of 8, zero
-// behind the width): what TMA cannot take as it is.
-struct Repack {
-  const __half* src;
-  __half* dst;  // null: nothing to do
-  int64_t rows, width, ld, pitch;
-};
-__device__ __forceinline__ void repack(const Repack& r, int64_t first, int64_t step) {
-  const int64_t pieces = r.pitch / 8;
-  for (int64_t i = first; i < r.rows * pieces; i += step) {
-    const int64_t row = i / pieces, c = i % pieces * 8;
-    *reinterpret_cast<uint4*>(r.dst + row * r.pitch + c) = load_halves(r.src + row * r.ld + c, r.width - c);
-  }
-}
-
-// Block 0 plans, the others lay out dy and lora_b anew where that is needed.
-__global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs p, const Plan plan, int warps,
-                                                                 int chunk_rows, int64_t counters, const Repack dy,
-                                                                 const Repack b) {
-  extern __shared__ int hist[];  // [warps][L]
-  __shared__ int warp_tot[32];
+// blockIdx.y: h or g, and which 32 of the step's rows.
+template <int RP>
+__global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q) {
+  using Cfg = SplitCfg<RP>;
+  __shared__ uint32_t top, runs[kStepRows / 32];
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x > 0) {
-    const int64_t first = (int64_t)(blockIdx.x - 1) * kPlanThreads + threadIdx.x;
-    const int64_t step = (int64_t)(gridDim.x - 1) * kPlanThreads;
-    if (dy.dst) repack(dy, first, step);
-    if (b.dst) repack(b, first, step);
-    return;
-  }
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int L = (int)p.L;
-  for (int i = tid; i < 2 * L; i += kPlanThreads) plan.amax[i] = 0u;
-  for (int64_t i = tid; i < counters; i += kPlanThreads) plan.count[i] = 0u;
-  for (int i = tid; i < warps * L; i += kPlanThreads) hist[i] = 0;
-  __syncthreads();
-  const int64_t per = ((p.M + warps - 1) / warps + 31) / 32 * 32;
-  const int64_t r0 = per * warp, r1 = r0 + per < p.M ? r0 + per : p.M;
-  int* const mine = hist + warp * L;
-  auto walk = [&](auto&& place) {
-    if (warp >= warps) return;
-    for (int64_t b = r0; b < r1; b += 32) {
-      const int64_t m = b + lane;
-      const int a = m < r1 ? (int)adapter_of(p, m) : -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, a);
-      const int rank = __popc(same & ((1u << lane) - 1u));
-      const int at = a >= 0 ? mine[a] : 0;
-      __syncwarp();
-      if (a >= 0 && rank == 0) mine[a] = at + __popc(same);
-      __syncwarp();
-      if (a >= 0) place(m, at + rank);
+  const int step = blockIdx.x, tid = threadIdx.x;
+  const int which = blockIdx.y % 2, row0 = blockIdx.y / 2 * kSplitRows;
+  const int steps = __ldcg(q.plan.total + 1);
+  const int4 info = __ldcg(reinterpret_cast<const int4*>(q.plan.steps) + step);  // there whatever the plan wrote
+  if (step >= steps) return;
+  const int adapter = info.x, rows = info.z, chunk = info.w;
+  const int* order = q.plan.order + info.y;
+  const uint32_t* tops = which ? q.top_g : q.top_h;
+  if (tid == 0) top = 0u;
+  if (blockIdx.y == 0) {  // a row a thread
+    const int m = tid < rows ? __ldcg(order + tid) : -1;
+    const int next = tid + 1 < rows ? __ldcg(order + tid + 1) : -1;
+    const bool run = m >= 0 && next == m + 1;
+    const uint32_t here = __ballot_sync(0xffffffffu, run);
+    if (tid % 32 == 0) runs[tid / 32] = here;
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t mask = 0u;
+      for (int g = 0; g < kStepRows / 8; ++g) mask |= ((runs[g / 4] >> g % 4 * 8 & 0x7Fu) == 0x7Fu ? 1u : 0u) << g;
+      const bool all = (runs[0] & runs[1] & runs[2]) == 0xFFFFFFFFu && runs[3] == 0x7FFFFFFFu;
+      q.runs[step] = make_int2(all ? m : -1, (int)mask);
     }
-  };
-  walk([](int64_t, int) {});
-  __syncthreads();
-  constexpr int kPer = (int)kLoraMaxAdapters / kPlanThreads;
-  int rows[kPer], sum = 0;
-  for (int i = 0; i < kPer; ++i) {
-    const int a = tid * kPer + i;
-    rows[i] = 0;
-    for (int w = 0; w < warps && a < L; ++w) rows[i] += hist[w * L + a];
-    sum += rows[i];
+  } else {
+    __syncthreads();
   }
-  int start = block_scan(sum, warp_tot);
-  int cuts[kPer], n_cuts = 0, joints = 0, parts = 0;
-  for (int i = 0; i < kPer; ++i) {
-    cuts[i] = tid * kPer + i < L ? (rows[i] + chunk_rows - 1) / chunk_rows : 0;
-    if (cuts[i] == 0 && tid * kPer + i < L) cuts[i] = 1;  // an adapter without rows has zeros to write
-    n_cuts += cuts[i];
-    joints += cuts[i] > 1;
-    parts += cuts[i] > 1 ? cuts[i] : 0;
-  }
-  int chunk = block_scan(n_cuts, warp_tot);
-  int joint = block_scan(joints, warp_tot);
-  int slot = block_scan(parts, warp_tot);
-  if (tid == kPlanThreads - 1) *plan.total = chunk + n_cuts;
-  for (int i = 0; i < kPer; ++i) {
-    const int a = tid * kPer + i;
-    if (a >= L) break;
-    for (int k = 0; k < cuts[i]; ++k) {
-      const int left = rows[i] - k * chunk_rows;
-      plan.chunks[chunk++] =
-          Chunk{a, start + k * chunk_rows, left < chunk_rows ? left : chunk_rows, k, cuts[i], joint, slot};
-    }
-    joint += cuts[i] > 1;
-    slot += cuts[i] > 1 ? cuts[i] : 0;
-    for (int w = 0; w < warps; ++w) {  // counts to positions
-      const int c = hist[w * L + a];
-      hist[w * L + a] = start;
-      start += c;
+  // the adapter's largest magnitude over the products' tiles
+  uint32_t bits = 0u;
+  for (int t = tid / 8; t < q.tiles; t += kSplitThreads / 8) {
+    const int64_t ids = (int64_t)t * kTileRows;
+#pragma unroll 4
+    for (int j = tid % 8; j < kTileRows; j += 8) {
+      if (__ldcg(q.tile_ids + ids + j) != (uint32_t)adapter) continue;
+#pragma unroll 4
+      for (int k = 0; k < q.split; ++k)
+        bits = max(bits, __ldcg(tops + ((int64_t)t * kMaxSplit + k) * kTileRows + j));
     }
   }
+  if (bits) atomicMax(&top, bits);
+  constexpr int kPieces = RP / 4, kRowStep = kSplitThreads / kPieces, kPasses = kSplitRows / kRowStep;
+  const int c = tid % kPieces * 4;
+  const float* src = which ? q.g : q.h;
+  float4 v[kPasses];
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int row = row0 + k * kRowStep + tid / kPieces;
+    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)__ldcg(order + row) * RP + c));
+  }
   __syncthreads();
-  walk([&](int64_t m, int at) { plan.order[at] = (int)m; });
+  // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
+  bits = top;
+  int e = bits == 0u || bits >= 0x7F800000u ? 0 : 14 - ((int)(bits >> 23) - 127);
+  e = e > 126 ? 126 : (e < -126 ? -126 : e);
+  const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+  if (row0 == 0 && tid == 0 && chunk >= 0) q.down[2 * chunk + which] = __uint_as_float((uint32_t)(127 - e) << 23);
+  uint8_t* image = q.images + ((int64_t)step * 2 + which) * Cfg::IMAGE + c / 64 * (kStepRows * 128);
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const float f[4] = {v[k].x * up, v[k].y * up, v[k].z * up, v[k].w * up};
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const __half2 h = __floats2half2_rn(f[2 * x], f[2 * x + 1]);
+      const float2 back = __half22float2(h);
+      const __half2 l = __floats2half2_rn(f[2 * x] - back.x, f[2 * x + 1] - back.y);
+      hi[x] = *reinterpret_cast<const uint32_t*>(&h);
+      lo[x] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+    uint8_t* at = image + swizzled(row0 + k * kRowStep + tid / kPieces, c % 64 / 8) + c % 8 * 2;
+    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(at + Cfg::HALF) = make_uint2(lo[0], lo[1]);
+  }
 }
 
 // -------------------------------------------------------------------- sums
 // A chunk of an adapter's rows and 128 columns of x (dA, and dx of those rows)
 // or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step:
-//   warps 8-10  copy the rows of x or dy (cp.async), a step each in turn, so that
-//               a warp's proxy fence waits for its own step's copies alone and
-//               three steps are in flight (TMA's four-row gathers were issued at
-//               one in 80 cycles: 12 GB/s an SM); warp 8 also an item's lora_a;
-//   warps 0-7   split the step's h or g for the tensor cores (below), and while
-//               those multiply take the step before's dx from TMEM to memory;
+//   warps 8-10  load a step each in turn: its image of h or g (one bulk copy) and
+//               its rows of x or dy, by TMA where they are consecutive, else copied
+//               (cp.async; a warp's proxy fence waits for its own step's copies
+//               alone, and three steps are in flight.  TMA's four-row gathers were
+//               issued at one in 80 cycles: 12 GB/s an SM); warp 8 also an item's
+//               lora_a;
 //   warp 11     issues tcgen05.mma: D[ranks][columns] += (h or g)^T v, both
 //               operands along MN since the rows are the reduction, and
-//               dx[rows][columns] = g A into one of two TMEM buffers.
-// HBM-bound by x and dy; operands along MN run at about half the tensor cores'
-// rate, so at rank 64 the products take as long as the copies.
-//
-// The tensor cores take fp16, h and g are fp32: scaled by a power of two that
-// puts the adapter's largest magnitude below 2^15, each is split into the nearest
-// fp16 and the nearest fp16 of the rest (22 bits together), so dA and dB keep what
-// an fp32 product would.  Up to rank 64 both halves are rows of one D (64 of
-// each) and are added when it is read.  dx, an fp16 result, takes the nearest
-// fp16 of g alone: its error stays below the result's own rounding.
+//               dx[rows][columns] = g A into one of two TMEM buffers;
+//   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
+// HBM-bound by x, dy and dx.  Up to rank 64 the two halves of h or g are rows of
+// one D (64 of each) and are added when it is read.  dx, an fp16 result, takes the
+// nearest fp16 of g alone: its error stays below the result's own rounding.
 //
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
 constexpr int kCols = 128;
-constexpr int kStepRows = 128;
 constexpr int kWorkers = 256;
-constexpr int kVStages = 3;  // and as many warps that copy
+constexpr int kWarpCols = kCols / (kWorkers / 128);  // columns of D or dx a worker warp reads, of 32 rows
+constexpr int kVStages = 3;                          // and as many warps that load
 constexpr int kMmaWarp = kWorkers / 32 + kVStages;
 constexpr int kSumThreads = (kMmaWarp + 1) * 32;
 
@@ -594,8 +708,10 @@ struct Sums {
   LoraArgs p;
   const __half* dy;
   int64_t dy_ld;
-  const float *h, *g;  // [M][RP]
-  Plan plan;
+  PlanArgs plan;
+  const uint8_t* images;
+  const float* down;
+  const int2* runs;
   __half* dx;
   float *da, *db;
   float* part;         // [chunk of a joint sum][tiles][kCols][RP]
@@ -603,26 +719,28 @@ struct Sums {
   int x_tiles, tiles;  // column tiles of x, and of x and dy together
   unsigned int* status;
 };
+struct SumMaps {
+  CUtensorMap x, dy;    // 128 rows of 64 columns
+  CUtensorMap x8, dy8;  // 8 rows of them
+  CUtensorMap a;        // 3-D
+};
+
 template <int RP>
 struct SumCfg {
   static constexpr bool STACK = RP <= 64;                        // a D's rows are 64 high and 64 low halves
-  static constexpr int NRANK = RP > 64 ? 128 : 64;               // ranks in whole 128-byte rows
   static constexpr int V_STAGE = kStepRows * kCols * 2;          // two blocks of 64 columns
-  static_assert(kStepRows * 128 == kStepRows * 64 * 2, "a block of 64 ranks or columns");
-  static constexpr int G_HALF = kStepRows * NRANK * 2;           // high or low halves, blocks of 64 ranks
-  static constexpr int G_BUFS = RP > 64 ? 1 : 2;
+  static constexpr int BLOCK = kStepRows * 128;                  // 64 ranks or columns of a step's rows
+  static constexpr int G_HALF = SplitCfg<RP>::HALF, G_STAGE = SplitCfg<RP>::IMAGE;
+  static constexpr int G_BUFS = RP > 64 ? 1 : kVStages;
   static constexpr int OFF_G = kVStages * V_STAGE;
-  static constexpr int OFF_A = OFF_G + G_BUFS * 2 * G_HALF;      // lora_a: two blocks of [RP][64 columns]
-  static constexpr int OFF_DX = OFF_A + RP * kCols * 2;          // dx of a step, [128 rows][128 columns] fp16
-  static constexpr int SMEM = OFF_DX + kStepRows * kCols * 2 + 1024;
-  static constexpr int XPITCH = kCols + 4;                       // floats of a row of the low halves' sums
-  static_assert(64 * XPITCH * 4 <= G_BUFS * 2 * G_HALF, "they fit where h or g were");
-  static constexpr int PER = RP / 8;                             // float4 of h or g per worker and step
+  static constexpr int OFF_A = OFF_G + G_BUFS * G_STAGE;         // lora_a: two blocks of [RP][64 columns]
+  static constexpr int OFF_X = OFF_A + RP * kCols * 2;           // 2 KB a worker warp, for transposing
+  static constexpr int SMEM = OFF_X + kWorkers / 32 * 2048 + 1024;
   static_assert(SMEM <= 226 * 1024, "shared memory budget");
 };
 
 struct SumShared {
-  uint64_t vfull[kVStages], vempty[kVStages], gfull[2], gempty[2], dxfull[2], dxempty[2];
+  uint64_t vfull[kVStages], vempty[kVStages], gfull[kVStages], dxfull[2], dxempty[2];
   uint64_t accfull, accempty, afull, aempty;
   uint32_t tmem;
   int last;
@@ -633,18 +751,35 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
   const int n = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void pair_sync(int pair) {  // two warps
+  asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory");
+}
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
 // One item of the persistent loop.
 struct Item {
   Chunk ck;
-  int tile, steps;
+  int chunk, tile, steps;
   bool is_x, sum, dx;  // columns of x; dA or dB wanted; dx wanted
   int64_t col0, width;
 };
 __device__ __forceinline__ Item item_at(const Sums& q, int64_t i) {
   Item t;
-  t.ck = q.plan.chunks[i / q.tiles];
+  t.chunk = (int)(i / q.tiles);
+  t.ck = q.plan.chunks[t.chunk];
   t.tile = (int)(i % q.tiles);
   t.is_x = t.tile < q.x_tiles;
   t.col0 = (int64_t)(t.is_x ? t.tile : t.tile - q.x_tiles) * kCols;
@@ -657,7 +792,7 @@ __device__ __forceinline__ Item item_at(const Sums& q, int64_t i) {
 
 template <int RP>
 __global__ void __launch_bounds__(kSumThreads, 1)
-    lora_sums_kernel(const __grid_constant__ Sums q, const __grid_constant__ CUtensorMap map_a) {
+    lora_sums_kernel(const __grid_constant__ Sums q, const __grid_constant__ SumMaps maps) {
   using Cfg = SumCfg<RP>;
   extern __shared__ uint8_t sum_smem[];
   __shared__ SumShared sh;
@@ -670,10 +805,9 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     for (int i = 0; i < kVStages; ++i) {
       mbar_init(&sh.vfull[i], 1);
       mbar_init(&sh.vempty[i], 1);
+      mbar_init(&sh.gfull[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.gfull[i], kWorkers / 32);
-      mbar_init(&sh.gempty[i], 1);
       mbar_init(&sh.dxfull[i], 1);
       mbar_init(&sh.dxempty[i], kWorkers / 32);
     }
@@ -693,13 +827,13 @@ __global__ void __launch_bounds__(kSumThreads, 1)
   const uint32_t tmem = sh.tmem;
   constexpr uint32_t kDx = 128;  // TMEM columns of the two dx buffers
   pdl_wait();
-  const int64_t items = (int64_t)*q.plan.total * q.tiles;
+  const int64_t items = (int64_t)q.plan.total[0] * q.tiles;
   bool ok = true;  // a bounded wait that ran out: go on without waiting
 
   if (warp >= kWorkers / 32 && warp < kMmaWarp) {
-    // ------------------------------------------------------------- copies
+    // -------------------------------------------------------------- loads
     const int slot = warp - kWorkers / 32;
-    uint32_t it = 0, ai = 0, uses = 0;
+    uint32_t it = 0, ai = 0;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
       const Item t = item_at(q, i);
       if (t.steps == 0) continue;
@@ -708,7 +842,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           if (ai > 0) ok = ok && mbar_wait(&sh.aempty, (ai - 1) & 1, q.status, kDevTimeoutEmpty);
           mbar_arrive_expect_tx(&sh.afull, RP * kCols * 2);
           for (int b = 0; b < 2; ++b)
-            tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &map_a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
+            tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &maps.a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
         }
         __syncwarp();
         ++ai;
@@ -717,29 +851,66 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       const int64_t ld = t.is_x ? p.x_ld : q.dy_ld;
       const int64_t c = t.col0 + lane % 16 * 8;
       const bool in_c = c < t.width;
+      const int* order = q.plan.order + t.ck.start;
       for (int step = 0; step < t.steps; ++step, ++it) {
         if (it % kVStages != (uint32_t)slot) continue;
+        const uint32_t gb = it % Cfg::G_BUFS;
+        const int2 runs = __ldcg(q.runs + t.ck.step0 + step);
+        const int rows = t.ck.count - step * kStepRows;
         int at[4];  // the step's rows, 32 k + lane
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = step * kStepRows + 32 * k + lane;
-          at[k] = r < t.ck.count ? __ldcg(q.plan.order + t.ck.start + r) : -1;
-        }
-        if (uses > 0) ok = ok && mbar_wait(&sh.vempty[slot], (uses - 1) & 1, q.status, kDevTimeoutEmpty);
-        ++uses;
-        const uint32_t dst = base + slot * Cfg::V_STAGE + lane % 16 / 8 * (kStepRows * 128);
-#pragma unroll
         for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {  // two rows of 256 bytes
-            const int row = 32 * k + 2 * j + lane / 16;
-            const int m = __shfl_sync(0xffffffffu, at[k], 2 * j + lane / 16);
-            const bool in = in_c && m >= 0;
-            cp_async16(dst + swizzled(row, lane % 8), v + (in ? m * ld + c : 0), in);
-          }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
+          at[k] = 32 * k + lane < rows ? __ldcg(order + step * kStepRows + 32 * k + lane) : -1;
+        const int head = lane % 16 * 8 < rows ? __ldcg(order + step * kStepRows + lane % 16 * 8) : -1;
+        // The products that read this stage are done; then those that read the
+        // image's buffer, which are at most two steps later (so that a barrier
+        // is never a whole turn ahead of its waiter).
+        if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[slot], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
+        uint8_t* const stage = smem + slot * Cfg::V_STAGE;
+        if (lane == 0 && runs.y) mbar_expect_tx(&sh.vfull[slot], (uint32_t)__popc(runs.y) * 2048u);
         __syncwarp();
+        if (runs.x >= 0) {
+          if (lane == 0)
+            for (int b = 0; b < 2; ++b)
+              tma_load_2d(stage + b * Cfg::BLOCK, t.is_x ? &maps.x : &maps.dy, &sh.vfull[slot], (int)t.col0 + b * 64,
+                          runs.x);
+        } else {
+          // groups of 8 consecutive rows by TMA, a group and a block of columns a lane
+          if (runs.y >> lane % 16 & 1)
+            tma_load_2d(stage + lane / 16 * Cfg::BLOCK + lane % 16 * 1024, t.is_x ? &maps.x8 : &maps.dy8,
+                        &sh.vfull[slot], (int)t.col0 + lane / 16 * 64, head);
+          const uint32_t dst = smem_u32(stage) + lane % 16 / 8 * Cfg::BLOCK;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+              // the products take no rows behind the last 16 that hold one
+              if ((runs.y >> (4 * k + g) & 1) || (4 * k + g) / 2 * 16 >= rows) continue;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {  // two rows of 256 bytes
+                const int in_k = g * 8 + 2 * j + lane / 16;
+                const int m = __shfl_sync(0xffffffffu, at[k], in_k);
+                const bool in = in_c && m >= 0;
+                cp_async16(dst + swizzled(32 * k + in_k, lane % 8), v + (in ? m * ld + c : 0), in);
+              }
+            }
+        }
+        if (lane == 0) {
+          if (it >= Cfg::G_BUFS) {
+            const uint32_t was = it - Cfg::G_BUFS;
+            ok = ok && mbar_wait(&sh.vempty[was % kVStages], (was / kVStages) & 1, q.status, kDevTimeoutEmpty);
+          }
+          mbar_arrive_expect_tx(&sh.gfull[gb], Cfg::G_STAGE);
+          bulk_copy(base + Cfg::OFF_G + gb * Cfg::G_STAGE,
+                    q.images + ((int64_t)(t.ck.step0 + step) * 2 + (t.is_x ? 1 : 0)) * Cfg::G_STAGE, Cfg::G_STAGE,
+                    &sh.gfull[gb]);
+        }
+        __syncwarp();
+        if (runs.x < 0) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         if (lane == 0) mbar_arrive(&sh.vfull[slot]);
       }
     }
@@ -752,7 +923,6 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
         const Item t = item_at(q, i);
         if (t.steps == 0) continue;
-        if (t.dx) ok = ok && mbar_wait(&sh.afull, ai & 1, q.status, kDevTimeoutFull);
         if (t.sum && sums > 0) ok = ok && mbar_wait(&sh.accempty, (sums - 1) & 1, q.status, kDevTimeoutAccum);
         for (int step = 0; step < t.steps; ++step, ++it) {
           const uint32_t s = it % kVStages, gb = it % Cfg::G_BUFS;
@@ -760,31 +930,37 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           ok = ok && mbar_wait(&sh.gfull[gb], (it / Cfg::G_BUFS) & 1, q.status, kDevTimeoutFull);
           if (t.dx && dxs >= 2) ok = ok && mbar_wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, q.status, kDevTimeoutAccum);
           tc_fence_after();
-          const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * 2 * Cfg::G_HALF;
-          if (t.sum) {
-            const uint64_t b = operand_mn(vs, kStepRows * 128);
-#pragma unroll
-            for (int half = 0; half < (Cfg::STACK ? 1 : 2); ++half) {
-              // both halves, 64 ranks of each, or one half's 128
-              const uint64_t a = operand_mn(gs + half * Cfg::G_HALF, kStepRows * 128);
-#pragma unroll
-              for (int kk = 0; kk < kStepRows / 16; ++kk)
-                tc_mma_ss(tmem, a + (uint64_t)(128 * kk), b + (uint64_t)(128 * kk), kSumDesc,
-                          step > 0 || half > 0 || kk > 0);
-            }
-          }
-          if (t.dx) {
+          const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * Cfg::G_STAGE;
+          auto dx = [&]() {
             const uint64_t b = operand_mn(base + Cfg::OFF_A, RP * 128);
 #pragma unroll
             for (int kk = 0; kk < RP / 16; ++kk) {
-              const uint64_t a = operand_k(gs + kk / 4 * (kStepRows * 128)) + (uint64_t)(2 * (kk % 4));
+              const uint64_t a = operand_k(gs + kk / 4 * Cfg::BLOCK) + (uint64_t)(2 * (kk % 4));
               tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, kk > 0);
             }
             tc_commit(&sh.dxfull[dxs & 1]);
             ++dxs;
+          };
+          if (t.dx && step > 0) dx();  // before the sums: the workers wait for it
+          if (t.sum) {
+            const int blocks = (t.ck.count - step * kStepRows + 15) / 16;
+            const uint64_t b = operand_mn(vs, Cfg::BLOCK);
+#pragma unroll
+            for (int half = 0; half < (Cfg::STACK ? 1 : 2); ++half) {
+              // both halves, 64 ranks of each, or one half's 128
+              const uint64_t a = operand_mn(gs + half * Cfg::G_HALF, Cfg::BLOCK);
+#pragma unroll
+              for (int kk = 0; kk < kStepRows / 16; ++kk)
+                if (kk < blocks)
+                  tc_mma_ss(tmem, a + (uint64_t)(128 * kk), b + (uint64_t)(128 * kk), kSumDesc,
+                            step > 0 || half > 0 || kk > 0);
+            }
+          }
+          if (t.dx && step == 0) {  // lora_a comes when the item before is done
+            ok = ok && mbar_wait(&sh.afull, ai & 1, q.status, kDevTimeoutFull);
+            dx();
           }
           tc_commit(&sh.vempty[s]);
-          tc_commit(&sh.gempty[gb]);
         }
         if (t.sum) {
           tc_commit(&sh.accfull);
@@ -801,68 +977,42 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     // ------------------------------------------------------------ workers
     const int quarter = warp % 4, upper = warp / 4;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    uint32_t it = 0, dxs = 0, sums = 0;
+    uint32_t dxs = 0, sums = 0;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
       const Item t = item_at(q, i);
       const Chunk& ck = t.ck;
       const int* order = q.plan.order + ck.start;
       float* out = t.is_x ? q.da : q.db;
-      // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
-      const uint32_t top = q.plan.amax[(t.is_x ? p.L : 0) + ck.adapter];
-      int e = top == 0u || top >= 0x7F800000u ? 0 : 14 - ((int)(top >> 23) - 127);
-      e = e > 126 ? 126 : (e < -126 ? -126 : e);
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-      const float* src = t.is_x ? q.g : q.h;
-      const int piece = tid % (RP / 4), row0 = tid / (RP / 4);
-      constexpr int kRowStep = kWorkers / (RP / 4);
-      // A worker's rows of a step, and their h or g a step later: the row numbers
-      // are read a step before they are needed.
-      float4 v[Cfg::PER];
-      int at[Cfg::PER];
-      auto fetch_rows = [&](int step) {
-#pragma unroll
-        for (int k = 0; k < Cfg::PER; ++k) {
-          const int r = step * kStepRows + row0 + k * kRowStep;
-          at[k] = r < ck.count ? __ldcg(order + r) : -1;
-        }
-      };
-      auto fetch = [&]() {
-#pragma unroll
-        for (int k = 0; k < Cfg::PER; ++k) {
-          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (at[k] >= 0) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)at[k] * RP) + piece);
-        }
-      };
-      int dx_row = -1;  // the row of dx that this lane writes next
-      auto fetch_dx_row = [&](int step) {
+      const float down = ck.count > 0 ? __ldcg(q.down + 2 * t.chunk + (t.is_x ? 1 : 0)) : 1.f;
+      // dx of a step: a row a lane and 64 columns a warp out of TMEM, through
+      // shared memory into pieces of 64 bytes of a row.  Added to what dx holds,
+      // it goes there directly, in fp32 up to its one rounding.
+      int next_row = -1;
+      auto fetch_row = [&](int step) {
         const int r = step * kStepRows + quarter * 32 + lane;
-        dx_row = r < ck.count ? __ldcg(order + r) : -1;
+        next_row = r < ck.count ? __ldcg(order + r) : -1;
       };
-      // dx of a step whose products are done: a row a lane and 64 columns a warp
-      // out of TMEM, through shared memory into whole rows of 256 bytes (32 bytes
-      // of 32 rows an instruction cost 2200 cycles a step).  Added to what dx
-      // holds, it goes there directly, in fp32 up to its one rounding.
-      auto store_dx = [&](int next) {
+      if (t.dx) fetch_row(0);
+      for (int step = 0; t.dx && step < t.steps; ++step, ++dxs) {
         const uint32_t b = dxs & 1;
-        const int mine = dx_row;
-        if (next < t.steps) fetch_dx_row(next);
+        const int mine = next_row;
+        if (step + 1 < t.steps) fetch_row(step + 1);
         ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
         tc_fence_after();
-        uint32_t d[4][16];
+        uint32_t d[kWarpCols / 16][16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * 64 + c * 16, d[c]);
+        for (int c = 0; c < kWarpCols / 16; ++c)
+          tmem_ld_32x32b_x16(tmem + lanes + kDx + b * kCols + upper * kWarpCols + c * 16, d[c]);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.dxempty[b]);
-        ++dxs;
         if (q.add_dx) {
-          if (mine < 0) return;
-          __half* row = q.dx + (int64_t)mine * p.K + t.col0 + upper * 64;
+          if (mine < 0) continue;
+          __half* row = q.dx + (int64_t)mine * p.K + t.col0 + upper * kWarpCols;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (t.col0 + upper * 64 + c * 16 >= t.width) continue;
+          for (int c = 0; c < kWarpCols / 16; ++c) {
+            if (t.col0 + upper * kWarpCols + c * 16 >= t.width) continue;
             uint32_t o[8];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -879,104 +1029,93 @@ __global__ void __launch_bounds__(kSumThreads, 1)
               *reinterpret_cast<uint4*>(row + c * 16 + 8 * x) =
                   make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
-          return;
+          continue;
         }
-        // the two warps of a lane quarter share its 32 rows
-        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");  // the step before's rows are read
-        const int row = quarter * 32 + lane;
+        const uint32_t area = base + Cfg::OFF_X + warp * 2048;  // 32 rows of 64 bytes, swizzled
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < 4; ++x) {
             uint32_t o[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const __half2 r = __floats2half2_rn(__uint_as_float(d[c][8 * x + 2 * y]) * down,
-                                                  __uint_as_float(d[c][8 * x + 2 * y + 1]) * down);
+              const uint32_t* v = &d[2 * h + x / 2][8 * (x % 2) + 2 * y];
+              const __half2 r = __floats2half2_rn(__uint_as_float(v[0]) * down, __uint_as_float(v[1]) * down);
               o[y] = *reinterpret_cast<const uint32_t*>(&r);
             }
-            sts16(base + Cfg::OFF_DX + row * 256 + (((upper * 8 + c * 2 + x) ^ (row & 7)) << 4),
-                  make_uint4(o[0], o[1], o[2], o[3]));
+            sts16(area + lane * 64 + ((x ^ (lane / 2 & 3)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
           }
-        asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory");
-        const int64_t col = t.col0 + lane % 16 * 8;
+          __syncwarp();
+          const int64_t col = t.col0 + upper * kWarpCols + h * 32 + lane % 4 * 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int in_quarter = upper * 16 + 2 * k + lane / 16, r = quarter * 32 + in_quarter;
-          const int m = __shfl_sync(0xffffffffu, mine, in_quarter);
-          uint4 v4;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v4.x), "=r"(v4.y), "=r"(v4.z), "=r"(v4.w)
-                       : "r"(base + Cfg::OFF_DX + r * 256 + (((lane % 16) ^ (r & 7)) << 4))
-                       : "memory");
-          if (m >= 0 && col < t.width) *reinterpret_cast<uint4*>(q.dx + (int64_t)m * p.K + col) = v4;
-        }
-      };
-      if (t.steps > 0) {
-        fetch_rows(0);
-        if (t.dx) fetch_dx_row(0);
-        fetch();
-        if (t.steps > 1) fetch_rows(1);
-      }
-      for (int step = 0; step < t.steps; ++step, ++it) {
-        const uint32_t gb = it % Cfg::G_BUFS;
-        // the products that read this buffer last are done
-        if (it >= Cfg::G_BUFS)
-          ok = ok && mbar_wait(&sh.gempty[gb], (it / Cfg::G_BUFS - 1) & 1, q.status, kDevTimeoutEmpty);
-        const uint32_t gs = base + Cfg::OFF_G + gb * 2 * Cfg::G_HALF;
-#pragma unroll
-        for (int k = 0; k < Cfg::PER; ++k) {
-          const int row = row0 + k * kRowStep, c = piece * 4;
-          const float f[4] = {v[k].x * up, v[k].y * up, v[k].z * up, v[k].w * up};
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const __half2 h = __floats2half2_rn(f[2 * x], f[2 * x + 1]);
-            const float2 back = __half22float2(h);
-            const __half2 l = __floats2half2_rn(f[2 * x] - back.x, f[2 * x + 1] - back.y);
-            hi[x] = *reinterpret_cast<const uint32_t*>(&h);
-            lo[x] = *reinterpret_cast<const uint32_t*>(&l);
+          for (int k = 0; k < 4; ++k) {
+            const int r = 8 * k + lane / 4;
+            const int m = __shfl_sync(0xffffffffu, mine, r);
+            const uint4 w = lds16(area + r * 64 + ((lane % 4 ^ (r / 2 & 3)) << 4));
+            if (m >= 0 && col < t.width) *reinterpret_cast<uint4*>(q.dx + (int64_t)m * p.K + col) = w;
           }
-          const uint32_t at = gs + c / 64 * (kStepRows * 128) + swizzled(row, c % 64 / 8) + (c % 8) * 2;
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[1]) : "memory");
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + Cfg::G_HALF), "r"(lo[0]), "r"(lo[1]) : "memory");
+          __syncwarp();
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.gfull[gb]);
-        if (step + 1 < t.steps) fetch();
-        if (step + 2 < t.steps) fetch_rows(step + 2);
-        if (t.dx && step > 0) store_dx(step);
       }
-      if (t.dx && t.steps > 0) store_dx(t.steps);
       if (!t.sum) continue;
 
-      // D[rank][column] of this chunk: a rank a lane, 64 columns a warp; the low
-      // halves' sums go to the high halves' warps through shared memory.
+      // D[rank][column] of this chunk: a rank a lane, 64 columns a warp, all read
+      // at once so that the next item's products may start.  The high and the low
+      // halves of a sum are in two warps: each gives the other 32 of its columns,
+      // 16 at a time through shared memory (2 KB, as 128 pieces of 16 bytes).
+      uint32_t d[4][16];
       if (t.steps > 0) {
         ok = ok && mbar_wait(&sh.accfull, sums & 1, q.status, kDevTimeoutAccum);
         ++sums;
         tc_fence_after();
-      }
-      const bool low = Cfg::STACK && quarter >= 2;
-      const int r = (Cfg::STACK ? quarter & 1 : quarter) * 32 + lane, c0 = upper * 64;
-      float* const exchange = reinterpret_cast<float*>(smem + Cfg::OFF_G) + r * Cfg::XPITCH + c0;
-      if (low && t.steps > 0) {
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 16) {
-          uint32_t d[16];
-          tmem_ld_32x32b_x16(tmem + lanes + c0 + c, d);
-          tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 16; x += 4)
-            *reinterpret_cast<uint4*>(exchange + c + x) = make_uint4(d[x], d[x + 1], d[x + 2], d[x + 3]);
-        }
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x16(tmem + lanes + upper * kWarpCols + c * 16, d[c]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.accempty);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) d[c][x] = 0u;
       }
-      if (Cfg::STACK) worker_sync();
-      // a chunk's sums lie [column][rank], those of the adapter's next chunk q.tiles further on
-      float* slots = q.part + (((int64_t)ck.slot0 * q.tiles + t.tile) * kCols + c0) * RP + r;
-      const int64_t apart = (int64_t)q.tiles * kCols * RP;
-      auto write = [&](int c, const float (&f)[16]) {
+      constexpr int kOwn = Cfg::STACK ? 2 : 4;  // 16s of columns that this warp finishes
+      const bool low = Cfg::STACK && quarter >= 2;
+      const int r = (Cfg::STACK ? quarter & 1 : quarter) * 32 + lane;
+      const int c0 = upper * kWarpCols + (low ? 32 : 0);
+      float f[kOwn][16];
+      if (Cfg::STACK) {
+        const uint32_t area = base + Cfg::OFF_X + warp * 2048, peer = base + Cfg::OFF_X + (warp ^ 2) * 2048;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint4 w;
+            w.x = low ? d[c][4 * x] : d[2 + c][4 * x];
+            w.y = low ? d[c][4 * x + 1] : d[2 + c][4 * x + 1];
+            w.z = low ? d[c][4 * x + 2] : d[2 + c][4 * x + 2];
+            w.w = low ? d[c][4 * x + 3] : d[2 + c][4 * x + 3];
+            sts16(area + lane * 64 + ((x ^ (lane / 2 & 3)) << 4), w);
+          }
+          pair_sync(quarter % 2 * 2 + upper);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint4 w = lds16(peer + lane * 64 + ((x ^ (lane / 2 & 3)) << 4));
+            f[c][4 * x] = __uint_as_float(low ? d[2 + c][4 * x] : d[c][4 * x]) + __uint_as_float(w.x);
+            f[c][4 * x + 1] = __uint_as_float(low ? d[2 + c][4 * x + 1] : d[c][4 * x + 1]) + __uint_as_float(w.y);
+            f[c][4 * x + 2] = __uint_as_float(low ? d[2 + c][4 * x + 2] : d[c][4 * x + 2]) + __uint_as_float(w.z);
+            f[c][4 * x + 3] = __uint_as_float(low ? d[2 + c][4 * x + 3] : d[c][4 * x + 3]) + __uint_as_float(w.w);
+          }
+          pair_sync(quarter % 2 * 2 + upper);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) f[c][x] = __uint_as_float(d[c % 4][x]);
+      }
+      auto write = [&](int c, const float (&v)[16]) {
         const int64_t col = t.col0 + c0 + c;
         if (r >= p.R) return;
         if (t.is_x) {
@@ -985,74 +1124,46 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 #pragma unroll
             for (int x = 0; x < 16; x += 4)
               *reinterpret_cast<float4*>(o + x) =
-                  make_float4(f[x] * down, f[x + 1] * down, f[x + 2] * down, f[x + 3] * down);
+                  make_float4(v[x] * down, v[x + 1] * down, v[x + 2] * down, v[x + 3] * down);
           }
         } else {
           float* o = out + ((int64_t)ck.adapter * t.width + col) * p.R + r;
 #pragma unroll
           for (int x = 0; x < 16; ++x)
-            if (col + x < t.width) o[x * p.R] = f[x] * down;
+            if (col + x < t.width) o[x * p.R] = v[x] * down;
         }
       };
-      if (!low) {
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 16) {
-          float f[16];
-          if (t.steps > 0) {
-            uint32_t d[16];
-            tmem_ld_32x32b_x16(tmem + lanes + c0 + c, d);
-            tmem_wait_ld();
+      if (ck.of == 1) {
 #pragma unroll
-            for (int x = 0; x < 16; ++x) f[x] = __uint_as_float(d[x]);
-            if (Cfg::STACK) {
-#pragma unroll
-              for (int x = 0; x < 16; x += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(exchange + c + x);
-                f[x] += w.x;
-                f[x + 1] += w.y;
-                f[x + 2] += w.z;
-                f[x + 3] += w.w;
-              }
-            }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) f[x] = 0.f;
-          }
-          if (ck.of == 1) {
-            write(c, f);
-          } else if (r < RP) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) __stcg(slots + ck.index * apart + (c + x) * RP, f[x]);
-          }
-        }
+        for (int c = 0; c < kOwn; ++c) write(c * 16, f[c]);
+        continue;
       }
-      if (t.steps > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.accempty);
+      // a chunk's sums lie [column][rank], those of the adapter's next chunk q.tiles further on
+      float* slots = q.part + (((int64_t)ck.slot0 * q.tiles + t.tile) * kCols + c0) * RP + r;
+      const int64_t apart = (int64_t)q.tiles * kCols * RP;
+      if (r < RP) {
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) __stcg(slots + ck.index * apart + (c * 16 + x) * RP, f[c][x]);
       }
-      if (ck.of > 1) {
+      __threadfence();
+      worker_sync();
+      if (tid == 0) sh.last = atomicAdd(q.plan.count + (int64_t)ck.joint * q.tiles + t.tile, 1u) == (uint32_t)ck.of - 1;
+      worker_sync();
+      if (sh.last && r < RP) {
         __threadfence();
-        worker_sync();
-        if (tid == 0)
-          sh.last = atomicAdd(q.plan.count + (int64_t)ck.joint * q.tiles + t.tile, 1u) == (uint32_t)ck.of - 1;
-        worker_sync();
-        const bool last = sh.last != 0;
-        if (last && !low && r < RP) {
-          __threadfence();
-#pragma unroll 1
-          for (int c = 0; c < 64; c += 16) {
-            float f[16];
 #pragma unroll
-            for (int x = 0; x < 16; ++x) f[x] = 0.f;
-            for (int k = 0; k < ck.of; ++k)
+        for (int c = 0; c < kOwn; ++c) {
 #pragma unroll
-              for (int x = 0; x < 16; ++x) f[x] += __ldcg(slots + k * apart + (c + x) * RP);
-            write(c, f);
-          }
+          for (int x = 0; x < 16; ++x) f[c][x] = 0.f;
+          for (int k = 0; k < ck.of; ++k)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) f[c][x] += __ldcg(slots + k * apart + (c * 16 + x) * RP);
+          write(c * 16, f[c]);
         }
       }
-      worker_sync();  // the low halves' sums are read before h or g go there again
+      worker_sync();  // all have read sh.last
     }
   }
   tc_fence_before();
@@ -1071,7 +1182,8 @@ struct GradSpace {
   int RP, x_tiles, tiles, chunk_rows;
   int64_t max_chunks, joints;
   int64_t dy_pitch, b_pitch;  // of dy and lora_b laid out anew (0: as they are)
-  size_t h, g, chunks, order, amax, count, part, dy, b, end;
+  int64_t max_steps;
+  size_t h, g, chunks, steps, order, count, part, dy, b, top, ids, images, down, runs, end;
 };
 GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_count) {
   GradSpace s;
@@ -1097,7 +1209,11 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.joints = M / (s.chunk_rows + 1);  // adapters of more than chunk_rows rows
   if (s.joints > L) s.joints = L;
   const int64_t parts = s.joints ? M / s.chunk_rows + s.joints : 0;  // their chunks
-  size_t at = 256;  // the chunks' total
+  s.max_steps = M / kStepRows + L;  // a whole step holds 128 rows, and an adapter has one that is not
+  if (s.max_steps > M) s.max_steps = M;
+  const size_t row_tiles = (size_t)((M + kTileRows - 1) / kTileRows);
+  const size_t image = (size_t)kStepRows * (s.RP > 64 ? 128 : 64) * 2 * 2;
+  size_t at = 256;  // the plan's totals
   auto take = [&](size_t bytes) {
     const size_t was = at;
     at += align256(bytes);
@@ -1106,8 +1222,13 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.h = take((size_t)M * s.RP * sizeof(float));
   s.g = take((size_t)M * s.RP * sizeof(float));
   s.chunks = take((size_t)s.max_chunks * sizeof(Chunk));
+  s.steps = take((size_t)s.max_steps * sizeof(Step));
   s.order = take((size_t)M * sizeof(int));
-  s.amax = take((size_t)2 * L * sizeof(uint32_t));
+  s.top = take(2 * row_tiles * kMaxSplit * kTileRows * sizeof(uint32_t));
+  s.ids = take(row_tiles * kTileRows * sizeof(uint32_t));
+  s.images = take((size_t)s.max_steps * 2 * image);
+  s.down = take((size_t)s.max_chunks * 2 * sizeof(float));
+  s.runs = take((size_t)s.max_steps * sizeof(int2));
   s.count = take((size_t)s.joints * s.tiles * sizeof(uint32_t));
   s.part = take((size_t)parts * s.tiles * kCols * s.RP * sizeof(float));
   s.dy_pitch = N % 8 ? (N + 7) / 8 * 8 : 0;
@@ -1119,7 +1240,8 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
 }
 
 template <int RP>
-cudaError_t launch_sums(const Sums& q, const CUtensorMap& map_a, int64_t items, int sm_count, bool pdl, cudaStream_t stream) {
+cudaError_t launch_sums(const Split& sp, const Sums& q, const SumMaps& maps, int64_t steps, int64_t items, int sm_count,
+                        bool pdl, cudaStream_t stream) {
   using Cfg = SumCfg<RP>;
   static thread_local int configured_dev = -1;
   int dev = 0;
@@ -1131,16 +1253,22 @@ cudaError_t launch_sums(const Sums& q, const CUtensorMap& map_a, int64_t items, 
     configured_dev = dev;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items < sm_count ? items : sm_count));
-  cfg.blockDim = dim3(kSumThreads);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RP>, q, map_a);
+  {
+    cfg.gridDim = dim3((unsigned)steps, 2 * kStepRows / kSplitRows);
+    cfg.blockDim = dim3(kSplitThreads);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, lora_split_kernel<RP>, sp);
+    if (e != cudaSuccess) return e;
+  }
+  cfg.gridDim = dim3((unsigned)(items < sm_count ? items : sm_count));
+  cfg.blockDim = dim3(kSumThreads);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  return cudaLaunchKernelEx(&cfg, lora_sums_kernel<RP>, q, maps);
 }
 
 }  // namespace
@@ -1156,7 +1284,6 @@ cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, voi
   q.a.w = static_cast<const __half*>(p.a);
   q.a.out16 = static_cast<__half*>(h16);
   q.lists = lists;
-  q.wait = true;
   q.status = status;
   return dispatch_products(q, sm_count, pdl, stream, err);
 }
@@ -1168,100 +1295,111 @@ size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L
 cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
                                  cudaStream_t stream, std::string* err) {
   cudaError_t e;
-  const GradSpace s = grad_space(p.M, p.N, p.K, p.R, p.L, sm_count);
-  uint8_t* base = static_cast<uint8_t*>(ws);
   if (p.L == 0) {  // nobody has an adapter
     return g.dx && !g.add_dx && p.M ? cudaMemsetAsync(g.dx, 0, (size_t)p.M * p.K * sizeof(__half), stream)
                                     : cudaSuccess;
   }
-  Plan plan;
-  plan.total = reinterpret_cast<int*>(base);
-  plan.chunks = reinterpret_cast<Chunk*>(base + s.chunks);
-  plan.order = reinterpret_cast<int*>(base + s.order);
-  plan.amax = reinterpret_cast<uint32_t*>(base + s.amax);
-  plan.count = reinterpret_cast<uint32_t*>(base + s.count);
+  if (p.M == 0) {  // no rows: the adapters' gradients are zero
+    e = g.da ? cudaMemsetAsync(g.da, 0, (size_t)p.L * p.R * p.K * sizeof(float), stream) : cudaSuccess;
+    if (e == cudaSuccess && g.db) e = cudaMemsetAsync(g.db, 0, (size_t)p.L * p.N * p.R * sizeof(float), stream);
+    return e;
+  }
+  const GradSpace s = grad_space(p.M, p.N, p.K, p.R, p.L, sm_count);
+  uint8_t* base = static_cast<uint8_t*>(ws);
   const __half *dy = static_cast<const __half*>(g.dy), *lora_b = static_cast<const __half*>(p.b);
   int64_t dy_ld = g.dy_ld;
-  bool anew = false;
-  {
-    // a warp's counters for every adapter; as many warps as fit 192 KB
-    int warps = (int)(192 * 1024 / (p.L * 4));
-    warps = warps > 32 ? 32 : warps;
-    static thread_local int configured_dev = -1;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (configured_dev != dev) {
-      e = cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024);
-      if (e != cudaSuccess) return e;
-      configured_dev = dev;
-    }
+  if (s.dy_pitch || s.b_pitch) {
     Repack rdy{}, rb{};
-    if (s.dy_pitch && p.M)
-      rdy = Repack{dy, reinterpret_cast<__half*>(base + s.dy), p.M, p.N, p.N, s.dy_pitch};
+    if (s.dy_pitch) rdy = Repack{dy, reinterpret_cast<__half*>(base + s.dy), p.M, p.N, p.N, s.dy_pitch};
     if (s.b_pitch) rb = Repack{lora_b, reinterpret_cast<__half*>(base + s.b), p.L * p.N, p.R, p.R, s.b_pitch};
     const int64_t pieces = (rdy.dst ? p.M * (s.dy_pitch / 8) : 0) + (rb.dst ? p.L * p.N * (s.b_pitch / 8) : 0);
-    const int64_t blocks = (pieces + kPlanThreads - 1) / kPlanThreads;
-    lora_plan_kernel<<<1 + (unsigned)(blocks < 2 * sm_count ? blocks : 2 * sm_count), kPlanThreads,
-                       (size_t)warps * p.L * 4, stream>>>(p, plan, warps, s.chunk_rows, s.joints * s.tiles, rdy, rb);
+    const int64_t blocks = (pieces + 255) / 256, most = 8 * (int64_t)sm_count;
+    lora_repack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(rdy, rb);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
     if (rdy.dst) {
       dy = rdy.dst;
       dy_ld = s.dy_pitch;
     }
     if (rb.dst) lora_b = rb.dst;
-    anew = rdy.dst || rb.dst;
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
-  if (p.M) {
-    Products q{};
-    q.p = p;
-    q.R8 = (p.R + 7) / 8 * 8;
-    q.a.v = static_cast<const __half*>(p.x);
-    q.a.ld = p.x_ld;
-    q.a.len = p.K;
-    q.a.w = static_cast<const __half*>(p.a);
-    q.a.out32 = reinterpret_cast<float*>(base + s.h);
-    q.a.amax = plan.amax;
-    q.b.v = dy;
-    q.b.ld = dy_ld;
-    q.b.len = p.N;
-    q.b.w = lora_b;
-    q.wait = anew;
-    q.b.out32 = reinterpret_cast<float*>(base + s.g);
-    q.b.amax = plan.amax + p.L;
-    q.status = g.status;
-    q.dx_zero = g.add_dx ? nullptr : static_cast<__half*>(g.dx);
-    if ((e = dispatch_products(q, sm_count, pdl, stream, err)) != cudaSuccess) return e;
-  }
-  Sums q{};
+  const int row_tiles = (int)((p.M + kTileRows - 1) / kTileRows);
+  uint32_t* top = reinterpret_cast<uint32_t*>(base + s.top);
+  Products q{};
   q.p = p;
-  q.h = reinterpret_cast<const float*>(base + s.h);
-  q.g = reinterpret_cast<const float*>(base + s.g);
-  q.plan = plan;
-  q.dx = static_cast<__half*>(g.dx);
-  q.da = g.da;
-  q.db = g.db;
-  q.part = reinterpret_cast<float*>(base + s.part);
-  q.add_dx = g.add_dx;
-  q.x_tiles = s.x_tiles;
-  q.tiles = s.tiles;
+  q.R8 = (p.R + 7) / 8 * 8;
+  q.a.v = static_cast<const __half*>(p.x);
+  q.a.ld = p.x_ld;
+  q.a.len = p.K;
+  q.a.w = static_cast<const __half*>(p.a);
+  q.a.out32 = reinterpret_cast<float*>(base + s.h);
+  q.a.top = top;
+  q.b.v = dy;
+  q.b.ld = dy_ld;
+  q.b.len = p.N;
+  q.b.w = lora_b;
+  q.b.out32 = reinterpret_cast<float*>(base + s.g);
+  q.b.top = top + (size_t)row_tiles * kMaxSplit * kTileRows;
+  q.tile_ids = reinterpret_cast<uint32_t*>(base + s.ids);
   q.status = g.status;
-  q.dy = dy;
-  q.dy_ld = dy_ld;
-  CUtensorMap map_a;
-  std::memset(&map_a, 0, sizeof(map_a));
-  {
-    const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.R, (uint64_t)p.L};
-    const uint64_t strides[2] = {(uint64_t)p.K * 2, (uint64_t)p.K * p.R * 2};
-    const uint32_t box[3] = {64, (uint32_t)s.RP, 1};
-    if (!encode_tmap_3d(&map_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                        err))
-      return cudaErrorInvalidValue;
-  }
+  q.dx_zero = g.add_dx ? nullptr : static_cast<__half*>(g.dx);
+  q.plan.total = reinterpret_cast<int*>(base);
+  q.plan.chunks = reinterpret_cast<Chunk*>(base + s.chunks);
+  q.plan.steps = reinterpret_cast<Step*>(base + s.steps);
+  q.plan.order = reinterpret_cast<int*>(base + s.order);
+  q.plan.count = reinterpret_cast<uint32_t*>(base + s.count);
+  q.plan.counters = s.joints * s.tiles;
+  q.plan.chunk_rows = s.chunk_rows;
+  if ((e = dispatch_products(q, sm_count, pdl, stream, err)) != cudaSuccess) return e;
+  Split sp{};
+  sp.p = p;
+  sp.plan = q.plan;
+  sp.h = q.a.out32;
+  sp.g = q.b.out32;
+  sp.top_h = q.a.top;
+  sp.top_g = q.b.top;
+  sp.tile_ids = q.tile_ids;
+  sp.tiles = q.tiles;
+  sp.split = q.split;
+  sp.images = base + s.images;
+  sp.down = reinterpret_cast<float*>(base + s.down);
+  sp.runs = reinterpret_cast<int2*>(base + s.runs);
+  Sums u{};
+  u.p = p;
+  u.dy = dy;
+  u.dy_ld = dy_ld;
+  u.plan = q.plan;
+  u.images = sp.images;
+  u.down = sp.down;
+  u.runs = sp.runs;
+  u.dx = static_cast<__half*>(g.dx);
+  u.da = g.da;
+  u.db = g.db;
+  u.part = reinterpret_cast<float*>(base + s.part);
+  u.add_dx = g.add_dx;
+  u.x_tiles = s.x_tiles;
+  u.tiles = s.tiles;
+  u.status = g.status;
+  SumMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.R, (uint64_t)p.L};
+  const uint64_t strides[2] = {(uint64_t)p.K * 2, (uint64_t)p.K * p.R * 2};
+  const uint32_t box[3] = {64, (uint32_t)s.RP, 1};
+  if (!encode_tmap_3d(&maps.a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                      err) ||
+      !encode_tmap_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, (uint64_t)p.K, (uint64_t)p.M,
+                      (uint64_t)p.x_ld * 2, 64, kStepRows, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
+      !encode_tmap_2d(&maps.x8, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p.x, (uint64_t)p.K, (uint64_t)p.M,
+                      (uint64_t)p.x_ld * 2, 64, 8, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
+      !encode_tmap_2d(&maps.dy, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy, (uint64_t)p.N, (uint64_t)p.M,
+                      (uint64_t)dy_ld * 2, 64, kStepRows, CU_TENSOR_MAP_SWIZZLE_128B, err) ||
+      !encode_tmap_2d(&maps.dy8, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dy, (uint64_t)p.N, (uint64_t)p.M,
+                      (uint64_t)dy_ld * 2, 64, 8, CU_TENSOR_MAP_SWIZZLE_128B, err))
+    return cudaErrorInvalidValue;
   const int64_t items = s.max_chunks * s.tiles;
-  if (p.R <= 16) return launch_sums<16>(q, map_a, items, sm_count, pdl, stream);
-  if (p.R <= 32) return launch_sums<32>(q, map_a, items, sm_count, pdl, stream);
-  if (p.R <= 64) return launch_sums<64>(q, map_a, items, sm_count, pdl, stream);
-  return launch_sums<128>(q, map_a, items, sm_count, pdl, stream);
+  if (p.R <= 16) return launch_sums<16>(sp, u, maps, s.max_steps, items, sm_count, pdl, stream);
+  if (p.R <= 32) return launch_sums<32>(sp, u, maps, s.max_steps, items, sm_count, pdl, stream);
+  if (p.R <= 64) return launch_sums<64>(sp, u, maps, s.max_steps, items, sm_count, pdl, stream);
+  return launch_sums<128>(sp, u, maps, s.max_steps, items, sm_count, pdl, stream);
 }
 
 }  // namespace qw
