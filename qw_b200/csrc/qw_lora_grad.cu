@@ -612,46 +612,60 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
   const int adapter = info.x, rows = info.z, chunk = info.w;
   const int* order = q.plan.order + info.y;
   const uint32_t* tops = which ? q.top_g : q.top_h;
-  if (tid == 0) top = 0u;
-  if (blockIdx.y == 0) {  // a row a thread
-    const int m = tid < rows ? __ldcg(order + tid) : -1;
-    const int next = tid + 1 < rows ? __ldcg(order + tid + 1) : -1;
-    const bool run = m >= 0 && next == m + 1;
-    const uint32_t here = __ballot_sync(0xffffffffu, run);
-    if (tid % 32 == 0) runs[tid / 32] = here;
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t mask = 0u;
-      for (int g = 0; g < kStepRows / 8; ++g) mask |= ((runs[g / 4] >> g % 4 * 8 & 0x7Fu) == 0x7Fu ? 1u : 0u) << g;
-      const bool all = (runs[0] & runs[1] & runs[2]) == 0xFFFFFFFFu && runs[3] == 0x7FFFFFFFu;
-      q.runs[step] = make_int2(all ? m : -1, (int)mask);
-    }
-  } else {
-    __syncthreads();
-  }
-  // the adapter's largest magnitude over the products' tiles
-  uint32_t bits = 0u;
-  for (int t = tid / 8; t < q.tiles; t += kSplitThreads / 8) {
-    const int64_t ids = (int64_t)t * kTileRows;
-#pragma unroll 4
-    for (int j = tid % 8; j < kTileRows; j += 8) {
-      if (__ldcg(q.tile_ids + ids + j) != (uint32_t)adapter) continue;
-#pragma unroll 4
-      for (int k = 0; k < q.split; ++k)
-        bits = max(bits, __ldcg(tops + ((int64_t)t * kMaxSplit + k) * kTileRows + j));
-    }
-  }
-  if (bits) atomicMax(&top, bits);
   constexpr int kPieces = RP / 4, kRowStep = kSplitThreads / kPieces, kPasses = kSplitRows / kRowStep;
   const int c = tid % kPieces * 4;
   const float* src = which ? q.g : q.h;
-  float4 v[kPasses];
+  // All that is read is asked for as early as its place is known: the time is the
+  // chain of reads (the plan, rows and tiles' adapters, values and maxima).
+  int m[kPasses];
 #pragma unroll
   for (int k = 0; k < kPasses; ++k) {
     const int row = row0 + k * kRowStep + tid / kPieces;
-    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < rows) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)__ldcg(order + row) * RP + c));
+    m[k] = row < rows ? __ldcg(order + row) : -1;
   }
+  const int mine = tid < rows ? __ldcg(order + tid) : -1, next = tid + 1 < rows ? __ldcg(order + tid + 1) : -1;
+  float4 v[kPasses];
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m[k] >= 0) v[k] = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)m[k] * RP + c));
+  }
+  if (tid == 0) top = 0u;
+  // the adapter's largest magnitude over the products' tiles, 16 of a tile's adapters a thread
+  uint32_t bits = 0u;
+  for (int t = tid / 8; t < q.tiles; t += kSplitThreads / 8) {
+    const int first = tid % 8 * 16;
+    uint4 id[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      id[j] = __ldcg(reinterpret_cast<const uint4*>(q.tile_ids + (int64_t)t * kTileRows + first) + j);
+    int at = -1;  // a tile names an adapter once
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = (uint32_t)adapter;
+      at = id[j].x == a ? 4 * j : id[j].y == a ? 4 * j + 1 : id[j].z == a ? 4 * j + 2 : id[j].w == a ? 4 * j + 3 : at;
+    }
+    if (at >= 0) {
+      const uint32_t* of = tops + (int64_t)t * kMaxSplit * kTileRows + first + at;
+      uint32_t b[kMaxSplit];
+#pragma unroll
+      for (int k = 0; k < kMaxSplit; ++k) b[k] = k < q.split ? __ldcg(of + k * kTileRows) : 0u;
+#pragma unroll
+      for (int k = 0; k < kMaxSplit; ++k) bits = b[k] > bits ? b[k] : bits;
+    }
+  }
+  if (blockIdx.y == 0) {  // a row a thread
+    const uint32_t here = __ballot_sync(0xffffffffu, mine >= 0 && next == mine + 1);
+    if (tid % 32 == 0) runs[tid / 32] = here;
+  }
+  __syncthreads();
+  if (blockIdx.y == 0 && tid == 0) {
+    uint32_t mask = 0u;
+    for (int g = 0; g < kStepRows / 8; ++g) mask |= ((runs[g / 4] >> g % 4 * 8 & 0x7Fu) == 0x7Fu ? 1u : 0u) << g;
+    const bool all = (runs[0] & runs[1] & runs[2]) == 0xFFFFFFFFu && runs[3] == 0x7FFFFFFFu;
+    q.runs[step] = make_int2(all ? mine : -1, (int)mask);
+  }
+  if (bits) atomicMax(&top, bits);
   __syncthreads();
   // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
   bits = top;
