@@ -234,9 +234,10 @@ struct Products {
 
 template <int RP>
 struct ProdCfg {
-  static constexpr int BLOCK = RP > 64 ? 128 : 64;    // TMEM columns of an adapter
+  static constexpr int BLOCK = RP > 64 ? 128 : 64;    // ranks in a step's rows of w
+  static constexpr int PITCH_T = RP < 32 ? 32 : RP;   // TMEM columns of an adapter
   static constexpr int COLUMNS = 256;                 // two CTAs an SM
-  static constexpr int GROUP = COLUMNS / BLOCK;       // adapters at a time
+  static constexpr int GROUP = COLUMNS / PITCH_T;     // adapters at a time
   static constexpr int V_STAGE = kTileRows * 128;
   static constexpr int W_STAGE = 64 * BLOCK * 2;
   static constexpr int STAGE = V_STAGE + W_STAGE;
@@ -326,12 +327,12 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   const uint32_t base = smem_u32(smem);
   bool ok = true;        // a bounded wait that ran out: go on without waiting
   uint32_t it0 = 0, vit0 = 0;  // steps and chunks of earlier rounds
-  constexpr uint32_t kDesc = mma_desc(kTileRows, TRANS ? Cfg::BLOCK : RP, false, TRANS);
+  constexpr uint32_t kDesc = mma_desc(kTileRows, RP, false, TRANS);
   auto multiply = [&](int chunk, int j, uint32_t vs, uint32_t ws) {
     const uint64_t a = operand_k(vs), b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
 #pragma unroll
     for (int kk = 0; kk < kChunk / 16; ++kk)
-      tc_mma_ss(sh.tmem + j * Cfg::BLOCK, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
+      tc_mma_ss(sh.tmem + j * Cfg::PITCH_T, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
                 chunk > 0 || kk > 0);
   };
 
@@ -392,7 +393,7 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       for (int c = 0; c < RP; c += 16) {
         uint32_t v[16];
         if (steps > 0) {
-          tmem_ld_32x32b_x16(sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::BLOCK + c, v);
+          tmem_ld_32x32b_x16(sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::PITCH_T + c, v);
           tmem_wait_ld();
         } else {
 #pragma unroll
