@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256) lora_repack_kernel(const Repack dy, const
 // above rank 64) and a row reads those of its own adapter: no row's sum ever
 // meets another adapter's values.  Sums over the cluster go through distributed
 // shared memory in rank order.
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 constexpr int kProdThreads = 128;
 constexpr int kChunk = 64;  // reduction values per step
 constexpr int kTileRows = 128;
@@ -240,11 +240,12 @@ struct ProdCfg {
   static constexpr int GROUP = COLUMNS / PITCH_T;     // adapters at a time
   static constexpr int V_STAGE = kTileRows * 128;
   static constexpr int W_STAGE = 64 * BLOCK * 2;
-  static constexpr int STAGE = V_STAGE + W_STAGE;
+  static constexpr int PER = RP > 64 ? 1 : 2;         // adapters a step
+  static constexpr int STAGE = V_STAGE + PER * W_STAGE;
   static constexpr int PITCH = RP + 4;                // floats of a row of sums
   static constexpr int SUMS = kTileRows * PITCH * 4;
   static constexpr int SMEM = (kStages * STAGE > SUMS ? kStages * STAGE : SUMS) + 1024;
-  static_assert(SMEM <= (RP > 64 ? 224 : 112) * 1024, "two CTAs an SM up to rank 64");
+  static_assert(SMEM <= 112 * 1024, "two CTAs an SM");
 };
 
 struct ProductMaps {
@@ -338,35 +339,41 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
 
   for (int j0 = 0; j0 < n; j0 += Cfg::GROUP) {
     const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
-    const int steps = (c1 - c0) * nj;
+    const int steps = (c1 - c0) * ((nj + Cfg::PER - 1) / Cfg::PER);
     if (warp == 1 && lane == 0) {  // loads
       uint32_t it = it0, vit = vit0;
       for (int c = c0; c < c1; ++c, ++vit) {
-        for (int j = 0; j < nj; ++j, ++it) {
+        for (int j = 0; j < nj; j += Cfg::PER, ++it) {
           const uint32_t s = it % kStages;
+          const int here = nj - j < Cfg::PER ? nj - j : Cfg::PER;
           if (it >= kStages)
             ok = ok && mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
-          mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) + (TRANS ? Cfg::W_STAGE : RP * 128)));
+          mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) +
+                                                        here * (TRANS ? Cfg::W_STAGE : RP * 128)));
           if (j == 0)
             tma_load_2d(smem + (vit % kStages) * Cfg::STAGE, map_v, &sh.full[s], c * kChunk, (int)m0);
-          uint8_t* dst = smem + s * Cfg::STAGE + Cfg::V_STAGE;
-          const int a = (int)sh.list[j0 + j];
-          if (TRANS) {
-            for (int b = 0; b < Cfg::BLOCK / 64; ++b)
-              tma_load_3d(dst + b * 8192, map_w, &sh.full[s], b * 64, c * kChunk, a);
-          } else {
-            tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
+          for (int i = 0; i < here; ++i) {
+            uint8_t* dst = smem + s * Cfg::STAGE + Cfg::V_STAGE + i * Cfg::W_STAGE;
+            const int a = (int)sh.list[j0 + j + i];
+            if (TRANS) {
+              for (int b = 0; b < Cfg::BLOCK / 64; ++b)
+                tma_load_3d(dst + b * 8192, map_w, &sh.full[s], b * 64, c * kChunk, a);
+            } else {
+              tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
+            }
           }
         }
       }
     } else if (warp == 0 && lane == 0) {  // products
       uint32_t it = it0, vit = vit0;
       for (int c = c0; c < c1; ++c, ++vit) {
-        for (int j = 0; j < nj; ++j, ++it) {
+        for (int j = 0; j < nj; j += Cfg::PER, ++it) {
           const uint32_t s = it % kStages;
           ok = ok && mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
           tc_fence_after();
-          multiply(c - c0, j, base + (vit % kStages) * Cfg::STAGE, base + s * Cfg::STAGE + Cfg::V_STAGE);
+          for (int i = 0; i < Cfg::PER && j + i < nj; ++i)
+            multiply(c - c0, j + i, base + (vit % kStages) * Cfg::STAGE,
+                     base + s * Cfg::STAGE + Cfg::V_STAGE + i * Cfg::W_STAGE);
           tc_commit(&sh.done[s]);
         }
       }
