@@ -6,7 +6,7 @@
 // with the sums over the rows of each adapter.
 //
 // Forward, two launches chained by programmatic dependent launch:
-//   rank_rows     h = s x A^T (below; a long forward: lora_products);
+//   rank_rows     h = s x A^T (below; many rows of a high rank: lora_products);
 //   the projection's own kernel: the decode kernel (at most 16 rows) adds h B^T
 //                 in its epilogue, the tcgen05 kernel takes h and B as further
 //                 columns of its reduction.
@@ -248,10 +248,10 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     q.lists.n = reinterpret_cast<uint32_t*>(base + f.second);
     q.lists.ids = reinterpret_cast<uint32_t*>(base + f.third);
     q.lists.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
-#ifndef TILE_M
-#define TILE_M 512
-#endif
-    if (p.M >= TILE_M) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
+    // Many rows of a high rank are worth the tcgen05 products' tiles of 128 rows
+    // (rank 64, 8 adapters, 5120 -> 5120, the whole call: 1024 rows in 116 us with
+    // them, 121 without; 512 rows 77 and 75; rank 32, 2048 rows to 17408: 395 and 388).
+    if (p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);

@@ -1,5 +1,5 @@
 // qw_lora_grad.cu -- gradient of the adapters beside a projection (and the
-// rank-space product of a long forward):
+// rank-space product of a forward with many rows of a high rank):
 //   h = s x A^T, g = s dy B                    per row, its adapter's A, B, s
 //   dA = g^T x, dB = dy^T h                    sums over the adapter's rows
 //   dx = g A (+ dx)
@@ -197,15 +197,18 @@ __global__ void __launch_bounds__(256) lora_repack_kernel(const Repack dy, const
 
 // ---------------------------------------------------------------- products
 // v W of each row's adapter, a tile of 128 rows at a time: out[m][r] = s sum_i
-// v[m][i] W[i][r].  HBM-bound by v, which is read once.
+// v[m][i] W[i][r].  HBM-bound by v, which is read once; short batches are bound by
+// the chain of loads, products and the cluster's sum.
 //
 // A cluster takes a tile and its CTAs split the reduction; a CTA walks 64 values
-// of it at a time, four TMA loads deep, and within those the adapters that the
-// tile's rows name, so v is staged once however mixed the rows are.
-// Every adapter has columns of its own in TMEM (four adapters at a time, two
-// above rank 64) and a row reads those of its own adapter: no row's sum ever
-// meets another adapter's values.  Sums over the cluster go through distributed
-// shared memory in rank order.
+// of it at a time, three steps of TMA loads deep, and within those the adapters
+// that the tile's rows name, two a step (one above rank 64), so v is staged once
+// however mixed the rows are.  Every adapter has columns of its own in TMEM (eight
+// adapters at a time, four above rank 32, two above 64) and a row reads those of
+// its own adapter: no row's sum ever meets another adapter's values.  Sums over
+// the cluster go through distributed shared memory in rank order.
+// x of 4096 x 17408 and dy of 4096 x 5120, rank 64: 53 us, 3.5 TB/s; one adapter a
+// step took 63, as tiles of several adapters were last.
 constexpr int kStages = 3;
 constexpr int kProdThreads = 128;
 constexpr int kChunk = 64;  // reduction values per step
@@ -441,10 +444,14 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       v.w *= s;
       if (f.out32) {
         *reinterpret_cast<float4*>(f.out32 + (m0 + row) * RP + c) = v;
-        const uint32_t b0 = __float_as_uint(fabsf(v.x)), b1 = __float_as_uint(fabsf(v.y));
-        const uint32_t b2 = __float_as_uint(fabsf(v.z)), b3 = __float_as_uint(fabsf(v.w));
-        const uint32_t lo = b0 > b1 ? b0 : b1, hi = b2 > b3 ? b2 : b3;
-        atomicMax(&sh.slot_max[slot], lo > hi ? lo : hi);  // a NaN is above every number
+        const float each[4] = {v.x, v.y, v.z, v.w};
+        uint32_t most = 0u;  // finite values alone: the others need no scale
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t b = __float_as_uint(fabsf(each[x]));
+          most = b < 0x7F800000u && b > most ? b : most;
+        }
+        atomicMax(&sh.slot_max[slot], most);
       } else if (c < q.R8) {
         // one rounding to fp16: the tensor cores take y's second product in fp16
         const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
@@ -579,12 +586,14 @@ int padded_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128
 
 // ------------------------------------------------------------------- split
 // The tensor cores take fp16, h and g are fp32: scaled by a power of two that
-// puts the adapter's largest magnitude below 2^15, each is split into the nearest
+// puts the adapter's largest finite magnitude below 2^15, each is split into the nearest
 // fp16 and the nearest fp16 of the rest (22 bits together), so dA and dB keep what
 // an fp32 product would.  A CTA lays out one step, 128 sorted rows of both, as the
 // sums' shared memory holds them: high halves then low halves, blocks of 64 ranks,
 // 128 rows of 128 swizzled bytes, so that a step is one bulk copy there however
-// many column tiles read it.
+// many column tiles read it (made anew by each column tile's CTA instead: 4096
+// rows to 5120 x 17408 columns, rank 64, 174 us, not 142).  Latency-bound, 4 us of
+// 256 rows' 19: three reads, each of what the one before names.
 template <int RP>
 struct SplitCfg {
   static constexpr int NRANK = RP > 64 ? 128 : 64;          // ranks in whole 128-byte rows
@@ -675,9 +684,9 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
   }
   if (bits) atomicMax(&top, bits);
   __syncthreads();
-  // 2^e brings the largest magnitude into [2^14, 2^15); nothing to scale by where it is 0 or not finite
+  // 2^e brings the largest magnitude into [2^14, 2^15)
   bits = top;
-  int e = bits == 0u || bits >= 0x7F800000u ? 0 : 14 - ((int)(bits >> 23) - 127);
+  int e = bits == 0u ? 0 : 14 - ((int)(bits >> 23) - 127);
   e = e > 126 ? 126 : (e < -126 ? -126 : e);
   const float up = __uint_as_float((uint32_t)(127 + e) << 23);
   if (row0 == 0 && tid == 0 && chunk >= 0) q.down[2 * chunk + which] = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -690,7 +699,8 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
     for (int x = 0; x < 2; ++x) {
       const __half2 h = __floats2half2_rn(f[2 * x], f[2 * x + 1]);
       const float2 back = __half22float2(h);
-      const __half2 l = __floats2half2_rn(f[2 * x] - back.x, f[2 * x + 1] - back.y);
+      // nothing is left of an infinity
+      const __half2 l = __floats2half2_rn(isinf(back.x) ? 0.f : f[2 * x] - back.x, isinf(back.y) ? 0.f : f[2 * x + 1] - back.y);
       hi[x] = *reinterpret_cast<const uint32_t*>(&h);
       lo[x] = *reinterpret_cast<const uint32_t*>(&l);
     }
@@ -702,18 +712,22 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 
 // -------------------------------------------------------------------- sums
 // A chunk of an adapter's rows and 128 columns of x (dA, and dx of those rows)
-// or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step:
+// or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step.
+// The CTAs take the column tiles in turns, so that at a time they read a stretch
+// of the same rows (equal shares of all the work, a range of columns each, took
+// 110 us where this takes 77):
 //   warps 8-10  load a step each in turn: its image of h or g (one bulk copy) and
-//               its rows of x or dy, by TMA where they are consecutive, else copied
-//               (cp.async; a warp's proxy fence waits for its own step's copies
-//               alone, and three steps are in flight.  TMA's four-row gathers were
-//               issued at one in 80 cycles: 12 GB/s an SM); warp 8 also an item's
-//               lora_a;
+//               its rows of x or dy, all 128 or 8 at a time by TMA where they are
+//               consecutive, else copied (cp.async; a warp's proxy fence waits for
+//               its own step's copies alone, and three steps are in flight.  TMA's
+//               four-row gathers were issued at one in 80 cycles: 12 GB/s an SM);
+//               warp 8 also an item's lora_a;
 //   warp 11     issues tcgen05.mma: D[ranks][columns] += (h or g)^T v, both
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers;
 //   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
-// HBM-bound by x, dy and dx.  Up to rank 64 the two halves of h or g are rows of
+// HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
+// rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
 // one D (64 of each) and are added when it is read.  dx, an fp16 result, takes the
 // nearest fp16 of g alone: its error stays below the result's own rounding.
 //
@@ -1214,7 +1228,7 @@ GradSpace grad_space(int64_t M, int64_t N, int64_t K, int R, int64_t L, int sm_c
   s.tiles = s.x_tiles + (int)((N + kCols - 1) / kCols);
   // The cuts of an adapter with all rows whose rounds of items take least, in
   // steps: an item's beginning and end cost about two, joining its sum two more
-  // (256 rows, 6144 x 5120: 15.9 us in one cut of two steps, 20 in two of one).
+  // (256 rows, 6144 x 5120: two cuts of one step took 4 us more than one of two).
   int64_t cuts = 1, best = 0;
   for (int64_t c = 1; c <= 8 && (c - 1) * kStepRows < M; ++c) {
     const int64_t rounds = (c * s.tiles + sm_count - 1) / sm_count;

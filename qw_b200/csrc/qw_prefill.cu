@@ -28,8 +28,9 @@
 // (adapter, r) hold lora_b of the tile's weight rows as A and h = s x A^T, fp16,
 // of the tokens that take that adapter as B, zero for the others.  Four more
 // warps write both (TMEM and the swizzled x slot) while the dequant warps are at
-// the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8 adapters of rank 32: the product
-// alone 291 us, a separate pass over y would read and write 214 MB more (33 us).
+// the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8
+// adapters of rank 32: the projection alone 368 to 396 us (power-capped clocks), with
+// adapters 2 to 6% more; a pass of its own over y would read and write 214 MB.
 // A zero times another adapter's infinity would be NaN: non-finite lora_b values
 // enter as zero and are added, for the tokens that own them, in the epilogue.
 //
