@@ -247,6 +247,73 @@ inline std::pair<Array, Array> top_k_candidate_logits(const Array& logits, int k
   return {idx, val};
 }
 
+// ---- adapters and distillation (no counterpart in the reference)
+namespace detail {
+// Scratch of one call: freed when the call's work is done (cudaFree waits).
+struct Scratch {
+  Array a;
+  int64_t bytes = 0;
+  template <class F>
+  explicit Scratch(F&& query) {
+    check(query(&bytes));
+    a = Array::empty({(bytes + 3) / 4}, DType::F32);
+  }
+};
+}  // namespace detail
+
+// quantized_linear_forward and, of each row's adapter, scale (x A^T) B^T
+inline Array quantized_linear_lora(const Array& x, const Array& w, const Array& scales, const Array* biases,
+                                   const Array* linear_bias, const Array& lora_a, const Array& lora_b,
+                                   const Array* lora_scales, const Array* adapter_idx, int group_size, int bits,
+                                   const std::string& mode, cudaStream_t s = nullptr) {
+  Array y = Array::empty(detail::with_last(x.shape(), w.shape()[0]), DType::F16);
+  const qw_array xd = x.desc(), wd = w.desc(), sd = scales.desc(), ad = lora_a.desc(), bd = lora_b.desc();
+  const detail::OptDesc qb(biases), lb(linear_bias), ls(lora_scales), ix(adapter_idx);
+  qw_array yd = y.desc();
+  const int64_t k = x.shape().empty() ? 1 : x.shape().back(), rank = lora_a.shape().size() == 3 ? lora_a.shape()[1] : 0;
+  const detail::Scratch ws([&](int64_t* n) {
+    return qw_quantized_linear_lora_workspace(k ? x.numel() / k : 0, w.shape()[0], rank, n);
+  });
+  check(qw_quantized_linear_lora(&xd, &wd, &sd, qb.p, lb.p, &ad, &bd, ls.p, ix.p, group_size, bits, mode.c_str(), &yd,
+                                 ws.a.data(), ws.bytes, s));
+  return y;
+}
+
+struct LoraGradients {
+  Array dx, da, db;  // f16 like x, f32 like lora_a and lora_b
+};
+inline LoraGradients lora_backward(const Array& x, const Array& dy, const Array& lora_a, const Array& lora_b,
+                                   const Array* lora_scales, const Array* adapter_idx, cudaStream_t s = nullptr) {
+  LoraGradients g{Array::empty(x.shape(), DType::F16), Array::empty(lora_a.shape(), DType::F32),
+                  Array::empty(lora_b.shape(), DType::F32)};
+  if (lora_a.shape().size() != 3 || lora_b.shape().size() != 3 || x.shape().empty())
+    throw Error(QW_EINVAL, "adapters are [L, R, K] and [L, N, R]");
+  const qw_array xd = x.desc(), yd = dy.desc(), ad = lora_a.desc(), bd = lora_b.desc();
+  const detail::OptDesc ls(lora_scales), ix(adapter_idx);
+  qw_array dx = g.dx.desc(), da = g.da.desc(), db = g.db.desc();
+  const int64_t k = x.shape().back();
+  const detail::Scratch ws([&](int64_t* n) {
+    return qw_lora_backward_workspace(k ? x.numel() / k : 0, lora_b.shape()[1], k, lora_a.shape()[1],
+                                      lora_a.shape()[0], n);
+  });
+  check(qw_lora_backward(&xd, &yd, &ad, &bd, ls.p, ix.p, 0, &dx, &da, &db, ws.a.data(), ws.bytes, s));
+  return g;
+}
+
+// (loss f32 [M], dlogits like logits) against a teacher's stored top logits
+inline std::pair<Array, Array> topk_distillation(const Array& logits, const Array& teacher_idx,
+                                                 const Array& teacher_values, const Array* temperature,
+                                                 const Array* row_weights, cudaStream_t s = nullptr) {
+  const int64_t v = logits.shape().empty() ? 1 : logits.shape().back();
+  Array loss = Array::empty({v ? logits.numel() / v : 0}, DType::F32);
+  Array grad = Array::empty(logits.shape(), logits.dtype());
+  const qw_array zd = logits.desc(), id = teacher_idx.desc(), td = teacher_values.desc();
+  const detail::OptDesc tp(temperature), rw(row_weights);
+  qw_array ld = loss.desc(), gd = grad.desc();
+  check(qw_topk_distill(&zd, &id, &td, tp.p, rw.p, &ld, &gd, s));
+  return {loss, grad};
+}
+
 // QuantizedWeight (layers.rs:35-174)
 struct QuantizedWeight {
   Array weight;  // u32 [N, K*bits/32]

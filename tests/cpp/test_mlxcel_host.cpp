@@ -6,6 +6,7 @@
 // (oracle/qw_oracle.h, linked as test infrastructure).  Needs a GPU; run by
 // tests/test_cpp_host.py.  Prints one line per test and exits non-zero on
 // the first failure.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -236,6 +237,73 @@ int main() {
       EXPECT(threw);
     }
     qw::top_k_candidate_logits(zd, 1);
+  });
+
+  // adapters: their term and its gradient against host sums, rows without one as the plain linear
+  run("adapters_forward_and_gradient", [] {
+    const int64_t M = 5, N = 64, K = 128, R = 4, L = 2;
+    const HostQuant q = random_quantized_weight(N, K, 21);
+    DevQuant d = upload(q, N, K);
+    const auto xh = normal_f16(M * K, 1.0, 22), ah = normal_f16(L * R * K, 0.1, 23), bh = normal_f16(L * N * R, 1.0, 24);
+    const auto gh = normal_f16(M * N, 0.5, 25);
+    const std::vector<uint32_t> ih = {1, 0xFFFFFFFFu, 0, 1, 7};
+    const std::vector<float> sh = {0.5f, 2.f};
+    qw::Array x = qw::Array::from_host(xh.data(), {M, K}, qw::DType::F16);
+    qw::Array a = qw::Array::from_host(ah.data(), {L, R, K}, qw::DType::F16);
+    qw::Array b = qw::Array::from_host(bh.data(), {L, N, R}, qw::DType::F16);
+    qw::Array sc = qw::Array::from_host(sh.data(), {L}, qw::DType::F32);
+    qw::Array ix = qw::Array::from_host(ih.data(), {M}, qw::DType::U32);
+    qw::Array dy = qw::Array::from_host(gh.data(), {M, N}, qw::DType::F16);
+    const auto f = [](const std::vector<uint16_t>& v, int64_t i) { return (double)qwo_f16_to_f32(v[(size_t)i]); };
+    const auto base = qw::quantized_linear_forward(x, d.w, d.s, &d.b, nullptr, 64, 4, "affine").to_host<uint16_t>();
+    const auto y = qw::quantized_linear_lora(x, d.w, d.s, &d.b, nullptr, a, b, &sc, &ix, 64, 4, "affine").to_host<uint16_t>();
+    const qw::LoraGradients g = qw::lora_backward(x, dy, a, b, &sc, &ix);
+    const auto da = g.da.to_host<float>(), db = g.db.to_host<float>();
+    std::vector<double> wa((size_t)(L * R * K)), wb((size_t)(L * N * R));
+    double worst = 0, big = 0;
+    for (int64_t m = 0; m < M; ++m) {
+      const int64_t l = ih[(size_t)m];
+      if (l >= L) {
+        for (int64_t n = 0; n < N; ++n) EXPECT(y[(size_t)(m * N + n)] == base[(size_t)(m * N + n)]);
+        continue;
+      }
+      for (int64_t r = 0; r < R; ++r) {
+        double h = 0, gr = 0;
+        for (int64_t k = 0; k < K; ++k) h += f(xh, m * K + k) * f(ah, (l * R + r) * K + k);
+        for (int64_t n = 0; n < N; ++n) gr += f(gh, m * N + n) * f(bh, (l * N + n) * R + r);
+        h *= sh[(size_t)l];
+        gr *= sh[(size_t)l];
+        for (int64_t k = 0; k < K; ++k) wa[(size_t)((l * R + r) * K + k)] += gr * f(xh, m * K + k);
+        for (int64_t n = 0; n < N; ++n) wb[(size_t)((l * N + n) * R + r)] += f(gh, m * N + n) * h;
+      }
+      for (int64_t n = 0; n < N; ++n) {
+        double t = f(base, m * N + n);
+        for (int64_t r = 0; r < R; ++r) {
+          double h = 0;
+          for (int64_t k = 0; k < K; ++k) h += f(xh, m * K + k) * f(ah, (l * R + r) * K + k);
+          t += sh[(size_t)l] * h * f(bh, (l * N + n) * R + r);
+        }
+        worst = std::max(worst, std::fabs(t - f(y, m * N + n)));
+        big = std::max(big, std::fabs(t));
+      }
+    }
+    EXPECT(worst <= big * 2e-3);  // base and y are each rounded to fp16
+    double ea = 0, eb = 0, ma = 0, mb = 0;
+    for (size_t i = 0; i < wa.size(); ++i) ea = std::max(ea, std::fabs(da[i] - wa[i])), ma = std::max(ma, std::fabs(wa[i]));
+    for (size_t i = 0; i < wb.size(); ++i) eb = std::max(eb, std::fabs(db[i] - wb[i])), mb = std::max(mb, std::fabs(wb[i]));
+    EXPECT(ea <= ma * 1e-4 && eb <= mb * 1e-4);
+  });
+
+  // a row whose logits are the teacher's, over all columns, has no loss and no gradient
+  run("distillation_of_a_teacher_by_itself", [] {
+    const int64_t V = 40;
+    const auto z = normal_f16(V, 2.0, 31);
+    std::vector<uint32_t> ids((size_t)V);
+    for (size_t i = 0; i < ids.size(); ++i) ids[i] = (uint32_t)i;
+    qw::Array zd = qw::Array::from_host(z.data(), {1, V}, qw::DType::F16);
+    auto [loss, grad] = qw::topk_distillation(zd, qw::Array::from_host(ids.data(), {1, V}, qw::DType::U32), zd, nullptr, nullptr);
+    EXPECT(std::fabs(loss.to_host<float>()[0]) <= 1e-5f);
+    for (uint16_t v : grad.to_host<uint16_t>()) EXPECT(std::fabs(qwo_f16_to_f32(v)) <= 1e-6f);
   });
 
   // the load-time validators (layers.rs:1286-1318, :1568-1570) as exceptions
