@@ -6,6 +6,7 @@
 
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -1145,6 +1146,15 @@ bool overlap(const qw_array* a, const qw_array* b, int64_t a_ld = 0, int64_t b_l
   return pa < pb + span(b, b_ld) && pb < pa + span(a, a_ld);
 }
 
+// Whether an output meets any of the arrays (null: not there) or the workspace.
+bool overlaps_any(const qw_array* out, std::initializer_list<const qw_array*> others, const void* workspace = nullptr,
+                  int64_t workspace_bytes = 0) {
+  for (const qw_array* o : others)
+    if (o && overlap(out, o)) return true;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(out->data), w = reinterpret_cast<uintptr_t>(workspace);
+  return workspace && p < w + (size_t)workspace_bytes && w < p + (size_t)numel(out) * dtype_bytes(out->dtype);
+}
+
 // The adapters of a call over M rows of x: A f16 [L, R, K], B f16 [L, N, R],
 // scales f32 [L] (nullable), idx u32 [M] (nullable).  Fills p.a .. p.R.
 int check_adapters(const qw_array* lora_a, const qw_array* lora_b, const qw_array* lora_scales,
@@ -1256,6 +1266,9 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
   const int token_tile = sa.M > 16 ? prefill_token_tile(sa.M) : 0;
   if ((rc = check_workspace(workspace, workspace_bytes, skinny + lora_forward_bytes(sa.M, la.R, token_tile))))
     return rc;
+  if (overlaps_any(y, {w, scales, biases, linear_bias, lora_a, lora_b, lora_scales, adapter_idx}, workspace,
+                   workspace_bytes))
+    return fail(QW_EINVAL, "y must not overlap another operand or the workspace");
   DeviceRes* res = nullptr;
   std::string err;
   if (!device_res(dev, &res, &err)) return fail(QW_ENOMEM, err);
@@ -1341,6 +1354,14 @@ int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora
     return fail(QW_EINVAL, "dy must be 16-byte aligned (2-byte where N is no multiple of 8)");
   if (dx && (overlap(dx, x, 0, la.x_ld) || overlap(dx, dy)))
     return fail(QW_EINVAL, "dx must not overlap x or dy");
+  for (const qw_array* out : {dx, da, db}) {
+    if (!out) continue;
+    if (overlap(out, x, 0, la.x_ld) ||
+        overlaps_any(out, {dy, lora_a, lora_b, lora_scales, adapter_idx, out == dx ? nullptr : dx,
+                           out == da ? nullptr : da, out == db ? nullptr : db},
+                     workspace, workspace_bytes))
+      return fail(QW_EINVAL, "dx, da and db must not overlap another operand or the workspace");
+  }
   int dev = 0;
   const cudaError_t cd = cudaGetDevice(&dev);
   if (cd != cudaSuccess) return cuda_fail(cd, "cudaGetDevice");
@@ -1408,6 +1429,10 @@ int qw_topk_distill(const qw_array* logits, const qw_array* teacher_idx, const q
     return fail(QW_EINVAL, "an array is misaligned");
   if (dlogits && dlogits->data != logits->data && overlap(dlogits, logits))
     return fail(QW_EINVAL, "dlogits must be the logits' own buffer or not overlap it");
+  if (dlogits && overlaps_any(dlogits, {teacher_idx, teacher_values, temperature, row_weights, loss}))
+    return fail(QW_EINVAL, "dlogits must not overlap another operand");
+  if (overlaps_any(loss, {logits, teacher_idx, teacher_values, temperature, row_weights}))
+    return fail(QW_EINVAL, "loss must not overlap another operand");
   DistillArgs a{};
   a.logits = logits->data;
   a.idx = static_cast<const uint32_t*>(teacher_idx->data);

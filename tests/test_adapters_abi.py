@@ -154,3 +154,19 @@ def test_adapter_stack_shapes_are_checked():
     with pytest.raises(ValueError, match="global scale"):
         qw_b200.QuantizedLinear(None, None, None, global_scale=torch.ones(1),
                                 lora=qw_b200.LoraAdapters(torch.zeros(2, 4, 8), torch.zeros(2, 8, 4)))
+
+
+@pytest.mark.parametrize("change", [dict(dx=arr([M, K], F16, 0x10100), x=arr([M, K], F16, 0x70000)),
+                                    dict(da=arr([L, R, K], F32, 0x40010)), dict(da=arr([L, R, K], F32, 0x9000c0)),
+                                    dict(db=arr([L, N, R], F32, 0xa1ff00)), dict(db=arr([L, N, R], F32, 0x10000))])
+def test_gradients_must_not_overlap_operands(change):
+    assert backward(**change) == _lib.QW_EINVAL
+    assert "overlap" in err()
+
+
+@pytest.mark.parametrize("change", [dict(dz=arr([M, V], F16, 0x10000 + 0x1000), z=arr([M, V], F16, 0x500000),
+                                         idx=arr([M, TOP], U32, 0x11770)),
+                                    dict(loss=arr([M], F32, 0x900000)), dict(loss=arr([M], F32, 0x10004))])
+def test_distillation_outputs_must_not_overlap_operands(change):
+    assert distill(**change) == _lib.QW_EINVAL
+    assert "overlap" in err()
