@@ -6,8 +6,8 @@
 // HBM-bound: z has to be read once and dz written once.  q needs the whole
 // row's maximum and sum before the first dz can leave, so a row is held on chip
 // in between: a thread-block cluster of up to 8 CTAs per row, each CTA a
-// contiguous share of it in shared memory (up to 72 KB, three CTAs of 256
-// threads an SM; longer rows up to 200 KB a CTA).  What a share has beyond that
+// contiguous share of it in shared memory (up to 40 KB, five CTAs of 128 threads
+// an SM, or 72 KB, three of 256; longer rows up to 200 KB a CTA).  What a share has beyond that
 // (rows of more than 1.6 MB) is read a second time, from L2.  Clusters are
 // persistent: behind each vector of dz that a thread writes, it starts the
 // asynchronous copy of the next row's vector into the same place, which only
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
 }
 
 constexpr int64_t kMaxSmem = 227 * 1024 - 2048;  // dynamic shared memory a CTA may take
-constexpr int64_t kShareBytes = 72 * 1024;       // share of a row that lets three CTAs sit on an SM
+constexpr int64_t kShortShare = 40 * 1024, kLongShare = 72 * 1024;  // shares of a row
 
 template <typename T, int TH, int PER_SM, bool EVEN>
 cudaError_t launch_even(const DistillArgs& p, int cluster, cudaStream_t stream) {
@@ -552,10 +552,18 @@ template <typename T>
 cudaError_t launch_type(const DistillArgs& p, int sm_count, cudaStream_t stream) {
   const int64_t bytes = p.V * (int64_t)sizeof(T);
   if (bytes <= 16384) return launch_rows<T, 128, 8>(p, 1, stream);
-  // shares of at most 72 KB; with few rows more CTAs, down to 8 KB a CTA, while they fit the SMs
-  int64_t cluster = (bytes + kShareBytes - 1) / kShareBytes;
+  // Many rows that a cluster holds in shares of 40 KB: five CTAs of 128 threads an
+  // SM, whose rows' reductions cover one another's (2048 rows of 151936 fp16 in 287
+  // us; 315 in shares of 72 KB, three CTAs of 256 threads; 333 rows of 32003 in 18.4
+  // and 19.3).  Few rows, where a row's own time counts: 256 threads, and more CTAs
+  // down to 8 KB a CTA while they fit the SMs (4 rows of 151936 in 7.8 us, 9.1 with
+  // 128).  Longer rows: shares of 72 KB.
+  const bool short_share = bytes <= kClusterMax * kShortShare;
+  const int64_t share = short_share ? kShortShare : kLongShare;
+  int64_t cluster = (bytes + share - 1) / share;
   while (cluster < kClusterMax && p.M * (cluster + 1) <= sm_count && bytes / (cluster + 1) >= 8192) ++cluster;
   if (cluster > kClusterMax) cluster = kClusterMax;
+  if (short_share && p.M * cluster > sm_count) return launch_rows<T, 128, 5>(p, (int)cluster, stream);
   return launch_rows<T, 256, 3>(p, (int)cluster, stream);
 }
 
