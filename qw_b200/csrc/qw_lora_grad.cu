@@ -736,8 +736,9 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 constexpr int kCols = 128;
 constexpr int kWorkers = 256;
 constexpr int kWarpCols = kCols / (kWorkers / 128);  // columns of D or dx a worker warp reads, of 32 rows
-constexpr int kVStages = 3;                          // and as many warps that load
-constexpr int kMmaWarp = kWorkers / 32 + kVStages;
+constexpr int kVStages = 3;                          // and two warps for each that load
+constexpr int kLoaders = 2;
+constexpr int kMmaWarp = kWorkers / 32 + kLoaders * kVStages;
 constexpr int kSumThreads = (kMmaWarp + 1) * 32;
 
 struct Sums {
@@ -839,7 +840,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kVStages; ++i) {
-      mbar_init(&sh.vfull[i], 1);
+      mbar_init(&sh.vfull[i], kLoaders);
       mbar_init(&sh.vempty[i], 1);
       mbar_init(&sh.gfull[i], 1);
     }
@@ -868,12 +869,13 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 
   if (warp >= kWorkers / 32 && warp < kMmaWarp) {
     // -------------------------------------------------------------- loads
-    const int slot = warp - kWorkers / 32;
+    const int slot = (warp - kWorkers / 32) / kLoaders, part = (warp - kWorkers / 32) % kLoaders;
+    constexpr int kQuarters = 4 / kLoaders;  // of the step's rows
     uint32_t it = 0, ai = 0;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
       const Item t = item_at(q, i);
       if (t.steps == 0) continue;
-      if (t.dx && slot == 0) {
+      if (t.dx && slot == 0 && part == 0) {
         if (lane == 0) {
           if (ai > 0) ok = ok && mbar_wait(&sh.aempty, (ai - 1) & 1, q.status, kDevTimeoutEmpty);
           mbar_arrive_expect_tx(&sh.afull, RP * kCols * 2);
@@ -893,45 +895,48 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         const uint32_t gb = it % Cfg::G_BUFS;
         const int2 runs = __ldcg(q.runs + t.ck.step0 + step);
         const int rows = t.ck.count - step * kStepRows;
-        int at[4];  // the step's rows, 32 k + lane
+        int at[kQuarters];  // this warp's rows of the step
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          at[k] = 32 * k + lane < rows ? __ldcg(order + step * kStepRows + 32 * k + lane) : -1;
+        for (int k = 0; k < kQuarters; ++k) {
+          const int r = 32 * (part * kQuarters + k) + lane;
+          at[k] = r < rows ? __ldcg(order + step * kStepRows + r) : -1;
+        }
         const int head = lane % 16 * 8 < rows ? __ldcg(order + step * kStepRows + lane % 16 * 8) : -1;
         // The products that read this stage are done; then those that read the
         // image's buffer, which are at most two steps later (so that a barrier
         // is never a whole turn ahead of its waiter).
         if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[slot], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
         uint8_t* const stage = smem + slot * Cfg::V_STAGE;
-        if (lane == 0 && runs.y) mbar_expect_tx(&sh.vfull[slot], (uint32_t)__popc(runs.y) * 2048u);
+        if (lane == 0 && part == 0 && runs.y) mbar_expect_tx(&sh.vfull[slot], (uint32_t)__popc(runs.y) * 2048u);
         __syncwarp();
         if (runs.x >= 0) {
-          if (lane == 0)
+          if (lane == 0 && part == 0)
             for (int b = 0; b < 2; ++b)
               tma_load_2d(stage + b * Cfg::BLOCK, t.is_x ? &maps.x : &maps.dy, &sh.vfull[slot], (int)t.col0 + b * 64,
                           runs.x);
         } else {
           // groups of 8 consecutive rows by TMA, a group and a block of columns a lane
-          if (runs.y >> lane % 16 & 1)
+          if (part == 0 && (runs.y >> lane % 16 & 1))
             tma_load_2d(stage + lane / 16 * Cfg::BLOCK + lane % 16 * 1024, t.is_x ? &maps.x8 : &maps.dy8,
                         &sh.vfull[slot], (int)t.col0 + lane / 16 * 64, head);
           const uint32_t dst = smem_u32(stage) + lane % 16 / 8 * Cfg::BLOCK;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < kQuarters; ++k)
 #pragma unroll 1
             for (int g = 0; g < 4; ++g) {
+              const int group = 4 * (part * kQuarters + k) + g;
               // the products take no rows behind the last 16 that hold one
-              if ((runs.y >> (4 * k + g) & 1) || (4 * k + g) / 2 * 16 >= rows) continue;
+              if ((runs.y >> group & 1) || group / 2 * 16 >= rows) continue;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {  // two rows of 256 bytes
                 const int in_k = g * 8 + 2 * j + lane / 16;
                 const int m = __shfl_sync(0xffffffffu, at[k], in_k);
                 const bool in = in_c && m >= 0;
-                cp_async16(dst + swizzled(32 * k + in_k, lane % 8), v + (in ? m * ld + c : 0), in);
+                cp_async16(dst + swizzled(group * 8 + 2 * j + lane / 16, lane % 8), v + (in ? m * ld + c : 0), in);
               }
             }
         }
-        if (lane == 0) {
+        if (lane == 0 && part == 0) {
           if (it >= Cfg::G_BUFS) {
             const uint32_t was = it - Cfg::G_BUFS;
             ok = ok && mbar_wait(&sh.vempty[was % kVStages], (was / kVStages) & 1, q.status, kDevTimeoutEmpty);
