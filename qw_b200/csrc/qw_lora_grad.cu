@@ -552,9 +552,11 @@ cudaError_t launch_products(Products& q, int sm_count, bool pdl, cudaStream_t st
   const int products = q.b.v ? 2 : 1;
   int64_t most = (q.a.len + kChunk - 1) / kChunk;
   if (q.b.v && (q.b.len + kChunk - 1) / kChunk > most) most = (q.b.len + kChunk - 1) / kChunk;
-  // Splits for about four CTAs an SM, each two SM's worth in flight: the loads of
-  // an SM run at 46 GB/s (a 128-byte row in 5 cycles), so all of them are needed.
-  // 16 CTAs to a cluster, twice the portable size, where the tiles are few.
+  // Splits for about four CTAs an SM, each two SM's worth in flight: an SM's TMA
+  // loads run at 46 GB/s (a 128-byte row in 5 cycles), so all SMs are needed.  16
+  // CTAs to a cluster, twice the portable size, where the tiles are few.  (Fewer
+  // CTAs of six stages, one an SM: 1024 rows, 17408 and 5120 columns, rank 64, 71 us
+  // a call; so 63.)
   int C = most < kMaxSplit ? (int)most : kMaxSplit;
   while (C > 1 && (int64_t)products * q.tiles * C > (C > 8 ? 1 : 4) * sm_count) --C;
   q.split = C;
@@ -716,13 +718,14 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // The CTAs take the column tiles in turns, so that at a time they read a stretch
 // of the same rows (equal shares of all the work, a range of columns each, took
 // 110 us where this takes 77):
-//   warps 8-10  load a step each in turn: its image of h or g (one bulk copy) and
-//               its rows of x or dy, all 128 or 8 at a time by TMA where they are
-//               consecutive, else copied (cp.async; a warp's proxy fence waits for
-//               its own step's copies alone, and three steps are in flight.  TMA's
-//               four-row gathers were issued at one in 80 cycles: 12 GB/s an SM);
-//               warp 8 also an item's lora_a;
-//   warp 11     issues tcgen05.mma: D[ranks][columns] += (h or g)^T v, both
+//   warps 8-13  load, two to a step in turn: its image of h or g (one bulk copy)
+//               and its rows of x or dy, all 128 or 8 at a time by TMA where they
+//               are consecutive, else copied (cp.async; a warp's proxy fence waits
+//               for its own step's copies alone, and three steps are in flight.
+//               One warp a step: 4096 rows in any order 187 us a call, not 173.
+//               TMA's four-row gathers were issued at one in 80 cycles: 12 GB/s an
+//               SM); warp 8 also an item's lora_a;
+//   warp 14     issues tcgen05.mma: D[ranks][columns] += (h or g)^T v, both
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers;
 //   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
