@@ -185,7 +185,8 @@ struct Repack {
 };
 __device__ __forceinline__ void repack(const Repack& r) {
   const int64_t pieces = r.pitch / 8;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < r.rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
+  const int64_t step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < r.rows * pieces; i += step) {
     const int64_t row = i / pieces, c = i % pieces * 8;
     *reinterpret_cast<uint4*>(r.dst + row * r.pitch + c) = load_halves(r.src + row * r.ld + c, r.width - c);
   }
@@ -702,7 +703,8 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
       const __half2 h = __floats2half2_rn(f[2 * x], f[2 * x + 1]);
       const float2 back = __half22float2(h);
       // nothing is left of an infinity
-      const __half2 l = __floats2half2_rn(isinf(back.x) ? 0.f : f[2 * x] - back.x, isinf(back.y) ? 0.f : f[2 * x + 1] - back.y);
+      const __half2 l = __floats2half2_rn(isinf(back.x) ? 0.f : f[2 * x] - back.x,
+                                          isinf(back.y) ? 0.f : f[2 * x + 1] - back.y);
       hi[x] = *reinterpret_cast<const uint32_t*>(&h);
       lo[x] = *reinterpret_cast<const uint32_t*>(&l);
     }
@@ -972,7 +974,8 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           const uint32_t s = it % kVStages, gb = it % Cfg::G_BUFS;
           ok = ok && mbar_wait(&sh.vfull[s], (it / kVStages) & 1, q.status, kDevTimeoutFull);
           ok = ok && mbar_wait(&sh.gfull[gb], (it / Cfg::G_BUFS) & 1, q.status, kDevTimeoutFull);
-          if (t.dx && dxs >= 2) ok = ok && mbar_wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, q.status, kDevTimeoutAccum);
+          if (t.dx && dxs >= 2)
+            ok = ok && mbar_wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, q.status, kDevTimeoutAccum);
           tc_fence_after();
           const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * Cfg::G_STAGE;
           auto dx = [&]() {
