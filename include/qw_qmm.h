@@ -294,7 +294,9 @@ int qw_quantized_linear_forward_global_scale(const qw_array* x, const qw_array* 
  * in fp32 rounded once.  x, w, scales, biases, linear_bias (nullable) as in
  * qw_quantized_linear_forward; y must not overlap x.  With more than 16 rows
  * the rank-space product scale * x A^T feeds the tensor cores as fp16 (so it
- * must stay below 65504); with up to 16 it stays fp32.
+ * must stay below 65504), and so do the weights, fp16(s q + b) rounded once;
+ * with up to 16 both stay fp32, and rows without an adapter have the bits of
+ * qw_quantized_linear_forward.
  * No counterpart in the reference, whose linears carry no adapters. */
 int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_array* scales, const qw_array* biases,
                              const qw_array* linear_bias, const qw_array* lora_a, const qw_array* lora_b,

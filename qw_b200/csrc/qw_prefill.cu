@@ -29,12 +29,14 @@
 // of the tokens that take that adapter as B, zero for the others.  Four more
 // warps write both (TMEM and the swizzled x slot) while the dequant warps are at
 // the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8
-// adapters of rank 32: the projection alone 368 to 396 us (power-capped clocks), with
-// adapters 2 to 6% more; a pass of its own over y would read and write 214 MB.
+// adapters of rank 32: 379 us, where the projection alone takes 368 to 396 (power-
+// capped clocks); a pass of its own over y would read and write 214 MB.
 // A zero times another adapter's infinity would be NaN: non-finite lora_b values
 // enter as zero and are added, for the tokens that own them, in the epilogue.
+// The weights are fp16(s q + b), rounded once: the result's error is half of that
+// with the two roundings below (2.8e-4 and 5.7e-4 of y in the mean, 2048 x 17408 x 5120).
 //
-// The weights the MMA consumes are exactly qw_dequantize's (fp16(fp16(s*q)
+// Otherwise the weights the MMA consumes are exactly qw_dequantize's (fp16(fp16(s*q)
 // + b)): pairs (1024 + q_even, 1024 + 16 q_odd) come from one prmt and one
 // and, fma.rn.f16x2 with (s, s/16) and (-1024 s, -64 s) gives fp16(s*q)
 // rounded once from the exact product, and add.rn.f16x2 adds b.  Scales too
@@ -171,6 +173,47 @@ __device__ __forceinline__ void dequant_group_slow(const uint32_t (&wd)[4], __ha
       const __half t0 = __hmul_rn(s, __uint2half_rn(q0));
       const __half t1 = __hmul_rn(s, __uint2half_rn(q1));
       out[4 * i + pp] = h2_bits(__halves2half2(__hadd_rn(t0, b), __hadd_rn(t1, b)));
+    }
+  }
+}
+
+// fp16(s q + b) of a block's 64 codes, rounded once.  A code's bits in the low
+// byte of a half are the subnormal 16 q 2^-24 (4 bits) or q 2^-24 (8 bits), exact:
+// one fma with s 2^20 or s 2^24, as long as that is finite; larger scales take
+// 1024 + 16 q (or q) less 1024, with s/16 (or s) and for the even 4-bit codes s.
+template <int BITS>
+__device__ __forceinline__ void weights_once(const uint32_t (&wd)[BITS * 2], __half s, uint32_t b2,
+                                             uint32_t (&out)[2][16]) {
+  const float sf = __half2float(s);
+  if (fabsf(sf) < (BITS == 4 ? 0.0624f : 0.0039f)) {
+    const __half up = __float2half_rn(sf * (BITS == 4 ? 1048576.f : 16777216.f));
+    const uint32_t up2 = h2_bits(__halves2half2(up, up));
+#pragma unroll
+    for (int i = 0; i < BITS * 2; ++i) {
+      if (BITS == 4) {
+        const uint32_t even = wd[i] << 4;
+#pragma unroll
+        for (int pp = 0; pp < 4; ++pp)
+          out[i / 4][4 * (i % 4) + pp] = hfma2_rn(prmt(even, wd[i], 0x0400u + 0x0101u * pp) & 0x00F000F0u, up2, b2);
+      } else {
+        out[i / 8][2 * (i % 8)] = hfma2_rn(prmt(wd[i], 0u, 0x5140u), up2, b2);
+        out[i / 8][2 * (i % 8) + 1] = hfma2_rn(prmt(wd[i], 0u, 0x5342u), up2, b2);
+      }
+    }
+  } else {
+    const uint32_t s2 = h2_bits(__halves2half2(s, BITS == 4 ? __float2half_rn(sf * 0.0625f) : s));
+#pragma unroll
+    for (int i = 0; i < BITS * 2; ++i) {
+      if (BITS == 4) {
+#pragma unroll
+        for (int pp = 0; pp < 4; ++pp) {
+          const uint32_t t = prmt(wd[i], 0x64646464u, 0x4040u + 0x0101u * pp) & 0xFFF0FF0Fu;
+          out[i / 4][4 * (i % 4) + pp] = hfma2_rn(hsub2_rn(t, 0x64006400u), s2, b2);
+        }
+      } else {
+        out[i / 8][2 * (i % 8)] = hfma2_rn(hsub2_rn(prmt(wd[i], 0x64646464u, 0x5140u), 0x64006400u), s2, b2);
+        out[i / 8][2 * (i % 8) + 1] = hfma2_rn(hsub2_rn(prmt(wd[i], 0x64646464u, 0x5342u), 0x64006400u), s2, b2);
+      }
     }
   }
 }
@@ -452,7 +495,9 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
         uint32_t out[2][16];
         const float sf = __half2float(sc);
         const uint32_t b2 = h2_bits(__halves2half2(bi, bi));
-        if (BITS == 4) {
+        if (LORA) {
+          weights_once<BITS>(wd, sc, b2, out);
+        } else if (BITS == 4) {
           const bool fast = fabsf(sf) >= 0.0009765625f && fabsf(sf) < 63.0f;  // s/16 exact, 1024 s finite
           if (fast) {
             const __half s16 = __float2half_rn(sf * 0.0625f);  // exact: s >= 2^-10

@@ -10,7 +10,7 @@ import torch
 
 import qw_b200
 from qw_b200 import _lib
-from tests.adapter_ref import close, half_step, lora_delta, lora_grads
+from tests.adapter_ref import U, close, half_step, lora_delta, lora_grads
 from tests.conftest import TOL, rel_err
 
 pytestmark = pytest.mark.gpu
@@ -74,18 +74,34 @@ def test_with_projection(cuda_dev, M, N, K, R, L, bits, gs):
     assert rel_err(y.cpu().numpy(), want.numpy()) <= TOL
 
 
+@pytest.mark.parametrize("bits,gs", [(4, 64), (8, 128)])
 @pytest.mark.parametrize("M", [1, 5, 16, 20, 300])
-def test_rows_without_adapter_are_the_projection(cuda_dev, M):
+def test_rows_without_adapter_are_the_projection(cuda_dev, M, bits, gs):
+    """Bit for bit up to 16 rows.  Above, the weights are rounded to fp16 once (half a step each) and y once; the
+    K products are added in fp32."""
     N, K = 264, 512
     x, a, b, s, _ = adapters(M, N, K, 16, 4, seed=M)
     a[:], b[:] = float("nan"), float("inf")
-    w = real_weights(N, K)
+    w = real_weights(N, K, bits, gs)
+    w[1][0], w[2][0] = 1e-4, -5e-4  # rows of a scale near fp16's subnormals, and beyond either side of the tensor
+    w[1][1], w[2][1] = 3.0, -20.0    # cores' dequantization rule
+    w[1][2], w[2][2] = 0.01, 0.1
+    w[1][3], w[2][3] = -3e-8, 0.25
+    plain = qw_b200.quantized_matmul(x, *w, group_size=gs, bits=bits)
+    q = (w[0].cpu()[..., None] >> torch.arange(0, 32, bits, dtype=torch.int32)) & (2 ** bits - 1)
+    W = (q.view(N, -1, gs).double() * w[1].cpu().double()[..., None] + w[2].cpu().double()[..., None]).view(N, K)
+    want, mags = x.cpu().double() @ W.T, x.cpu().double().abs() @ W.abs().T
+    bound = (half_step(torch.float16) + (K + 4) * U) * mags + 2.0 ** -25 * x.cpu().double().abs().sum(1, keepdim=True)
+    bound = bound + half_step(torch.float16) * (want.abs() + bound) + 2.0 ** -25
     for none in (-1, 4, -2, 2 ** 31 - 1):
         idx = torch.full((M,), none, dtype=torch.int32, device="cuda")
-        y = qw_b200.quantized_linear_lora(x, *w, a, b, s, idx)
-        assert torch.equal(y, qw_b200.quantized_matmul(x, *w))
-    empty = qw_b200.quantized_linear_lora(x, *w, a[:0], b[:0], s[:0], None)
-    assert torch.equal(empty, qw_b200.quantized_matmul(x, *w))
+        y = qw_b200.quantized_linear_lora(x, *w, a, b, s, idx, group_size=gs, bits=bits)
+        if M <= 16:
+            assert torch.equal(y, plain)
+        else:
+            close(y, want, bound, "y")
+    empty = qw_b200.quantized_linear_lora(x, *w, a[:0], b[:0], s[:0], None, group_size=gs, bits=bits)
+    assert torch.equal(empty, y)
 
 
 @pytest.mark.parametrize("M", [2, 16, 40, 280])
