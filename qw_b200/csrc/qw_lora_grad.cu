@@ -333,17 +333,23 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   bool ok = true;        // a bounded wait that ran out: go on without waiting
   uint32_t it0 = 0, vit0 = 0;  // steps and chunks of earlier rounds
   constexpr uint32_t kDesc = mma_desc(kTileRows, RP, false, TRANS);
+  // Few adapters: two sums of every other chunk, as the tensor cores' additions
+  // truncate and an error grows with the number that follow one another.
+  constexpr int kHalf = Cfg::GROUP / 2;
+  bool two = false;
   auto multiply = [&](int chunk, int j, uint32_t vs, uint32_t ws) {
     const uint64_t a = operand_k(vs), b = TRANS ? operand_mn(ws, 8192) : operand_k(ws);
+    const int col = (j + (two && (chunk & 1) ? kHalf : 0)) * Cfg::PITCH_T;
 #pragma unroll
     for (int kk = 0; kk < kChunk / 16; ++kk)
-      tc_mma_ss(sh.tmem + j * Cfg::PITCH_T, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
-                chunk > 0 || kk > 0);
+      tc_mma_ss(sh.tmem + col, a + (uint64_t)(2 * kk), b + (uint64_t)((TRANS ? 128 : 2) * kk), kDesc,
+                chunk > (two ? 1 : 0) || kk > 0);
   };
 
   for (int j0 = 0; j0 < n; j0 += Cfg::GROUP) {
     const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
     const int steps = (c1 - c0) * ((nj + Cfg::PER - 1) / Cfg::PER);
+    two = nj <= kHalf && c1 - c0 > 1;
     if (warp == 1 && lane == 0) {  // loads
       uint32_t it = it0, vit = vit0;
       for (int c = c0; c < c1; ++c, ++vit) {
@@ -404,8 +410,16 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       for (int c = 0; c < RP; c += 16) {
         uint32_t v[16];
         if (steps > 0) {
-          tmem_ld_32x32b_x16(sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::PITCH_T + c, v);
+          const uint32_t at = sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::PITCH_T + c;
+          tmem_ld_32x32b_x16(at, v);
           tmem_wait_ld();
+          if (two) {
+            uint32_t w[16];
+            tmem_ld_32x32b_x16(at + kHalf * Cfg::PITCH_T, w);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(w[i]));
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = 0u;  // this CTA has no part of the reduction
