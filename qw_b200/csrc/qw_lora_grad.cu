@@ -745,6 +745,9 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers;
 //   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
+// Odd steps of a long chunk have a D of their own: the tensor cores' additions
+// truncate, and an error grows with the number that follow one another (4096 rows:
+// dA to 1.3e-6 of its size, 2.3e-6 in one sum, 131 us a call in one and 133 in two).
 // HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
 // rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
 // one D (64 of each) and are added when it is read.  dx, an fp16 result, takes the
@@ -753,6 +756,7 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
 constexpr int kCols = 128;
+constexpr int kOneSum = 4;  // steps
 constexpr int kWorkers = 256;
 constexpr int kWarpCols = kCols / (kWorkers / 128);  // columns of D or dx a worker warp reads, of 32 rows
 constexpr int kVStages = 3;                          // and two warps for each that load
@@ -881,7 +885,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  constexpr uint32_t kDx = 128;  // TMEM columns of the two dx buffers
+  constexpr uint32_t kDx = 128, kOdd = 384;  // TMEM columns of the two dx buffers, and of D's odd steps
   pdl_wait();
   const int64_t items = (int64_t)q.plan.total[0] * q.tiles;
   bool ok = true;  // a bounded wait that ran out: go on without waiting
@@ -1005,6 +1009,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           if (t.dx && step > 0) dx();  // before the sums: the workers wait for it
           if (t.sum) {
             const int blocks = (t.ck.count - step * kStepRows + 15) / 16;
+            const bool two = t.steps > kOneSum;
             const uint64_t b = operand_mn(vs, Cfg::BLOCK);
 #pragma unroll
             for (int half = 0; half < (Cfg::STACK ? 1 : 2); ++half) {
@@ -1013,8 +1018,8 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < kStepRows / 16; ++kk)
                 if (kk < blocks)
-                  tc_mma_ss(tmem, a + (uint64_t)(128 * kk), b + (uint64_t)(128 * kk), kSumDesc,
-                            step > 0 || half > 0 || kk > 0);
+                  tc_mma_ss(tmem + (two && (step & 1) ? kOdd : 0u), a + (uint64_t)(128 * kk),
+                            b + (uint64_t)(128 * kk), kSumDesc, step > (two ? 1 : 0) || half > 0 || kk > 0);
             }
           }
           if (t.dx && step == 0) {  // lora_a comes when the item before is done
@@ -1132,6 +1137,17 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x16(tmem + lanes + upper * kWarpCols + c * 16, d[c]);
         tmem_wait_ld();
+        if (t.steps > kOneSum) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+            tmem_ld_32x32b_x16(tmem + lanes + kOdd + upper * kWarpCols + c * 16, w);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              d[c][x] = __float_as_uint(__uint_as_float(d[c][x]) + __uint_as_float(w[x]));
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.accempty);
