@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 //   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
 // Odd steps of a long chunk have a D of their own: the tensor cores' additions
 // truncate, and an error grows with the number that follow one another (4096 rows:
-// dA to 1.3e-6 of its size, 2.3e-6 in one sum, 131 us a call in one and 133 in two).
+// dA to 1.3e-6 of its size, 2.3e-6 in one sum; the time is the same).
 // HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
 // rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
 // one D (64 of each) and are added when it is read.  dx, an fp16 result, takes the
