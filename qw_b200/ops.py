@@ -326,11 +326,11 @@ def topk_distillation(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_v
     """(loss fp32 [...], dlogits like logits or None): T^2 KL(teacher || student)
     of each row, the teacher a softmax over its stored top logits (``topk``,
     ``quantized_matmul_topk``), times ``row_weights``, with its gradient.
-    ``teacher_idx`` int32 or int64 (int64 costs a cast), -1 for no entry;
+    ``teacher_idx`` int32 or int64 (int64 costs a copy), -1 for no entry;
     ``temperature`` an fp32 tensor of one element on the device (None: 1).
     ``dlogits`` (optional) receives the gradient and may be ``logits``."""
     if teacher_idx.dtype == torch.int64:
-        teacher_idx = teacher_idx.to(torch.int32)
+        teacher_idx = teacher_idx.clamp(-1, 2 ** 31 - 1).to(torch.int32)  # an id past int32 is no entry, not another
     if dlogits is None and grad:
         dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
     loss = logits.new_empty(logits.shape[:-1] or (1,), dtype=torch.float32)

@@ -145,3 +145,13 @@ def test_no_rows(cuda_dev):
     z, idx, t, w = batch(0, 100, 4, torch.float16)
     loss, dz = qw_b200.topk_distillation(z, idx, t, row_weights=w)
     assert loss.shape == (0,) and dz.shape == (0, 100)
+
+
+def test_int64_ids_past_int32_are_no_entries(cuda_dev):
+    z, idx, t, w = batch(3, 500, 6, torch.float16, seed=1)
+    far = idx.to(torch.int64)
+    idx[0, 2], idx[1, 0], idx[2, 5] = -1, -1, -1
+    far[0, 2], far[1, 0], far[2, 5] = 2 ** 32 + 7, -2 ** 32 + 7, 2 ** 40
+    want = qw_b200.topk_distillation(z, idx, t, row_weights=w)
+    got = qw_b200.topk_distillation(z, far, t, row_weights=w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
