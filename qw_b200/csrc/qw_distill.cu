@@ -254,6 +254,9 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
   uint32_t rank, C;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
+  // A CTA's shared memory may be written by its cluster only once it runs: met
+  // before the rows, so that rows without shares need no barrier either.
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int V = (int)p.V, M = (int)p.M;
   const T* const z0 = reinterpret_cast<const T*>(p.logits);
@@ -284,6 +287,8 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     for (int e = 0; e < n; e += TH) copy_async16(mine + e * 16, z + lay.first + e * VT::N);
     if (lay.edge >= 0) ze = to_f32(z[lay.edge]);
   }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // behind the first row's copies
   const float temp = p.temperature ? *p.temperature : 1.f;
   const float inv = 1.f / temp;
   const float c = inv * kLog2e;
