@@ -34,6 +34,11 @@ _DESC_CACHE: dict = {}
 _DESC_CACHE_MAX = 8192
 
 
+# Zero strides mean row-contiguous to the library, so a value expanded over a
+# shape cannot be told from an array of that shape.
+_ONE_VALUE = "an operand must be row-contiguous, not one value expanded over its shape"
+
+
 def _arr(t: Optional[torch.Tensor]):
     """torch tensor -> pointer to a qw_array (None -> NULL)."""
     if t is None:
@@ -46,6 +51,8 @@ def _arr(t: Optional[torch.Tensor]):
         raise TypeError(f"unsupported dtype {t.dtype}")
     if t.dim() < 1 or t.dim() > 4:
         raise ValueError("qw arrays have 1 to 4 dimensions")
+    if not t.is_contiguous() and not any(t.stride()):
+        raise ValueError(_ONE_VALUE)
     a = _lib.QwArray()
     a.data = t.data_ptr() if t.numel() else 0
     a.dtype = _DT[t.dtype]
@@ -88,7 +95,10 @@ def _desc(t: Optional[torch.Tensor]) -> Optional[bytes]:
     pad = _PAD[n]
     if t.is_contiguous():
         return _PACK(t.data_ptr(), dt, n, *shape, *pad, 0, 0, 0, 0)
-    return _PACK(t.data_ptr(), dt, n, *shape, *pad, *t.stride(), *pad)
+    stride = t.stride()
+    if not any(stride):
+        raise ValueError(_ONE_VALUE)
+    return _PACK(t.data_ptr(), dt, n, *shape, *pad, *stride, *pad)
 
 
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: Optional[torch.Tensor],
