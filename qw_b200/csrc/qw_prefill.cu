@@ -73,11 +73,15 @@ struct PfCfg {
   // barriers: xfull, wpfull, wpempty, afull, aempty (per stage), dfull, dempty
   static constexpr int NBAR = 5 * STAGES + 2;
   static constexpr int OFF_BAR = OFF_WP + STAGES * WP_STAGE;
-  // LORA: per tile parity, whether a weight row has non-finite lora_b values
+  // LORA: whether a weight row has non-finite lora_b values, a slot for each of the
+  // last STAGES tiles.  The slot of a tile STAGES further on is written with its last
+  // block, when the block STAGES before that one has been multiplied.  The tiles from
+  // the next on have at least STAGES + 1 blocks together (one each, two where adapters
+  // are), so that block belongs to them, and their products wait for this tile's epilogue.
   static constexpr int OFF_BAD = OFF_BAR + NBAR * 8 + 64;
-  static constexpr int OFF_XGO = OFF_BAD + 2 * BM;  // LORA: barriers, the producer has freed the stage for an adapters' block
+  static constexpr int OFF_XGO = OFF_BAD + STAGES * BM;  // LORA: barriers, the producer has freed the stage for an adapters' block
   static constexpr int SMEM = OFF_BAD + 1024;
-  static constexpr int SMEM_LORA = SMEM + 2 * BM + 8 * STAGES;
+  static constexpr int SMEM_LORA = SMEM + STAGES * BM + 8 * STAGES;
   // TMEM: D (BT fp32 columns) at 0, then the A stages (32 columns each)
   static constexpr uint32_t D_COL = 0;
   static constexpr uint32_t A_COL = BT >= 128 ? BT : 128;
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   const int total_tiles = p.n_tiles * p.m_tiles;
-  uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [parity][BM]
+  uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [tile % STAGES][BM]
   uint64_t* const xgo = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_XGO);  // LORA
   // k blocks of a token tile: the weights' groups, then its adapters'
   auto blocks_of = [&](int mt) {
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
           out[c / 4][4 * (c % 4) + 2] = finite_pair(v[c].z, &bad);
           out[c / 4][4 * (c % 4) + 3] = finite_pair(v[c].w, &bad);
         }
-        if (g + 1 == blocks) bad_rows[(tile_count & 1) * BM + lane_row] = bad;
+        if (g + 1 == blocks) bad_rows[tile_count % STAGES * BM + lane_row] = bad;
         tc_fence_after();
         tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
         tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
       bool bad = false;  // non-finite lora_b values in this row
       if (LORA) {
         if (p.lora.bias && row_ok) bias = __half2float(reinterpret_cast<const __half*>(p.lora.bias)[row]);
-        bad = blocks > p.groups && bad_rows[(tile_count & 1) * BM + quarter * 32 + lane];
+        bad = blocks > p.groups && bad_rows[tile_count % STAGES * BM + quarter * 32 + lane];
       }
       auto store_tile = [&](auto with_bad) {
 #pragma unroll 1
