@@ -517,6 +517,9 @@ class QuantizedMlp:
     @classmethod
     def from_fused(cls, gate_up: QuantizedLinear, intermediate_size: int, down: QuantizedLinear):
         """Gate and up stored as one [2I, ...] projection (rows 0..I-1 gate)."""
+        if gate_up.lora is not None:
+            raise ValueError("attach adapters to the gate and up projections, not to the matrix that holds both")
+
         def half(t, i):
             return None if t is None else t[i * intermediate_size:(i + 1) * intermediate_size]
         g = QuantizedLinear(half(gate_up.weight, 0), half(gate_up.scales, 0), half(gate_up.biases, 0),

@@ -16,3 +16,19 @@ def test_one_value_over_a_shape_is_no_array(pack, shape):
     pack(torch.ones(shape))
     pack(torch.ones(4).expand(3, 4))  # strides (0, 1): refused by the library itself
     pack(torch.ones(0).expand(2, 0))
+
+
+def linear(n, k=64, lora=None):
+    return ops.QuantizedLinear(torch.zeros(n, k // 8, dtype=torch.int32), torch.zeros(n, 1, dtype=torch.float16),
+                               torch.zeros(n, 1, dtype=torch.float16), lora=lora)
+
+
+def stack(n, k=64, adapters=2, rank=4):
+    return ops.LoraAdapters(torch.zeros(adapters, rank, k).half(), torch.zeros(adapters, n, rank).half())
+
+
+def test_a_fused_gate_and_up_with_adapters_is_not_split():
+    """Its halves would have lost them."""
+    with pytest.raises(ValueError, match="adapters"):
+        ops.QuantizedMlp.from_fused(linear(32, lora=stack(32)), 16, linear(64, 16 * 4))
+    assert ops.QuantizedMlp.from_fused(linear(32), 16, linear(64)).fused
