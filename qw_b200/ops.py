@@ -530,7 +530,7 @@ class QuantizedMlp:
 
     def forward_hidden(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
         g, u = self.gate, self.up
-        if self.fused:
+        if self.fused and g.lora is None and u.lora is None:  # adapters may have come since
             return quantized_matmul_swiglu(x, g.weight, g.scales, g.biases, u.weight, u.scales, u.biases,
                                            g.group_size, g.bits, g.mode, out=out)
         return compiled_swiglu_activation(g(x, adapter_idx=adapter_idx), u(x, adapter_idx=adapter_idx), out=out)

@@ -32,3 +32,37 @@ def test_a_fused_gate_and_up_with_adapters_is_not_split():
     with pytest.raises(ValueError, match="adapters"):
         ops.QuantizedMlp.from_fused(linear(32, lora=stack(32)), 16, linear(64, 16 * 4))
     assert ops.QuantizedMlp.from_fused(linear(32), 16, linear(64)).fused
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Calls of the operators below the layer types, as (name, keyword arguments); each returns zeros."""
+    log = []
+
+    def fake(name, width):
+        def f(x, *args, **kw):
+            log.append((name, args, kw))
+            return torch.zeros(*x.shape[:-1], width or args[0].shape[0])
+        monkeypatch.setattr(ops, name, f)
+    for name in ("quantized_matmul_swiglu", "quantized_linear_lora", "quantized_linear_forward"):
+        fake(name, None)
+    fake("compiled_swiglu_activation", 16)
+    return log
+
+
+@pytest.mark.parametrize("which", ["gate", "up"])
+def test_adapters_attached_to_an_mlp_in_use(calls, which):
+    mlp = ops.QuantizedMlp(linear(16), linear(16), linear(64, 64))
+    x, idx = torch.zeros(3, 64), torch.zeros(3, dtype=torch.int32)
+    mlp.forward_hidden(x)
+    assert [c[0] for c in calls] == ["quantized_matmul_swiglu"]
+    calls.clear()
+    setattr(getattr(mlp, which), "lora", stack(16))
+    mlp.forward_hidden(x, adapter_idx=idx)
+    names = [c[0] for c in calls]
+    assert sorted(names) == ["compiled_swiglu_activation", "quantized_linear_forward", "quantized_linear_lora"]
+    assert calls[names.index("quantized_linear_lora")][1][6] is idx
+    calls.clear()
+    getattr(mlp, which).lora = None
+    mlp.forward_hidden(x)
+    assert [c[0] for c in calls] == ["quantized_matmul_swiglu"]
