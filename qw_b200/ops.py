@@ -439,6 +439,8 @@ class QuantizedLinear:
 
     def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
         if self.lora is not None:
+            if self.global_scale is not None:
+                raise ValueError("a projection with a global scale takes no adapters")
             return quantized_linear_lora(x, self.weight, self.scales, self.biases, self.lora.a, self.lora.b,
                                          self.lora.scales, adapter_idx, self.bias, self.group_size, self.bits,
                                          self.mode, out=out)

@@ -66,3 +66,12 @@ def test_adapters_attached_to_an_mlp_in_use(calls, which):
     getattr(mlp, which).lora = None
     mlp.forward_hidden(x)
     assert [c[0] for c in calls] == ["quantized_matmul_swiglu"]
+
+
+def test_adapters_attached_beside_a_global_scale_are_refused(calls):
+    """The adapters' kernel would leave the scale out."""
+    lin = linear(16, lora=stack(16))
+    lin.global_scale = torch.ones(1)
+    with pytest.raises(ValueError, match="global scale"):
+        lin(torch.zeros(3, 64))
+    assert not calls
