@@ -418,6 +418,8 @@ class QuantizedLinear:
     ``UnifiedLinear::forward`` (layers.rs:2023-2093).  With ``lora`` (adapters
     of many requests, LoraAdapters) forward adds each row's adapter."""
 
+    lora: Optional[LoraAdapters] = None  # of objects stored before there were adapters too
+
     def __init__(self, w, scales, biases, group_size: int = 64, bits: int = 4, mode: str = "affine",
                  bias: Optional[torch.Tensor] = None, global_scale: Optional[torch.Tensor] = None,
                  lora: Optional[LoraAdapters] = None):
@@ -454,6 +456,16 @@ class QuantizedLinear:
     __call__ = forward
 
 
+def _adapters_of(linear) -> Optional[LoraAdapters]:
+    """Adapters of a projection; a caller's own projection type need not know any."""
+    return getattr(linear, "lora", None)
+
+
+def _adapter_kw(adapter_idx) -> dict:
+    """Rows' adapters as a keyword for a projection, which gets none unless the caller names some."""
+    return {} if adapter_idx is None else {"adapter_idx": adapter_idx}
+
+
 class QuantizedFusedLinear:
     """Projections of one input fused into one quantized matmul: the planes'
     weights, scales and biases concatenated along the output rows, the output
@@ -480,7 +492,7 @@ class QuantizedFusedLinear:
                 raise ValueError("fused planes must share input width and quantization")
             if l.bias is not None or l.global_scale is not None:
                 raise ValueError("fused planes take no linear bias or global scale")
-            if l.lora is not None:
+            if _adapters_of(l) is not None:
                 raise ValueError("attach adapters to the fused projection, not to its planes")
         cat = lambda ts: torch.cat(ts, 0).contiguous()  # noqa: E731
         fused = QuantizedLinear(cat([l.weight for l in linears]), cat([l.scales for l in linears]),
@@ -489,7 +501,7 @@ class QuantizedFusedLinear:
         return cls(fused, [l.out_features for l in linears])
 
     def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None):
-        y = self.linear(x, out=out, adapter_idx=adapter_idx)
+        y = self.linear(x, out=out, **_adapter_kw(adapter_idx))
         views, c = [], 0
         for n in self.sizes:
             views.append(y[..., c:c + n])
@@ -513,13 +525,13 @@ class QuantizedMlp:
         self.fused = (gate.group_size == up.group_size and gate.bits == up.bits and gate.mode == up.mode
                       and gate.bias is None and up.bias is None
                       and gate.global_scale is None and up.global_scale is None
-                      and gate.lora is None and up.lora is None
+                      and _adapters_of(gate) is None and _adapters_of(up) is None
                       and gate.out_features == up.out_features)
 
     @classmethod
     def from_fused(cls, gate_up: QuantizedLinear, intermediate_size: int, down: QuantizedLinear):
         """Gate and up stored as one [2I, ...] projection (rows 0..I-1 gate)."""
-        if gate_up.lora is not None:
+        if _adapters_of(gate_up) is not None:
             raise ValueError("attach adapters to the gate and up projections, not to the matrix that holds both")
 
         def half(t, i):
@@ -532,12 +544,14 @@ class QuantizedMlp:
 
     def forward_hidden(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
         g, u = self.gate, self.up
-        if self.fused and g.lora is None and u.lora is None:  # adapters may have come since
+        if self.fused and _adapters_of(g) is None and _adapters_of(u) is None:  # some may have come since
             return quantized_matmul_swiglu(x, g.weight, g.scales, g.biases, u.weight, u.scales, u.biases,
                                            g.group_size, g.bits, g.mode, out=out)
-        return compiled_swiglu_activation(g(x, adapter_idx=adapter_idx), u(x, adapter_idx=adapter_idx), out=out)
+        kw = _adapter_kw(adapter_idx)
+        return compiled_swiglu_activation(g(x, **kw), u(x, **kw), out=out)
 
     def forward(self, x: torch.Tensor, out=None, adapter_idx: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return self.down(self.forward_hidden(x, adapter_idx=adapter_idx), out=out, adapter_idx=adapter_idx)
+        kw = _adapter_kw(adapter_idx)
+        return self.down(self.forward_hidden(x, **kw), out=out, **kw)
 
     __call__ = forward

@@ -75,3 +75,32 @@ def test_adapters_attached_beside_a_global_scale_are_refused(calls):
     with pytest.raises(ValueError, match="global scale"):
         lin(torch.zeros(3, 64))
     assert not calls
+
+
+class OwnLinear:
+    """A caller's projection, as the layer types took it before there were adapters."""
+    weight, scales, biases = torch.zeros(16, 8, dtype=torch.int32), torch.zeros(16, 1).half(), torch.zeros(16, 1).half()
+    group_size, bits, mode, bias, global_scale, in_features, out_features = 64, 4, "affine", None, None, 64, 16
+
+    def __call__(self, x, out=None):
+        return torch.full((*x.shape[:-1], 16), 2.0)
+
+
+def test_projections_that_know_no_adapters(calls):
+    x = torch.zeros(3, 64)
+    mlp = ops.QuantizedMlp(OwnLinear(), OwnLinear(), lambda h, out=None: h + 1)
+    assert mlp.fused and torch.equal(mlp(x), torch.ones(3, 16))
+    other = OwnLinear()
+    other.bias = torch.zeros(16)
+    assert torch.equal(ops.QuantizedMlp(OwnLinear(), other, lambda h, out=None: h + 1)(x), torch.ones(3, 16))
+    a, b = ops.QuantizedFusedLinear(OwnLinear(), [10, 6])(x)
+    assert a.shape == (3, 10) and b.shape == (3, 6)
+    assert ops.QuantizedFusedLinear.from_linears([OwnLinear(), OwnLinear()]).linear.out_features == 32
+    assert ops.QuantizedMlp.from_fused(OwnLinear(), 8, lambda h, out=None: h).fused
+
+
+def test_a_projection_stored_before_there_were_adapters(calls):
+    lin = linear(16)
+    del lin.__dict__["lora"]
+    lin(torch.zeros(3, 64))
+    assert [c[0] for c in calls] == ["quantized_linear_forward"]
