@@ -251,7 +251,8 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     // Many rows of a high rank are worth the tcgen05 products' tiles of 128 rows
     // (rank 64, 8 adapters, 5120 -> 5120, the whole call: 1024 rows in 116 us with
     // them, 121 without; 512 rows 77 and 75; rank 32, 2048 rows to 17408: 395 and 388).
-    if (p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
+    // (An empty stack has no tensor maps.)
+    if (p.L > 0 && p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);

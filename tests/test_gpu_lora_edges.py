@@ -6,7 +6,7 @@ import torch
 
 import qw_b200
 from tests.adapter_ref import close
-from tests.test_gpu_lora import adapters, delta_of, zero_weights
+from tests.test_gpu_lora import adapters, delta_of, real_weights, zero_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,15 @@ def test_non_finite_b_of_an_adapter_in_use(cuda_dev, M, R, bits, gs):
     y = qw_b200.quantized_linear_lora(x, *zero_weights(N, K, bits, gs), a, b, s, idx, group_size=gs, bits=bits)
     close(y, want, bound, "y")
     assert not torch.isfinite(y[0, 0]) and torch.isfinite(y[5]).all()
+
+
+@pytest.mark.parametrize("M,R", [(600, 64), (513, 33), (1025, 128)])
+def test_an_empty_stack_of_a_high_rank(cuda_dev, M, R):
+    N, K = 136, 256
+    x, a, b, s, _ = adapters(M, N, K, R, 1, seed=R)
+    w = real_weights(N, K)
+    empty = qw_b200.quantized_linear_lora(x, *w, a[:0], b[:0], s[:0], None)
+    none = torch.full((M,), -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(empty, qw_b200.quantized_linear_lora(x, *w, a, b, s, none))
+    dx, da, db = qw_b200.lora_backward(x, empty, a[:0], b[:0], s[:0], None)
+    assert not dx.any() and da.shape == (0, R, K) and db.shape == (0, N, R)
