@@ -318,11 +318,11 @@ int qw_quantized_linear_lora_workspace(int64_t m, int64_t n, int64_t rank, int64
  * adapter are left as they are.  x f16 [..., K] (rows may be strided as in
  * qw_quantized_matmul), K a multiple of 64; dy f16 [..., N] row-contiguous; dx
  * must not overlap x or dy; x, dx, da, db and, where N is a multiple of 8, dy
- * are 16-byte aligned.  Products are accumulated in fp32; h and g enter
- * the sums over rows with 22 significant bits relative to their largest
- * magnitude in the adapter, g enters dx rounded to fp16 at that scale.  Results do not depend on scheduling: the same
- * inputs give the same bits.  Non-finite values in dy or x of an adapter's
- * rows make that adapter's gradients non-finite. */
+ * are 16-byte aligned.  Products are accumulated in fp32; h and g enter the
+ * sums and dx with 22 significant bits relative to their largest magnitude in
+ * the adapter.  Results do not depend on scheduling: the same inputs give the
+ * same bits.  Non-finite values in dy or x of an adapter's rows make that
+ * adapter's gradients non-finite. */
 int qw_lora_backward(const qw_array* x, const qw_array* dy, const qw_array* lora_a, const qw_array* lora_b,
                      const qw_array* lora_scales, const qw_array* adapter_idx, int accumulate_dx, qw_array* dx,
                      qw_array* da, qw_array* db, void* workspace, int64_t workspace_bytes, void* stream);

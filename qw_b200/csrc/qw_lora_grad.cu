@@ -750,8 +750,7 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // dA to 1.3e-6 of its size, 2.3e-6 in one sum; the time is the same).
 // HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
 // rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
-// one D (64 of each) and are added when it is read.  dx, an fp16 result, takes the
-// nearest fp16 of g alone: its error stays below the result's own rounding.
+// one D (64 of each) and are added when it is read; dx takes both into one sum.
 //
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
@@ -999,10 +998,13 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           auto dx = [&]() {
             const uint64_t b = operand_mn(base + Cfg::OFF_A, RP * 128);
 #pragma unroll
-            for (int kk = 0; kk < RP / 16; ++kk) {
-              const uint64_t a = operand_k(gs + kk / 4 * Cfg::BLOCK) + (uint64_t)(2 * (kk % 4));
-              tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, kk > 0);
-            }
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int kk = 0; kk < RP / 16; ++kk) {
+                const uint64_t a =
+                    operand_k(gs + half * Cfg::G_HALF + kk / 4 * Cfg::BLOCK) + (uint64_t)(2 * (kk % 4));
+                tc_mma_ss(tmem + kDx + (dxs & 1) * kCols, a, b + (uint64_t)(128 * kk), kDxDesc, half > 0 || kk > 0);
+              }
             tc_commit(&sh.dxfull[dxs & 1]);
             ++dxs;
           };
