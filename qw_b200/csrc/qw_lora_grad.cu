@@ -409,6 +409,7 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
 #pragma unroll
       for (int c = 0; c < RP; c += 16) {
         uint32_t v[16];
+        __syncwarp();  // tcgen05.ld takes a whole warp, stores below are some lanes'
         if (steps > 0) {
           const uint32_t at = sh.tmem + ((uint32_t)(warp * 32) << 16) + b * Cfg::PITCH_T + c;
           tmem_ld_32x32b_x16(at, v);
@@ -1066,6 +1067,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         const int mine = next_row;
         if (step + 1 < t.steps) fetch_row(step + 1);
         ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
+        __syncwarp();  // lanes without a row came early
         tc_fence_after();
         uint32_t d[kWarpCols / 16][16];
 #pragma unroll
@@ -1135,6 +1137,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       if (t.steps > 0) {
         ok = ok && mbar_wait(&sh.accfull, sums & 1, q.status, kDevTimeoutAccum);
         ++sums;
+        __syncwarp();
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x16(tmem + lanes + upper * kWarpCols + c * 16, d[c]);

@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
           out[c / 4][4 * (c % 4) + 3] = finite_pair(v[c].w, &bad);
         }
         if (g + 1 == blocks) bad_rows[tile_count % STAGES * BM + lane_row] = bad;
+        __syncwarp();
         tc_fence_after();
         tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
         tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
@@ -554,6 +555,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
         // write A stage s once the MMAs that read it last have completed
         if (it >= STAGES && !*abort_flag && !mbar_wait(&aempty[s], ph ^ 1, p.status, kDevTimeoutEmpty))
           *abort_flag = 1;
+        __syncwarp();  // scales of two kinds took two ways
         tc_fence_after();
         tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
         tmem_st_x16(tmem + lane_base + A_COL + s * 32 + 16, out[1]);
@@ -576,6 +578,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
 #pragma unroll 1
         for (int cb = khalf * (BT / 32); cb < (khalf + 1) * (BT / 32); ++cb) {
           uint32_t v[16];
+          __syncwarp();  // lanes past the last row came early
           tmem_ld_32x32b_x16(tmem + lane_base + D_COL + cb * 16, v);
           tmem_wait_ld();
           if (p.swiglu) {
