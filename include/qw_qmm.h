@@ -293,8 +293,8 @@ int qw_quantized_linear_forward_global_scale(const qw_array* x, const qw_array* 
  * and scale of each row's adapter: y f16 [..., N], the sum of the three terms
  * in fp32 rounded once.  x, w, scales, biases, linear_bias (nullable) as in
  * qw_quantized_linear_forward; y must not overlap x.  With more than 16 rows
- * the rank-space product scale * x A^T feeds the tensor cores as fp16 (so it
- * must stay below 65504), and so do the weights, fp16(s q + b) rounded once;
+ * the rank-space product scale * x A^T feeds the tensor cores as fp16 (values
+ * beyond fp16 are added in fp32), and so do the weights, fp16(s q + b) rounded once;
  * with up to 16 both stay fp32, and rows without an adapter have the bits of
  * qw_quantized_linear_forward.
  * No counterpart in the reference, whose linears carry no adapters. */

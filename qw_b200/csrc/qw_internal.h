@@ -120,6 +120,7 @@ int check_qmm_call(const qw_array* x, const qw_array* w, const qw_array* scales,
 // token tile, the adapters its tokens name.
 struct PrefillLora {
   const void* h;             // fp16 [M][R8], R8 the rank rounded up to 8, zero-padded
+  const float* full;         // [M][R8] fp32 values of h where that is not finite
   const void* b;             // fp16 [L][N][R]
   const uint32_t* idx;       // [M] or null (adapter 0)
   const uint32_t* tile_n;    // [token tiles]
@@ -239,9 +240,9 @@ PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, c
 size_t lora_backward_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t L, int sm_count);
 cudaError_t launch_lora_backward(const LoraArgs& p, const LoraGrads& g, void* ws, int sm_count, bool pdl,
                                  cudaStream_t stream, std::string* err);
-// h = s x A^T in fp16 [M][R8] and the token tiles' lists, for a long forward.
-cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, unsigned int* status,
-                                 int sm_count, bool pdl, cudaStream_t stream, std::string* err);
+// h = s x A^T in fp16 [M][R8], its fp32 values where that is not finite, and the token tiles' lists, for a long forward.
+cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, float* full,
+                                 unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err);
 
 // Distillation from a teacher's top logits (qw_distill.cu).
 struct DistillArgs {

@@ -40,7 +40,8 @@ namespace {
 struct RankRows {
   LoraArgs p;
   float* h32;         // [M][R] fp32 (at most 16 rows), or
-  __half* h16;        // [M][R8] fp16, zero-padded rank
+  __half* h16;        // [M][R8] fp16, zero-padded rank, and
+  float* full;        // [M][R8] fp32, where that is not finite
   int R8;
   int tiles, groups;  // row tiles, adapter groups per tile
   TokenLists lists;
@@ -156,8 +157,13 @@ __global__ void __launch_bounds__(WARPS * 32, RT <= 2 ? 5 : (RT <= 4 ? 4 : 2)) r
       if (q.h32) {
         if (c < p.R) q.h32[(m0 + row) * p.R + c] = v;
       } else if (c < q.R8) {
-        // one rounding to fp16: the tensor cores take y's second product in fp16
-        q.h16[(m0 + row) * q.R8 + c] = __float2half_rn(v);
+        // One rounding to fp16, relative to the adapter's term what y's own rounding is to
+        // y: the tensor cores take the second product in fp16, and a second term of h
+        // would double the adapters' k blocks.  Values beyond fp16 are kept in fp32.
+        const int64_t at = (m0 + row) * q.R8 + c;
+        const __half h = c < p.R ? __float2half_rn(v) : __half(0);
+        q.h16[at] = h;
+        if (!isfinite(__half2float(h))) q.full[at] = v;
       }
     }
     if (C > 1) cluster_sync();  // the peers' sums are read before they change or go
@@ -167,21 +173,22 @@ __global__ void __launch_bounds__(WARPS * 32, RT <= 2 ? 5 : (RT <= 4 ? 4 : 2)) r
 constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int round8(int r) { return (r + 7) / 8 * 8; }
 
-// Forward workspace: at most 16 rows, h fp32; above, h fp16 (zero-padded rank)
-// and the token tiles' lists.
+// Forward workspace: at most 16 rows, h fp32; above, h fp16 (zero-padded rank),
+// the token tiles' lists, and h fp32.
 struct ForwardSpace {
-  size_t second, third, fourth, end;
+  size_t second, third, fourth, full, end;
 };
 ForwardSpace forward_space(int64_t M, int R, int token_tile) {
   ForwardSpace f;
   if (token_tile == 0) {
-    f.second = f.third = f.fourth = f.end = align256((size_t)M * R * sizeof(float));
+    f.second = f.third = f.fourth = f.full = f.end = align256((size_t)M * R * sizeof(float));
   } else {
     const size_t tiles = (size_t)((M + token_tile - 1) / token_tile);
     f.second = align256((size_t)M * round8(R) * sizeof(__half));
     f.third = f.second + align256(tiles * sizeof(uint32_t));
     f.fourth = f.third + align256(tiles * token_tile * sizeof(uint32_t));
-    f.end = f.fourth + align256((size_t)M * sizeof(uint32_t));
+    f.full = f.fourth + align256((size_t)M * sizeof(uint32_t));
+    f.end = f.full + align256((size_t)M * round8(R) * sizeof(float));
   }
   return f;
 }
@@ -243,6 +250,7 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     q.prefetch = 1;
   } else {
     q.h16 = reinterpret_cast<__half*>(base);
+    q.full = reinterpret_cast<float*>(base + f.full);
     q.lists.tile = token_tile;
     q.lists.tiles = (int)((p.M + token_tile - 1) / token_tile);
     q.lists.n = reinterpret_cast<uint32_t*>(base + f.second);
@@ -252,7 +260,7 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     // (rank 64, 8 adapters, 5120 -> 5120, the whole call: 1024 rows in 116 us with
     // them, 121 without; 512 rows 77 and 75; rank 32, 2048 rows to 17408: 395 and 388).
     // (An empty stack has no tensor maps.)
-    if (p.L > 0 && p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, status, sm_count, pdl, stream, err);
+    if (p.L > 0 && p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, q.full, status, sm_count, pdl, stream, err);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);
@@ -273,6 +281,7 @@ PrefillLora lora_prefill_operands(const LoraArgs& p, int token_tile, void* ws, c
   uint8_t* base = static_cast<uint8_t*>(ws);
   PrefillLora l{};
   l.h = base;
+  l.full = reinterpret_cast<const float*>(base + f.full);
   l.b = p.b;
   l.idx = p.idx;
   l.tile_n = reinterpret_cast<uint32_t*>(base + f.second);

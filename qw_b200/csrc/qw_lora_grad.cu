@@ -221,7 +221,8 @@ struct Product {
   int64_t ld, len;
   const __half* w;  // [L][R][len], or for the second product [L][len][R8]
   float* out32;     // [M][RP] fp32, RP the kernel's padded rank (null: out16)
-  __half* out16;    // [M][R8] fp16
+  __half* out16;    // [M][R8] fp16, zero-padded rank, and
+  float* full;      // [M][R8] fp32, where that is not finite
   uint32_t* top;    // [tiles][kMaxSplit][kTileRows] largest magnitude of out32 by adapter, as fp32 bits
 };
 struct Products {
@@ -469,10 +470,15 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
         }
         atomicMax(&sh.slot_max[slot], most);
       } else if (c < q.R8) {
-        // one rounding to fp16: the tensor cores take y's second product in fp16
-        const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+        // one rounding to fp16, as rank_rows has it
+        const int left = p.R - c;
+        const __half2 x = __floats2half2_rn(left > 0 ? v.x : 0.f, left > 1 ? v.y : 0.f);
+        const __half2 y = __floats2half2_rn(left > 2 ? v.z : 0.f, left > 3 ? v.w : 0.f);
         *reinterpret_cast<uint2*>(f.out16 + (m0 + row) * q.R8 + c) =
             make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+        const float2 bx = __half22float2(x), by = __half22float2(y);
+        if (!isfinite(bx.x) || !isfinite(bx.y) || !isfinite(by.x) || !isfinite(by.y))
+          *reinterpret_cast<float4*>(f.full + (m0 + row) * q.R8 + c) = v;
       }
     }
     fence_proxy_async_smem();   // TMA writes there next
@@ -1355,8 +1361,8 @@ cudaError_t launch_sums(const Split& sp, const Sums& q, const SumMaps& maps, int
 
 }  // namespace
 
-cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, unsigned int* status,
-                                 int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
+cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, void* h16, float* full,
+                                 unsigned int* status, int sm_count, bool pdl, cudaStream_t stream, std::string* err) {
   Products q{};
   q.p = p;
   q.R8 = (p.R + 7) / 8 * 8;
@@ -1365,6 +1371,7 @@ cudaError_t launch_lora_products(const LoraArgs& p, const TokenLists& lists, voi
   q.a.len = p.K;
   q.a.w = static_cast<const __half*>(p.a);
   q.a.out16 = static_cast<__half*>(h16);
+  q.a.full = full;
   q.lists = lists;
   q.status = status;
   return dispatch_products(q, sm_count, pdl, stream, err);

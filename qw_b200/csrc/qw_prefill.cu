@@ -31,8 +31,9 @@
 // the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8
 // adapters of rank 32: 379 us, where the projection alone takes 368 to 396 (power-
 // capped clocks); a pass of its own over y would read and write 214 MB.
-// A zero times another adapter's infinity would be NaN: non-finite lora_b values
-// enter as zero and are added, for the tokens that own them, in the epilogue.
+// A zero times another adapter's infinity would be NaN: lora_b and h values that
+// are not finite fp16 enter as zero, and their terms, with h in fp32, are added in
+// the epilogue for the tokens that own them (so h may pass 65504).
 // The weights are fp16(s q + b), rounded once: the result's error is half of that
 // with the two roundings below (2.8e-4 and 5.7e-4 of y in the mean, 2048 x 17408 x 5120).
 //
@@ -80,8 +81,9 @@ struct PfCfg {
   // are), so that block belongs to them, and their products wait for this tile's epilogue.
   static constexpr int OFF_BAD = OFF_BAR + NBAR * 8 + 64;
   static constexpr int OFF_XGO = OFF_BAD + STAGES * BM;  // LORA: barriers, the producer has freed the stage for an adapters' block
+  static constexpr int OFF_WIDE = OFF_XGO + 8 * STAGES;  // LORA: of the same tiles, whether a warp met such values in h
   static constexpr int SMEM = OFF_BAD + 1024;
-  static constexpr int SMEM_LORA = SMEM + STAGES * BM + 8 * STAGES;
+  static constexpr int SMEM_LORA = SMEM + STAGES * BM + 12 * STAGES;
   // TMEM: D (BT fp32 columns) at 0, then the A stages (32 columns each)
   static constexpr uint32_t D_COL = 0;
   static constexpr uint32_t A_COL = BT >= 128 ? BT : 128;
@@ -133,11 +135,22 @@ __device__ __forceinline__ uint4 lora_chunk(const __half* row, int r0, int R) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Two fp16 values with non-finite ones (exponent all ones) replaced by zero.
-__device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool* bad) {
-  const bool lo = (w & 0x7C00u) == 0x7C00u, hi = (w & 0x7C000000u) == 0x7C000000u;
-  *bad = *bad || lo || hi;
-  return (lo ? 0u : w & 0xFFFFu) | (hi ? 0u : w & 0xFFFF0000u);
+// Replaces non-finite fp16 values (exponent all ones) by zero; whether there were
+// any.  One more in the exponent's place carries into the sign's where it is all
+// ones, so that the usual case takes two operations a pair.
+__device__ __forceinline__ bool make_finite(uint4 (&v)[8]) {
+  uint32_t met = 0u;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    met |= ((v[c].x & 0x7C007C00u) + 0x04000400u) | ((v[c].y & 0x7C007C00u) + 0x04000400u) |
+           ((v[c].z & 0x7C007C00u) + 0x04000400u) | ((v[c].w & 0x7C007C00u) + 0x04000400u);
+  if ((met & 0x80008000u) == 0u) return false;
+  auto finite = [](uint32_t w) {
+    return ((w & 0x7C00u) == 0x7C00u ? 0u : w & 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0u : w & 0xFFFF0000u);
+  };
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = make_uint4(finite(v[c].x), finite(v[c].y), finite(v[c].z), finite(v[c].w));
+  return true;
 }
 __device__ __forceinline__ uint32_t lora_adapter_of(const PrefillLora& l, int tok, int M) {
   if (tok >= M) return 0xFFFFFFFFu;
@@ -222,6 +235,25 @@ __device__ __forceinline__ void weights_once(const uint32_t (&wd)[BITS * 2], __h
   }
 }
 
+// Terms of a token's own adapter in which lora_b or h is not finite fp16.  No part of
+// the epilogue's code: inlined, it made the usual case slower too (37 x 4099 x 2560
+// 33.4 us, not 31.6; 2048 x 17408 x 5120 390, not 377).
+__device__ __noinline__ float own_terms(const PrefillParams& p, int tok, int row) {
+  const PrefillLora& l = p.lora;
+  const uint32_t a = lora_adapter_of(l, tok, p.M);
+  if (a >= (uint32_t)l.L) return 0.f;
+  const __half* h = reinterpret_cast<const __half*>(l.h) + (size_t)tok * 8 * p.lora_r8;
+  const float* full = l.full + (size_t)tok * 8 * p.lora_r8;
+  const __half* b = reinterpret_cast<const __half*>(l.b) + ((size_t)a * p.N + row) * l.R;
+  float f = 0.f;
+  for (int r = 0; r < l.R; ++r) {
+    const float bv = __half2float(b[r]), hr = __half2float(h[r]);
+    if (!isfinite(hr)) f += __ldcg(full + r) * bv;
+    else if (!isfinite(bv)) f += hr * bv;
+  }
+  return f;
+}
+
 template <int BITS, int BT_, bool LORA>
 __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
     qmm_prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
@@ -249,6 +281,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
   const int lane = threadIdx.x % 32;
   const int total_tiles = p.n_tiles * p.m_tiles;
   uint8_t* const bad_rows = smem + Cfg::OFF_BAD;  // LORA: [tile % STAGES][BM]
+  uint32_t* const wide_tiles = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_WIDE);  // LORA: [tile % STAGES], a byte a warp
   uint64_t* const xgo = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_XGO);  // LORA
   // k blocks of a token tile: the weights' groups, then its adapters'
   auto blocks_of = [&](int mt) {
@@ -378,7 +411,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
       const uint32_t* list = p.lora.tile_ids + (size_t)mt * BT;
       const int row = nt * BM + lane_row;
       const bool row_ok = row < p.N;
-      bool bad = false;
+      bool bad = false, wide = false;
       for (int g = p.groups; g < blocks; ++g) {
         const int s = (int)((it0 + (uint32_t)g) % STAGES);
         // chunk c (8 wide) of the block is ranks 8 rc .. of entry j of the tile's list
@@ -416,20 +449,26 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
             if ((uint32_t)j == slot[i]) hv[c] = __ldcg(h + rc);
             if (++rc == r8) rc = 0, ++j;
           }
+          wide |= make_finite(hv);
           uint8_t* dst = smem + OFF_X + s * X_STAGE + t * 128;
 #pragma unroll
           for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(dst + ((c ^ (t & 7)) << 4)) = hv[c];
         }
         fence_proxy_async_smem();
+        bad |= make_finite(v);
         uint32_t out[2][16];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          out[c / 4][4 * (c % 4)] = finite_pair(v[c].x, &bad);
-          out[c / 4][4 * (c % 4) + 1] = finite_pair(v[c].y, &bad);
-          out[c / 4][4 * (c % 4) + 2] = finite_pair(v[c].z, &bad);
-          out[c / 4][4 * (c % 4) + 3] = finite_pair(v[c].w, &bad);
+          out[c / 4][4 * (c % 4)] = v[c].x;
+          out[c / 4][4 * (c % 4) + 1] = v[c].y;
+          out[c / 4][4 * (c % 4) + 2] = v[c].z;
+          out[c / 4][4 * (c % 4) + 3] = v[c].w;
         }
-        if (g + 1 == blocks) bad_rows[tile_count % STAGES * BM + lane_row] = bad;
+        if (g + 1 == blocks) {
+          bad_rows[tile_count % STAGES * BM + lane_row] = bad;
+          const bool met = __any_sync(0xffffffffu, wide);
+          if (lane == 0) reinterpret_cast<uint8_t*>(wide_tiles + tile_count % STAGES)[quarter] = met;
+        }
         __syncwarp();
         tc_fence_after();
         tmem_st_x16(tmem + lane_base + A_COL + s * 32, out[0]);
@@ -569,10 +608,11 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
       if (!*abort_flag && !mbar_wait(dfull, tile_count & 1, p.status, kDevTimeoutAccum)) *abort_flag = 1;
       tc_fence_after();
       float bias = 0.f;
-      bool bad = false;  // non-finite lora_b values in this row
+      bool bad = false, wide = false;  // non-finite lora_b values in this row, h values in this tile
       if (LORA) {
         if (p.lora.bias && row_ok) bias = __half2float(reinterpret_cast<const __half*>(p.lora.bias)[row]);
         bad = blocks > p.groups && bad_rows[tile_count % STAGES * BM + quarter * 32 + lane];
+        wide = blocks > p.groups && wide_tiles[tile_count % STAGES] != 0u;
       }
       auto store_tile = [&](auto with_bad) {
 #pragma unroll 1
@@ -614,15 +654,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
               float f = __uint_as_float(v[q]);
               if constexpr (LORA) {
                 f += bias;
-                if (decltype(with_bad)::value && bad) {  // the non-finite terms of this token's own adapter
-                  const uint32_t a = lora_adapter_of(p.lora, tok, p.M);
-                  const __half* h = reinterpret_cast<const __half*>(p.lora.h) + (size_t)tok * 8 * p.lora_r8;
-                  const __half* b = reinterpret_cast<const __half*>(p.lora.b) + ((size_t)a * p.N + row) * p.lora.R;
-                  for (int r = 0; a < (uint32_t)p.lora.L && r < p.lora.R; ++r) {
-                    const float bv = __half2float(b[r]);
-                    if (!isfinite(bv)) f += __half2float(h[r]) * bv;
-                  }
-                }
+                if (decltype(with_bad)::value && (bad || wide)) f += own_terms(p, tok, row);
                 reinterpret_cast<__half*>(p.y)[idx] = __float2half_rn(f);
                 continue;
               }
@@ -633,7 +665,7 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
         }
       };
       // a branch an element for the rare case would cost the whole epilogue (2048 x 17408 x 5120: 45 us of 499)
-      if (LORA && __any_sync(0xffffffffu, bad)) store_tile(std::true_type{});
+      if (LORA && __any_sync(0xffffffffu, bad || wide)) store_tile(std::true_type{});
       else store_tile(std::false_type{});
       tc_fence_before();
       __syncwarp();

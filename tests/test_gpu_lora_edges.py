@@ -63,3 +63,40 @@ def test_an_empty_stack_of_a_high_rank(cuda_dev, M, R):
     assert torch.equal(empty, qw_b200.quantized_linear_lora(x, *w, a, b, s, none))
     dx, da, db = qw_b200.lora_backward(x, empty, a[:0], b[:0], s[:0], None)
     assert not dx.any() and da.shape == (0, R, K) and db.shape == (0, N, R)
+
+
+@pytest.mark.parametrize("M,R,L", [(17, 8, 3), (32, 5, 2), (48, 16, 6), (300, 12, 300), (600, 48, 4), (700, 128, 2)])
+def test_rank_products_beyond_fp16(cuda_dev, M, R, L):
+    """h of some rows passes 65504, y does not: as finite as up to 16 rows.  One such rank meets an infinite lora_b."""
+    N, K = 200, 256
+    x, a, b, s, idx = adapters(M, N, K, R, L, seed=M + R)
+    a, b = (a * 16).half(), (b * 2.0 ** -8).half()
+    x[::3] = (x[::3] * 8192).half()
+    idx[0], idx[3], idx[4] = 0, 1, 0
+    h = s[idx.long().clamp_min(0)][:, None] * torch.einsum("mk,mrk->mr", x.float(), a.float()[idx.long().clamp_min(0)])
+    assert (h.abs() > 66000).any() and (h.abs() < 60000).any()
+    want, bound = delta_of(x, a, b, s, idx)
+    assert want.abs().max() < 60000
+    y = qw_b200.quantized_linear_lora(x, *zero_weights(N, K), a, b, s, idx)
+    close(y, want, bound, "y")
+    few = torch.cat([qw_b200.quantized_linear_lora(x[i:i + 16], *zero_weights(N, K), a, b, s, idx[i:i + 16])
+                     for i in range(0, M, 16)])
+    close(few, want, bound, "y in calls of 16 rows")
+    bad = [(0, 7, R - 1, INF), (1, 150, 0, -INF)]
+    for l, n, r, v in bad:
+        b[l, n, r] = v
+    close(qw_b200.quantized_linear_lora(x, *zero_weights(N, K), a, b, s, idx),
+          with_bad_b(want, x, a, b, s, idx, bad), bound, "y")
+
+
+@pytest.mark.parametrize("M,R", [(20, 5), (40, 12), (300, 3), (600, 44)])
+def test_an_infinite_input_is_no_nan(cuda_dev, M, R):
+    """Ranks that pad h stay zero: infinity times the zeros beside them would be NaN."""
+    N, K = 136, 128
+    x, a, b, s, _ = adapters(M, N, K, R, 1, seed=R)
+    x, a, b = x.abs(), a.abs() + 2.0 ** -6, b.abs() + 2.0 ** -6
+    ones = torch.ones(N, K // 64, dtype=torch.float16, device="cuda")
+    w = (torch.zeros(N, K // 8, dtype=torch.int32, device="cuda"), torch.zeros_like(ones), ones)
+    x[1, 70] = INF
+    y = qw_b200.quantized_linear_lora(x, *w, a.half(), b.half(), s, None)
+    assert (y[1] == INF).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
