@@ -324,8 +324,13 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     float tmax = -INFINITY, tsum = 0.f;
-    for (int j = lane; j < p.k; j += 32) tmax = fmaxf(tmax, tval[j]);
+    bool unknown = false;
+    for (int j = lane; j < p.k; j += 32) {
+      tmax = fmaxf(tmax, tval[j]);
+      unknown = unknown || tval[j] != tval[j];
+    }
     tmax = warp_max(tmax);
+    if (__any_sync(0xffffffffu, unknown)) tmax = NAN;  // a teacher of NaN alone is no row without entries
     // Writes the row from `value` of each element and, behind each vector's
     // store, starts the next row's copy into its place.
     auto write_row = [&](auto&& value) {
