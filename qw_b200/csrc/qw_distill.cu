@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
   uint32_t rank, C;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
-  // A CTA's shared memory may be written by its cluster only once it runs: met
-  // before the rows, so that rows without shares need no barrier either.
+  // A CTA's shared memory may be written by its cluster only once it runs: waited
+  // for before the first share, which the first row's loads come before.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int V = (int)p.V, M = (int)p.M;
@@ -287,8 +287,6 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     for (int e = 0; e < n; e += TH) copy_async16(mine + e * 16, z + lay.first + e * VT::N);
     if (lay.edge >= 0) ze = to_f32(z[lay.edge]);
   }
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // behind the first row's copies
   const float temp = p.temperature ? *p.temperature : 1.f;
   const float inv = 1.f / temp;
   const float c = inv * kLog2e;
@@ -297,6 +295,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
   // teacher's by row, the shares by row that reached the cluster barrier (a CTA
   // may be ahead of its cluster by rows that skip it, but by one barrier only).
   int met = 0;
+  bool begun = false;
   for (int parity = 0; m < M; parity ^= 1) {
     uint32_t* const ids = teacher + parity * p.k;
     float* const tval = reinterpret_cast<float*>(teacher) + (2 + parity) * p.k;
@@ -439,6 +438,11 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     for (int j = tid + TH; j < p.k; j += TH)
       if (ids[j] >= (uint32_t)cur.lo && ids[j] < (uint32_t)cur.hi) entry(j, tval[j], to_f32(z[ids[j]]));
     if (__any_sync(0xffffffffu, gap != 0.0)) gap = warp_sum(gap);
+    if (!begun) {
+      __syncwarp();
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      begun = true;
+    }
     if (lane < C) {  // this warp's share into CTA `lane` of the cluster
       uint32_t to;
       asm("mapa.shared::cluster.u32 %0, %1, %2;"
@@ -501,6 +505,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     }
     m = next;
   }
+  if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // no row had a share
 }
 
 constexpr int64_t kMaxSmem = 227 * 1024 - 2048;  // dynamic shared memory a CTA may take
