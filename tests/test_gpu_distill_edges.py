@@ -43,3 +43,25 @@ def test_a_teacher_of_nan_is_not_a_row_without_entries(cuda_dev, V, vdtype):
     named = torch.zeros(3, V, dtype=torch.bool, device="cuda").scatter_(1, idx[:3].long(), True)
     assert torch.equal(dz[:3].isnan(), named)
     assert torch.equal(dz[:3][~named], plain[:3][~named])
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 500000), (torch.float32, 500003), (torch.float16, 1000000),
+                                     (torch.bfloat16, 1000003)])
+def test_rows_longer_than_a_cluster_s_shared_memory(cuda_dev, dtype, V):
+    """What a share has beyond shared memory is read again; teacher ids all over the row, the ends of every CTA's share
+    (the part that is read again) among them."""
+    M, k = 3, 64
+    z, idx, t, w = batch(M, V, k, dtype, seed=5)
+    ends = (torch.arange(1, 9, device="cuda") * V) // 8
+    idx[:, :24] = torch.cat([ends - 40, ends - 8, ends - 1]).int()
+    idx[:, 24:28] = torch.tensor([0, 1, V - 17, V // 3], device="cuda", dtype=torch.int32)
+    z[0, V - 30], z[1, V // 8 - 50] = 9.0, 11.0  # a maximum where it is not held
+    w[2] = 0.0
+    want, bound = distill(z, idx, t, 1.0, w)
+    loss, dz = check(z, idx, t, 1.0, w)
+    for shift in (0, 1):  # in place, from an aligned and an odd start
+        own = torch.empty(M * V + shift, dtype=dtype, device="cuda")[shift:].view(M, V)
+        own.copy_(z)
+        loss, _ = qw_b200.topk_distillation(own, idx, t, row_weights=w, dlogits=own)
+        close(loss, want[0], bound[0], "loss in place")
+        close(own, want[1], bound[1], "dlogits in place")
