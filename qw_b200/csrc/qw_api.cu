@@ -1059,6 +1059,7 @@ static int linear_common(const qw_array* x, const qw_array* w, const qw_array* s
     if ((rc = check_array(linear_bias, "linear_bias"))) return rc;
     if (linear_bias->dtype != QW_F16 || numel(linear_bias) != w->shape[0])
       return fail(QW_EINVAL, "linear_bias must be float16 with N elements");
+    if (!aligned(linear_bias->data, 2)) return fail(QW_EINVAL, "linear_bias is misaligned");
   }
   if ((rc = run_qmm(x, w, scales, biases, 1, group_size, bits, mode, y, stream))) return rc;
   const int64_t N = w->shape[0];
@@ -1251,6 +1252,7 @@ int qw_quantized_linear_lora(const qw_array* x, const qw_array* w, const qw_arra
     if ((rc = check_array(linear_bias, "linear_bias"))) return rc;
     if (linear_bias->dtype != QW_F16 || numel(linear_bias) != sa.N)
       return fail(QW_EINVAL, "linear_bias must be float16 with N elements");
+    if (!aligned(linear_bias->data, 2)) return fail(QW_EINVAL, "linear_bias is misaligned");
   }
   LoraArgs la{};
   if ((rc = check_adapters(lora_a, lora_b, lora_scales, adapter_idx, sa.M, sa.N, sa.K, &la))) return rc;

@@ -170,3 +170,12 @@ def test_gradients_must_not_overlap_operands(change):
 def test_distillation_outputs_must_not_overlap_operands(change):
     assert distill(**change) == _lib.QW_EINVAL
     assert "overlap" in err()
+
+
+def test_a_misaligned_bias_is_refused():
+    assert forward(bias=arr([N], F16, 0x20001)) == _lib.QW_EINVAL
+    assert "misaligned" in err()
+    assert _lib.load().qw_quantized_linear_forward(
+        arr([M, K], F16), arr([N, K // 8], U32), arr([N, K // 64], F16), arr([N, K // 64], F16),
+        arr([N], F16, 0x20001), 64, 4, b"affine", arr([M, N], F16, 0x900000), None) == _lib.QW_EINVAL
+    assert "misaligned" in err()
