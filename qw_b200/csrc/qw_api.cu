@@ -1056,7 +1056,7 @@ static int linear_common(const qw_array* x, const qw_array* w, const qw_array* s
       return fail(QW_EINVAL, "global_scale must be a float32 scalar");
   }
   if (linear_bias) {
-    if ((rc = check_array(linear_bias, "linear_bias"))) return rc;
+    if ((rc = check_array(linear_bias, "linear_bias")) || (rc = check_array(w, "w"))) return rc;
     if (linear_bias->dtype != QW_F16 || numel(linear_bias) != w->shape[0])
       return fail(QW_EINVAL, "linear_bias must be float16 with N elements");
     if (!aligned(linear_bias->data, 2)) return fail(QW_EINVAL, "linear_bias is misaligned");

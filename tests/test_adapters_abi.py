@@ -179,3 +179,11 @@ def test_a_misaligned_bias_is_refused():
         arr([M, K], F16), arr([N, K // 8], U32), arr([N, K // 64], F16), arr([N, K // 64], F16),
         arr([N], F16, 0x20001), 64, 4, b"affine", arr([M, N], F16, 0x900000), None) == _lib.QW_EINVAL
     assert "misaligned" in err()
+
+
+def test_a_bias_without_weights_is_refused():
+    assert forward(w=None, bias=arr([N], F16)) == _lib.QW_EINVAL
+    assert _lib.load().qw_quantized_linear_forward(
+        arr([M, K], F16), None, arr([N, K // 64], F16), arr([N, K // 64], F16), arr([N], F16), 64, 4, b"affine",
+        arr([M, N], F16, 0x900000), None) == _lib.QW_EINVAL
+    assert "w is null" in err()
