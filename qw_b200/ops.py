@@ -341,6 +341,8 @@ def topk_distillation(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_v
     ``dlogits`` (optional) receives the gradient and may be ``logits``."""
     if teacher_idx.dtype == torch.int64:
         teacher_idx = teacher_idx.clamp(-1, 2 ** 31 - 1).to(torch.int32)  # an id past int32 is no entry, not another
+    if temperature is not None and temperature.dim() == 0:
+        temperature = temperature.reshape(1)
     if dlogits is None and grad:
         dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
     loss = logits.new_empty(logits.shape[:-1] or (1,), dtype=torch.float32)

@@ -65,3 +65,10 @@ def test_rows_longer_than_a_cluster_s_shared_memory(cuda_dev, dtype, V):
         loss, _ = qw_b200.topk_distillation(own, idx, t, row_weights=w, dlogits=own)
         close(loss, want[0], bound[0], "loss in place")
         close(own, want[1], bound[1], "dlogits in place")
+
+
+def test_a_temperature_without_dimensions(cuda_dev):
+    z, idx, t, w = batch(3, 900, 5, torch.float16)
+    want = qw_b200.topk_distillation(z, idx, t, torch.tensor([2.0], device="cuda"), w)
+    got = qw_b200.topk_distillation(z, idx, t, torch.tensor(2.0, device="cuda"), w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
