@@ -258,7 +258,7 @@ struct ProductMaps {
 };
 struct ProdShared {
   uint32_t row_id[kTileRows], row_slot[kTileRows], list[2 * kTileRows], slot_max[kTileRows];
-  uint64_t full[kStages], done[kStages];
+  uint64_t full[kStages], done[kStages], drained;
   int list_n;
   uint32_t tmem;
 };
@@ -331,8 +331,9 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
   const int chunks = (int)((f.len + kChunk - 1) / kChunk);
   const int c0 = (int)((int64_t)chunks * rank / C), c1 = (int)((int64_t)chunks * (rank + 1) / C);
   const uint32_t base = smem_u32(smem);
-  bool ok = true;        // a bounded wait that ran out: go on without waiting
+  bool ok = true;        // false: a bounded wait ran out, nothing more is loaded or multiplied
   uint32_t it0 = 0, vit0 = 0;  // steps and chunks of earlier rounds
+  uint32_t issued = 0;         // steps loaded, by the thread that loads
   constexpr uint32_t kDesc = mma_desc(kTileRows, RP, false, TRANS);
   // Few adapters: two sums of every other chunk, as the tensor cores' additions
   // truncate and an error grows with the number that follow one another.
@@ -351,14 +352,17 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
     const int nj = n - j0 < Cfg::GROUP ? n - j0 : Cfg::GROUP;
     const int steps = (c1 - c0) * ((nj + Cfg::PER - 1) / Cfg::PER);
     two = nj <= kHalf && c1 - c0 > 1;
-    if (warp == 1 && lane == 0) {  // loads
+    const bool working = ok;
+    if (warp == 1 && lane == 0 && working) {  // loads
       uint32_t it = it0, vit = vit0;
-      for (int c = c0; c < c1; ++c, ++vit) {
+      for (int c = c0; c < c1 && ok; ++c, ++vit) {
         for (int j = 0; j < nj; j += Cfg::PER, ++it) {
           const uint32_t s = it % kStages;
           const int here = nj - j < Cfg::PER ? nj - j : Cfg::PER;
-          if (it >= kStages)
-            ok = ok && mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
+          if (it >= kStages) {
+            ok = mbar_wait(&sh.done[s], (it / kStages - 1) & 1, q.status, kDevTimeoutEmpty);
+            if (!ok) break;
+          }
           mbar_arrive_expect_tx(&sh.full[s], (uint32_t)((j == 0 ? Cfg::V_STAGE : 0) +
                                                         here * (TRANS ? Cfg::W_STAGE : RP * 128)));
           if (j == 0)
@@ -373,14 +377,16 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
               tma_load_3d(dst, map_w, &sh.full[s], c * kChunk, 0, a);
             }
           }
+          issued = it + 1;
         }
       }
-    } else if (warp == 0 && lane == 0) {  // products
+    } else if (warp == 0 && lane == 0 && working) {  // products
       uint32_t it = it0, vit = vit0;
-      for (int c = c0; c < c1; ++c, ++vit) {
+      for (int c = c0; c < c1 && ok; ++c, ++vit) {
         for (int j = 0; j < nj; j += Cfg::PER, ++it) {
           const uint32_t s = it % kStages;
-          ok = ok && mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
+          ok = mbar_wait(&sh.full[s], (it / kStages) & 1, q.status, kDevTimeoutFull);
+          if (!ok) break;
           tc_fence_after();
           for (int i = 0; i < Cfg::PER && j + i < nj; ++i)
             multiply(c - c0, j + i, base + (vit % kStages) * Cfg::STAGE,
@@ -399,8 +405,17 @@ __device__ void product_tile(const Products& q, const Product& f, const CUtensor
       __syncthreads();
       ok = ok && mbar_wait(&sh.done[(it0 - 1) % kStages], ((it0 - 1) / kStages) & 1, q.status, kDevTimeoutAccum);
     }
+    ok = !__syncthreads_or(!ok);
+    if (working && !ok) {  // loads and products under way end before their memory goes
+      if (tid == 0) {
+        tc_commit(&sh.drained);
+        mbar_wait(&sh.drained, 0, q.status, kDevTimeoutAccum);
+      }
+      for (uint32_t u = issued < kStages ? 0 : issued - kStages; u < issued; ++u)
+        mbar_wait(&sh.full[u % kStages], (u / kStages) & 1, q.status, kDevTimeoutFull);
+      __syncthreads();
+    }
     tc_fence_after();
-    __syncthreads();
 
     // each row's own columns, to shared memory
     float* const sums = reinterpret_cast<float*>(smem);
@@ -514,6 +529,7 @@ __global__ void __launch_bounds__(kProdThreads) lora_products_kernel(const __gri
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.done[i], 1);
     }
+    mbar_init(&sh.drained, 1);
     fence_barrier_init();
   }
   if (threadIdx.x < 32) {
@@ -807,9 +823,10 @@ struct SumCfg {
 
 struct SumShared {
   uint64_t vfull[kVStages], vempty[kVStages], gfull[kVStages], dxfull[2], dxempty[2];
-  uint64_t accfull, accempty, afull, aempty;
+  uint64_t accfull, accempty, afull, aempty, drained;
   uint32_t tmem;
   int last;
+  int late;  // a bounded wait ran out
 };
 
 // 16 bytes from src (zeros where !valid)
@@ -881,6 +898,8 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     mbar_init(&sh.accempty, kWorkers / 32);
     mbar_init(&sh.afull, 1);
     mbar_init(&sh.aempty, 1);
+    mbar_init(&sh.drained, 1);
+    sh.late = 0;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -894,19 +913,32 @@ __global__ void __launch_bounds__(kSumThreads, 1)
   constexpr uint32_t kDx = 128, kOdd = 384;  // TMEM columns of the two dx buffers, and of D's odd steps
   pdl_wait();
   const int64_t items = (int64_t)q.plan.total[0] * q.tiles;
-  bool ok = true;  // a bounded wait that ran out: go on without waiting
+  // After a bounded wait that ran out the workers go on without waiting (they meet at
+  // barriers of their own); the others stop, one after the other, and see to what they
+  // have under way.
+  bool ok = true;
+  int last_image = -1;  // the last step whose image this thread loaded
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int code) {
+    if (ok && !mbar_wait(bar, parity, q.status, code)) {
+      ok = false;
+      sh.late = 1;
+    }
+  };
 
   if (warp >= kWorkers / 32 && warp < kMmaWarp) {
     // -------------------------------------------------------------- loads
     const int slot = (warp - kWorkers / 32) / kLoaders, part = (warp - kWorkers / 32) % kLoaders;
     constexpr int kQuarters = 4 / kLoaders;  // of the step's rows
     uint32_t it = 0, ai = 0;
-    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    int last = -1;  // the last step that this warp loaded
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const Item t = item_at(q, i);
       if (t.steps == 0) continue;
       if (t.dx && slot == 0 && part == 0) {
+        if (lane == 0 && ai > 0) wait(&sh.aempty, (ai - 1) & 1, kDevTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (lane == 0) {
-          if (ai > 0) ok = ok && mbar_wait(&sh.aempty, (ai - 1) & 1, q.status, kDevTimeoutEmpty);
           mbar_arrive_expect_tx(&sh.afull, RP * kCols * 2);
           for (int b = 0; b < 2; ++b)
             tma_load_3d(smem + Cfg::OFF_A + b * RP * 128, &maps.a, &sh.afull, (int)t.col0 + b * 64, 0, t.ck.adapter);
@@ -934,7 +966,10 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         // The products that read this stage are done; then those that read the
         // image's buffer, which are at most two steps later (so that a barrier
         // is never a whole turn ahead of its waiter).
-        if (it >= kVStages) ok = ok && mbar_wait(&sh.vempty[slot], (it / kVStages - 1) & 1, q.status, kDevTimeoutEmpty);
+        if (it >= kVStages) wait(&sh.vempty[slot], (it / kVStages - 1) & 1, kDevTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        last = (int)it;
         uint8_t* const stage = smem + slot * Cfg::V_STAGE;
         if (lane == 0 && part == 0 && runs.y) mbar_expect_tx(&sh.vfull[slot], (uint32_t)__popc(runs.y) * 2048u);
         __syncwarp();
@@ -968,12 +1003,15 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         if (lane == 0 && part == 0) {
           if (it >= Cfg::G_BUFS) {
             const uint32_t was = it - Cfg::G_BUFS;
-            ok = ok && mbar_wait(&sh.vempty[was % kVStages], (was / kVStages) & 1, q.status, kDevTimeoutEmpty);
+            wait(&sh.vempty[was % kVStages], (was / kVStages) & 1, kDevTimeoutEmpty);
           }
-          mbar_arrive_expect_tx(&sh.gfull[gb], Cfg::G_STAGE);
-          bulk_copy(base + Cfg::OFF_G + gb * Cfg::G_STAGE,
-                    q.images + ((int64_t)(t.ck.step0 + step) * 2 + (t.is_x ? 1 : 0)) * Cfg::G_STAGE, Cfg::G_STAGE,
-                    &sh.gfull[gb]);
+          if (ok) {
+            last_image = (int)it;
+            mbar_arrive_expect_tx(&sh.gfull[gb], Cfg::G_STAGE);
+            bulk_copy(base + Cfg::OFF_G + gb * Cfg::G_STAGE,
+                      q.images + ((int64_t)(t.ck.step0 + step) * 2 + (t.is_x ? 1 : 0)) * Cfg::G_STAGE, Cfg::G_STAGE,
+                      &sh.gfull[gb]);
+          }
         }
         __syncwarp();
         if (runs.x < 0) {
@@ -984,22 +1022,30 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         if (lane == 0) mbar_arrive(&sh.vfull[slot]);
       }
     }
+    // What is under way lands before the CTA goes (a step counts as landed when both
+    // its warps have arrived, so the one that gives up does).
+    if (lane == 0 && part == 1 && !ok) mbar_arrive(&sh.vfull[slot]);
+    if (lane == 0 && part == 0) {
+      if (last >= 0) mbar_wait(&sh.vfull[slot], (last / kVStages) & 1, q.status, kDevTimeoutFull);
+      if (ai > 0) mbar_wait(&sh.afull, (ai - 1) & 1, q.status, kDevTimeoutFull);
+    }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------- products
     uint32_t it = 0, dxs = 0, sums = 0, ai = 0;
     if (lane == 0) {
       constexpr uint32_t kSumDesc = mma_desc(128, kCols, true, true);
       constexpr uint32_t kDxDesc = mma_desc(kStepRows, kCols, false, true);
-      for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+      for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
         const Item t = item_at(q, i);
         if (t.steps == 0) continue;
-        if (t.sum && sums > 0) ok = ok && mbar_wait(&sh.accempty, (sums - 1) & 1, q.status, kDevTimeoutAccum);
+        if (t.sum && sums > 0) wait(&sh.accempty, (sums - 1) & 1, kDevTimeoutAccum);
         for (int step = 0; step < t.steps; ++step, ++it) {
           const uint32_t s = it % kVStages, gb = it % Cfg::G_BUFS;
-          ok = ok && mbar_wait(&sh.vfull[s], (it / kVStages) & 1, q.status, kDevTimeoutFull);
-          ok = ok && mbar_wait(&sh.gfull[gb], (it / Cfg::G_BUFS) & 1, q.status, kDevTimeoutFull);
-          if (t.dx && dxs >= 2)
-            ok = ok && mbar_wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, q.status, kDevTimeoutAccum);
+          wait(&sh.vfull[s], (it / kVStages) & 1, kDevTimeoutFull);
+          wait(&sh.gfull[gb], (it / Cfg::G_BUFS) & 1, kDevTimeoutFull);
+          if (t.dx && dxs >= 2) wait(&sh.dxempty[dxs & 1], (dxs / 2 - 1) & 1, kDevTimeoutAccum);
+          if (!ok) break;
           tc_fence_after();
           const uint32_t vs = base + s * Cfg::V_STAGE, gs = base + Cfg::OFF_G + gb * Cfg::G_STAGE;
           auto dx = [&]() {
@@ -1032,8 +1078,8 @@ __global__ void __launch_bounds__(kSumThreads, 1)
             }
           }
           if (t.dx && step == 0) {  // lora_a comes when the item before is done
-            ok = ok && mbar_wait(&sh.afull, ai & 1, q.status, kDevTimeoutFull);
-            dx();
+            wait(&sh.afull, ai & 1, kDevTimeoutFull);
+            if (ok) dx();
           }
           tc_commit(&sh.vempty[s]);
         }
@@ -1046,6 +1092,9 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           ++ai;
         }
       }
+      // every product and every arrival has ended before the CTA's memory goes
+      tc_commit(&sh.drained);
+      mbar_wait(&sh.drained, 0, q.status, kDevTimeoutAccum);
     }
     __syncwarp();
   } else {
@@ -1072,7 +1121,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
         const uint32_t b = dxs & 1;
         const int mine = next_row;
         if (step + 1 < t.steps) fetch_row(step + 1);
-        ok = ok && mbar_wait(&sh.dxfull[b], (dxs / 2) & 1, q.status, kDevTimeoutAccum);
+        wait(&sh.dxfull[b], (dxs / 2) & 1, kDevTimeoutAccum);
         __syncwarp();  // lanes without a row came early
         tc_fence_after();
         uint32_t d[kWarpCols / 16][16];
@@ -1141,7 +1190,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
       // 16 at a time through shared memory (2 KB, as 128 pieces of 16 bytes).
       uint32_t d[4][16];
       if (t.steps > 0) {
-        ok = ok && mbar_wait(&sh.accfull, sums & 1, q.status, kDevTimeoutAccum);
+        wait(&sh.accfull, sums & 1, kDevTimeoutAccum);
         ++sums;
         __syncwarp();
         tc_fence_after();
@@ -1260,6 +1309,8 @@ __global__ void __launch_bounds__(kSumThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (sh.late && last_image >= 0)  // images too, where products did not wait for them
+    mbar_wait(&sh.gfull[last_image % Cfg::G_BUFS], (last_image / Cfg::G_BUFS) & 1, q.status, kDevTimeoutFull);
 }
 
 constexpr size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }

@@ -355,6 +355,11 @@ __global__ void __launch_bounds__(LORA ? THREADS_LORA : THREADS, 1)
           }
         }
       }
+      // what is under way lands before the CTA goes, whoever gave up waiting for it
+      for (uint32_t u = it < (uint32_t)STAGES ? 0u : it - STAGES; u < it; ++u) {
+        mbar_wait(&xfull[u % STAGES], (u / STAGES) & 1, p.status, kDevTimeoutFull);
+        mbar_wait(&wpfull[u % STAGES], (u / STAGES) & 1, p.status, kDevTimeoutFull);
+      }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
