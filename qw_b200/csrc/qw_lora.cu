@@ -256,9 +256,10 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     q.lists.n = reinterpret_cast<uint32_t*>(base + f.second);
     q.lists.ids = reinterpret_cast<uint32_t*>(base + f.third);
     q.lists.slots = reinterpret_cast<uint32_t*>(base + f.fourth);
-    // Many rows of a high rank are worth the tcgen05 products' tiles of 128 rows
-    // (rank 64, 8 adapters, 5120 -> 5120, the whole call: 1024 rows in 116 us with
-    // them, 121 without; 512 rows 77 and 75; rank 32, 2048 rows to 17408: 395 and 388).
+    // Many rows of a high rank are worth the tcgen05 products' tiles of 128 rows.  The
+    // whole call in us with them and without, 8 adapters, 5120 -> 5120: 1024 rows of
+    // rank 64 113 and 119, of rank 128 156 and 165; 512 rows 75 and 74, 98 and 93;
+    // 300 rows 68 and 62, 82 and 73; rank 32 at 2048 rows 154 and 150.
     // (An empty stack has no tensor maps.)
     if (p.L > 0 && p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, q.full, status, sm_count, pdl, stream, err);
   }

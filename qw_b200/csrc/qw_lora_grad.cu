@@ -768,9 +768,10 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 //               operands along MN since the rows are the reduction, and
 //               dx[rows][columns] = g A into one of two TMEM buffers;
 //   warps 0-7   take a step's dx from TMEM to memory, and an item's D.
-// Odd steps of a long chunk have a D of their own: the tensor cores' additions
-// truncate, and an error grows with the number that follow one another (4096 rows:
-// dA to 1.3e-6 of its size, 2.3e-6 in one sum; the time is the same).
+// Odd steps of a chunk have a D of their own: the tensor cores' additions truncate,
+// and an error grows with the number that follow one another (dA of 4096 rows to
+// 1.2e-6 of its size, 2.0e-6 in one sum; of 256 rows 4.0e-7 and 5.4e-7; the plain
+// fp32 form 1.4e-6 and 4.8e-7; the times are the same, 135.1 and 19.8 us).
 // HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
 // rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
 // one D (64 of each) and are added when it is read; dx takes both into one sum.
@@ -778,7 +779,6 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.
 constexpr int kCols = 128;
-constexpr int kOneSum = 4;  // steps
 constexpr int kWorkers = 256;
 constexpr int kWarpCols = kCols / (kWorkers / 128);  // columns of D or dx a worker warp reads, of 32 rows
 constexpr int kVStages = 3;                          // and two warps for each that load
@@ -1064,7 +1064,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
           if (t.dx && step > 0) dx();  // before the sums: the workers wait for it
           if (t.sum) {
             const int blocks = (t.ck.count - step * kStepRows + 15) / 16;
-            const bool two = t.steps > kOneSum;
+            const bool two = t.steps > 1;
             const uint64_t b = operand_mn(vs, Cfg::BLOCK);
 #pragma unroll
             for (int half = 0; half < (Cfg::STACK ? 1 : 2); ++half) {
@@ -1197,7 +1197,7 @@ __global__ void __launch_bounds__(kSumThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x16(tmem + lanes + upper * kWarpCols + c * 16, d[c]);
         tmem_wait_ld();
-        if (t.steps > kOneSum) {
+        if (t.steps > 1) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t w[16];
