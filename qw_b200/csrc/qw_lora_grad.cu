@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // or of dy (dB) at a time, by a persistent grid of one CTA an SM, 128 rows a step.
 // The CTAs take the column tiles in turns, so that at a time they read a stretch
 // of the same rows (equal shares of all the work, a range of columns each, took
-// 110 us where this takes 77):
+// 110 us where this took 77):
 //   warps 8-13  load, two to a step in turn: its image of h or g (one bulk copy)
 //               and its rows of x or dy, all 128 or 8 at a time by TMA where they
 //               are consecutive, else copied (cp.async; a warp's proxy fence waits
@@ -772,9 +772,9 @@ __global__ void __launch_bounds__(kSplitThreads) lora_split_kernel(const Split q
 // and an error grows with the number that follow one another (dA of 4096 rows to
 // 1.2e-6 of its size, 2.0e-6 in one sum; of 256 rows 4.0e-7 and 5.4e-7; the plain
 // fp32 form 1.4e-6 and 4.8e-7; the times are the same, 135.1 and 19.8 us).
-// HBM-bound by x, dy and dx (5 TB/s of them over 4096 rows, 17408 and 5120 columns,
-// rank 64: 77 us; 6.3 TB/s within an item).  Up to rank 64 the two halves of h or g are rows of
-// one D (64 of each) and are added when it is read; dx takes both into one sum.
+// HBM-bound by x, dy and dx (4.1 TB/s of them over 4096 rows, 17408 and 5120 columns,
+// rank 64: 80 us).  Up to rank 64 the two halves of h or g are rows of one D (64 of
+// each) and are added when it is read; dx takes both into one sum.
 //
 // A sum of several chunks is joined by the last CTA to finish one of them, from
 // fp32 partial sums in chunk order, so that results do not depend on timing.

@@ -29,13 +29,15 @@
 // of the tokens that take that adapter as B, zero for the others.  Four more
 // warps write both (TMEM and the swizzled x slot) while the dequant warps are at
 // the weights; the producer only passes the stage on.  2048 x 17408 x 5120 with 8
-// adapters of rank 32: 379 us, where the projection alone takes 368 to 396 (power-
-// capped clocks); a pass of its own over y would read and write 214 MB.
+// adapters of rank 32: 380 us, where the projection alone takes 369 (421 and 418 once
+// the power cap lowers the clocks); a pass of its own over y would read and write 214 MB.
 // A zero times another adapter's infinity would be NaN: lora_b and h values that
 // are not finite fp16 enter as zero, and their terms, with h in fp32, are added in
 // the epilogue for the tokens that own them (so h may pass 65504).
 // The weights are fp16(s q + b), rounded once: the result's error is half of that
-// with the two roundings below (2.8e-4 and 5.7e-4 of y in the mean, 2048 x 17408 x 5120).
+// with the two roundings below (2.8e-4 and 5.7e-4 of y in the mean, 2048 x 17408 x 5120;
+// y's own rounding alone is 2.1e-4).  The rest would take a second fp16 term, twice the
+// products and the tensor memory.
 //
 // Otherwise the weights the MMA consumes are exactly qw_dequantize's (fp16(fp16(s*q)
 // + b)): pairs (1024 + q_even, 1024 + 16 q_odd) come from one prmt and one

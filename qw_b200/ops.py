@@ -293,7 +293,8 @@ def quantized_linear_lora(x: torch.Tensor, w, scales, biases, lora_a: torch.Tens
     (A, B, s) of each row, many adapters in one call: ``lora_a`` fp16
     [L, R, K], ``lora_b`` fp16 [L, N, R], ``lora_scales`` fp32 [L] (None: 1),
     ``adapter_idx`` int32, one per row in any order, -1 for none (None: adapter
-    0 for every row)."""
+    0 for every row).  No part of torch's autograd: the adapters' gradient is
+    lora_backward's."""
     if out is None:
         out = x.new_empty((*x.shape[:-1], w.shape[0]), dtype=torch.float16)
     L = _lib.load()
