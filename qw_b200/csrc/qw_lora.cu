@@ -261,7 +261,8 @@ cudaError_t launch_lora_rank(const LoraArgs& p, int token_tile, void* ws, void* 
     // rank 64 113 and 119, of rank 128 156 and 165; 512 rows 75 and 74, 98 and 93;
     // 300 rows 68 and 62, 82 and 73; rank 32 at 2048 rows 154 and 150.
     // (An empty stack has no tensor maps.)
-    if (p.L > 0 && p.R > 32 && p.M > 512) return launch_lora_products(p, q.lists, q.h16, q.full, status, sm_count, pdl, stream, err);
+    if (p.L > 0 && p.R > 32 && p.M > 512)
+      return launch_lora_products(p, q.lists, q.h16, q.full, status, sm_count, pdl, stream, err);
   }
   q.tiles = (int)((p.M + 15) / 16);
   q.zero = static_cast<uint4*>(zero);

@@ -82,8 +82,10 @@ struct PfCfg {
   // the next on have at least STAGES + 1 blocks together (one each, two where adapters
   // are), so that block belongs to them, and their products wait for this tile's epilogue.
   static constexpr int OFF_BAD = OFF_BAR + NBAR * 8 + 64;
-  static constexpr int OFF_XGO = OFF_BAD + STAGES * BM;  // LORA: barriers, the producer has freed the stage for an adapters' block
-  static constexpr int OFF_WIDE = OFF_XGO + 8 * STAGES;  // LORA: of the same tiles, whether a warp met such values in h
+  // LORA: barriers, the producer has freed the stage for an adapters' block
+  static constexpr int OFF_XGO = OFF_BAD + STAGES * BM;
+  // LORA: of the same tiles as OFF_BAD's, whether a warp met such values in h
+  static constexpr int OFF_WIDE = OFF_XGO + 8 * STAGES;
   static constexpr int SMEM = OFF_BAD + 1024;
   static constexpr int SMEM_LORA = SMEM + STAGES * BM + 12 * STAGES;
   // TMEM: D (BT fp32 columns) at 0, then the A stages (32 columns each)
