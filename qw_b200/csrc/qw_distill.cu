@@ -453,6 +453,7 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
                    "f"(mx), "f"(sum)
                    : "memory");
     }
+    __syncwarp();  // .aligned takes a whole warp
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     met ^= 1;
     // two shares a lane, joined by every warp
@@ -506,7 +507,10 @@ __global__ void __launch_bounds__(TH, PER_SM) distill_rows_kernel(const DistillA
     }
     m = next;
   }
-  if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // no row had a share
+  if (!begun) {  // no row had a share
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
 }
 
 constexpr int64_t kMaxSmem = 227 * 1024 - 2048;  // dynamic shared memory a CTA may take

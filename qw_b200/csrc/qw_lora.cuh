@@ -25,6 +25,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // .aligned takes a whole warp
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
