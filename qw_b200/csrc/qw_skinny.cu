@@ -533,6 +533,12 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
         }
       }
     }
+    // With adapters, what is under way lands before the CTA goes, whoever gave up
+    // waiting for it.  (In the plain kernel these waits cost 0.5% of a decode stack.)
+    if (LORA && lane == 0)
+#pragma unroll 1
+      for (int u = issued < WST ? 0 : issued - WST; u < issued; ++u)
+        mbar_wait(&wfull[u % WST], (u / WST) & 1, p.status, kDevTimeoutFull);
     return;
   }
 
@@ -570,6 +576,9 @@ __global__ void __launch_bounds__((SkinnyCfg<MT, BITS, WIDE>::THREADS), 1)
           if (++c == op.C) c = 0;
         }
       }
+#pragma unroll 1
+      for (int u = issued < SST ? 0 : issued - SST; LORA && u < issued; ++u)
+        mbar_wait(&sfull[u % SST], (u / SST) & 1, p.status, kDevTimeoutFull);
     }
     return;
   }
